@@ -13,6 +13,14 @@
  *   tq_paged_mixed    a step's decode rows (with their cache write) and prefill
  *                     rows in one launch
  *
+ * three operators for models with position rotation, grouped K/V heads and a 16-bit pool, and for
+ * steps of several new tokens per sequence (prompt chunks, drafted tokens):
+ *
+ *   tq_rope_cache_write  norms and rotates each new token's query and key heads, writes the queries out
+ *                     and the keys and values into the pool
+ *   tq_paged_chunk    causal attention of chunks of new tokens (from one on) straight off a 16-bit pool
+ *   tq_verify_drafts  drafted tokens against the target's logits, and the token drawn after them
+ *
  * plus two kernels of the model step around them:
  *
  *   tq_argmax_rows    index of each logit row's maximum (greedy sampling)
@@ -44,8 +52,8 @@
  *     out-of-range block id, slot or length. Such an entry is skipped (the
  *     kernel never reads or writes outside the pool), so the result for that
  *     row is undefined but the launch is memory safe.
- *   - Only head_dim == 64 is supported (GPT-2 family). block_size may be any
- *     value in [1, 1024].
+ *   - Only head_dim == 64 is supported (GPT-2 family), and 64 and 128 by tq_rope_cache_write and
+ *     tq_paged_chunk. block_size may be any value in [1, 1024].
  *   - Calls are not thread safe with respect to the same pool: the caller
  *     (one engine thread) orders them on one stream.
  */
@@ -72,6 +80,12 @@ typedef enum tq_status {
 #define TQ_DEVERR_SLOT 2       /* a slot_mapping entry >= num_blocks * block_size */
 #define TQ_DEVERR_LENGTH 4     /* a context / query length the block table cannot hold */
 #define TQ_DEVERR_ORDER 8      /* a seq_order entry outside [0, num_seqs) */
+#define TQ_DEVERR_POSITION 16  /* a position outside the rotation table */
+#define TQ_DEVERR_TOKEN 32     /* a drafted token outside [0, vocab) */
+#define TQ_DEVERR_VALUE 64     /* a logit row that has no distribution (a NaN or +inf, or nothing above -inf) */
+
+/* Element types of the entry points that take one (tq_paged_chunk, tq_rope_cache_write, tq_verify_drafts). */
+typedef enum tq_dtype { TQ_F32 = 0, TQ_F16 = 1, TQ_BF16 = 2 } tq_dtype;
 
 /* Human-readable name of a status code (static storage, never NULL). */
 const char* tq_status_string(tq_status status);
@@ -450,6 +464,117 @@ tq_status tq_embed_rows(float* x, int64_t x_stride, const int64_t* ids, const in
                         const int64_t* tokens, const int64_t* positions, const float* wte, const float* wpe,
                         int64_t rows, int32_t C, int64_t vocab, int64_t n_positions, int32_t* d_error,
                         void* stream);
+
+/*
+ * Cache write with the position rotation applied on the way (and each head's norm, if weights are
+ * given). For every token n in [0, num_tokens), every query head h and key head h:
+ *
+ *   q_out[n, h] = R_p(norm(q[n, h]; q_norm))
+ *   pool[slot / block_size][layer][0][h][slot % block_size] = R_p(norm(k[n, h]; k_norm))
+ *   pool[slot / block_size][layer][1][h][slot % block_size] = v[n, h]                     (bit exact)
+ *
+ * with p = positions[n] and slot = slot_mapping[n]; a negative slot marks a padded token: its queries are
+ * written out, the pool is not touched. norm(x; w) = x w / sqrt(mean(x^2) + eps) over the head's dims; a null
+ * q_norm or k_norm leaves those heads as they are. R_p turns the first rotary_dim dims,
+ * for i < rotary_dim / 2, the pair (a, b) = dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where interleaved is 1:
+ *
+ *   (a, b) -> (a c - b s, b c + a s),  c = table[p][i], s = table[p][rotary_dim / 2 + i]
+ *
+ * and leaves the others. table is fp32 [num_positions, rotary_dim], contiguous. All arithmetic is fp32, rounded once
+ * to dtype (tq_dtype), the type of q_out, q, k, v, q_norm, k_norm and pool; the pool has num_kv_heads heads, and
+ * num_heads need not be a multiple of it here. head_dim 64 or 128; rotary_dim a multiple of 16, at most
+ * head_dim. Pointers 16-byte aligned and row strides multiples of 16 bytes. q_out may be q (the same rows in
+ * place); no other output may overlap an input. A position outside the table sets
+ * TQ_DEVERR_POSITION and skips its token, a slot >= num_blocks * block_size sets TQ_DEVERR_SLOT and
+ * skips its cache write. Slots other than negative ones must differ.
+ *
+ * No counterpart in the reference (GPT-2 adds learned position embeddings, tokquay/model.py:172); the cache write
+ * is PagedBatch.write's (tokquay/kv_cache.py:228-232).
+ */
+tq_status tq_rope_cache_write(void* q_out, int64_t q_out_row_stride, const void* q, int64_t q_row_stride,
+                              const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride,
+                              void* pool, int64_t num_blocks, int32_t num_layers, int32_t num_heads,
+                              int32_t num_kv_heads, int32_t block_size, int32_t head_dim, int32_t layer,
+                              const int64_t* slot_mapping, const int64_t* positions, const float* table,
+                              int64_t num_positions, int32_t rotary_dim, int32_t interleaved,
+                              const void* q_norm, const void* k_norm, float eps, int64_t num_tokens,
+                              int32_t dtype, int32_t* d_error, void* stream);
+
+/*
+ * Attention of chunks of new tokens over a 16-bit paged cache with grouped heads. Sequence b feeds
+ * n_b = cu_seqlens_q[b+1] - cu_seqlens_q[b] tokens (one: a decode row; a few: drafted tokens; many: a prompt or
+ * a piece of one) at positions q_start[b] .. q_start[b] + n_b - 1, whose q rows are
+ * q + (cu_seqlens_q[b] + i) * q_row_stride. Its K/V for positions [0, q_start[b] + n_b) must already be
+ * in the pool. Causal:
+ *
+ *   out[row, h] = softmax_{j <= q_start[b] + i}(scale * q[row, h] . K_b[h / G][j]) @ V_b[h / G][j],  G = num_heads / num_kv_heads
+ *
+ * pool[num_blocks][num_layers][2][num_kv_heads][block_size][head_dim], q and out are of dtype (TQ_F16 or TQ_BF16),
+ * head_dim 64 or 128. Scores, weights and sums are fp32; each weight is rounded to dtype before it meets V, and the
+ * output once. What the pool holds behind a sequence's last position, or at positions a row does not see, never
+ * reaches that row, infinities and NaN included. scale is any finite number.
+ *
+ * cu_seqlens_q has num_seqs + 1 entries and is non-decreasing; sequences may be empty, and rows of q and out
+ * outside every sequence are left alone. max_query_len >= every n_b and max_context_len >= every
+ * q_start[b] + n_b size the launch: a sequence past them, past num_q_rows or past its block table sets
+ * TQ_DEVERR_LENGTH and gets no output. Bad block ids set TQ_DEVERR_BLOCK_ID (that sequence's output is undefined).
+ * q and pool 16-byte aligned, out 8-byte, q_row_stride a multiple of 8 elements, out_row_stride of 4. out
+ * must not overlap q.
+ *
+ * Keys are split into parts where the rows alone do not fill the GPU; the parts' sums are joined by a second
+ * launch, in a fixed order, and kept in tq_paged_chunk_workspace_size(...) bytes of workspace (16-byte aligned, any
+ * contents; calls that may run at the same time need one each).
+ *
+ * Does for such models what tq_paged_decode and tq_paged_prefill do for the reference's (tokquay/kv_cache.py:208-214,
+ * :234-242; tokquay/model.py:94-96).
+ */
+tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                         const void* pool, int64_t num_blocks, int32_t num_layers, int32_t num_heads,
+                         int32_t num_kv_heads, int32_t block_size, int32_t head_dim, int32_t layer,
+                         const int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks_per_seq,
+                         const int32_t* cu_seqlens_q, const int32_t* q_start, int32_t num_seqs,
+                         int32_t num_q_rows, int32_t max_query_len, int32_t max_context_len, float scale,
+                         int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* d_error, void* stream);
+
+/* Bytes of workspace tq_paged_chunk needs for these sizes (0 if none). */
+size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                     int32_t num_q_rows, int32_t max_query_len, int32_t max_context_len);
+
+/*
+ * Verification of drafted tokens against the target's logits, from given random numbers (speculative
+ * sampling). Sequence b has n_b = cu_seqlens_q[b+1] - cu_seqlens_q[b] rows from lo = cu_seqlens_q[b] on: rows
+ * lo + i, i < n_b - 1, judge its drafted tokens x_i = draft_tokens[lo + i] in order, and the last row follows all of
+ * them (the rows tq_paged_chunk computes for the last token and the drafted ones fed after it). With
+ * p_i = softmax(logits[lo + i] / temperature[b]), or all of it on tq_argmax_rows' column of the row where
+ * temperature[b] is not above 0, and q_i = draft_probs[lo + i], or all of it on x_i where draft_probs is null:
+ *
+ *   x_i stands while uniforms[lo + i] * q_i(x_i) < p_i(x_i); accepted[b] = r counts those before the first that does not
+ *   next token ~ max(p_r - q_r, 0) where one does not stand (~ p_r where that leaves nothing), ~ p of the last row else
+ *   tokens[b] = x_0 .. x_{r-1}, next, -1, -1 ..                (max_query_len entries)
+ *
+ * The draw from weights w is the lowest j with w_0 + .. + w_j > u (w_0 + w_1 + ..), u = uniforms[last row] (the last
+ * j with w_j > 0 where rounding leaves none). Weights and sums are fp64. With
+ * independent uniform numbers and drafts drawn from q the tokens are distributed as the target's own. A sequence of no rows gets r = 0 and only -1.
+ *
+ * logits: [num_rows, vocab] of dtype (tq_dtype), row stride logits_row_stride; -inf masks a token. draft_probs:
+ * fp32 [num_rows, vocab], row stride probs_row_stride (rows of no drafted token, the last ones, are not read).
+ * A row of a sequence with a temperature that holds a NaN or +inf, or nothing above -inf, has no distribution: it is
+ * taken greedily and sets TQ_DEVERR_VALUE if the sequence came to it. A drafted token outside [0, vocab) sets
+ * TQ_DEVERR_TOKEN and does not stand. A sequence that does not fit num_rows or max_query_len sets
+ * TQ_DEVERR_LENGTH and is treated as one of no rows. tokens is int64 [num_seqs, max_query_len], accepted int32 [num_seqs].
+ *
+ * Needs tq_verify_drafts_workspace_size(...) bytes of workspace (16-byte aligned, any contents; calls that may
+ * run at the same time need one each). No counterpart in the reference; it stands beside Engine._sample
+ * (tokquay/engine.py:83-92, :189-194).
+ */
+tq_status tq_verify_drafts(int64_t* tokens, int32_t* accepted, const void* logits, int64_t logits_row_stride,
+                           const float* draft_probs, int64_t probs_row_stride, const int64_t* draft_tokens,
+                           const float* uniforms, const float* temperature, const int32_t* cu_seqlens_q,
+                           int32_t num_seqs, int32_t num_rows, int32_t max_query_len, int32_t vocab, int32_t dtype,
+                           void* workspace, size_t workspace_bytes, int32_t* d_error, void* stream);
+
+/* Bytes of workspace tq_verify_drafts needs for these sizes. */
+size_t tq_verify_drafts_workspace_size(int32_t num_seqs, int32_t num_rows, int32_t vocab);
 
 #ifdef __cplusplus
 }

@@ -23,6 +23,9 @@ DEVERR_BLOCK_ID = 1
 DEVERR_SLOT = 2
 DEVERR_LENGTH = 4
 DEVERR_ORDER = 8
+DEVERR_POSITION = 16
+DEVERR_TOKEN = 32
+DEVERR_VALUE = 64
 
 # name -> (restype, argtypes); the order of argtypes is the C declaration's.
 SIGNATURES: dict[str, tuple] = {
@@ -176,6 +179,46 @@ SIGNATURES: dict[str, tuple] = {
             ctypes.c_int64, ctypes.c_int64, c_i32p, ctypes.c_void_p,  # vocab, n_positions, d_error, stream
         ],
     ),
+    "tq_rope_cache_write": (
+        ctypes.c_int,
+        [
+            ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,  # q_out, stride, q, stride
+            ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,  # k, stride, v, stride
+            ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,  # pool, num_blocks, num_layers, num_heads
+            ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,  # num_kv_heads, block_size, head_dim, layer
+            c_i64p, c_i64p, c_f32p, ctypes.c_int64,  # slot_mapping, positions, table, num_positions
+            ctypes.c_int32, ctypes.c_int32,  # rotary_dim, interleaved
+            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float, ctypes.c_int64,  # q_norm, k_norm, eps, num_tokens
+            ctypes.c_int32, c_i32p, ctypes.c_void_p,  # dtype, d_error, stream
+        ],
+    ),
+    "tq_paged_chunk": (
+        ctypes.c_int,
+        [
+            ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,  # out, stride, q, stride
+            ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,  # pool, num_blocks, num_layers, num_heads
+            ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,  # num_kv_heads, block_size, head_dim, layer
+            c_i32p, ctypes.c_int64, ctypes.c_int32,  # block_tables, block_table_stride, max_blocks_per_seq
+            c_i32p, c_i32p,  # cu_seqlens_q, q_start
+            ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,  # num_seqs, num_q_rows, max_query_len, max_context_len
+            ctypes.c_float, ctypes.c_int32,  # scale, dtype
+            ctypes.c_void_p, ctypes.c_size_t,  # workspace, workspace_bytes
+            c_i32p, ctypes.c_void_p,  # d_error, stream
+        ],
+    ),
+    "tq_paged_chunk_workspace_size": (ctypes.c_size_t, [ctypes.c_int32] * 7),
+    "tq_verify_drafts": (
+        ctypes.c_int,
+        [
+            c_i64p, c_i32p, ctypes.c_void_p, ctypes.c_int64,  # tokens, accepted, logits, logits_row_stride
+            c_f32p, ctypes.c_int64, c_i64p, c_f32p, c_f32p,  # draft_probs, stride, draft_tokens, uniforms, temperature
+            c_i32p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,  # cu_seqlens_q, num_seqs, num_rows, max_query_len
+            ctypes.c_int32, ctypes.c_int32,  # vocab, dtype
+            ctypes.c_void_p, ctypes.c_size_t,  # workspace, workspace_bytes
+            c_i32p, ctypes.c_void_p,  # d_error, stream
+        ],
+    ),
+    "tq_verify_drafts_workspace_size": (ctypes.c_size_t, [ctypes.c_int32] * 3),
     "tq_argmax_rows": (
         ctypes.c_int,
         [c_i64p, c_f32p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p],  # out, logits, rows, cols, row_stride, stream

@@ -322,6 +322,184 @@ void linear(at::Tensor out, const at::Tensor& x, const at::Tensor& weight, const
         "tq_linear");
 }
 
+// ---- rotated cache append, chunk attention and draft verification: pools of three types, grouped heads
+
+int32_t dtype_of(at::ScalarType t) {
+  return t == at::kFloat ? TQ_F32 : t == at::kHalf ? TQ_F16 : t == at::kBFloat16 ? TQ_BF16 : -1;
+}
+
+// A contiguous pool of one of the types, with heads of 64 or 128 dims.
+Pool typed_pool_of(const char* op, const at::Tensor& pool, int64_t layer, bool float32) {
+  const bool type = pool.scalar_type() == at::kHalf || pool.scalar_type() == at::kBFloat16 ||
+                    (float32 && pool.scalar_type() == at::kFloat);
+  TORCH_CHECK(pool.dim() == 6 && pool.size(2) == 2 && type && pool.is_contiguous() && pool.is_cuda(), op,
+              ": pool must be a contiguous ", float32 ? "float32, float16 or bfloat16" : "float16 or bfloat16",
+              " [num_blocks, n_layer, 2, n_kv_head, block_size, d_head] tensor on a HIP device");
+  TORCH_CHECK(pool.size(5) == 64 || pool.size(5) == 128, op, ": only d_head 64 and 128 are supported, got ",
+              pool.size(5));
+  TORCH_CHECK(layer >= 0 && layer < pool.size(1), op, ": layer ", layer, " out of range [0, ", pool.size(1), ")");
+  TORCH_CHECK(pool.size(0) >= 1 && pool.size(3) >= 1 && pool.size(4) >= 1 && pool.size(4) <= 1024 &&
+                  pool.size(0) <= INT32_MAX && pool.size(1) <= INT32_MAX && pool.size(3) <= 65535,
+              op, ": pool must hold blocks and heads, in blocks of at most 1024 slots");
+  return {pool.size(0), (int32_t)pool.size(1), (int32_t)pool.size(3), (int32_t)pool.size(4), (int32_t)pool.size(5),
+          pool.device()};
+}
+
+// Rows [N, heads, d_head] or [N, heads * d_head] of the pool's type, each row's elements contiguous, rows `align`
+// bytes aligned. `heads` 0: any number (3-dimensional tensors tell it, others by their width); it is returned.
+int64_t typed_rows_of(const char* op, const char* name, const at::Tensor& t, int64_t rows, int64_t& heads,
+                      const at::Tensor& pool, const Pool& p, int64_t align) {
+  on_device(op, name, t, p);
+  TORCH_CHECK(t.scalar_type() == pool.scalar_type(), op, ": ", name, " must be of the pool's type ",
+              pool.scalar_type(), ", got ", t.scalar_type());
+  bool ok = t.dim() == 3 ? t.size(2) == p.head_dim && t.stride(2) == 1 && (t.size(1) <= 1 || t.stride(1) == p.head_dim)
+                         : t.dim() == 2 && t.size(1) % p.head_dim == 0 && (t.size(1) <= 1 || t.stride(1) == 1);
+  if (ok) {
+    const int64_t has = t.dim() == 3 ? t.size(1) : t.size(1) / p.head_dim;
+    ok = has >= 1 && has <= 65535 && (heads == 0 || has == heads);
+    if (ok) heads = has;
+  }
+  TORCH_CHECK(ok, op, ": ", name, " must be [N, heads, ", p.head_dim, "] or [N, heads * ", p.head_dim,
+              "] with contiguous rows", heads > 0 ? " of " + std::to_string(heads) + " heads" : std::string());
+  const int64_t width = heads * p.head_dim;
+  TORCH_CHECK(t.size(0) >= rows, op, ": ", name, " has ", t.size(0), " rows, needs ", rows);
+  const int64_t stride = t.size(0) > 1 ? t.stride(0) : width;
+  TORCH_CHECK(rows <= 1 || stride >= width, op, ": ", name, "'s rows overlap (row stride ", stride, ")");
+  TORCH_CHECK((uintptr_t)t.data_ptr() % align == 0 && (rows <= 1 || stride * t.element_size() % align == 0), op, ": ",
+              name, "'s rows must be ", align, "-byte aligned");
+  return rows <= 1 ? width : stride;
+}
+
+void norm_of(const char* op, const char* name, const c10::optional<at::Tensor>& t, const at::Tensor& pool,
+             const Pool& p) {
+  if (!t.has_value()) return;
+  on_device(op, name, *t, p);
+  TORCH_CHECK(t->scalar_type() == pool.scalar_type() && t->dim() == 1 && t->size(0) == p.head_dim &&
+                  t->is_contiguous() && (uintptr_t)t->data_ptr() % 16 == 0,
+              op, ": ", name, " must be a contiguous, 16-byte aligned [", p.head_dim, "] tensor of the pool's type");
+}
+
+void rope_cache_write(at::Tensor q_out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor pool,
+                      int64_t layer, const at::Tensor& slot_mapping, const at::Tensor& positions,
+                      const at::Tensor& table, bool interleaved, const c10::optional<at::Tensor>& q_norm,
+                      const c10::optional<at::Tensor>& k_norm, double eps, const c10::optional<at::Tensor>& d_error) {
+  const char* op = "tokquay_amd::rope_cache_write";
+  const Pool p = typed_pool_of(op, pool, layer, true);
+  vector_of(op, "slot_mapping", slot_mapping, at::kLong, 0, p);
+  const int64_t n = slot_mapping.numel();
+  vector_of(op, "positions", positions, at::kLong, n, p);
+  int64_t heads = 0, kv_heads = p.heads;
+  const int64_t qs = typed_rows_of(op, "q", q, n, heads, pool, p, 16);
+  const int64_t os = typed_rows_of(op, "q_out", q_out, n, heads, pool, p, 16);
+  const int64_t ks = typed_rows_of(op, "k", k, n, kv_heads, pool, p, 16);
+  const int64_t vs = typed_rows_of(op, "v", v, n, kv_heads, pool, p, 16);
+  on_device(op, "table", table, p);
+  TORCH_CHECK(table.scalar_type() == at::kFloat && table.dim() == 2 && table.is_contiguous() &&
+                  (uintptr_t)table.data_ptr() % 16 == 0 && table.size(1) >= 16 && table.size(1) <= p.head_dim &&
+                  table.size(1) % 16 == 0,
+              op, ": table must be a contiguous float32 [positions, rotary] tensor, rotary a multiple of 16 up to ",
+              p.head_dim);
+  norm_of(op, "q_norm", q_norm, pool, p);
+  norm_of(op, "k_norm", k_norm, pool, p);
+  error_word_of(op, d_error, p);
+  check(tq_rope_cache_write(q_out.data_ptr(), os, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+                            pool.data_ptr(), p.blocks, p.layers, (int32_t)heads, p.heads, p.block_size, p.head_dim,
+                            (int32_t)layer, slot_mapping.data_ptr<int64_t>(), positions.data_ptr<int64_t>(),
+                            table.data_ptr<float>(), table.size(0), (int32_t)table.size(1), interleaved ? 1 : 0,
+                            ptr<void>(q_norm), ptr<void>(k_norm), (float)eps, n, dtype_of(pool.scalar_type()),
+                            ptr<int32_t>(d_error), stream_of(pool)),
+        "tq_rope_cache_write");
+}
+
+void paged_chunk(at::Tensor out, const at::Tensor& q, const at::Tensor& pool, int64_t layer,
+                 const at::Tensor& block_tables, const at::Tensor& cu_seqlens_q, const at::Tensor& q_start,
+                 int64_t max_query_len, int64_t max_context_len, double scale,
+                 const c10::optional<at::Tensor>& workspace, const c10::optional<at::Tensor>& d_error) {
+  const char* op = "tokquay_amd::paged_chunk";
+  const Pool p = typed_pool_of(op, pool, layer, false);
+  vector_of(op, "q_start", q_start, at::kInt, 0, p);
+  const int64_t n = q_start.numel();
+  TORCH_CHECK(n <= INT32_MAX, op, ": too many sequences");
+  vector_of(op, "cu_seqlens_q", cu_seqlens_q, at::kInt, n + 1, p);
+  TORCH_CHECK(cu_seqlens_q.numel() == n + 1, op, ": cu_seqlens_q must have num_seqs + 1 entries");
+  TORCH_CHECK(q.dim() >= 1 && q.size(0) <= INT32_MAX, op, ": q has too many rows");
+  const int64_t rows = q.size(0);
+  int64_t heads = 0;
+  const int64_t qs = typed_rows_of(op, "q", q, rows, heads, pool, p, 16);
+  const int64_t os = typed_rows_of(op, "out", out, rows, heads, pool, p, 8);
+  TORCH_CHECK(heads % p.heads == 0, op, ": ", heads, " query heads are no multiple of the pool's ", p.heads);
+  const int64_t ts = tables_of(op, "block_tables", block_tables, n, p);
+  TORCH_CHECK(block_tables.size(1) <= INT32_MAX, op, ": block_tables has too many columns");
+  TORCH_CHECK(max_query_len >= 0 && max_query_len <= INT32_MAX && max_context_len >= 0 &&
+                  max_context_len <= INT32_MAX, op, ": max_query_len and max_context_len must be lengths");
+  error_word_of(op, d_error, p);
+  size_t ws = workspace_of(op, workspace, p);
+  const size_t need = tq_paged_chunk_workspace_size((int32_t)n, (int32_t)heads, p.heads, p.head_dim, (int32_t)rows,
+                                                    (int32_t)max_query_len, (int32_t)max_context_len);
+  at::Tensor own;  // from torch's allocator: safe on any stream and under graph capture
+  void* at_ws = ptr<void>(workspace);
+  if (need > 0 && !workspace.has_value()) {
+    own = at::empty({(int64_t)need}, pool.options().dtype(at::kByte));
+    at_ws = own.data_ptr();
+    ws = need;
+  }
+  check(tq_paged_chunk(out.data_ptr(), os, q.data_ptr(), qs, pool.data_ptr(), p.blocks, p.layers, (int32_t)heads,
+                       p.heads, p.block_size, p.head_dim, (int32_t)layer, block_tables.data_ptr<int32_t>(), ts,
+                       (int32_t)block_tables.size(1), cu_seqlens_q.data_ptr<int32_t>(), q_start.data_ptr<int32_t>(),
+                       (int32_t)n, (int32_t)rows, (int32_t)max_query_len, (int32_t)max_context_len, (float)scale,
+                       dtype_of(pool.scalar_type()), at_ws, ws, ptr<int32_t>(d_error), stream_of(pool)),
+        "tq_paged_chunk");
+}
+
+// A [rows, vocab] tensor with contiguous rows on p's device; its row stride.
+int64_t vocab_rows_of(const char* op, const char* name, const at::Tensor& t, int64_t rows, int64_t vocab) {
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == vocab && (vocab <= 1 || t.stride(1) == 1), op, ": ",
+              name, " must be [", rows, ", ", vocab, "] with contiguous rows");
+  TORCH_CHECK(rows <= 1 || t.stride(0) >= vocab, op, ": ", name, "'s rows overlap");
+  return rows > 1 ? t.stride(0) : vocab;
+}
+
+void verify_drafts(at::Tensor tokens, at::Tensor accepted, const at::Tensor& logits,
+                   const c10::optional<at::Tensor>& draft_probs, const at::Tensor& draft_tokens,
+                   const at::Tensor& uniforms, const at::Tensor& temperature, const at::Tensor& cu_seqlens_q,
+                   const c10::optional<at::Tensor>& d_error) {
+  const char* op = "tokquay_amd::verify_drafts";
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && dtype_of(logits.scalar_type()) >= 0, op,
+              ": logits must be a float32, float16 or bfloat16 [rows, vocab] tensor on a HIP device");
+  const int64_t rows = logits.size(0), vocab = logits.size(1), n = temperature.numel();
+  TORCH_CHECK(rows <= INT32_MAX && vocab >= 1 && vocab <= 1 << 30 && n <= INT32_MAX, op, ": sizes out of range");
+  const int64_t ls = vocab_rows_of(op, "logits", logits, rows, vocab);
+  const auto vector = [&](const char* name, const at::Tensor& t, at::ScalarType type, int64_t entries) {
+    TORCH_CHECK(t.device() == logits.device() && t.scalar_type() == type && t.dim() == 1 && t.is_contiguous() &&
+                    t.numel() == entries,
+                op, ": ", name, " must be a contiguous ", type, " [", entries, "] tensor on the logits' device");
+  };
+  vector("draft_tokens", draft_tokens, at::kLong, rows);
+  vector("uniforms", uniforms, at::kFloat, rows);
+  vector("temperature", temperature, at::kFloat, n);
+  vector("cu_seqlens_q", cu_seqlens_q, at::kInt, n + 1);
+  vector("accepted", accepted, at::kInt, n);
+  if (d_error.has_value()) vector("d_error", *d_error, at::kInt, 1);
+  TORCH_CHECK(tokens.device() == logits.device() && tokens.scalar_type() == at::kLong && tokens.dim() == 2 &&
+                  tokens.size(0) == n && tokens.size(1) >= 1 && tokens.size(1) <= INT32_MAX && tokens.is_contiguous(),
+              op, ": tokens must be a contiguous int64 [", n, ", max_query_len] tensor on the logits' device");
+  int64_t ps = vocab;
+  if (draft_probs.has_value()) {
+    TORCH_CHECK(draft_probs->device() == logits.device() && draft_probs->scalar_type() == at::kFloat, op,
+                ": draft_probs must be a float32 tensor on the logits' device");
+    ps = vocab_rows_of(op, "draft_probs", *draft_probs, rows, vocab);
+  }
+  const size_t need = tq_verify_drafts_workspace_size((int32_t)n, (int32_t)rows, (int32_t)vocab);
+  at::Tensor workspace;
+  if (need > 0) workspace = at::empty({(int64_t)need}, logits.options().dtype(at::kByte));
+  check(tq_verify_drafts(tokens.data_ptr<int64_t>(), accepted.data_ptr<int32_t>(), logits.data_ptr(), ls,
+                         ptr<float>(draft_probs), ps, draft_tokens.data_ptr<int64_t>(), uniforms.data_ptr<float>(),
+                         temperature.data_ptr<float>(), cu_seqlens_q.data_ptr<int32_t>(), (int32_t)n, (int32_t)rows,
+                         (int32_t)tokens.size(1), (int32_t)vocab, dtype_of(logits.scalar_type()),
+                         need > 0 ? workspace.data_ptr() : nullptr, need, ptr<int32_t>(d_error), stream_of(logits)),
+        "tq_verify_drafts");
+}
+
 }  // namespace
 
 TORCH_LIBRARY(tokquay_amd, m) {
@@ -342,6 +520,14 @@ TORCH_LIBRARY(tokquay_amd, m) {
         "Tensor(c!)? d_error) -> ()");
   m.def("argmax_rows(Tensor logits, Tensor(a!) out) -> ()");
   m.def("linear(Tensor(a!) out, Tensor x, Tensor weight, Tensor? bias, bool gelu) -> ()");
+  m.def("rope_cache_write(Tensor(a!) q_out, Tensor q, Tensor k, Tensor v, Tensor(b!) pool, int layer, "
+        "Tensor slot_mapping, Tensor positions, Tensor table, bool interleaved, Tensor? q_norm, Tensor? k_norm, "
+        "float eps, Tensor(c!)? d_error) -> ()");
+  m.def("paged_chunk(Tensor(a!) out, Tensor q, Tensor pool, int layer, Tensor block_tables, Tensor cu_seqlens_q, "
+        "Tensor q_start, int max_query_len, int max_context_len, float scale, Tensor(b!)? workspace, "
+        "Tensor(c!)? d_error) -> ()");
+  m.def("verify_drafts(Tensor(a!) tokens, Tensor(b!) accepted, Tensor logits, Tensor? draft_probs, "
+        "Tensor draft_tokens, Tensor uniforms, Tensor temperature, Tensor cu_seqlens_q, Tensor(c!)? d_error) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(tokquay_amd, CUDA, m) {
@@ -353,4 +539,7 @@ TORCH_LIBRARY_IMPL(tokquay_amd, CUDA, m) {
   m.impl("paged_gather", &paged_gather);
   m.impl("argmax_rows", &argmax_rows);
   m.impl("linear", &linear);
+  m.impl("rope_cache_write", &rope_cache_write);
+  m.impl("paged_chunk", &paged_chunk);
+  m.impl("verify_drafts", &verify_drafts);
 }

@@ -495,6 +495,125 @@ def embed_rows(ids: torch.Tensor, positions: torch.Tensor, wte: torch.Tensor, wp
 
 
 
+# ------------------------------------------- 16-bit pools, grouped heads, chunks of new tokens, drafts
+@functools.lru_cache(maxsize=None)
+def _overload(name: str):
+    return getattr(torch_ops.load(), name).default
+
+
+def _checked_op(name: str, *args) -> None:
+    """``_op`` for operators whose arguments are checked by the operator alone: what it refuses is a ``ValueError``."""
+    try:
+        _overload(name)(*args)
+    except RuntimeError as e:
+        first = str(e).splitlines()[0] if str(e) else ""
+        if first.startswith(f"tokquay_amd::{name}: "):
+            raise ValueError(first.split("::", 1)[1]) from None
+        if " failed: " in first and first.startswith("tq_"):
+            raise _lib.KernelError(first) from None
+        raise
+
+
+def rope_table(num_positions: int, rotary_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """``rope_cache_write``'s table, float32 ``[num_positions, rotary_dim]``: the cosines, then the sines, of the angles
+    ``p base^(-2 i / rotary_dim)``, ``i < rotary_dim / 2``, computed in float64. Any other table of that
+    layout (scaled or stretched angles) does as well."""
+    if num_positions < 1 or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("a table needs positions and an even number of dims")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64, device=device)
+    angles = torch.arange(num_positions, dtype=torch.float64, device=device)[:, None] * base ** (-2.0 * i / rotary_dim)
+    return torch.cat([angles.cos(), angles.sin()], dim=1).float()
+
+
+def rope_cache_write(
+    q_out: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    pool: torch.Tensor,
+    layer: int,
+    slot_mapping: torch.Tensor,
+    positions: torch.Tensor,
+    table: torch.Tensor,
+    interleaved: bool = False,
+    q_norm: torch.Tensor | None = None,
+    k_norm: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    d_error: torch.Tensor | None = None,
+) -> None:
+    """``cache_write`` for models with position rotation, in one pass: each row's query heads normed (where
+    ``q_norm`` is given: RMS norm over the head's dims) and rotated into ``q_out`` (may be ``q`` itself), its key heads normed and
+    rotated into ``pool[:, layer]`` at ``slot_mapping``, its value heads copied there. Padded rows (slot -1)
+    write their queries only. float32, float16 or bfloat16 rows and pool, heads of 64 or 128 dims, any number of
+    query heads; ``positions`` int64 ``[N]`` index ``table`` (``rope_table``), whose width is the rotated part of each
+    head (a multiple of 16); pairs are half the width apart, or neighbours where ``interleaved``."""
+    _checked_op("rope_cache_write", q_out, q, k, v, pool, layer, slot_mapping, positions, table, interleaved, q_norm,
+                k_norm, eps, d_error)  # fmt: skip
+
+
+def chunk_workspace_bytes(num_seqs: int, n_head: int, n_kv_head: int, d_head: int, num_q_rows: int,
+                          max_query_len: int, max_context_len: int) -> int:  # fmt: skip
+    return int(_lib.lib().tq_paged_chunk_workspace_size(num_seqs, n_head, n_kv_head, d_head, num_q_rows, max_query_len,
+                                                        max_context_len))  # fmt: skip
+
+
+def paged_chunk(
+    out: torch.Tensor,
+    q: torch.Tensor,
+    pool: torch.Tensor,
+    layer: int,
+    block_tables: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    q_start: torch.Tensor,
+    max_query_len: int,
+    max_context_len: int,
+    scale: float | None = None,
+    workspace: torch.Tensor | None = None,
+    d_error: torch.Tensor | None = None,
+) -> None:
+    """Causal attention of each sequence's new rows over its keys ``0 .. q_start[b] + n_b - 1`` in a float16 or bfloat16 pool,
+    whose K/V heads each serve ``n_head / n_kv_head`` neighbouring query heads: ``paged_prefill`` and ``paged_decode`` (rows of one
+    token) for such pools, heads of 64 or 128 dims. The rows' own K/V must be in the pool already
+    (``rope_cache_write``). ``max_query_len`` and ``max_context_len`` (the longest ``q_start[b] + n_b``) size the launch; in a captured graph,
+    which replays with other lengths, give the largest. Rows of no sequence are left alone."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(pool.size(-1))
+    _checked_op("paged_chunk", out, q, pool, layer, block_tables, cu_seqlens_q, q_start, max_query_len, max_context_len,
+                scale, workspace, d_error)  # fmt: skip
+
+
+def verify_drafts(
+    logits: torch.Tensor,
+    draft_tokens: torch.Tensor,
+    uniforms: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    max_query_len: int,
+    temperature: torch.Tensor,
+    draft_probs: torch.Tensor | None = None,
+    d_error: torch.Tensor | None = None,
+    tokens: torch.Tensor | None = None,
+    accepted: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Speculative sampling's accept / resample rule over a batch, from given random numbers: ``(tokens, accepted)``, int64
+    ``[B, max_query_len]`` (each sequence's accepted drafts and the token drawn after them, then -1) and int32 ``[B]``.
+
+    ``cu_seqlens_q`` is ``paged_chunk``'s: sequence b has ``n_b - 1`` drafts, judged by its rows of ``logits`` (``[N, vocab]``, float32,
+    float16 or bfloat16) in order, and a last row behind them. ``draft_tokens`` (int64) and ``uniforms`` (float32 in [0, 1)) have
+    an entry per row: the draft that the row judges (unused in a last row), and the random number that decides on it
+    (in a last row: that the next token is drawn with). ``temperature`` float32 ``[B]``: 0 is greedy. ``draft_probs``
+    (float32 ``[N, vocab]``): what each draft was drawn from; without it drafts are taken as certain (prompt lookup, a greedy draft
+    model). Mask tokens with -inf logits."""
+    if tokens is None:
+        tokens = torch.empty(temperature.numel(), max_query_len, dtype=torch.int64, device=logits.device)
+    elif tokens.dim() != 2 or tokens.size(1) != max_query_len:
+        raise ValueError(f"tokens must be [{temperature.numel()}, {max_query_len}]")
+    if accepted is None:
+        accepted = torch.empty(temperature.numel(), dtype=torch.int32, device=logits.device)
+    _checked_op("verify_drafts", tokens, accepted, logits, draft_probs, draft_tokens, uniforms, temperature, cu_seqlens_q,
+                d_error)  # fmt: skip
+    return tokens, accepted
+
+
 # ------------------------------------------------------------------------------ library GEMMs
 # hipBLASLt's default fp32 kernel for a given shape depends on the operand layout. Measured on the
 # device (a spin kernel holding the stream while ten calls per layout queue behind it, best of three

@@ -1,6 +1,6 @@
 """``torch.ops.tokquay_amd.*``: the paged-attention entry points as torch operators.
 
-``csrc/torch_ops.cpp`` (built into ``_torch_ops.so`` next to ``libtokquay_amd.so``) registers eight
+``csrc/torch_ops.cpp`` (built into ``_torch_ops.so`` next to ``libtokquay_amd.so``) registers
 out-variant operators with torch's dispatcher; each is a thin call into the C ABI on the current
 HIP stream. This module loads that library and registers the operators' fake (shape-only)
 implementations, so programs that record torch calls (``make_fx``, FX graphs on fake tensors)
@@ -21,6 +21,12 @@ or entries, overlapping rows:
   gathered copy)
 * ``argmax_rows(logits, out!)``
 * ``linear(out!, x, weight, bias?, gelu)``
+* ``rope_cache_write(q_out!, q, k, v, pool!, layer, slot_mapping, positions, table, interleaved, q_norm?,
+  k_norm?, eps, d_error!?)``
+* ``paged_chunk(out!, q, pool, layer, block_tables, cu_seqlens_q, q_start, max_query_len, max_context_len,
+  scale, workspace!?, d_error!?)``
+* ``verify_drafts(tokens!, accepted!, logits, draft_probs?, draft_tokens, uniforms, temperature,
+  cu_seqlens_q, d_error!?)``
 
 (``!``: written in place.) ``tokquay_amd.ops`` checks the tensors with the reference's messages
 and calls these operators; there is no fallback when the library is missing.
@@ -35,7 +41,7 @@ import torch
 from tokquay_amd.build import TORCH_OPS_PATH
 
 OPS = ("cache_write", "paged_decode", "paged_decode_write", "paged_prefill", "paged_mixed", "paged_gather",
-       "argmax_rows", "linear")
+       "argmax_rows", "linear", "rope_cache_write", "paged_chunk", "verify_drafts")
 
 _loaded = False
 
@@ -235,6 +241,137 @@ def _fake_linear(out, x, weight, bias, gelu):
         _fail(op, "out must be a float32 [rows, N] tensor on x's device with contiguous rows")
     if rows > 1 and out.stride(0) < n:
         _fail(op, "out's rows overlap")
+
+
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _typed_pool_of(op, pool, layer, float32):
+    ok = pool.dtype in (_TYPES if float32 else _TYPES[1:])
+    if not (pool.dim() == 6 and pool.size(2) == 2 and ok and pool.is_contiguous() and pool.is_cuda):
+        _fail(op, f"pool must be a contiguous {'float32, float16 or bfloat16' if float32 else 'float16 or bfloat16'} "
+                  "[num_blocks, n_layer, 2, n_kv_head, block_size, d_head] tensor on a HIP device")  # fmt: skip
+    if pool.size(5) not in (64, 128):
+        _fail(op, f"only d_head 64 and 128 are supported, got {pool.size(5)}")
+    if not 0 <= layer < pool.size(1):
+        _fail(op, f"layer {layer} out of range [0, {pool.size(1)})")
+    if not (pool.size(0) >= 1 and 1 <= pool.size(3) <= 65535 and 1 <= pool.size(4) <= 1024):
+        _fail(op, "pool must hold blocks and heads, in blocks of at most 1024 slots")
+
+
+def _typed_rows_of(op, name, t, rows, heads, pool, align):
+    _on_device(op, name, t, pool)
+    if t.dtype != pool.dtype:
+        _fail(op, f"{name} must be of the pool's type {pool.dtype}, got {t.dtype}")
+    d = pool.size(5)
+    if t.dim() == 3:
+        ok = t.size(2) == d and t.stride(2) == 1 and (t.size(1) <= 1 or t.stride(1) == d)
+    else:
+        ok = t.dim() == 2 and t.size(1) % d == 0 and (t.size(1) <= 1 or t.stride(1) == 1)
+    if ok:
+        has = t.size(1) if t.dim() == 3 else t.size(1) // d
+        ok = 1 <= has <= 65535 and heads in (0, has)
+        heads = has if ok else heads
+    if not ok:
+        of = f" of {heads} heads" if heads else ""
+        _fail(op, f"{name} must be [N, heads, {d}] or [N, heads * {d}] with contiguous rows{of}")
+    if t.size(0) < rows:
+        _fail(op, f"{name} has {t.size(0)} rows, needs {rows}")
+    stride = t.stride(0) if t.size(0) > 1 else heads * d
+    if rows > 1 and stride < heads * d:
+        _fail(op, f"{name}'s rows overlap (row stride {stride})")
+    # (A fake tensor has no address: its offset stands for it.)
+    if t.storage_offset() * t.element_size() % align or (rows > 1 and stride * t.element_size() % align):
+        _fail(op, f"{name}'s rows must be {align}-byte aligned")
+    return heads
+
+
+def _norm_of(op, name, t, pool):
+    if t is None:
+        return
+    _on_device(op, name, t, pool)
+    if not (t.dtype == pool.dtype and t.shape == (pool.size(5),) and t.is_contiguous()
+            and t.storage_offset() * t.element_size() % 16 == 0):  # fmt: skip
+        _fail(op, f"{name} must be a contiguous, 16-byte aligned [{pool.size(5)}] tensor of the pool's type")
+
+
+def _fake_rope_cache_write(q_out, q, k, v, pool, layer, slot_mapping, positions, table, interleaved, q_norm, k_norm,
+                           eps, d_error):  # fmt: skip
+    op = "rope_cache_write"
+    _typed_pool_of(op, pool, layer, True)
+    _vector_of(op, "slot_mapping", slot_mapping, torch.int64, 0, pool)
+    n = slot_mapping.numel()
+    _vector_of(op, "positions", positions, torch.int64, n, pool)
+    heads = _typed_rows_of(op, "q", q, n, 0, pool, 16)
+    _typed_rows_of(op, "q_out", q_out, n, heads, pool, 16)
+    _typed_rows_of(op, "k", k, n, pool.size(3), pool, 16)
+    _typed_rows_of(op, "v", v, n, pool.size(3), pool, 16)
+    _on_device(op, "table", table, pool)
+    if not (table.dtype == torch.float32 and table.dim() == 2 and table.is_contiguous()
+            and table.storage_offset() % 4 == 0 and 16 <= table.size(1) <= pool.size(5)
+            and table.size(1) % 16 == 0):  # fmt: skip
+        _fail(op, "table must be a contiguous float32 [positions, rotary] tensor, rotary a multiple of 16 up to "
+                  f"{pool.size(5)}")  # fmt: skip
+    _norm_of(op, "q_norm", q_norm, pool)
+    _norm_of(op, "k_norm", k_norm, pool)
+    _error_word(op, d_error, pool)
+
+
+def _fake_paged_chunk(out, q, pool, layer, block_tables, cu_seqlens_q, q_start, max_query_len, max_context_len, scale,
+                      workspace, d_error):  # fmt: skip
+    op = "paged_chunk"
+    _typed_pool_of(op, pool, layer, False)
+    _vector_of(op, "q_start", q_start, torch.int32, 0, pool)
+    n = q_start.numel()
+    _vector_of(op, "cu_seqlens_q", cu_seqlens_q, torch.int32, n + 1, pool)
+    if cu_seqlens_q.numel() != n + 1:
+        _fail(op, "cu_seqlens_q must have num_seqs + 1 entries")
+    heads = _typed_rows_of(op, "q", q, q.size(0) if q.dim() else 0, 0, pool, 16)
+    _typed_rows_of(op, "out", out, q.size(0), heads, pool, 8)
+    if heads % pool.size(3):
+        _fail(op, f"{heads} query heads are no multiple of the pool's {pool.size(3)}")
+    _tables_of(op, "block_tables", block_tables, n, pool)
+    if not (0 <= max_query_len < 2**31 and 0 <= max_context_len < 2**31):
+        _fail(op, "max_query_len and max_context_len must be lengths")
+    _error_word(op, d_error, pool)
+    _workspace(op, workspace, pool)
+
+
+def _fake_verify_drafts(tokens, accepted, logits, draft_probs, draft_tokens, uniforms, temperature, cu_seqlens_q,
+                        d_error):  # fmt: skip
+    op = "verify_drafts"
+    if not (logits.is_cuda and logits.dim() == 2 and logits.dtype in _TYPES):
+        _fail(op, "logits must be a float32, float16 or bfloat16 [rows, vocab] tensor on a HIP device")
+    rows, vocab = logits.shape
+    n = temperature.numel()
+    if not 1 <= vocab <= 1 << 30:
+        _fail(op, "sizes out of range")
+
+    def vocab_rows(name, t):
+        if not (t.dim() == 2 and tuple(t.shape) == (rows, vocab) and (vocab <= 1 or t.stride(1) == 1)):
+            _fail(op, f"{name} must be [{rows}, {vocab}] with contiguous rows")
+        if rows > 1 and t.stride(0) < vocab:
+            _fail(op, f"{name}'s rows overlap")
+
+    def vector(name, t, dtype, entries):
+        if not (t.device == logits.device and t.dtype == dtype and t.shape == (entries,) and t.is_contiguous()):
+            _fail(op, f"{name} must be a contiguous {dtype} [{entries}] tensor on the logits' device")
+
+    vocab_rows("logits", logits)
+    vector("draft_tokens", draft_tokens, torch.int64, rows)
+    vector("uniforms", uniforms, torch.float32, rows)
+    vector("temperature", temperature, torch.float32, n)
+    vector("cu_seqlens_q", cu_seqlens_q, torch.int32, n + 1)
+    vector("accepted", accepted, torch.int32, n)
+    if d_error is not None:
+        vector("d_error", d_error, torch.int32, 1)
+    if not (tokens.device == logits.device and tokens.dtype == torch.int64 and tokens.dim() == 2
+            and tokens.size(0) == n and tokens.size(1) >= 1 and tokens.is_contiguous()):  # fmt: skip
+        _fail(op, f"tokens must be a contiguous int64 [{n}, max_query_len] tensor on the logits' device")
+    if draft_probs is not None:
+        if draft_probs.device != logits.device or draft_probs.dtype != torch.float32:
+            _fail(op, "draft_probs must be a float32 tensor on the logits' device")
+        vocab_rows("draft_probs", draft_probs)
 
 
 FAKES = {name: globals()[f"_fake_{name}"] for name in OPS}
