@@ -97,47 +97,103 @@ __device__ __forceinline__ int swizzle(int key) {
   return D == 128 ? key & 15 : (key >> 1) & 7;
 }
 
-// Starts the copy of keys kt .. kt + 31 of one K/V head into LDS (K, then V), by one wave. Keys from kend on
-// are the last one again: finite wherever it is, and masked.
-template <int D>
-__device__ __forceinline__ void load_tile(const ChunkArgs& a, const int32_t* bt, const uint16_t* head_base, int kt,
-                                          int kend, uint16_t* s_k, uint16_t* s_v) {
-  constexpr int kLanes = D / 8;             // lanes a key row takes, 16 bytes each
-  constexpr int kKeys = kWave / kLanes;     // keys of one instruction
-  const int lane = threadIdx.x & (kWave - 1);
+// Zeros in place of the infinities and NaN among a wave's `pieces` 16-byte pieces of V in LDS; whether there were any (uniform).
+// For tiles with keys that some row does not see: a weight of zero times infinity is NaN. The rows that do see them get them
+// back at the end (add_left_out).
+template <typename T>
+__device__ __forceinline__ bool clean_values(uint16_t* s_v, int pieces) {
+  bool any = false;
+#pragma unroll 1
+  for (int j = threadIdx.x & (kWave - 1); j < pieces; j += kWave) {
+    u32x4 v = reinterpret_cast<const u32x4*>(s_v)[j];
+    bool bad = false;
 #pragma unroll
-  for (int j = 0; j < kTileKeys / kKeys; ++j) {
-    const int local = j * kKeys + lane / kLanes;
-    const int key = min(kt + local, kend - 1);
-    const int ti = key / a.block_size;
-    int32_t blk = bt[ti];
-    if ((uint32_t)blk >= (uint32_t)a.num_blocks) {
-      flag_error(a.d_error, TQ_DEVERR_BLOCK_ID);
-      blk = 0;
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = v[e];
+      const bool lo = (x & T::kExponent) == T::kExponent, hi = ((x >> 16) & T::kExponent) == T::kExponent;
+      v[e] = (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
+      bad |= lo || hi;
     }
-    const uint16_t* src = head_base + (int64_t)blk * a.block_stride + (int64_t)(key - ti * a.block_size) * D +
-                          8 * ((lane % kLanes) ^ swizzle<D>(local));
-    typedef const __attribute__((address_space(1))) void* Global;
-    typedef __attribute__((address_space(3))) void* Lds;
-    __builtin_amdgcn_global_load_lds((Global)src, (Lds)(s_k + j * kKeys * D), 16, 0, 0);
-    __builtin_amdgcn_global_load_lds((Global)(src + a.kv_stride), (Lds)(s_v + j * kKeys * D), 16, 0, 0);
+    if (bad) reinterpret_cast<u32x4*>(s_v)[j] = v;
+    any |= bad;
+  }
+  return __builtin_amdgcn_ballot_w64(any) != 0;
+}
+
+// Values of four dims of a row that the products left out, added to `o`: those of keys from..to - 1 (to: past the row's last
+// key) that are infinities or NaN. head_base is at the first of the dims in the K slab.
+template <typename T>
+__device__ __forceinline__ void add_left_out(const ChunkArgs& a, const int32_t* bt, const uint16_t* head_base, int D,
+                                             int from, int to, f32x4& o) {
+#pragma unroll 1
+  for (int key = from; key < to; ++key) {
+    const int ti = key / a.block_size;
+    const int32_t blk = bt[ti];
+    if ((uint32_t)blk >= (uint32_t)a.num_blocks) continue;  // flagged by the loads
+    const u32x2 v = *reinterpret_cast<const u32x2*>(head_base + (int64_t)blk * a.block_stride + a.kv_stride +
+                                                    (int64_t)(key - ti * a.block_size) * D);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = (v[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+      if ((x & T::kExponent) == T::kExponent) o[e] += T::load((uint16_t)x);
+    }
   }
 }
 
-// s_waitcnt vmcnt(0) lgkmcnt(0): the tile that was loaded is in LDS, and what was read of the other one is in registers.
-__device__ __forceinline__ void wait_tile() {
-  __builtin_amdgcn_s_waitcnt(0x0070);
-  __builtin_amdgcn_sched_barrier(0);
+// The block id of key kt + lane % KEYS of a sequence (keys from kend on: the last one's).
+template <int KEYS>
+__device__ __forceinline__ int32_t block_ids(const ChunkArgs& a, const int32_t* bt, int kt, int kend) {
+  const int key = min(kt + (int)(threadIdx.x & (KEYS - 1)), kend - 1);
+  return bt[key / a.block_size];
 }
 
-// The rows of one wave: queries, sums, running maxima.
-template <int D, int NT, typename T>
+// Starts the copy of keys kt + FIRST .. of one K/V head into LDS by one wave, J instructions of 1024 bytes. Keys
+// from kend on are the last one again: finite wherever it is, and masked. `ids` is block_ids(kt); bad ones are flagged
+// and block 0 is read in their place.
+template <int D, int J>
+struct Loader {
+  static constexpr int kLanes = D / 8;          // lanes a key row takes, 16 bytes each
+  static constexpr int kKeys = kWave / kLanes;  // keys of one instruction
+  const uint16_t* src[J];                       // K; V is kv_stride on
+
+  __device__ __forceinline__ void aim(const ChunkArgs& a, const uint16_t* head_base, int32_t ids, int kt, int first,
+                                      int kend) {
+    const int lane = threadIdx.x & (kWave - 1);
+    if ((uint32_t)ids >= (uint32_t)a.num_blocks) {
+      flag_error(a.d_error, TQ_DEVERR_BLOCK_ID);
+      ids = 0;
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int local = first + j * kKeys + lane / kLanes;
+      const int key = min(kt + local, kend - 1);
+      const int32_t blk = __shfl(ids, local);
+      src[j] = head_base + (int64_t)blk * a.block_stride + (int64_t)(key % a.block_size) * D +
+               8 * ((lane % kLanes) ^ swizzle<D>(local));
+    }
+  }
+
+  // `to`: the tile's row `first` in LDS.
+  __device__ __forceinline__ void start(uint16_t* to, int64_t offset) const {
+    typedef const __attribute__((address_space(1))) void* Global;
+    typedef __attribute__((address_space(3))) void* Lds;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      __builtin_amdgcn_global_load_lds((Global)(src[j] + offset), (Lds)(to + j * kKeys * D), 16, 0, 0);
+  }
+};
+
+// The rows of one wave: queries, sums, running maxima. KS: 32-key steps of a tile.
+template <int D, int NT, int KS, typename T>
 struct Rows {
   u32x4 q[NT][D / 32];
   f32x4 o[NT][D / 16];
   float m[NT], mthr[NT], l[NT];
   int qpos[NT];
   int lo, hi;  // positions of the first and last row (uniform)
+
+  typedef f32x4 Scores[2 * KS][NT];  // of keys 16 h + 4 g + 0..3 with row i of row tile n
+  typedef u32x4 Weights[KS][NT];     // rounded: of keys 32 k + 4 g + 0..3 and 32 k + 16 + 4 g + 0..3
 
   __device__ __forceinline__ void init(const ChunkArgs& a, const Seq& s, int kvh, int r0) {
     const int lane = threadIdx.x & (kWave - 1), i = lane & 15, g = lane >> 4;
@@ -147,8 +203,7 @@ struct Rows {
       const int r = min(r0 + kTileRows * n + i, last), t = r / a.group;
       const uint16_t* qp = a.q + (int64_t)(s.row0 + t) * a.q_stride + (kvh * a.group + r - t * a.group) * D + 8 * g;
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k)
-        q[n][k] = *reinterpret_cast<const u32x4*>(qp + 32 * k) ^ a.q_sign;
+      for (int k = 0; k < D / 32; ++k) q[n][k] = *reinterpret_cast<const u32x4*>(qp + 32 * k);
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
       qpos[n] = s.start + t;
@@ -156,42 +211,78 @@ struct Rows {
       mthr[n] = -FLT_MAX;
       l[n] = 0.f;
     }
-    lo = s.start + min(r0, last) / a.group;
-    hi = s.start + min(r0 + kTileRows * NT - 1, last) / a.group;
+    lo = __builtin_amdgcn_readfirstlane(s.start + min(r0, last) / a.group);
+    hi = __builtin_amdgcn_readfirstlane(s.start + min(r0 + kTileRows * NT - 1, last) / a.group);
   }
 
-  // One tile of keys kt .. kt + 31, of which those from kend on are not there.
-  __device__ __forceinline__ void tile(const ChunkArgs& a, int kt, const uint16_t* s_k, const uint16_t* s_v) {
+  __device__ __forceinline__ void flip(uint32_t sign) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) q[n][k] ^= sign;
+  }
+
+  // K of keys 16 h + 0..15 as the first operand of D / 32 products.
+  static __device__ __forceinline__ void read_k(const uint16_t* s_k, int h, u32x4 (&kf)[D / 32]) {
     const int lane = threadIdx.x & (kWave - 1), i = lane & 15, g = lane >> 4;
-    f32x4 s[2][NT];
+    const int key = 16 * h + i;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int k = 0; k < D / 32; ++k)
+      kf[k] = *reinterpret_cast<const u32x4*>(s_k + key * D + 8 * ((4 * k + g) ^ swizzle<D>(key)));
+  }
+
+  // The same beside loads into LDS (values_beside_loads).
+  static __device__ __forceinline__ void read_k_beside_loads(const uint16_t* s_k, int h, u32x4 (&kf)[D / 32]) {
+    const int lane = threadIdx.x & (kWave - 1), i = lane & 15, g = lane >> 4;
+    const int key = 16 * h + i;
+    typedef __attribute__((address_space(3))) const u32x4* Lds;
+    Lds at[D / 32];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[h][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < D / 32; ++k) at[k] = (Lds)(s_k + key * D + 8 * ((4 * k + g) ^ swizzle<D>(key)));
+    if constexpr (D == 128)
+      asm volatile(
+          "ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\tds_read_b128 %3, %7\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(kf[0]), "=&v"(kf[1]), "=&v"(kf[2]), "=&v"(kf[3])
+          : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+          : "memory");
+    else
+      asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(kf[0]), "=&v"(kf[1])
+                   : "v"(at[0]), "v"(at[1])
+                   : "memory");
+  }
+
+  __device__ __forceinline__ void scores(const u32x4 (&kf)[D / 32], f32x4 (&s)[NT]) const {
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        const int key = 16 * h + i;
-        const u32x4 kf = *reinterpret_cast<const u32x4*>(s_k + key * D + 8 * ((4 * k + g) ^ swizzle<D>(key)));
+    for (int n = 0; n < NT; ++n) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[h][n] = T::mfma(kf, q[n][k], s[h][n]);
-      }
-    }
-    const bool masked = kt + kTileKeys - 1 > lo;  // uniform: some row does not see some key
-    if (masked) {
+    for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n] = T::mfma(kf[k], q[n][k], s[n]);
+  }
+
+  // Whether some row does not see some key of the tile (uniform).
+  __device__ __forceinline__ bool masked(int kt) const { return kt + 32 * KS - 1 > lo; }
+
+  // Masks the scores of the tile of keys kt .. and raises the running maxima where they are passed.
+  __device__ __forceinline__ void maxima(const ChunkArgs& a, int kt, Scores& s) {
+    const int g = (threadIdx.x & (kWave - 1)) >> 4;
+    if (masked(kt)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2 * KS; ++h)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             s[h][n][e] = kt + 16 * h + 4 * g + e <= qpos[n] ? s[h][n][e] : -INFINITY;
     }
-    float p[NT][8];
-    u32x4 pf[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float top = max2(max2(max2(s[0][n][0], s[0][n][1]), max2(s[0][n][2], s[0][n][3])),
-                       max2(max2(s[1][n][0], s[1][n][1]), max2(s[1][n][2], s[1][n][3])));
+      float top = max2(max2(s[0][n][0], s[0][n][1]), max2(s[0][n][2], s[0][n][3]));
+#pragma unroll
+      for (int h = 1; h < 2 * KS; ++h)
+        top = max2(max2(max2(top, s[h][n][0]), s[h][n][1]), max2(s[h][n][2], s[h][n][3]));
       top *= a.c;
       if (__builtin_amdgcn_ballot_w64(top > mthr[n]) != 0) {
         top = max2(top, __shfl_xor(top, 16));
@@ -205,93 +296,126 @@ struct Rows {
         m[n] = next;
         mthr[n] = next + kSlack;
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) p[n][e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][n][e & 3], a.c, -m[n]));
-      l[n] += ((p[n][0] + p[n][1]) + (p[n][2] + p[n][3])) + ((p[n][4] + p[n][5]) + (p[n][6] + p[n][7]));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pf[n][e] = pack2<T>(p[n][2 * e], p[n][2 * e + 1]);
     }
-    if (masked && not_finite(s_v)) {
-      visible_values(kt, s_v, p);
-      return;
+  }
+
+  // The weights of keys 16 h + 0..15, added to the rows' sums.
+  __device__ __forceinline__ void weights(const ChunkArgs& a, int h, const f32x4 (&s)[NT], Weights& w) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], a.c, -m[n]));
+      l[n] += (p[0] + p[1]) + (p[2] + p[3]);
+      w[h / 2][n][2 * (h % 2)] = pack2<T>(p[0], p[1]);
+      w[h / 2][n][2 * (h % 2) + 1] = pack2<T>(p[2], p[3]);
     }
+  }
+
+  __device__ __forceinline__ void values(const uint16_t* s_v, const Weights& w) {
+    u32x4 vf[2];
+    vf[0] = read_v(s_v, 0);
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) {
-      const u32x4 vf = read_v(s_v, d);
+    for (int j = 0; j < KS * D / 16; ++j) {
+      const int k = j / (D / 16), d = j % (D / 16), jn = j + 1;
+      if (jn < KS * D / 16) vf[jn & 1] = read_v(s_v + 32 * (jn / (D / 16)) * D, jn % (D / 16));
 #pragma unroll
-      for (int n = 0; n < NT; ++n) o[n][d] = T::mfma(vf, pf[n], o[n][d]);
+      for (int n = 0; n < NT; ++n) o[n][d] = T::mfma(vf[j & 1], w[k][n], o[n][d]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // The same for callers with loads into LDS on their way, for all of which the compiler waits before the builtin's reads (it
+  // cannot tell them apart): the reads and the wait for them in one block, four dim tiles at a time.
+  __device__ __forceinline__ void values_beside_loads(const uint16_t* s_v, const Weights& w) {
+#pragma unroll
+    for (int j = 0; j < KS * D / 64; ++j) {
+      const int k = j / (D / 64), d = j % (D / 64) * 4;
+      const uint16_t* base = s_v + 32 * k * D;
+      u32x2 lo[4], hi[4];
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %4, %8 offset:%12\n\t"
+          "ds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %5, %9 offset:%12\n\t"
+          "ds_read_b64_tr_b16 %2, %10\n\tds_read_b64_tr_b16 %6, %10 offset:%12\n\t"
+          "ds_read_b64_tr_b16 %3, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3])
+          : "v"(v_address(base, d)), "v"(v_address(base, d + 1)), "v"(v_address(base, d + 2)),
+            "v"(v_address(base, d + 3)), "n"(16 * D * 2)
+          : "memory");
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          o[n][d + e] = T::mfma(u32x4{lo[e][0], lo[e][1], hi[e][0], hi[e][1]}, w[k][n], o[n][d + e]);
     }
   }
 
   // V^T of dims 16 d + 0..15: dim 16 d + i, keys 4 g + 0..3 and 16 + 4 g + 0..3. Of 16 lanes, lane 4 a + b names
   // four values of key a and gets value (its own index) of keys 0..3.
   static __device__ __forceinline__ u32x4 read_v(const uint16_t* s_v, int d) {
-    const int lane = threadIdx.x & (kWave - 1), i = lane & 15, g = lane >> 4;
     u32x2 half[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int key = 16 * h + 4 * g + (i >> 2), piece = 2 * d + ((i >> 1) & 1);
-      const uint16_t* at = s_v + key * D + 8 * (piece ^ swizzle<D>(key)) + 4 * (i & 1);
-      half[h] = __builtin_bit_cast(
-          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at)));
-    }
+    for (int h = 0; h < 2; ++h)  // 16 keys on, the swizzle is the same
+      half[h] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(v_address(s_v, d) + 4 * h * D));
     return u32x4{half[0][0], half[0][1], half[1][0], half[1][1]};
   }
 
-  // Whether the tile's V holds an infinity or a NaN (uniform).
-  static __device__ __forceinline__ bool not_finite(const uint16_t* s_v) {
-    const int lane = threadIdx.x & (kWave - 1);
-    bool bad = false;
-#pragma unroll 1
-    for (int j = lane; j < kTileKeys * D / 8; j += kWave) {
-      const u32x4 v = reinterpret_cast<const u32x4*>(s_v)[j];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        bad |= (v[e] & T::kExponent) == T::kExponent || ((v[e] >> 16) & T::kExponent) == T::kExponent;
-    }
-    return __builtin_amdgcn_ballot_w64(bad) != 0;
+  typedef __attribute__((address_space(3))) s16x4* Lds;
+  static __device__ __forceinline__ Lds v_address(const uint16_t* s_v, int d) {
+    const int lane = threadIdx.x & (kWave - 1), i = lane & 15, g = lane >> 4;
+    const int key = 4 * g + (i >> 2), piece = 2 * d + ((i >> 1) & 1);
+    return (Lds)(s_v + key * D + 8 * (piece ^ swizzle<D>(key)) + 4 * (i & 1));
   }
 
-  // The second product of a tile whose V is not finite and that some row does not see all of: a weight of
-  // zero times infinity is NaN, so each key's values reach only the rows that see it.
-  __device__ __forceinline__ void visible_values(int kt, const uint16_t* s_v, const float (&p)[NT][8]) {
-    const int lane = threadIdx.x & (kWave - 1), i = lane & 15, g = lane >> 4;
-#pragma unroll 1
-    for (int key = 0; key < kTileKeys; ++key) {
-      const int from = 16 * ((key >> 2) & 3) + i, slot = 4 * (key >> 4) + (key & 3);
-      float w[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        w[n] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[n] = e == slot ? p[n][e] : w[n];
-        w[n] = __shfl(w[n], from);
-      }
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        const int dim = 16 * d + 4 * g;
-        const u32x2 v = *reinterpret_cast<const u32x2*>(s_v + key * D + 8 * ((dim >> 3) ^ swizzle<D>(key)) + (dim & 7));
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float f = T::load((uint16_t)(v[r >> 1] >> (16 * (r & 1))));
-#pragma unroll
-          for (int n = 0; n < NT; ++n) o[n][d][r] = kt + key <= qpos[n] ? fmaf(w[n], f, o[n][d][r]) : o[n][d][r];
-        }
-      }
-    }
+  // The four lanes of a row have its maximum; each has the weights of its own keys.
+  __device__ __forceinline__ float weight_sum(int n) const {
+    float sum = l[n];
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    return sum;
   }
 };
 
+// Waits until at most N loads are on their way (they end in order); the compiler does not know which loads into LDS a read
+// of LDS needs.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "vmcnt has six bits");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
+// Waits until what was read of LDS is in registers: its place is free for other loads.
+__device__ __forceinline__ void wait_reads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The workgroup's waves meet, with their LDS accesses done; loads may be on their way.
+__device__ __forceinline__ void barrier() {
+  wait_reads();
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
 // Few rows: a workgroup takes 16 NT rows and one part of the keys; its waves take every fourth tile of the
-// part, each with its own two tile buffers in LDS and no barrier, and join their sums in LDS at the end.
+// part, each with its own two K and two V buffers in LDS and no barrier, and join their sums in LDS at the end.
+//
+// K and V of the next tile and V of this one are on their way while a tile's scores are computed: 24 KB a wave,
+// 96 KB a CU (D = 128), which covers the latency of HBM at its full rate.
 template <int D, int NT, typename T>
 __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkArgs a) {
   constexpr int kTileElems = kTileKeys * D;
-  // Two buffers of K and V for each wave; at the end the waves' sums (D + 4 floats a row keep rows apart).
-  constexpr int kSumFloats = kWaves * kTileRows * NT * (D + 4);
-  constexpr int kBytes = kWaves * 4 * kTileElems * 2 > kSumFloats * 4 ? kWaves * 4 * kTileElems * 2 : kSumFloats * 4;
-  __shared__ __attribute__((aligned(16))) char s_mem[kBytes];
+  __shared__ __attribute__((aligned(16))) uint16_t s_k0[kWaves * kTileElems], s_v0[kWaves * kTileElems],
+      s_k1[kWaves * kTileElems], s_v1[kWaves * kTileElems];
   __shared__ float s_ml[kWaves][kTileRows * NT][2];
+  __shared__ int s_dirty[kWaves];
   const int lane = threadIdx.x & (kWave - 1), i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   int idx = blockIdx.x;
@@ -304,36 +428,75 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
   if (!seq_of(a, b, part == 0 && tile == 0 && kvh == 0, s)) return;
   const int r0 = tile * kTileRows * NT, rows = min(kTileRows * NT, s.nq * a.group - r0);
   if (rows <= 0) return;
-  Rows<D, NT, T> w;
-  w.init(a, s, kvh, r0);
-  const int kend = w.hi + 1, kbeg = part * a.part_tokens;
+  const int last = (s.start + min(r0 + kTileRows * NT - 1, s.nq * a.group - 1) / a.group);
+  const int kend = last + 1, kbeg = part * a.part_tokens;
   if (kbeg >= kend) return;
   const int kstop = min(kend, kbeg + a.part_tokens);
 
   const int32_t* bt = a.block_tables + (int64_t)b * a.bt_stride;
   const uint16_t* head_base = a.pool_layer + (int64_t)kvh * a.head_stride;
-  uint16_t* s_tile = reinterpret_cast<uint16_t*>(s_mem) + wave * 4 * kTileElems;
   constexpr int kStep = kWaves * kTileKeys;
-  int kt = kbeg + wave * kTileKeys, buf = 0;
-  if (kt < kstop) load_tile<D>(a, bt, head_base, kt, kend, s_tile, s_tile + kTileElems);
-  for (; kt < kstop; kt += kStep) {
-    wait_tile();
-    const int nbuf = buf ^ 1;
-    if (kt + kStep < kstop)
-      load_tile<D>(a, bt, head_base, kt + kStep, kend, s_tile + nbuf * 2 * kTileElems,
-                   s_tile + nbuf * 2 * kTileElems + kTileElems);
-    w.tile(a, kt, s_tile + buf * 2 * kTileElems, s_tile + buf * 2 * kTileElems + kTileElems);
-    buf = nbuf;
+  constexpr int J = kTileElems * 2 / 1024;
+  typedef Rows<D, NT, 1, T> R;
+  R w;
+  Loader<D, J> load;
+  uint16_t *k0 = s_k0 + wave * kTileElems, *v0 = s_v0 + wave * kTileElems, *k1 = s_k1 + wave * kTileElems,
+           *v1 = s_v1 + wave * kTileElems;
+  int kt = kbeg + wave * kTileKeys;
+  // Tiles past the part's end are loaded too (their keys clamped into the sequence), so that the count of loads behind the
+  // one that is waited for stays the same: K and V of two tiles are always on their way, of which a wait takes the first.
+  int32_t id0 = block_ids<kTileKeys>(a, bt, kt, kend), id1 = block_ids<kTileKeys>(a, bt, kt + kStep, kend);
+  int32_t id2 = block_ids<kTileKeys>(a, bt, kt + 2 * kStep, kend), id3 = block_ids<kTileKeys>(a, bt, kt + 3 * kStep, kend);
+  w.init(a, s, kvh, r0);
+  load.aim(a, head_base, id0, kt, 0, kend);
+  load.start(k0, 0);
+  load.start(v0, a.kv_stride);
+  load.aim(a, head_base, id1, kt + kStep, 0, kend);
+  load.start(k1, 0);
+  load.start(v1, a.kv_stride);
+  w.flip(a.q_sign);
+  bool dirty = false;
+  auto step = [&](uint16_t* s_k, uint16_t* s_v) {
+    typename R::Scores sc;
+    typename R::Weights wt;
+    u32x4 kf[2][D / 32];
+    wait_loads<3 * J>();  // behind K of this tile: V, K and V of the next
+    R::read_k_beside_loads(s_k, 0, kf[0]);
+    R::read_k_beside_loads(s_k, 1, kf[1]);
+    w.scores(kf[0], sc[0]);
+    w.scores(kf[1], sc[1]);
+    wait_reads();
+    load.aim(a, head_base, id2, kt + 2 * kStep, 0, kend);
+    load.start(s_k, 0);
+    id2 = id3;
+    id3 = block_ids<kTileKeys>(a, bt, kt + 4 * kStep, kend);
+    w.maxima(a, kt, sc);
+    w.weights(a, 0, sc[0], wt);
+    w.weights(a, 1, sc[1], wt);
+    wait_loads<3 * J>();
+    if (w.masked(kt)) dirty |= clean_values<T>(s_v, kTileElems / 8);
+    w.values_beside_loads(s_v, wt);
+    wait_reads();
+    load.start(s_v, a.kv_stride);
+    kt += kStep;
+  };
+  while (kt < kstop) {
+    step(k0, v0);
+    if (kt >= kstop) break;
+    step(k1, v1);
   }
 
-  // Join: m is the same in the four lanes of a row, l is each lane's own keys'.
+  // Join: wave v's sums go to the v-th array, 16-byte pieces permuted by row.
+  wait_loads<0>();  // of tiles that were not needed
+  if (lane == 0) s_dirty[wave] = dirty;
   __syncthreads();
-  float* s_o = reinterpret_cast<float*>(s_mem);
+  float* s_o[kWaves] = {reinterpret_cast<float*>(s_k0), reinterpret_cast<float*>(s_v0), reinterpret_cast<float*>(s_k1),
+                        reinterpret_cast<float*>(s_v1)};
+  float* mine = wave == 0 ? s_o[0] : wave == 1 ? s_o[1] : wave == 2 ? s_o[2] : s_o[3];
+  static_assert(kTileRows * NT * D * 4 <= kWaves * kTileElems * 2, "a wave's sums fit one array");
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    float l = w.l[n];
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    const float l = w.weight_sum(n);
     const int r = kTileRows * n + i;
     if (g == 0) {
       s_ml[wave][r][0] = w.m[n];
@@ -341,11 +504,12 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
     }
 #pragma unroll
     for (int d = 0; d < D / 16; ++d)
-      *reinterpret_cast<f32x4*>(s_o + (wave * kTileRows * NT + r) * (D + 4) + 16 * d + 4 * g) = w.o[n][d];
+      *reinterpret_cast<f32x4*>(mine + r * D + 4 * ((4 * d + g) ^ (r & (D / 4 - 1)))) = w.o[n][d];
   }
   __syncthreads();
+  dirty = (s_dirty[0] | s_dirty[1] | s_dirty[2] | s_dirty[3]) != 0;
   for (int e = threadIdx.x; e < rows * (D / 4); e += kWave * kWaves) {
-    const int r = e / (D / 4), d = 4 * (e % (D / 4));
+    const int r = e / (D / 4), piece = e % (D / 4), d = 4 * piece;
     float top = s_ml[0][r][0];
 #pragma unroll
     for (int v = 1; v < kWaves; ++v) top = fmaxf(top, s_ml[v][r][0]);
@@ -355,11 +519,13 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
     for (int v = 0; v < kWaves; ++v) {
       const float f = __builtin_amdgcn_exp2f(s_ml[v][r][0] - top);
       l = fmaf(f, s_ml[v][r][1], l);
-      const f32x4 ov = *reinterpret_cast<const f32x4*>(s_o + (v * kTileRows * NT + r) * (D + 4) + d);
+      const f32x4 ov = *reinterpret_cast<const f32x4*>(s_o[v] + r * D + 4 * (piece ^ (r & (D / 4 - 1))));
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[k] = fmaf(f, ov[k], o[k]);
     }
     const int t = (r0 + r) / a.group, h = kvh * a.group + (r0 + r) - t * a.group;
+    if (dirty)
+      add_left_out<T>(a, bt, head_base + d, D, max(kbeg, (w.lo + 1) / kTileKeys * kTileKeys), min(kstop, s.start + t + 1), o);
     if (a.parts == 1) {
       const float inv = 1.f / l;
       *reinterpret_cast<u32x2*>(a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + d) =
@@ -368,6 +534,157 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
       const int64_t at = ((int64_t)(s.row0 + t) * a.num_heads + h) * a.parts + part;
       *reinterpret_cast<f32x4*>(a.part_o + at * D + d) = o;
       if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = f32x2{top, l};
+    }
+  }
+}
+
+// Many rows: a workgroup takes 64 NT rows, 16 NT a wave, and one part of the keys; its waves share the tiles of 64 keys
+// in LDS, each loading a quarter. The scores of tile t + 1 are computed beside the weights of tile t (matrix and
+// vector instructions of one iteration do not depend on each other), so one barrier a tile is enough: behind it K of t + 1
+// and V of t are in LDS, and the buffers of K of t and V of t - 1 are free for K of t + 2 and V of t + 1.
+template <int D, int NT, typename T>
+__global__ __launch_bounds__(kWave* kWaves, 2) void chunk_tiles_kernel(const ChunkArgs a) {
+  constexpr int kKeys = 64, kTileElems = kKeys * D;
+  constexpr int J = kTileElems * 2 / 1024 / kWaves;  // load instructions of a wave for K, and for V
+  __shared__ __attribute__((aligned(16))) uint16_t s_k0[kTileElems], s_v0[kTileElems], s_k1[kTileElems], s_v1[kTileElems];
+  __shared__ int s_dirty;
+  const int lane = threadIdx.x & (kWave - 1), i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  // The last row tiles see the most keys: they go first. Tiles of one K/V head and part follow each other every 8th
+  // workgroup, so on one XCD where these are a multiple of 8.
+  int idx = blockIdx.x;
+  const int units = a.num_seqs * a.kv_heads * a.parts;
+  const int tile = a.row_tiles - 1 - idx / units;
+  idx %= units;
+  const int kvh = idx % a.kv_heads;
+  idx /= a.kv_heads;
+  const int part = idx % a.parts, b = idx / a.parts;
+  Seq s;
+  if (!seq_of(a, b, part == 0 && tile == 0 && kvh == 0, s)) return;
+  constexpr int kRows = kTileRows * NT;
+  const int r0 = tile * kRows * kWaves, total = s.nq * a.group;
+  if (r0 >= total) return;
+  const int kend = s.start + min(r0 + kRows * kWaves - 1, total - 1) / a.group + 1, kbeg = part * a.part_tokens;
+  if (kbeg >= kend) return;
+  const int kstop = min(kend, kbeg + a.part_tokens);
+  const int tiles = (kstop - kbeg + kKeys - 1) / kKeys;
+
+  const int32_t* bt = a.block_tables + (int64_t)b * a.bt_stride;
+  const uint16_t* head_base = a.pool_layer + (int64_t)kvh * a.head_stride;
+  typedef Rows<D, NT, 2, T> R;
+  R w;
+  const int wr0 = r0 + wave * kRows;  // the wave's first row; from total on: it only loads
+  w.init(a, s, kvh, wr0);
+  const bool has_rows = wr0 < total;
+  const int lo = s.start + r0 / a.group;  // the workgroup's first position
+  if (threadIdx.x == 0) s_dirty = 0;
+  Loader<D, J> load;
+  const int first = wave * (kKeys / kWaves);
+  const int at = first * D;
+  auto ids_of = [&](int t) { return block_ids<kKeys>(a, bt, kbeg + t * kKeys, kend); };
+  auto aim = [&](int32_t ids, int t) { load.aim(a, head_base, ids, kbeg + t * kKeys, first, kend); };
+  // Tiles past the last one repeat its last key.
+  int32_t id2, id3;
+  {
+    const int32_t id0 = ids_of(0), id1 = ids_of(1);
+    id2 = ids_of(2);
+    id3 = ids_of(3);
+    aim(id0, 0);
+    load.start(s_k0 + at, 0);
+    load.start(s_v0 + at, a.kv_stride);
+    aim(id1, 1);
+    load.start(s_k1 + at, 0);
+  }
+  w.flip(a.q_sign);
+  typename R::Scores sc;
+  wait_loads<0>();
+  barrier();
+  if (has_rows) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      u32x4 kf[D / 32];
+      R::read_k(s_k0, h, kf);
+      w.scores(kf, sc[h]);
+    }
+  }
+  // The loader is aimed at tile t + 1 at the start.
+  auto step = [&](int t, uint16_t* k_next, uint16_t* k_free, uint16_t* v_this, uint16_t* v_free) {
+    wait_loads<0>();
+    const int kt = kbeg + t * kKeys;
+    if (kt + kKeys - 1 > lo && clean_values<T>(v_this + at, kTileElems / 8 / kWaves)) s_dirty = 1;
+    barrier();
+    load.start(v_free + at, a.kv_stride);
+    aim(id2, t + 2);
+    load.start(k_free + at, 0);
+    id2 = id3;
+    id3 = ids_of(t + 4);
+    if (has_rows && kt <= w.hi) {
+      u32x4 kf[2][D / 32];
+      R::read_k(k_next, 0, kf[0]);
+      w.maxima(a, kt, sc);
+      typename R::Weights wt;
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {  // scores of the next tile beside the weights of this one
+        if (h < 3) R::read_k(k_next, h + 1, kf[(h + 1) & 1]);
+        f32x4 sn[NT];
+        w.scores(kf[h & 1], sn);
+        w.weights(a, h, sc[h], wt);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sc[h][n] = sn[n];
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      w.values(v_this, wt);
+    }
+  };
+  for (int t = 0; t < tiles; t += 2) {
+    step(t, s_k1, s_k0, s_v0, s_v1);
+    if (t + 1 >= tiles) break;
+    step(t + 1, s_k0, s_k1, s_v1, s_v0);
+  }
+  wait_loads<0>();  // of tiles that were not needed
+  if (!has_rows) return;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float l = w.weight_sum(n);
+    const int r = wr0 + kTileRows * n + i;
+    if (r >= total) continue;
+    const int t = r / a.group, h = kvh * a.group + r - t * a.group;
+    if (a.parts == 1) {
+      const float inv = 1.f / l;
+      uint16_t* op = a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + 4 * g;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+        *reinterpret_cast<u32x2*>(op + 16 * d) =
+            u32x2{pack2<T>(w.o[n][d][0] * inv, w.o[n][d][1] * inv), pack2<T>(w.o[n][d][2] * inv, w.o[n][d][3] * inv)};
+    } else {
+      const int64_t to = ((int64_t)(s.row0 + t) * a.num_heads + h) * a.parts + part;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4*>(a.part_o + to * D + 16 * d + 4 * g) = w.o[n][d];
+      if (g == 0) *reinterpret_cast<f32x2*>(a.part_ml + to * 2) = f32x2{w.m[n], l};
+    }
+  }
+  if (s_dirty == 0) return;
+  // What was left out goes into what was just written, by the lane that wrote it.
+  const int from = max(kbeg, (lo + 1) / kKeys * kKeys);
+#pragma unroll 1
+  for (int n = 0; n < NT; ++n) {
+    const int r = wr0 + kTileRows * n + i;
+    if (r >= total) continue;
+    const int t = r / a.group, h = kvh * a.group + r - t * a.group;
+#pragma unroll 1
+    for (int d = 4 * g; d < D; d += 16) {
+      f32x4 more = {0.f, 0.f, 0.f, 0.f};
+      add_left_out<T>(a, bt, head_base + d, D, from, min(kstop, s.start + t + 1), more);
+      if (a.parts == 1) {
+        uint16_t* op = a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (more[e] != 0.f) op[e] = (uint16_t)pack2<T>(more[e] + T::load(op[e]), 0.f);
+      } else {
+        float* op = a.part_o + (((int64_t)(s.row0 + t) * a.num_heads + h) * a.parts + part) * D + d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) op[e] += more[e];
+      }
     }
   }
 }
@@ -402,22 +719,26 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkArgs a) {
       u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
 }
 
-// How a call is split: row tiles of 16 nt rows per (sequence, K/V head), key parts of part_tokens.
+// How a call is split: row tiles of `rows` rows per (sequence, K/V head), key parts of part_tokens.
 struct Plan {
-  int nt, row_tiles, parts, part_tokens;
+  int rows, row_tiles, parts, part_tokens;
+  bool tiles;  // chunk_tiles_kernel, else chunk_rows_kernel
 };
 
 constexpr int kCus = 256;
+constexpr int kTilesNt = 2;  // 16-row tiles of a wave of chunk_tiles_kernel
 
 Plan plan_of(int num_seqs, int kv_heads, int group, int max_query_len, int max_context) {
   Plan p;
   const int64_t rows = (int64_t)max_query_len * group;
-  p.nt = rows > 48 ? 4 : rows > 32 ? 3 : rows > 16 ? 2 : 1;
-  p.row_tiles = (int)((rows + kTileRows * p.nt - 1) / (kTileRows * p.nt));
+  p.tiles = rows > 64;
+  p.rows = p.tiles ? kTileRows * kTilesNt * kWaves : rows > 48 ? 64 : rows > 32 ? 48 : rows > 16 ? 32 : 16;
+  p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
   constexpr int kStep = kWaves * kTileKeys;
   const int64_t steps = ((int64_t)max_context + kStep - 1) / kStep;
   const int64_t groups = (int64_t)num_seqs * kv_heads * p.row_tiles;
-  int64_t parts = (kCus + groups - 1) / groups;
+  const int64_t want = p.tiles ? 2 * kCus : kCus;
+  int64_t parts = (want + groups - 1) / groups;
   if (parts > steps) parts = steps;
   const int64_t per = (steps + parts - 1) / parts;
   p.part_tokens = (int)(per * kStep > 0x7fffffff - kStep ? 0x7fffffff / kStep * kStep : per * kStep);
@@ -441,12 +762,15 @@ tq_status launch(const ChunkArgs& a, const Plan& p, hipStream_t stream) {
   const int64_t join = (int64_t)a.num_seqs * (((int64_t)a.max_query_len * a.num_heads + 1024 / D - 1) / (1024 / D));
   if (grid > 0x7fffffffLL || (a.parts > 1 && join > 0x7fffffffLL)) return TQ_ERR_UNSUPPORTED;
   const dim3 g((unsigned)grid), t(kWave * kWaves);
-  switch (p.nt) {
-    case 1: hipLaunchKernelGGL((chunk_rows_kernel<D, 1, T>), g, t, 0, stream, a); break;
-    case 2: hipLaunchKernelGGL((chunk_rows_kernel<D, 2, T>), g, t, 0, stream, a); break;
-    case 3: hipLaunchKernelGGL((chunk_rows_kernel<D, 3, T>), g, t, 0, stream, a); break;
-    default: hipLaunchKernelGGL((chunk_rows_kernel<D, 4, T>), g, t, 0, stream, a); break;
-  }
+  if (p.tiles)
+    hipLaunchKernelGGL((chunk_tiles_kernel<D, kTilesNt, T>), g, t, 0, stream, a);
+  else
+    switch (p.rows) {
+      case 16: hipLaunchKernelGGL((chunk_rows_kernel<D, 1, T>), g, t, 0, stream, a); break;
+      case 32: hipLaunchKernelGGL((chunk_rows_kernel<D, 2, T>), g, t, 0, stream, a); break;
+      case 48: hipLaunchKernelGGL((chunk_rows_kernel<D, 3, T>), g, t, 0, stream, a); break;
+      default: hipLaunchKernelGGL((chunk_rows_kernel<D, 4, T>), g, t, 0, stream, a); break;
+    }
   tq_status st = check_launch();
   if (st != TQ_OK || a.parts == 1) return st;
   hipLaunchKernelGGL((chunk_join_kernel<D, T>), dim3((unsigned)join), dim3(256), 0, stream, a);
