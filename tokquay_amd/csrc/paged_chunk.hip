@@ -59,6 +59,7 @@ struct ChunkArgs {
   int32_t kv_heads;
   int32_t group;
   int32_t block_size;
+  uint32_t inv_block;  // ceil(2^21 / block_size)
   int32_t max_blocks;
   int32_t num_q_rows;
   int32_t max_query_len;
@@ -140,36 +141,103 @@ __device__ __forceinline__ void add_left_out(const ChunkArgs& a, const int32_t* 
   }
 }
 
-// The block id of key kt + lane % KEYS of a sequence (keys from kend on: the last one's).
-template <int KEYS>
-__device__ __forceinline__ int32_t block_ids(const ChunkArgs& a, const int32_t* bt, int kt, int kend) {
-  const int key = min(kt + (int)(threadIdx.x & (KEYS - 1)), kend - 1);
-  return bt[key / a.block_size];
+// A block-table entry, or block 0 for a bad one, which is flagged.
+__device__ __forceinline__ int32_t checked(const ChunkArgs& a, int32_t id) {
+  if ((uint32_t)id < (uint32_t)a.num_blocks) return id;
+  flag_error(a.d_error, TQ_DEVERR_BLOCK_ID);
+  return 0;
 }
 
-// Starts the copy of keys kt + FIRST .. of one K/V head into LDS by one wave, J instructions of 1024 bytes. Keys
-// from kend on are the last one again: finite wherever it is, and masked. `ids` is block_ids(kt); bad ones are flagged
-// and block 0 is read in their place.
+// A tile's first key and its place in the sequence's blocks. Keys from `stop` on are the last one before it again:
+// finite wherever that one is, and masked.
+struct Cursor {
+  int kt, stop;          // uniform, as is all of it
+  int q, r;              // kt = q block_size + r
+  int end_q, end_r;      // stop - 1
+  int step_q, step_r;    // the step to the next tile
+
+  __device__ __forceinline__ void init(const ChunkArgs& a, int first, int until, int step) {
+    kt = first;
+    stop = until;
+    q = kt / a.block_size;
+    r = kt - q * a.block_size;
+    end_q = (stop - 1) / a.block_size;
+    end_r = stop - 1 - end_q * a.block_size;
+    step_q = step / a.block_size;
+    step_r = step - step_q * a.block_size;
+  }
+  __device__ __forceinline__ void next(const ChunkArgs& a, int step) {
+    kt += step;
+    q += step_q;
+    r += step_r;
+    if (r >= a.block_size) {
+      r -= a.block_size;
+      ++q;
+    }
+  }
+  __device__ __forceinline__ int first_entry() const { return kt < stop ? q : end_q; }
+  // Table entry and slot in its block of the tile's key `local` (below 64). With x below 1024 + 64 and inv_block =
+  // ceil(2^21 / block_size), x inv_block / 2^21 exceeds x / block_size by less than 1 / block_size.
+  __device__ __forceinline__ void place(const ChunkArgs& a, int local, int& entry, int& slot) const {
+    const bool in = kt < stop;
+    const uint32_t x = (uint32_t)((in ? r : end_r) + min(local, in ? stop - 1 - kt : 0));
+    const int b = (int)(__umul24(x, a.inv_block) >> 21);
+    entry = (in ? q : end_q) + b;
+    slot = (int)x - b * a.block_size;
+  }
+};
+
+// The block ids of one wave's tiles: 64 consecutive table entries in its lanes, and the 64 that come next on their
+// way, so that a tile waits for none.
+struct Window {
+  int base, next_base;
+  int32_t ids, next;
+
+  __device__ __forceinline__ int32_t entries(const int32_t* bt, const Cursor& c, int from) const {
+    return bt[min(from + (int)(threadIdx.x & (kWave - 1)), c.end_q)];
+  }
+  // The entries from the first later tile on that passes these.
+  __device__ __forceinline__ void ahead(const ChunkArgs& a, const int32_t* bt, const Cursor& c, int step) {
+    const int64_t left = (int64_t)(base + kWave) * a.block_size - (kTileKeys - 1) - c.kt;
+    const int64_t at = c.kt + (left <= 0 ? step : (left + step - 1) / step * step);
+    next_base = (int)(min(at, (int64_t)c.stop - 1) / a.block_size);
+    next = entries(bt, c, next_base);
+  }
+  __device__ __forceinline__ void init(const ChunkArgs& a, const int32_t* bt, const Cursor& c, int step) {
+    base = c.first_entry();
+    ids = entries(bt, c, base);
+    ahead(a, bt, c, step);
+    ids = checked(a, ids);
+  }
+  // Moves on where the cursor's tile passes the entries at hand.
+  __device__ __forceinline__ void move(const ChunkArgs& a, const int32_t* bt, const Cursor& c, int step) {
+    if (min(c.kt + kTileKeys, c.stop) - 1 < (int64_t)(base + kWave) * a.block_size) return;  // uniform
+    base = next_base;
+    ids = checked(a, next);
+    asm volatile("" : "+v"(ids));  // waited for here, not by every tile
+    ahead(a, bt, c, step);
+  }
+};
+
+// The copy of `J` times 1024 bytes of a tile of one K/V head into LDS by one wave, from key FIRST of the tile on.
 template <int D, int J>
 struct Loader {
   static constexpr int kLanes = D / 8;          // lanes a key row takes, 16 bytes each
   static constexpr int kKeys = kWave / kLanes;  // keys of one instruction
   const uint16_t* src[J];                       // K; V is kv_stride on
 
-  __device__ __forceinline__ void aim(const ChunkArgs& a, const uint16_t* head_base, int32_t ids, int kt, int first,
-                                      int kend) {
+  // `ids`: lane l has the block id of table entry base + l, or (BY_KEY) of the tile's key l.
+  template <bool BY_KEY>
+  __device__ __forceinline__ void aim(const ChunkArgs& a, const uint16_t* head_base, const Cursor& c, int first,
+                                      int32_t ids, int base) {
     const int lane = threadIdx.x & (kWave - 1);
-    if ((uint32_t)ids >= (uint32_t)a.num_blocks) {
-      flag_error(a.d_error, TQ_DEVERR_BLOCK_ID);
-      ids = 0;
-    }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int local = first + j * kKeys + lane / kLanes;
-      const int key = min(kt + local, kend - 1);
-      const int32_t blk = __shfl(ids, local);
-      src[j] = head_base + (int64_t)blk * a.block_stride + (int64_t)(key % a.block_size) * D +
-               8 * ((lane % kLanes) ^ swizzle<D>(local));
+      int entry, slot;
+      c.place(a, local, entry, slot);
+      const int32_t blk = __shfl(ids, BY_KEY ? local : entry - base);
+      src[j] = head_base + (int64_t)blk * a.block_stride + slot * D + 8 * ((lane % kLanes) ^ swizzle<D>(local));
     }
   }
 
@@ -443,15 +511,22 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
   uint16_t *k0 = s_k0 + wave * kTileElems, *v0 = s_v0 + wave * kTileElems, *k1 = s_k1 + wave * kTileElems,
            *v1 = s_v1 + wave * kTileElems;
   int kt = kbeg + wave * kTileKeys;
-  // Tiles past the part's end are loaded too (their keys clamped into the sequence), so that the count of loads behind the
-  // one that is waited for stays the same: K and V of two tiles are always on their way, of which a wait takes the first.
-  int32_t id0 = block_ids<kTileKeys>(a, bt, kt, kend), id1 = block_ids<kTileKeys>(a, bt, kt + kStep, kend);
-  int32_t id2 = block_ids<kTileKeys>(a, bt, kt + 2 * kStep, kend), id3 = block_ids<kTileKeys>(a, bt, kt + 3 * kStep, kend);
   w.init(a, s, kvh, r0);
-  load.aim(a, head_base, id0, kt, 0, kend);
+  Cursor c;
+  c.init(a, kt, kstop, kStep);
+  Window ids;
+  ids.init(a, bt, c, kStep);
+  // Tiles past the part's end are loaded too (its last key again and again), so that the count of loads behind the
+  // one that is waited for stays the same: K and V of two tiles are always on their way, of which a wait takes the first.
+  auto aim = [&] {
+    ids.move(a, bt, c, kStep);
+    load.template aim<false>(a, head_base, c, 0, ids.ids, ids.base);
+    c.next(a, kStep);
+  };
+  aim();
   load.start(k0, 0);
   load.start(v0, a.kv_stride);
-  load.aim(a, head_base, id1, kt + kStep, 0, kend);
+  aim();
   load.start(k1, 0);
   load.start(v1, a.kv_stride);
   w.flip(a.q_sign);
@@ -466,10 +541,8 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
     w.scores(kf[0], sc[0]);
     w.scores(kf[1], sc[1]);
     wait_reads();
-    load.aim(a, head_base, id2, kt + 2 * kStep, 0, kend);
+    aim();
     load.start(s_k, 0);
-    id2 = id3;
-    id3 = block_ids<kTileKeys>(a, bt, kt + 4 * kStep, kend);
     w.maxima(a, kt, sc);
     w.weights(a, 0, sc[0], wt);
     w.weights(a, 1, sc[1], wt);
@@ -581,18 +654,29 @@ __global__ __launch_bounds__(kWave* kWaves, 2) void chunk_tiles_kernel(const Chu
   Loader<D, J> load;
   const int first = wave * (kKeys / kWaves);
   const int at = first * D;
-  auto ids_of = [&](int t) { return block_ids<kKeys>(a, bt, kbeg + t * kKeys, kend); };
-  auto aim = [&](int32_t ids, int t) { load.aim(a, head_base, ids, kbeg + t * kKeys, first, kend); };
+  Cursor c, ahead;  // the tile to aim at, and the one to fetch block ids of
+  c.init(a, kbeg, kend, kKeys);
+  ahead = c;
+  auto fetch_ids = [&] {  // by key
+    int entry, slot;
+    ahead.place(a, lane, entry, slot);
+    ahead.next(a, kKeys);
+    return bt[entry];
+  };
+  auto aim = [&](int32_t ids) {
+    load.template aim<true>(a, head_base, c, first, checked(a, ids), 0);
+    c.next(a, kKeys);
+  };
   // Tiles past the last one repeat its last key.
   int32_t id2, id3;
   {
-    const int32_t id0 = ids_of(0), id1 = ids_of(1);
-    id2 = ids_of(2);
-    id3 = ids_of(3);
-    aim(id0, 0);
+    const int32_t id0 = fetch_ids(), id1 = fetch_ids();
+    id2 = fetch_ids();
+    id3 = fetch_ids();
+    aim(id0);
     load.start(s_k0 + at, 0);
     load.start(s_v0 + at, a.kv_stride);
-    aim(id1, 1);
+    aim(id1);
     load.start(s_k1 + at, 0);
   }
   w.flip(a.q_sign);
@@ -614,10 +698,10 @@ __global__ __launch_bounds__(kWave* kWaves, 2) void chunk_tiles_kernel(const Chu
     if (kt + kKeys - 1 > lo && clean_values<T>(v_this + at, kTileElems / 8 / kWaves)) s_dirty = 1;
     barrier();
     load.start(v_free + at, a.kv_stride);
-    aim(id2, t + 2);
+    aim(id2);
     load.start(k_free + at, 0);
     id2 = id3;
-    id3 = ids_of(t + 4);
+    id3 = fetch_ids();
     if (has_rows && kt <= w.hi) {
       u32x4 kf[2][D / 32];
       R::read_k(k_next, 0, kf[0]);
@@ -689,34 +773,65 @@ __global__ __launch_bounds__(kWave* kWaves, 2) void chunk_tiles_kernel(const Chu
   }
 }
 
-// Joins the parts of each (row, head): D / 4 lanes a pair, four dims each.
+// Joins the parts of each (row, head): one wave a pair. A lane first takes a part's maximum and weight sum, then D / 64 dims
+// of all parts, whose loads do not depend on each other.
 template <int D, typename T>
 __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkArgs a) {
-  constexpr int kLanes = D / 4, kPairs = 256 / kLanes;
-  const int tiles = (a.max_query_len * a.num_heads + kPairs - 1) / kPairs;
-  const int b = blockIdx.x / tiles, pair = (blockIdx.x - b * tiles) * kPairs + threadIdx.x / kLanes;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int tiles = (a.max_query_len * a.num_heads + 3) / 4;
+  const int b = blockIdx.x / tiles;
+  const int pair = __builtin_amdgcn_readfirstlane((blockIdx.x - b * tiles) * 4 + threadIdx.x / kWave);
   Seq s;
   if (!seq_of(a, b, false, s)) return;
   const int t = pair / a.num_heads, h = pair - t * a.num_heads;
   if (t >= s.nq) return;
-  const int d = 4 * (threadIdx.x % kLanes);
   const int parts = (s.start + t) / a.part_tokens + 1;  // parts that the row sees
   const int64_t at = ((int64_t)(s.row0 + t) * a.num_heads + h) * a.parts;
-  float top = -FLT_MAX, l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < parts; ++p) {
-    const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + (at + p) * 2);
-    const f32x4 op = *reinterpret_cast<const f32x4*>(a.part_o + (at + p) * D + d);
-    const float next = fmaxf(top, ml[0]);
-    const float f = __builtin_amdgcn_exp2f(top - next), fp = __builtin_amdgcn_exp2f(ml[0] - next);
-    l = fmaf(fp, ml[1], l * f);
+  constexpr int kDims = D / kWave;
+  float top = -FLT_MAX, l = 0.f, o[kDims] = {};
+  for (int p0 = 0; p0 < parts; p0 += kWave) {
+    const int n = min(kWave, parts - p0);
+    const f32x2 ml = lane < n ? *reinterpret_cast<const f32x2*>(a.part_ml + (at + p0 + lane) * 2) : f32x2{-FLT_MAX, 0.f};
+    float most = ml[0];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = fmaf(fp, op[k], o[k] * f);
+    for (int off = kWave / 2; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off));
+    const float next = fmaxf(top, most), f = __builtin_amdgcn_exp2f(top - next);
+    const float fp = lane < n ? __builtin_amdgcn_exp2f(ml[0] - next) : 0.f;
+    float sum = lane < n ? fp * ml[1] : 0.f;
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+    l = fmaf(l, f, sum);
     top = next;
+#pragma unroll
+    for (int k = 0; k < kDims; ++k) o[k] *= f;
+    const float* op = a.part_o + (at + p0) * D + lane * kDims;
+    auto weight = [&](int p) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, fp), p)); };
+    int p = 0;
+    for (; p + 8 <= n; p += 8) {
+      float x[8][kDims];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int k = 0; k < kDims; ++k) x[e][k] = op[(int64_t)(p + e) * D + k];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float w = weight(p + e);
+#pragma unroll
+        for (int k = 0; k < kDims; ++k) o[k] = fmaf(w, x[e][k], o[k]);
+      }
+    }
+    for (; p < n; ++p) {
+      const float w = weight(p);
+#pragma unroll
+      for (int k = 0; k < kDims; ++k) o[k] = fmaf(w, op[(int64_t)p * D + k], o[k]);
+    }
   }
   const float inv = 1.f / l;
-  *reinterpret_cast<u32x2*>(a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + d) =
-      u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+  uint16_t* to = a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + lane * kDims;
+  if constexpr (kDims == 2)
+    *reinterpret_cast<uint32_t*>(to) = pack2<T>(o[0] * inv, o[1] * inv);
+  else
+    *to = (uint16_t)pack2<T>(o[0] * inv, 0.f);
 }
 
 // How a call is split: row tiles of `rows` rows per (sequence, K/V head), key parts of part_tokens.
@@ -759,7 +874,7 @@ size_t workspace_of(const Plan& p, int32_t num_q_rows, int32_t num_heads, int32_
 template <int D, typename T>
 tq_status launch(const ChunkArgs& a, const Plan& p, hipStream_t stream) {
   const int64_t grid = (int64_t)a.num_seqs * a.kv_heads * a.row_tiles * a.parts;
-  const int64_t join = (int64_t)a.num_seqs * (((int64_t)a.max_query_len * a.num_heads + 1024 / D - 1) / (1024 / D));
+  const int64_t join = (int64_t)a.num_seqs * (((int64_t)a.max_query_len * a.num_heads + 3) / 4);
   if (grid > 0x7fffffffLL || (a.parts > 1 && join > 0x7fffffffLL)) return TQ_ERR_UNSUPPORTED;
   const dim3 g((unsigned)grid), t(kWave * kWaves);
   if (p.tiles)
@@ -851,6 +966,7 @@ extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const voi
   a.kv_heads = num_kv_heads;
   a.group = group;
   a.block_size = block_size;
+  a.inv_block = ((1u << 21) + block_size - 1) / block_size;
   a.max_blocks = max_blocks_per_seq;
   a.num_q_rows = num_q_rows;
   a.max_query_len = max_query_len;
