@@ -42,7 +42,7 @@ struct ChunkArgs {
   const uint16_t* q;
   int64_t q_stride;
   const uint16_t* pool_layer;
-  int64_t block_stride;
+  uint32_t block_stride;
   int64_t kv_stride;
   int64_t head_stride;
   const int32_t* block_tables;
@@ -51,6 +51,7 @@ struct ChunkArgs {
   const int32_t* q_start;
   float* part_o;   // [num_q_rows][num_heads][parts][D] sums of each part, or null: one part
   float* part_ml;  // [num_q_rows][num_heads][parts][2] maximum and weight sum
+  int32_t* queue;  // kQueueHead words, then (sequence, row tile) pairs: chunk_order_kernel; or null
   int32_t* d_error;
   float c;         // |scale| log2(e)
   uint32_t q_sign; // 0x80008000 where the scale is negative: the queries' signs are flipped
@@ -77,25 +78,30 @@ struct Seq {
   int row0, nq, start;
 };
 
+__device__ __forceinline__ bool fits(const ChunkArgs& a, const Seq& s, int64_t nq) {
+  const int64_t end = (int64_t)s.start + nq;
+  return nq > 0 && nq <= a.max_query_len && s.row0 >= 0 && s.row0 + nq <= a.num_q_rows && s.start >= 0 &&
+         end <= a.max_context && end <= (int64_t)a.max_blocks * a.block_size;
+}
+
 // False where the sequence has no rows or its lengths do not fit (flagged by the workgroup that `reports`).
 __device__ __forceinline__ bool seq_of(const ChunkArgs& a, int b, bool reports, Seq& s) {
   s.row0 = __builtin_amdgcn_readfirstlane(a.cu_q[b]);
   const int64_t nq = (int64_t)__builtin_amdgcn_readfirstlane(a.cu_q[b + 1]) - s.row0;
   s.start = __builtin_amdgcn_readfirstlane(a.q_start[b]);
-  if (nq == 0) return false;
-  const int64_t end = (int64_t)s.start + nq;
-  const bool ok = nq > 0 && nq <= a.max_query_len && s.row0 >= 0 && s.row0 + nq <= a.num_q_rows && s.start >= 0 &&
-                  end <= a.max_context && end <= (int64_t)a.max_blocks * a.block_size;
-  if (!ok && reports && threadIdx.x == 0) flag_error(a.d_error, TQ_DEVERR_LENGTH);
   s.nq = (int)nq;
+  if (nq == 0) return false;
+  const bool ok = fits(a, s, nq);
+  if (!ok && reports && threadIdx.x == 0) flag_error(a.d_error, TQ_DEVERR_LENGTH);
   return ok;
 }
 
-// 16-byte piece p of a tile's key `key` lies at piece p ^ swizzle(key) of the key's row in LDS: reads take
-// the same piece of 16 consecutive keys, or two neighbouring ones, and 256 bytes cover all banks once.
+// 16-byte piece p of a tile's key `key` lies at piece p ^ swizzle(key) of the key's row in LDS. K is read as one piece of 16
+// consecutive keys: 8 of them differ in the low three bits, so they cover 128 bytes of banks. V is read as two neighbouring
+// pieces of 4 consecutive keys: these differ in the two bits above the lowest.
 template <int D>
 __device__ __forceinline__ int swizzle(int key) {
-  return D == 128 ? key & 15 : (key >> 1) & 7;
+  return (key & 3) << 1 | ((key >> 2) & 1) | (D == 128 ? key & 8 : 0);
 }
 
 // Zeros in place of the infinities and NaN among a wave's `pieces` 16-byte pieces of V in LDS; whether there were any (uniform).
@@ -226,18 +232,30 @@ struct Loader {
   static constexpr int kKeys = kWave / kLanes;  // keys of one instruction
   const uint16_t* src[J];                       // K; V is kv_stride on
 
-  // `ids`: lane l has the block id of table entry base + l, or (BY_KEY) of the tile's key l.
-  template <bool BY_KEY>
-  __device__ __forceinline__ void aim(const ChunkArgs& a, const uint16_t* head_base, const Cursor& c, int first,
-                                      int32_t ids, int base) {
+  // `ids`: lane l has the block id of table entry base + l.
+  __device__ __forceinline__ void aim(const ChunkArgs& a, const uint16_t* head_base, const Cursor& c, int32_t ids, int base) {
     const int lane = threadIdx.x & (kWave - 1);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const int local = first + j * kKeys + lane / kLanes;
+      const int local = j * kKeys + lane / kLanes;
       int entry, slot;
       c.place(a, local, entry, slot);
-      const int32_t blk = __shfl(ids, BY_KEY ? local : entry - base);
-      src[j] = head_base + (int64_t)blk * a.block_stride + slot * D + 8 * ((lane % kLanes) ^ swizzle<D>(local));
+      const uint32_t blk = __shfl(ids, entry - base);
+      src[j] = head_base + ((uint64_t)blk * a.block_stride + slot * D + 8 * ((lane % kLanes) ^ swizzle<D>(local)));
+    }
+  }
+  // The same for a quarter of a 64-key tile, its keys from `first` on: lane l has the block id of the tile's key l.
+  __device__ __forceinline__ void aim_by_key(const ChunkArgs& a, const uint16_t* head_base, const Cursor& c, int first,
+                                             int32_t id) {
+    const int lane = threadIdx.x & (kWave - 1);
+    int entry, slot;
+    c.place(a, lane, entry, slot);
+    const uint64_t row = (uint64_t)(uint32_t)id * a.block_stride + slot * D;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int local = first + j * kKeys + lane / kLanes;
+      const uint64_t lo = (uint32_t)__shfl((int)(uint32_t)row, local), hi = (uint32_t)__shfl((int)(row >> 32), local);
+      src[j] = head_base + (hi << 32 | lo) + 8 * ((lane % kLanes) ^ swizzle<D>(local));
     }
   }
 
@@ -380,15 +398,21 @@ struct Rows {
     }
   }
 
+  // Four dim tiles' V at a time, the next four's on their way.
   __device__ __forceinline__ void values(const uint16_t* s_v, const Weights& w) {
-    u32x4 vf[2];
-    vf[0] = read_v(s_v, 0);
+    u32x4 vf[2][4];
 #pragma unroll
-    for (int j = 0; j < KS * D / 16; ++j) {
-      const int k = j / (D / 16), d = j % (D / 16), jn = j + 1;
-      if (jn < KS * D / 16) vf[jn & 1] = read_v(s_v + 32 * (jn / (D / 16)) * D, jn % (D / 16));
+    for (int e = 0; e < 4; ++e) vf[0][e] = read_v(s_v, e);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) o[n][d] = T::mfma(vf[j & 1], w[k][n], o[n][d]);
+    for (int j = 0; j < KS * D / 64; ++j) {
+      const int k = j / (D / 64), d = j % (D / 64) * 4, jn = j + 1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (jn < KS * D / 64) vf[jn & 1][e] = read_v(s_v + 32 * (jn / (D / 64)) * D, jn % (D / 64) * 4 + e);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[n][d + e] = T::mfma(vf[j & 1][e], w[k][n], o[n][d + e]);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -520,7 +544,7 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
   // one that is waited for stays the same: K and V of two tiles are always on their way, of which a wait takes the first.
   auto aim = [&] {
     ids.move(a, bt, c, kStep);
-    load.template aim<false>(a, head_base, c, 0, ids.ids, ids.base);
+    load.aim(a, head_base, c, ids.ids, ids.base);
     c.next(a, kStep);
   };
   aim();
@@ -616,24 +640,12 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
 // vector instructions of one iteration do not depend on each other), so one barrier a tile is enough: behind it K of t + 1
 // and V of t are in LDS, and the buffers of K of t and V of t - 1 are free for K of t + 2 and V of t + 1.
 template <int D, int NT, typename T>
-__global__ __launch_bounds__(kWave* kWaves, 2) void chunk_tiles_kernel(const ChunkArgs a) {
+__device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b, int tile, int kvh, int part,
+                                         uint16_t* s_k0, uint16_t* s_v0, uint16_t* s_k1, uint16_t* s_v1, int& s_dirty) {
   constexpr int kKeys = 64, kTileElems = kKeys * D;
   constexpr int J = kTileElems * 2 / 1024 / kWaves;  // load instructions of a wave for K, and for V
-  __shared__ __attribute__((aligned(16))) uint16_t s_k0[kTileElems], s_v0[kTileElems], s_k1[kTileElems], s_v1[kTileElems];
-  __shared__ int s_dirty;
   const int lane = threadIdx.x & (kWave - 1), i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  // The last row tiles see the most keys: they go first. Tiles of one K/V head and part follow each other every 8th
-  // workgroup, so on one XCD where these are a multiple of 8.
-  int idx = blockIdx.x;
-  const int units = a.num_seqs * a.kv_heads * a.parts;
-  const int tile = a.row_tiles - 1 - idx / units;
-  idx %= units;
-  const int kvh = idx % a.kv_heads;
-  idx /= a.kv_heads;
-  const int part = idx % a.parts, b = idx / a.parts;
-  Seq s;
-  if (!seq_of(a, b, part == 0 && tile == 0 && kvh == 0, s)) return;
   constexpr int kRows = kTileRows * NT;
   const int r0 = tile * kRows * kWaves, total = s.nq * a.group;
   if (r0 >= total) return;
@@ -655,7 +667,7 @@ __global__ __launch_bounds__(kWave* kWaves, 2) void chunk_tiles_kernel(const Chu
   const int first = wave * (kKeys / kWaves);
   const int at = first * D;
   Cursor c, ahead;  // the tile to aim at, and the one to fetch block ids of
-  c.init(a, kbeg, kend, kKeys);
+  c.init(a, kbeg, kstop, kKeys);
   ahead = c;
   auto fetch_ids = [&] {  // by key
     int entry, slot;
@@ -664,7 +676,7 @@ __global__ __launch_bounds__(kWave* kWaves, 2) void chunk_tiles_kernel(const Chu
     return bt[entry];
   };
   auto aim = [&](int32_t ids) {
-    load.template aim<true>(a, head_base, c, first, checked(a, ids), 0);
+    load.aim_by_key(a, head_base, c, first, checked(a, ids));
     c.next(a, kKeys);
   };
   // Tiles past the last one repeat its last key.
@@ -773,6 +785,136 @@ __global__ __launch_bounds__(kWave* kWaves, 2) void chunk_tiles_kernel(const Chu
   }
 }
 
+// One workgroup a (sequence, K/V head, part, row tile). The last row tiles see the most keys and go first. Tiles of one K/V
+// head and part follow each other every 8th workgroup, so on one XCD, where these are a multiple of 8.
+template <int D, int NT, typename T>
+__global__ __launch_bounds__(kWave* kWaves, 2) void chunk_tiles_kernel(const ChunkArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t s_k0[64 * D], s_v0[64 * D], s_k1[64 * D], s_v1[64 * D];
+  __shared__ int s_dirty;
+  int idx = blockIdx.x;
+  const int units = a.num_seqs * a.kv_heads * a.parts;
+  const int tile = a.row_tiles - 1 - idx / units;
+  idx %= units;
+  const int kvh = idx % a.kv_heads;
+  idx /= a.kv_heads;
+  const int part = idx % a.parts, b = idx / a.parts;
+  Seq s;
+  if (!seq_of(a, b, part == 0 && tile == 0 && kvh == 0, s)) return;
+  row_tile<D, NT, T>(a, s, b, tile, kvh, part, s_k0, s_v0, s_k1, s_v1, s_dirty);
+}
+
+// With more row tiles than run at once, workgroups that stay and take them from a queue, the most keys first: dispatched
+// workgroups go to an XCD's CUs in turn, and one that has to wait for its CU holds up those behind it (4 x 2,048 tokens behind 768
+// to 5,376: 330 of 512 workgroups at work on average).
+constexpr int kXcds = 8;
+constexpr int kQueueLine = 32;                           // words between counters: a 128-byte line each
+constexpr int kQueueHead = (kXcds + 1) * kQueueLine;     // [0] pairs, then the counter of each XCD's share
+constexpr int kOrderThreads = 1024, kBuckets = 2048;
+
+__host__ __device__ inline int64_t queue_pairs(int64_t num_q_rows, int group, int rows_per_tile, int num_seqs) {
+  return num_q_rows * group / rows_per_tile + num_seqs;  // a sequence's last row tile may be partly filled
+}
+
+// The (sequence, row tile) pairs by keys, most first (to 1 / kBuckets of the longest context), and the counters at zero.
+__global__ __launch_bounds__(kOrderThreads) void chunk_order_kernel(const ChunkArgs a, int rows_per_tile) {
+  __shared__ int s_count[kBuckets];
+  __shared__ int s_wave[kOrderThreads / kWave];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  for (int i = tid; i < kBuckets; i += kOrderThreads) s_count[i] = 0;
+  if (tid < kXcds) a.queue[(tid + 1) * kQueueLine] = 0;
+  __syncthreads();
+  const int64_t all = (int64_t)a.num_seqs * a.row_tiles;
+  // The pair's bucket, or -1: no such tile.
+  auto bucket = [&](int64_t i, int& b, int& tile) {
+    b = (int)(i / a.row_tiles);
+    tile = (int)(i - (int64_t)b * a.row_tiles);
+    Seq s;
+    s.row0 = a.cu_q[b];
+    s.start = a.q_start[b];
+    const int64_t nq = (int64_t)a.cu_q[b + 1] - s.row0;
+    if (!fits(a, s, nq)) {
+      if (nq != 0 && tile == 0) flag_error(a.d_error, TQ_DEVERR_LENGTH);
+      return -1;
+    }
+    const int64_t r0 = (int64_t)tile * rows_per_tile, total = nq * a.group;
+    if (r0 >= total) return -1;
+    const int64_t keys = s.start + (min(r0 + rows_per_tile, total) - 1) / a.group;  // below max_context
+    return kBuckets - 1 - (int)(keys * kBuckets / a.max_context);
+  };
+  int b, tile;
+  for (int64_t i = tid; i < all; i += kOrderThreads) {
+    const int k = bucket(i, b, tile);
+    if (k >= 0) atomicAdd(&s_count[k], 1);
+  }
+  __syncthreads();
+  // Counts to starts: two buckets a thread, summed over the wave, then over the waves.
+  static_assert(kBuckets == 2 * kOrderThreads, "two buckets a thread");
+  const int c0 = s_count[2 * tid], c1 = s_count[2 * tid + 1];
+  int sum = c0 + c1;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const int up = __shfl_up(sum, off);
+    if (lane >= off) sum += up;
+  }
+  if (lane == kWave - 1) s_wave[wave] = sum;
+  __syncthreads();
+  int before = 0;
+  for (int v = 0; v < wave; ++v) before += s_wave[v];
+  s_count[2 * tid] = before + sum - c0 - c1;
+  s_count[2 * tid + 1] = before + sum - c1;
+  // More only where sequences share rows (cu_seqlens_q falls somewhere): those are left out.
+  const int64_t room = queue_pairs(a.num_q_rows, a.group, rows_per_tile, a.num_seqs);
+  if (tid == kOrderThreads - 1) {
+    a.queue[0] = (int)min((int64_t)(before + sum), room);
+    if (before + sum > room) flag_error(a.d_error, TQ_DEVERR_LENGTH);
+  }
+  __syncthreads();
+  for (int64_t i = tid; i < all; i += kOrderThreads) {
+    const int k = bucket(i, b, tile);
+    if (k < 0) continue;
+    const int at = atomicAdd(&s_count[k], 1);
+    if (at >= room) continue;
+    a.queue[kQueueHead + 2 * (int64_t)at] = b;
+    a.queue[kQueueHead + 2 * (int64_t)at + 1] = tile;
+  }
+}
+
+// Item f is pair f / kv_heads with K/V head f % kv_heads. XCD x takes the items f % 8 = x (with a multiple of 8 heads, heads of
+// its own), then those that others left.
+template <int D, int NT, typename T>
+__global__ __launch_bounds__(kWave* kWaves, 2) void chunk_queue_kernel(const ChunkArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t s_k0[64 * D], s_v0[64 * D], s_k1[64 * D], s_v1[64 * D];
+  __shared__ int s_dirty;
+  __shared__ int64_t s_item;
+  const int64_t items = (int64_t)a.queue[0] * a.kv_heads;
+  int turn = 0;  // shares that were found empty
+  for (;;) {
+    if (threadIdx.x == 0) {
+      int64_t item = -1;
+      while (turn < kXcds && item < 0) {
+        const int x = (blockIdx.x + turn) % kXcds;
+        const int64_t f = x + (int64_t)kXcds * atomicAdd(&a.queue[(x + 1) * kQueueLine], 1);
+        if (f < items)
+          item = f;
+        else
+          ++turn;
+      }
+      s_item = item;
+    }
+    __syncthreads();
+    const int64_t item = s_item;
+    if (item < 0) return;
+    const int pair = __builtin_amdgcn_readfirstlane((int)(item / a.kv_heads));
+    const int kvh = __builtin_amdgcn_readfirstlane((int)(item - (int64_t)pair * a.kv_heads));
+    const int b = __builtin_amdgcn_readfirstlane(a.queue[kQueueHead + 2 * (int64_t)pair]);
+    const int tile = __builtin_amdgcn_readfirstlane(a.queue[kQueueHead + 2 * (int64_t)pair + 1]);
+    Seq s;
+    seq_of(a, b, false, s);
+    row_tile<D, NT, T>(a, s, b, tile, kvh, 0, s_k0, s_v0, s_k1, s_v1, s_dirty);
+    __syncthreads();  // the buffers and s_item are free
+  }
+}
+
 // Joins the parts of each (row, head): one wave a pair. A lane first takes a part's maximum and weight sum, then D / 64 dims
 // of all parts, whose loads do not depend on each other.
 template <int D, typename T>
@@ -837,11 +979,13 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkArgs a) {
 // How a call is split: row tiles of `rows` rows per (sequence, K/V head), key parts of part_tokens.
 struct Plan {
   int rows, row_tiles, parts, part_tokens;
-  bool tiles;  // chunk_tiles_kernel, else chunk_rows_kernel
+  bool tiles;  // chunk_tiles_kernel or chunk_queue_kernel, else chunk_rows_kernel
+  bool queue;
 };
 
 constexpr int kCus = 256;
-constexpr int kTilesNt = 2;  // 16-row tiles of a wave of chunk_tiles_kernel
+constexpr int kTilesNt = 2;   // 16-row tiles of a wave of chunk_tiles_kernel
+constexpr int kTilesPerCu = 2;
 
 Plan plan_of(int num_seqs, int kv_heads, int group, int max_query_len, int max_context) {
   Plan p;
@@ -852,12 +996,13 @@ Plan plan_of(int num_seqs, int kv_heads, int group, int max_query_len, int max_c
   constexpr int kStep = kWaves * kTileKeys;
   const int64_t steps = ((int64_t)max_context + kStep - 1) / kStep;
   const int64_t groups = (int64_t)num_seqs * kv_heads * p.row_tiles;
-  const int64_t want = p.tiles ? 2 * kCus : kCus;
+  const int64_t want = p.tiles ? kTilesPerCu * kCus : kCus;
   int64_t parts = (want + groups - 1) / groups;
   if (parts > steps) parts = steps;
   const int64_t per = (steps + parts - 1) / parts;
   p.part_tokens = (int)(per * kStep > 0x7fffffff - kStep ? 0x7fffffff / kStep * kStep : per * kStep);
   p.parts = (int)((steps + per - 1) / per);
+  p.queue = p.tiles && p.parts == 1 && groups > want;
   return p;
 }
 
@@ -867,7 +1012,9 @@ bool sizes_ok(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t
          num_q_rows >= 0 && max_query_len >= 0 && max_context >= 0;
 }
 
-size_t workspace_of(const Plan& p, int32_t num_q_rows, int32_t num_heads, int32_t head_dim) {
+size_t workspace_of(const Plan& p, int32_t num_seqs, int32_t num_q_rows, int32_t num_heads, int32_t group,
+                    int32_t head_dim) {
+  if (p.queue) return (kQueueHead + 2 * (size_t)queue_pairs(num_q_rows, group, p.rows, num_seqs)) * sizeof(int32_t);
   return p.parts <= 1 ? 0 : (size_t)num_q_rows * num_heads * p.parts * (head_dim + 2) * sizeof(float);
 }
 
@@ -877,7 +1024,12 @@ tq_status launch(const ChunkArgs& a, const Plan& p, hipStream_t stream) {
   const int64_t join = (int64_t)a.num_seqs * (((int64_t)a.max_query_len * a.num_heads + 3) / 4);
   if (grid > 0x7fffffffLL || (a.parts > 1 && join > 0x7fffffffLL)) return TQ_ERR_UNSUPPORTED;
   const dim3 g((unsigned)grid), t(kWave * kWaves);
-  if (p.tiles)
+  if (p.queue) {
+    hipLaunchKernelGGL(chunk_order_kernel, dim3(1), dim3(kOrderThreads), 0, stream, a, p.rows);
+    const tq_status st = check_launch();
+    if (st != TQ_OK) return st;
+    hipLaunchKernelGGL((chunk_queue_kernel<D, kTilesNt, T>), dim3(kTilesPerCu * kCus), t, 0, stream, a);
+  } else if (p.tiles)
     hipLaunchKernelGGL((chunk_tiles_kernel<D, kTilesNt, T>), g, t, 0, stream, a);
   else
     switch (p.rows) {
@@ -902,8 +1054,9 @@ extern "C" size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_he
   if (!sizes_ok(num_seqs, num_heads, num_kv_heads, head_dim, num_q_rows, max_query_len, max_context_len) ||
       num_seqs == 0 || num_q_rows == 0 || max_query_len == 0 || max_context_len == 0)
     return 0;
-  return workspace_of(plan_of(num_seqs, num_kv_heads, num_heads / num_kv_heads, max_query_len, max_context_len),
-                      num_q_rows, num_heads, head_dim);
+  const int32_t group = num_heads / num_kv_heads;
+  return workspace_of(plan_of(num_seqs, num_kv_heads, group, max_query_len, max_context_len), num_seqs, num_q_rows,
+                      num_heads, group, head_dim);
 }
 
 extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
@@ -935,25 +1088,27 @@ extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const voi
 
   const int32_t group = num_heads / num_kv_heads;
   const Plan p = plan_of(num_seqs, num_kv_heads, group, max_query_len, max_context_len);
-  const size_t need = workspace_of(p, num_q_rows, num_heads, head_dim);
+  const size_t need = workspace_of(p, num_seqs, num_q_rows, num_heads, group, head_dim);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 16 != 0))
     return TQ_ERR_WORKSPACE;
 
   const PoolGeom g = pool_geom(num_layers, num_kv_heads, block_size, head_dim, layer);
+  if (g.block_stride > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
   ChunkArgs a;
   a.out = static_cast<uint16_t*>(out);
   a.out_stride = out_row_stride;
   a.q = static_cast<const uint16_t*>(q);
   a.q_stride = q_row_stride;
   a.pool_layer = static_cast<const uint16_t*>(pool) + g.layer_offset;
-  a.block_stride = g.block_stride;
+  a.block_stride = (uint32_t)g.block_stride;
   a.kv_stride = g.kv_stride;
   a.head_stride = g.head_stride;
   a.block_tables = block_tables;
   a.bt_stride = block_table_stride;
   a.cu_q = cu_seqlens_q;
   a.q_start = q_start;
-  a.part_o = static_cast<float*>(workspace);
+  a.queue = p.queue ? static_cast<int32_t*>(workspace) : nullptr;
+  a.part_o = p.parts > 1 ? static_cast<float*>(workspace) : nullptr;
   a.part_ml = a.part_o == nullptr ? nullptr : a.part_o + (size_t)num_q_rows * num_heads * p.parts * head_dim;
   a.d_error = d_error;
   // A scale of zero weighs every visible key alike: the smallest positive factor does the same, and keeps
