@@ -25,6 +25,8 @@
 // that one LDS read takes lie in different banks.
 #include <float.h>
 
+#include <utility>
+
 #include "half_types.h"
 
 namespace tq {
@@ -225,38 +227,37 @@ struct Window {
   }
 };
 
-// The copy of `J` times 1024 bytes of a tile of one K/V head into LDS by one wave, from key FIRST of the tile on.
+// The copy of J times 1024 bytes of a tile of one K/V head into LDS by one wave, from key `first` of the tile on. kLanes lanes
+// take a key's row, so instruction j copies the keys first + j kKeys + lane / kLanes; lane l looks up the key of
+// instruction l % J, and hands where its row lies to the others that copy it (a broadcast in rows of 16 or 4 lanes).
 template <int D, int J>
 struct Loader {
-  static constexpr int kLanes = D / 8;          // lanes a key row takes, 16 bytes each
-  static constexpr int kKeys = kWave / kLanes;  // keys of one instruction
-  const uint16_t* src[J];                       // K; V is kv_stride on
+  static constexpr int kLanes = D / 8;
+  static constexpr int kKeys = kWave / kLanes;
+  static_assert(J <= 4 || (J == 8 && kLanes == 16), "J lanes that copy the same keys lie in one row");
+  const uint16_t* src[J];  // K; V is kv_stride on
 
-  // `ids`: lane l has the block id of table entry base + l.
-  __device__ __forceinline__ void aim(const ChunkArgs& a, const uint16_t* head_base, const Cursor& c, int32_t ids, int base) {
+  static __device__ __forceinline__ int own_key(int first) {
     const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int local = j * kKeys + lane / kLanes;
-      int entry, slot;
-      c.place(a, local, entry, slot);
-      const uint32_t blk = __shfl(ids, entry - base);
-      src[j] = head_base + ((uint64_t)blk * a.block_stride + slot * D + 8 * ((lane % kLanes) ^ swizzle<D>(local)));
-    }
+    return first + kKeys * (lane % J) + lane / kLanes;
   }
-  // The same for a quarter of a 64-key tile, its keys from `first` on: lane l has the block id of the tile's key l.
-  __device__ __forceinline__ void aim_by_key(const ChunkArgs& a, const uint16_t* head_base, const Cursor& c, int first,
-                                             int32_t id) {
+  template <int FROM>
+  static __device__ __forceinline__ uint32_t broadcast(uint32_t v) {
+    constexpr int kRowBroadcast = 0x150;  // of the row's lane FROM; else of the quad's
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, J == 8 ? kRowBroadcast + FROM : 0x55 * FROM, 0xF, 0xF, true);
+  }
+  // `id`, `slot`: block and slot of this lane's own_key.
+  __device__ __forceinline__ void aim(const ChunkArgs& a, const uint16_t* head_base, int first, int32_t id, int slot) {
+    aim_each(a, head_base, first, (uint64_t)(uint32_t)id * a.block_stride + slot * D, std::make_integer_sequence<int, J>());
+  }
+  template <int... j>
+  __device__ __forceinline__ void aim_each(const ChunkArgs& a, const uint16_t* head_base, int first, uint64_t row,
+                                           std::integer_sequence<int, j...>) {
     const int lane = threadIdx.x & (kWave - 1);
-    int entry, slot;
-    c.place(a, lane, entry, slot);
-    const uint64_t row = (uint64_t)(uint32_t)id * a.block_stride + slot * D;
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int local = first + j * kKeys + lane / kLanes;
-      const uint64_t lo = (uint32_t)__shfl((int)(uint32_t)row, local), hi = (uint32_t)__shfl((int)(row >> 32), local);
-      src[j] = head_base + (hi << 32 | lo) + 8 * ((lane % kLanes) ^ swizzle<D>(local));
-    }
+    ((src[j] = head_base +
+               ((uint64_t)broadcast<j>((uint32_t)(row >> 32)) << 32 | broadcast<j>((uint32_t)row)) +
+               8 * ((lane % kLanes) ^ swizzle<D>(first + j * kKeys + lane / kLanes))),
+     ...);
   }
 
   // `to`: the tile's row `first` in LDS.
@@ -544,7 +545,9 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
   // one that is waited for stays the same: K and V of two tiles are always on their way, of which a wait takes the first.
   auto aim = [&] {
     ids.move(a, bt, c, kStep);
-    load.aim(a, head_base, c, ids.ids, ids.base);
+    int entry, slot;
+    c.place(a, Loader<D, J>::own_key(0), entry, slot);
+    load.aim(a, head_base, 0, __shfl(ids.ids, entry - ids.base), slot);
     c.next(a, kStep);
   };
   aim();
@@ -669,14 +672,16 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
   Cursor c, ahead;  // the tile to aim at, and the one to fetch block ids of
   c.init(a, kbeg, kstop, kKeys);
   ahead = c;
-  auto fetch_ids = [&] {  // by key
+  auto fetch_ids = [&] {
     int entry, slot;
-    ahead.place(a, lane, entry, slot);
+    ahead.place(a, Loader<D, J>::own_key(first), entry, slot);
     ahead.next(a, kKeys);
     return bt[entry];
   };
-  auto aim = [&](int32_t ids) {
-    load.aim_by_key(a, head_base, c, first, checked(a, ids));
+  auto aim = [&](int32_t id) {
+    int entry, slot;
+    c.place(a, Loader<D, J>::own_key(first), entry, slot);
+    load.aim(a, head_base, first, checked(a, id), slot);
     c.next(a, kKeys);
   };
   // Tiles past the last one repeat its last key.
