@@ -86,9 +86,11 @@ class Chunk:
     def expected(self, scale=None):
         """(out, bound) float64; rows of no sequence are NaN in both. The bound on ``|out - kernel|``:
 
-        * the output's rounding, and each weight's before it meets V: half a step of |out| (of the smallest normal
-          value below that) and of sum w |v|;
-          for weights that are subnormal in float16, 2^-25 of each |v| instead (the largest weight is at least 1);
+        * the output's rounding: half a step of |out| (of the smallest normal value below that);
+        * each weight's before it meets V and is summed: with w_j (1 + d_j), |d_j| <= d = half a step, in place of w_j (their sum
+          1), sum w (1 + d_j) v / sum w (1 + d_j) - sum w v = sum w d_j (v - out) / sum w (1 + d_j), at most
+          d (sum w |v| + |out|) / (1 - d); for weights that are subnormal in float16, 2^-25 of each |v| + |out| instead (the
+          largest weight is at least 1);
         * scores: D products summed in float32, off by at most (D + 8) 2^-24 sum |q k| scale, which changes a weight by
           that share; the sum of the weights, and of the products, (keys + 16) 2^-23 more."""
         scale = 1 / math.sqrt(self.dim) if scale is None else scale
@@ -109,9 +111,10 @@ class Chunk:
                 size = w @ vh.abs()
                 off = ((q.abs() @ kh.abs().t()).masked_fill(unseen, 0).amax(-1, keepdim=True) * abs(scale)
                        * (self.dim + 8) * 2.0**-24)  # fmt: skip
-                sub = 2.0**-25 * vh.abs().sum(0) if self.dtype == torch.float16 else 0.0
+                mine = out[r0 : r0 + n, h].abs()
+                sub = 2.0**-25 * (vh.abs().sum(0) + (s + n) * mine) if self.dtype == torch.float16 else 0.0
                 sub = sub + step * torch.finfo(self.dtype).tiny
-                bound[r0 : r0 + n, h] = (step * (out[r0 : r0 + n, h].abs() + size) * (1 + 2.0**-6)
+                bound[r0 : r0 + n, h] = ((step * mine + step * (size + mine)) * (1 + 2.0**-6)
                                          + size * (2 * off + (s + n + 16) * 2.0**-23) + sub)  # fmt: skip
         return out, bound
 

@@ -16,6 +16,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 struct Bf16 {
   typedef __bf16 x2 __attribute__((ext_vector_type(2)));
   typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+  static constexpr uint32_t kOnes = 0x3f803f80u;  // 1, 1
   static constexpr uint32_t kExponent = 0x7f80u;  // all ones: an infinity or a NaN
   static __device__ __forceinline__ float load(uint16_t bits) { return __uint_as_float((uint32_t)bits << 16); }
   // C/D: column lane % 16, rows 4 (lane / 16) + 0..3. A: row, B: column lane % 16, depth 8 (lane / 16) + 0..7.
@@ -27,6 +28,7 @@ struct Bf16 {
 struct Fp16 {
   typedef _Float16 x2 __attribute__((ext_vector_type(2)));
   typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+  static constexpr uint32_t kOnes = 0x3c003c00u;
   static constexpr uint32_t kExponent = 0x7c00u;
   static __device__ __forceinline__ float load(uint16_t bits) { return (float)__builtin_bit_cast(_Float16, bits); }
   static __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {

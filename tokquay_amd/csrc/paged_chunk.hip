@@ -14,11 +14,11 @@
 //   O^T[dim][row] += V^T[dim][key] P^T[key][row]     one depth step for each 16 dims
 //
 // The transposed scores leave lane (i, g) = (lane % 16, lane / 16) with row i and the keys 4 g + 0..3 and
-// 16 + 4 g + 0..3, so one lane's scores belong to one row (its position is one register, its maximum and
-// sum are taken in the lane and across four lanes at the end) and are, rounded to 16 bits, the B operand
+// 16 + 4 g + 0..3, so one lane's scores belong to one row (its position is one register, its maximum
+// is taken in the lane and across four lanes) and are, rounded to 16 bits, the B operand
 // of the second product with no exchange: that product may take the keys in any order, and V^T is read in
 // the same one (two transposing LDS reads of 4 keys each). Rounding p to the cache's type costs each weight half a
-// step, as much as the rounding of the output; its sum is taken before the rounding.
+// step, about as much as the rounding of the output; the rounded weights are summed, so equal values come out exactly.
 //
 // K and V come in 32-key tiles straight from HBM into LDS (16 bytes a lane, no registers), a tile ahead
 // of the products. 16-byte pieces are permuted inside a row as they arrive (swizzled), so that the 16 keys
@@ -98,12 +98,14 @@ __device__ __forceinline__ bool seq_of(const ChunkArgs& a, int b, bool reports, 
   return ok;
 }
 
-// 16-byte piece p of a tile's key `key` lies at piece p ^ swizzle(key) of the key's row in LDS. K is read as one piece of 16
-// consecutive keys: 8 of them differ in the low three bits, so they cover 128 bytes of banks. V is read as two neighbouring
-// pieces of 4 consecutive keys: these differ in the two bits above the lowest.
+// 16-byte piece p of a tile's key `key` lies at piece p ^ swizzle(key) of the key's row in LDS, so that the banks (64 of 4
+// bytes) are each met once a clock: a read of K takes one piece of 16 keys, 16 lanes a clock (quads of lanes 0, 3 of one lane
+// group and 1, 2 of the next); one of V two neighbouring pieces of 8 consecutive keys. The first asks for distinct
+// swizzle(key) ^ group, the second for distinct swizzle(key) / 2 (at D = 64 with the key's lowest bit above, which picks
+// the half of the 256 bytes). No conflicts counted; with key & 15 a quarter of the reading clocks.
 template <int D>
 __device__ __forceinline__ int swizzle(int key) {
-  return (key & 3) << 1 | ((key >> 2) & 1) | (D == 128 ? key & 8 : 0);
+  return D == 128 ? (key & 7) << 1 ^ (key & 8 ? 9 : 0) : (key & 6) ^ (key & 8 ? 5 : 0);
 }
 
 // Zeros in place of the infinities and NaN among a wave's `pieces` 16-byte pieces of V in LDS; whether there were any (uniform).
@@ -275,7 +277,8 @@ template <int D, int NT, int KS, typename T>
 struct Rows {
   u32x4 q[NT][D / 32];
   f32x4 o[NT][D / 16];
-  float m[NT], mthr[NT], l[NT];
+  f32x4 l[NT];  // sum of the weights, four times
+  float m[NT], mthr[NT];
   int qpos[NT];
   int lo, hi;  // positions of the first and last row (uniform)
 
@@ -296,7 +299,7 @@ struct Rows {
       qpos[n] = s.start + t;
       m[n] = -FLT_MAX;
       mthr[n] = -FLT_MAX;
-      l[n] = 0.f;
+      l[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     lo = __builtin_amdgcn_readfirstlane(s.start + min(r0, last) / a.group);
     hi = __builtin_amdgcn_readfirstlane(s.start + min(r0 + kTileRows * NT - 1, last) / a.group);
@@ -386,17 +389,26 @@ struct Rows {
     }
   }
 
-  // The weights of keys 16 h + 0..15, added to the rows' sums.
+  // The weights of keys 16 h + 0..15.
   __device__ __forceinline__ void weights(const ChunkArgs& a, int h, const f32x4 (&s)[NT], Weights& w) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float p[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], a.c, -m[n]));
-      l[n] += (p[0] + p[1]) + (p[2] + p[3]);
       w[h / 2][n][2 * (h % 2)] = pack2<T>(p[0], p[1]);
       w[h / 2][n][2 * (h % 2) + 1] = pack2<T>(p[2], p[3]);
     }
+  }
+
+  // Adds the weights to their rows' sums, by a product with ones: on the matrix cores, which have the time (4 instructions
+  // for 32 additions and their joining across lanes), and of the rounded weights that meet V.
+  __device__ __forceinline__ void sums(const Weights& w) {
+    const u32x4 ones = {T::kOnes, T::kOnes, T::kOnes, T::kOnes};
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) l[n] = T::mfma(ones, w[k][n], l[n]);
   }
 
   // Four dim tiles' V at a time, the next four's on their way.
@@ -459,14 +471,6 @@ struct Rows {
     const int lane = threadIdx.x & (kWave - 1), i = lane & 15, g = lane >> 4;
     const int key = 4 * g + (i >> 2), piece = 2 * d + ((i >> 1) & 1);
     return (Lds)(s_v + key * D + 8 * (piece ^ swizzle<D>(key)) + 4 * (i & 1));
-  }
-
-  // The four lanes of a row have its maximum; each has the weights of its own keys.
-  __device__ __forceinline__ float weight_sum(int n) const {
-    float sum = l[n];
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    return sum;
   }
 };
 
@@ -575,6 +579,7 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
     w.weights(a, 1, sc[1], wt);
     wait_loads<3 * J>();
     if (w.masked(kt)) dirty |= clean_values<T>(s_v, kTileElems / 8);
+    w.sums(wt);
     w.values_beside_loads(s_v, wt);
     wait_reads();
     load.start(s_v, a.kv_stride);
@@ -596,7 +601,7 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
   static_assert(kTileRows * NT * D * 4 <= kWaves * kTileElems * 2, "a wave's sums fit one array");
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float l = w.weight_sum(n);
+    const float l = w.l[n][0];
     const int r = kTileRows * n + i;
     if (g == 0) {
       s_ml[wave][r][0] = w.m[n];
@@ -734,6 +739,7 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
         for (int n = 0; n < NT; ++n) sc[h][n] = sn[n];
         __builtin_amdgcn_sched_barrier(0);
       }
+      w.sums(wt);
       w.values(v_this, wt);
     }
   };
@@ -746,7 +752,7 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
   if (!has_rows) return;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float l = w.weight_sum(n);
+    const float l = w.l[n][0];
     const int r = wr0 + kTileRows * n + i;
     if (r >= total) continue;
     const int t = r / a.group, h = kvh * a.group + r - t * a.group;
