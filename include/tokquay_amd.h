@@ -556,7 +556,7 @@ size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_heads, int32_
  * j with w_j > 0 where rounding leaves none). Weights and sums are fp64. With
  * independent uniform numbers and drafts drawn from q the tokens are distributed as the target's own. A sequence of no rows gets r = 0 and only -1.
  *
- * logits: [num_rows, vocab] of dtype (tq_dtype), row stride logits_row_stride; -inf masks a token. draft_probs:
+ * logits: [num_rows, vocab] of dtype (tq_dtype), vocab at most 2^21, row stride logits_row_stride; -inf masks a token. draft_probs:
  * fp32 [num_rows, vocab], row stride probs_row_stride (rows of no drafted token, the last ones, are not read).
  * A row of a sequence with a temperature that holds a NaN or +inf, or nothing above -inf, has no distribution: it is
  * taken greedily and sets TQ_DEVERR_VALUE if the sequence came to it. A drafted token outside [0, vocab) sets

@@ -208,7 +208,7 @@ def verify_call(tokens=P, accepted=P, logits=P, ls=90, probs=None, ps=90, drafts
 
 @pytest.mark.parametrize("status,more", [
     (INVALID, dict(seqs=-1)), (INVALID, dict(rows=-1)), (INVALID, dict(mr=-1)), (INVALID, dict(vocab=0)),
-    (UNSUPPORTED, dict(dtype=5)), (UNSUPPORTED, dict(vocab=(1 << 30) + 1)), (OK, dict(seqs=0)), (INVALID, dict(mr=0)),
+    (UNSUPPORTED, dict(dtype=5)), (UNSUPPORTED, dict(vocab=(1 << 21) + 1)), (OK, dict(seqs=0)), (INVALID, dict(mr=0)),
     (INVALID, dict(tokens=None)), (INVALID, dict(accepted=None)), (INVALID, dict(logits=None)), (INVALID, dict(drafts=None)),
     (INVALID, dict(u=None)), (INVALID, dict(temp=None)), (INVALID, dict(cu=None)), (INVALID, dict(ls=89)),
     (INVALID, dict(probs=P, ps=89)), (WORKSPACE, dict(ws=None)), (WORKSPACE, dict(wb=8)), (WORKSPACE, dict(ws=P + 8)),

@@ -467,7 +467,8 @@ void verify_drafts(at::Tensor tokens, at::Tensor accepted, const at::Tensor& log
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && dtype_of(logits.scalar_type()) >= 0, op,
               ": logits must be a float32, float16 or bfloat16 [rows, vocab] tensor on a HIP device");
   const int64_t rows = logits.size(0), vocab = logits.size(1), n = temperature.numel();
-  TORCH_CHECK(rows <= INT32_MAX && vocab >= 1 && vocab <= 1 << 30 && n <= INT32_MAX, op, ": sizes out of range");
+  TORCH_CHECK(rows <= INT32_MAX && vocab >= 1 && vocab <= 1 << 21 && n <= INT32_MAX, op,
+              ": logits must have 1 to 2097152 columns");
   const int64_t ls = vocab_rows_of(op, "logits", logits, rows, vocab);
   const auto vector = [&](const char* name, const at::Tensor& t, at::ScalarType type, int64_t entries) {
     TORCH_CHECK(t.device() == logits.device() && t.scalar_type() == type && t.dim() == 1 && t.is_contiguous() &&

@@ -11,11 +11,11 @@
 // close: exponentials and sums are fp64 (fp64 FMAs run at the fp32 rate here), which also makes the order of a sum
 // not matter. Two launches:
 //
-// 1. stats: one workgroup per row and kChunk columns keeps its logits in registers and leaves their maximum, its
-//    lowest column and their sum of exponentials. The logits are read once: HBM bound.
-// 2. draw: one workgroup per sequence and kChunk columns joins the rows' statistics, finds the first token that
-//    does not stand and sums its chunk's weights of that row; the last workgroup of a sequence to finish
-//    finds the chunk the draw falls in, and the column in it.
+// 1. stats: one workgroup per row and chunk of columns keeps its logits in registers and leaves their maximum and their
+//    sum of exponentials. The logits are read once: HBM bound.
+// 2. draw: one workgroup per sequence and chunk joins the rows' statistics, finds the first token that does not
+//    stand and sums its chunk's weights of that row; the last workgroup of a sequence to finish finds the chunk the draw
+//    falls in, and the column in it.
 
 #include <float.h>
 
@@ -25,12 +25,11 @@ namespace tq {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 32;                 // columns of a thread
-constexpr int kChunk = kThreads * kPer;  // columns of a workgroup
+constexpr int kWaves = kThreads / kWave;
 
 struct Stat {  // of one row's chunk
   double sum;      // of exp((logit - max) / T); 0 at T = 0
-  uint64_t key;    // argmax_key of its largest logit
+  uint64_t key;    // argmax_key of its largest logit (the column: where T = 0 or the maximum is not finite)
 };
 
 struct VerifyArgs {
@@ -55,25 +54,27 @@ struct VerifyArgs {
   int32_t chunks;
 };
 
-// e^x for x <= 0 (0 for NaN): 2^k 2^f, the second factor by its Taylor series (|f ln 2| < 0.35: the first term left
-// out is below 7e-15).
-__device__ __forceinline__ double exp_neg(double x) {
-  const double t = __builtin_fmax(x * 1.4426950408889634, -1100.0);  // below it: 0
-  const double k = __builtin_rint(t);
-  const double f = (t - k) * 0.6931471805599453;
-  double r = 2.505210838544172e-08;                // 1 / 11!
-  r = __builtin_fma(r, f, 2.755731922398589e-07);  // 1 / 10!
-  r = __builtin_fma(r, f, 2.755731922398589e-06);
-  r = __builtin_fma(r, f, 2.48015873015873e-05);
-  r = __builtin_fma(r, f, 1.984126984126984e-04);
-  r = __builtin_fma(r, f, 1.388888888888889e-03);
-  r = __builtin_fma(r, f, 8.333333333333333e-03);
-  r = __builtin_fma(r, f, 4.1666666666666664e-02);
-  r = __builtin_fma(r, f, 1.6666666666666666e-01);
-  r = __builtin_fma(r, f, 0.5);
+// 2^t for t <= 0: 2^k 2^f with k the nearest integer (read off the low bits of t + 1.5 2^52), the second factor by its Taylor
+// series (|f ln 2| < 0.35: the first term left out is below 3e-13). Below -1000, and for NaN: 2^-1000, which no sum of theirs
+// notices.
+__device__ __forceinline__ double exp2_neg(double t) {
+  t = __builtin_fmax(t, -1000.0);
+  const double shifted = t + 0x1.8p52;
+  const double f = t - (shifted - 0x1.8p52);
+  double r = 7.054911620801121e-09;  // ln(2)^10 / 10!
+  r = __builtin_fma(r, f, 1.0178086009239696e-07);
+  r = __builtin_fma(r, f, 1.3215486790144305e-06);
+  r = __builtin_fma(r, f, 1.525273380405984e-05);
+  r = __builtin_fma(r, f, 1.540353039338161e-04);
+  r = __builtin_fma(r, f, 1.3333558146428441e-03);
+  r = __builtin_fma(r, f, 9.618129107628477e-03);
+  r = __builtin_fma(r, f, 5.5504108664821576e-02);
+  r = __builtin_fma(r, f, 2.402265069591007e-01);
+  r = __builtin_fma(r, f, 6.931471805599453e-01);
   r = __builtin_fma(r, f, 1.0);
-  r = __builtin_fma(r, f, 1.0);
-  return __builtin_ldexp(r, (int)k);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, r);
+  const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, shifted);
+  return __builtin_bit_cast(double, bits + ((uint64_t)k << 52));
 }
 
 template <typename T>
@@ -102,6 +103,33 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
+// PER columns of a chunk as floats, columns past n as -inf. Thread t has the 16-byte pieces t, t + 256, .. (RUNS false) or
+// PER columns in a row (true), in order. Rows start at any element.
+template <typename T, int PER, bool RUNS, typename F>
+__device__ __forceinline__ void columns(const void* row, int base, int n, F&& put) {
+  constexpr int kVec = __is_same(T, float) ? 4 : 8;
+#pragma unroll
+  for (int v = 0; v < PER / kVec; ++v) {
+    const int at = RUNS ? (int)threadIdx.x * PER + v * kVec : (v * kThreads + (int)threadIdx.x) * kVec;
+    if (at + kVec <= n) {
+      u32x4 w;
+      __builtin_memcpy(&w, static_cast<const char*>(row) + (int64_t)(base + at) * (16 / kVec), 16);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        if constexpr (__is_same(T, float))
+          put(v * kVec + e, at + e, __uint_as_float(w[e]));
+        else
+          put(v * kVec + e, at + e, T::load((uint16_t)(w[e / 2] >> (16 * (e & 1)))));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) put(v * kVec + e, at + e, at + e < n ? logit_at<T>(row, base + at + e) : -INFINITY);
+    }
+  }
+}
+
+constexpr double kLog2e = 1.4426950408889634;
+
 // The sequence that a row belongs to: the last with cu[b] <= row (empty sequences hold no row).
 __device__ __forceinline__ int sequence_of(const VerifyArgs& a, int row) {
   int lo = 0, hi = a.num_seqs;  // cu[lo] <= row < cu[hi]
@@ -115,106 +143,152 @@ __device__ __forceinline__ int sequence_of(const VerifyArgs& a, int row) {
   return lo;
 }
 
-template <typename T>
+template <typename T, int PER>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs a) {
-  __shared__ uint64_t s_key[kThreads / kWave];
-  __shared__ double s_sum[kThreads / kWave];
+  __shared__ float s_top[kWaves];
+  __shared__ double s_sum[kWaves];
+  __shared__ int s_col;
   const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks;
   if (row < a.num_seqs && chunk == 0 && threadIdx.x == 0) a.arrived[row] = 0;  // for the second launch
   if (row >= a.num_rows) return;
-  const int b = sequence_of(a, row);
-  const float temp = a.temperature[b];
-  const void* lp = row_of<T>(a, row);
-  const int base = chunk * kChunk, n = min(kChunk, a.vocab - base);
-  float x[kPer];
-  uint64_t key = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int j = i * kThreads + threadIdx.x;
-    x[i] = j < n ? logit_at<T>(lp, base + j) : -INFINITY;
-    if (j < n) key = max_u64(key, argmax_key(x[i], base + j));
-  }
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int base = chunk * kThreads * PER, n = min(kThreads * PER, a.vocab - base);
+  float x[PER], top = -INFINITY;
+  const void* lp = row_of<T>(a, row);
+  columns<T, PER, false>(lp, base, n, [&](int i, int, float v) { x[i] = v; });
+  const float temp = a.temperature[sequence_of(a, row)];
 #pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) key = max_u64(key, __shfl_xor(key, off));
-  if (lane == 0) s_key[wave] = key;
+  for (int i = 0; i < PER; ++i) top = __builtin_elementwise_maximum(top, x[i]);  // NaN, if any is
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, off));
+  if (lane == 0) s_top[wave] = top;
+  if (threadIdx.x == 0) s_col = 0x7fffffff;
   __syncthreads();
 #pragma unroll
-  for (int v = 0; v < kThreads / kWave; ++v) key = max_u64(key, s_key[v]);
-  const float top = key_value(key);
+  for (int v = 0; v < kWaves; ++v) top = __builtin_elementwise_maximum(top, s_top[v]);
   double sum = 0.0;
-  if (temp > 0.f && top > -INFINITY && top < INFINITY) {  // else no distribution, or none needed
-    const double inv = 1.0 / (double)temp;
+  int col = 0;
+  if (temp > 0.f && top > -INFINITY && top < INFINITY) {  // uniform
+    const double c = kLog2e / (double)temp, t0 = (double)top;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) sum += exp_neg(((double)x[i] - (double)top) * inv);
+    for (int i = 0; i < PER; ++i) sum += exp2_neg(((double)x[i] - t0) * c);
+    sum = wave_sum(sum);
+    if (lane == 0) s_sum[wave] = sum;
+  } else {  // no distribution, or none needed: the first column that holds the maximum
+    constexpr int kVec = __is_same(T, float) ? 4 : 8;
+    int mine = 0x7fffffff;
+#pragma unroll
+    for (int i = PER - 1; i >= 0; --i) {
+      const int at = (i / kVec * kThreads + (int)threadIdx.x) * kVec + i % kVec;
+      if (at < n && (top != top ? x[i] != x[i] : x[i] == top)) mine = at;
+    }
+    atomicMin(&s_col, mine);
+    if (lane == 0) s_sum[wave] = 0.0;
   }
-  sum = wave_sum(sum);
-  if (lane == 0) s_sum[wave] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
+    sum = s_sum[0];
 #pragma unroll
-    for (int v = 1; v < kThreads / kWave; ++v) sum += s_sum[v];
-    a.stats[(int64_t)row * a.chunks + chunk] = Stat{sum, key};
+    for (int v = 1; v < kWaves; ++v) sum += s_sum[v];
+    if (s_col != 0x7fffffff) col = s_col;
+    a.stats[(int64_t)row * a.chunks + chunk] = Stat{sum, argmax_key(top, base + col)};
   }
 }
 
-// A row's distribution: exp((logit - top) / T) / sum, or all of it on column best.
+// A row's distribution: 2^((logit - top) c) / sum, or all of it on column best.
 struct Dist {
-  double sum, inv;
-  float top;
+  double sum, c;
   int64_t best;
+  float top;
   bool peak;
 };
 
+// By one wave; every lane gets it.
 __device__ __forceinline__ Dist dist_of(const VerifyArgs& a, int row, float temp) {
   const Stat* st = a.stats + (int64_t)row * a.chunks;
+  const int lane = threadIdx.x & (kWave - 1);
   uint64_t key = 0;
-  for (int c = 0; c < a.chunks; ++c) key = max_u64(key, st[c].key);
+  for (int c = lane; c < a.chunks; c += kWave) key = max_u64(key, st[c].key);
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) key = max_u64(key, __shfl_xor(key, off));
   Dist d;
   d.top = key_value(key);
   d.best = argmax_key_column(key);
-  d.inv = 1.0 / (double)temp;
+  d.c = kLog2e / (double)temp;
   d.peak = !(temp > 0.f) || !(d.top > -INFINITY && d.top < INFINITY);
   d.sum = 0.0;
   if (!d.peak) {
-    for (int c = 0; c < a.chunks; ++c) {
+    for (int c = lane; c < a.chunks; c += kWave) {
       const float m = key_value(st[c].key);
-      if (m > -INFINITY) d.sum += st[c].sum * exp_neg(((double)m - (double)d.top) * d.inv);
+      if (m > -INFINITY) d.sum += st[c].sum * exp2_neg(((double)m - (double)d.top) * d.c);
     }
+    d.sum = wave_sum(d.sum);
   }
   return d;
 }
 
-// p of column j, times sum (the draw needs no division).
-template <typename T>
-__device__ __forceinline__ double mass_at(const Dist& d, const void* row, int64_t j) {
-  if (d.peak) return j == d.best ? 1.0 : 0.0;
-  return exp_neg(((double)logit_at<T>(row, j) - (double)d.top) * d.inv);
+// p of a column, times sum (the draw needs no division). A logit of -inf has none.
+__device__ __forceinline__ double mass_of(const Dist& d, float logit, int64_t col) {
+  if (d.peak) return col == d.best ? 1.0 : 0.0;
+  const double t = ((double)logit - (double)d.top) * d.c;
+  return t >= -1000.0 ? exp2_neg(t) : 0.0;
 }
 
-// The draw's weight of column j: all of p's (mode 0), p - q where positive (1), p without the draft (2). Times d.sum.
-template <typename T>
-__device__ __forceinline__ double weight_at(const Dist& d, const void* row, const float* qrow, int64_t draft, int mode,
-                                            int64_t j) {
-  const double p = mass_at<T>(d, row, j);
-  if (mode == 0) return p;
-  if (mode == 2) return j == draft ? 0.0 : p;
-  const double w = d.peak ? p - (double)qrow[j] : p - (double)qrow[j] * d.sum;
+enum Mode { kAll, kLess, kWithout };  // the draw is from p, from p - q where positive, from p without the draft
+
+// The draw's weight of a column, times sum.
+__device__ __forceinline__ double weight_of(const Dist& d, float logit, double q, int64_t draft, int mode, int64_t col) {
+  const double p = mass_of(d, logit, col);
+  if (mode == kAll) return p;
+  if (mode == kWithout) return col == draft ? 0.0 : p;
+  const double w = p - (d.peak ? q : q * d.sum);
   return w > 0.0 ? w : 0.0;
 }
 
-template <typename T>
+// The weights of PER columns of a chunk.
+template <typename T, int PER, bool RUNS, typename F>
+__device__ __forceinline__ void weights(const Dist& d, const void* row, const float* qrow, int64_t draft, int mode,
+                                        int base, int n, F&& put) {
+  float x[PER];
+  columns<T, PER, RUNS>(row, base, n, [&](int i, int, float v) { x[i] = v; });
+  constexpr int kVec = __is_same(T, float) ? 4 : 8;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = RUNS ? (int)threadIdx.x * PER + i : (i / kVec * kThreads + (int)threadIdx.x) * kVec + i % kVec;
+    const double q = mode == kLess && at < n ? (double)qrow[base + at] : 0.0;
+    put(i, at < n ? weight_of(d, x[i], q, draft, mode, base + at) : 0.0);
+  }
+}
+
+// Inclusive sums over the workgroup's threads, in order; s_part: a word a wave.
+__device__ __forceinline__ double scan(double v, double* s_part) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const double up = __shfl_up(v, off);
+    if (lane >= off) v += up;
+  }
+  if (lane == kWave - 1) s_part[wave] = v;
+  __syncthreads();
+  double before = 0.0;
+  for (int u = 0; u < wave; ++u) before += s_part[u];
+  __syncthreads();
+  return before + v;
+}
+
+template <typename T, int PER>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs a) {
-  __shared__ int s_first, s_bad;
+  __shared__ int s_first, s_bad, s_turn;
   __shared__ Dist s_dist;
-  __shared__ double s_sum[kThreads];
-  __shared__ int s_last;
+  __shared__ double s_part[kWaves], s_goal;
+  constexpr int kChunk = kThreads * PER;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int chunk = blockIdx.x % a.chunks, b = blockIdx.x / a.chunks;
   const int lo = a.cu[b];
   const int64_t rows64 = (int64_t)a.cu[b + 1] - lo;
   int64_t* out = a.tokens + (int64_t)b * a.max_rows;
   const bool lead = chunk == 0;
-  if (lo < 0 || rows64 < 0 || lo + rows64 > a.num_rows || rows64 > a.max_rows || rows64 == 0) {
+  if (lo < 0 || rows64 <= 0 || lo + rows64 > a.num_rows || rows64 > a.max_rows) {
     if (lead) {
       if (rows64 != 0 && threadIdx.x == 0) flag_error(a.d_error, TQ_DEVERR_LENGTH);
       for (int i = threadIdx.x; i < a.max_rows; i += kThreads) out[i] = -1;
@@ -222,158 +296,161 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs 
     }
     return;
   }
-  const int rows = (int)rows64, drafts = rows - 1;
+  const int drafts = (int)rows64 - 1;
   const float temp = a.temperature[b];
   if (threadIdx.x == 0) {
     s_first = drafts;
-    s_bad = rows;
+    s_bad = drafts + 1;
   }
   __syncthreads();
-  // The first drafted token that does not stand.
-  for (int i = threadIdx.x; i < drafts; i += kThreads) {
+  // The first drafted token that does not stand: a wave a row. (Rows behind one that does not are left out.)
+  for (int i = wave; i <= drafts && i <= *(volatile int*)&s_first; i += kWaves) {
     const Dist d = dist_of(a, lo + i, temp);
+    if (d.peak && temp > 0.f && lane == 0) atomicMin(&s_bad, i);
+    if (i == drafts) break;
     const int64_t x = a.drafts[lo + i];
-    const bool in = x >= 0 && x < a.vocab;
-    if (!in && lead) flag_error(a.d_error, TQ_DEVERR_TOKEN);
     bool stands = false;
-    if (in) {
-      const double p = d.peak ? (x == d.best ? 1.0 : 0.0) : mass_at<T>(d, row_of<T>(a, lo + i), x) / d.sum;
+    if (x >= 0 && x < a.vocab) {
+      const double p = d.peak ? (x == d.best ? 1.0 : 0.0) : mass_of(d, logit_at<T>(row_of<T>(a, lo + i), x), x) / d.sum;
       const double q = a.probs == nullptr ? 1.0 : (double)a.probs[(int64_t)(lo + i) * a.probs_stride + x];
       stands = (double)a.uniforms[lo + i] * q < p;
     }
-    if (!stands) atomicMin(&s_first, i);
-    if (d.peak && temp > 0.f) atomicMin(&s_bad, i);
+    if (!stands && lane == 0) atomicMin(&s_first, i);
   }
   __syncthreads();
   const int first = s_first, row = lo + first;
-  if (threadIdx.x == 0) {
-    s_dist = dist_of(a, row, temp);
-    if (lead && temp > 0.f && (s_dist.peak || s_bad < first)) flag_error(a.d_error, TQ_DEVERR_VALUE);
+  if (wave == 0) {
+    const Dist d = dist_of(a, row, temp);
+    if (lane == 0) s_dist = d;
+  }
+  if (lead) {
+    for (int i = threadIdx.x; i < a.max_rows; i += kThreads)
+      if (i != first) out[i] = i < first ? a.drafts[lo + i] : -1;
+    if (threadIdx.x == 0) {
+      a.accepted[b] = first;
+      if (s_bad <= first) flag_error(a.d_error, TQ_DEVERR_VALUE);
+      if (first < drafts && (a.drafts[row] < 0 || a.drafts[row] >= a.vocab)) flag_error(a.d_error, TQ_DEVERR_TOKEN);
+    }
   }
   __syncthreads();
   const Dist d = s_dist;
   const void* lp = row_of<T>(a, row);
   const float* qrow = a.probs == nullptr ? nullptr : a.probs + (int64_t)row * a.probs_stride;
   const int64_t draft = first < drafts ? a.drafts[row] : -1;
-  int mode = first == drafts ? 0 : a.probs != nullptr ? 1 : 2;
-  if (lead) {
-    for (int i = threadIdx.x; i < a.max_rows; i += kThreads)
-      if (i != first) out[i] = i < first ? a.drafts[lo + i] : -1;
-    if (threadIdx.x == 0) a.accepted[b] = first;
-  }
-  // This chunk's weights, a run of kPer columns a thread.
-  const int base = chunk * kChunk + threadIdx.x * kPer;
+  int mode = first == drafts ? kAll : qrow != nullptr ? kLess : kWithout;
+  const int base = chunk * kChunk, n = min(kChunk, a.vocab - base);
   double w = 0.0;
-  for (int i = 0; i < kPer; ++i)
-    if (base + i < a.vocab) w += weight_at<T>(d, lp, qrow, draft, mode, base + i);
+  weights<T, PER, false>(d, lp, qrow, draft, mode, base, n, [&](int, double v) { w += v; });
   w = wave_sum(w);
-  if (threadIdx.x % kWave == 0) s_sum[threadIdx.x / kWave] = w;
+  if (lane == 0) s_part[wave] = w;
   __syncthreads();
+  double* sums = a.sums + (int64_t)b * a.chunks;
   if (threadIdx.x == 0) {
-    double total = s_sum[0];
-    for (int v = 1; v < kThreads / kWave; ++v) total += s_sum[v];
-    __hip_atomic_store(&a.sums[(int64_t)b * a.chunks + chunk], total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_last = __hip_atomic_fetch_add(&a.arrived[b], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
-             (uint32_t)a.chunks - 1;
+    for (int v = 1; v < kWaves; ++v) w += s_part[v];
+    __hip_atomic_store(&sums[chunk], w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s_turn = (int)__hip_atomic_fetch_add(&a.arrived[b], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  if (!s_last) return;
+  if (s_turn != a.chunks - 1) return;
 
-  // The last workgroup of the sequence: the chunk, then the thread's run, then the column.
-  __shared__ double s_goal;
-  __shared__ int s_chunk;
-  const double u = (double)a.uniforms[lo + drafts];
-  if (threadIdx.x == 0) {
-    double total = 0.0;
-    for (int c = 0; c < a.chunks; ++c)
-      total += __hip_atomic_load(&a.sums[(int64_t)b * a.chunks + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_chunk = -1;
-    s_goal = u * total;
-    if (total > 0.0) {
-      double before = 0.0;
-      int pick = -1;
-      double pick_before = 0.0;
-      for (int c = 0; c < a.chunks; ++c) {
-        const double part =
-            __hip_atomic_load(&a.sums[(int64_t)b * a.chunks + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (part > 0.0) {  // the last one with weight, should rounding leave none above the goal
-          pick = c;
-          pick_before = before;
-        }
-        before += part;
-        if (part > 0.0 && before > s_goal) break;
-      }
-      s_chunk = pick;
-      s_goal -= pick_before;
+  // The last workgroup of the sequence: the chunk that the draw falls in (the last one with weight where rounding
+  // leaves none above the goal), a chunk a thread.
+  const int c = threadIdx.x;
+  double mine = c < a.chunks ? __hip_atomic_load(&sums[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+  double upto = scan(mine, s_part);
+  if (c == kThreads - 1) s_goal = upto;
+  __syncthreads();
+  if (!(s_goal > 0.0)) {
+    // Nothing left where q covers p (to rounding): the draw is from p itself, whose chunks' sums the statistics have.
+    mode = kAll;
+    mine = 0.0;
+    if (c < a.chunks) {
+      const Stat st = a.stats[(int64_t)row * a.chunks + c];
+      const float m = key_value(st.key);
+      if (d.peak)
+        mine = c == (int)(d.best / kChunk) ? 1.0 : 0.0;
+      else if (m > -INFINITY)
+        mine = st.sum * exp2_neg(((double)m - (double)d.top) * d.c);
     }
+    upto = scan(mine, s_part);
+    if (c == kThreads - 1) s_goal = upto;
+    __syncthreads();
+  }
+  const double goal = (double)a.uniforms[lo + drafts] * s_goal;
+  if (c == 0) s_first = 0x7fffffff, s_turn = -1;
+  __syncthreads();
+  if (mine > 0.0) {
+    if (upto > goal) atomicMin(&s_first, c);
+    atomicMax(&s_turn, c);
   }
   __syncthreads();
-  int c0 = s_chunk, c1 = c0 + 1;
-  double goal = s_goal;
-  bool whole = false;
-  if (c0 < 0) {
-    // Nothing left where q covers p (to rounding): the draw is from p itself, over all chunks.
-    mode = 0;
-    c0 = 0;
-    c1 = a.chunks;
-    whole = true;
-    goal = d.peak ? u : u * d.sum;
+  const int chosen = s_first != 0x7fffffff ? s_first : s_turn;
+  if (chosen < 0) {  // no weight anywhere: draft probabilities that are not numbers
+    if (c == 0) out[first] = d.best;
+    return;
   }
-  __shared__ int64_t s_token;
-  for (int c = c0; c < c1; ++c) {
-    const int at = c * kChunk + threadIdx.x * kPer;
-    double run = 0.0;
-    for (int i = 0; i < kPer; ++i)
-      if (at + i < a.vocab) run += weight_at<T>(d, lp, qrow, draft, mode, at + i);
-    s_sum[threadIdx.x] = run;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      double before = 0.0;
-      int64_t token = -1;
-      for (int v = 0; v < kThreads && token < 0; ++v) {
-        if (!(s_sum[v] > 0.0)) continue;
-        // The column: inside this run if the goal falls in it; the last weighted column where the chunk ends first.
-        double cum = before;
-        int64_t lastw = -1;
-        const int from = c * kChunk + v * kPer;
-        const bool inside = before + s_sum[v] > goal;
-        bool more = false;
-        for (int vv = v + 1; vv < kThreads && !more; ++vv) more = s_sum[vv] > 0.0;
-        if (inside || (!more && (!whole || c == c1 - 1))) {
-          for (int i = 0; i < kPer && from + i < a.vocab; ++i) {
-            const double wi = weight_at<T>(d, lp, qrow, draft, mode, from + i);
-            if (!(wi > 0.0)) continue;
-            cum += wi;
-            lastw = from + i;
-            if (cum > goal) break;
-          }
-          token = lastw;
-        }
-        before += s_sum[v];
+  if (c == chosen) s_goal = goal - (upto - mine);
+  __syncthreads();
+  const double rest = s_goal;
+  // The column in it: runs of PER columns a thread.
+  const int at = chosen * kChunk, m = min(kChunk, a.vocab - at);
+  double ws[PER], run = 0.0;
+  weights<T, PER, true>(d, lp, qrow, draft, mode, at, m, [&](int i, double v) {
+    ws[i] = v;
+    run += v;
+  });
+  upto = scan(run, s_part);
+  if (c == 0) s_first = 0x7fffffff, s_turn = -1;
+  __syncthreads();
+  if (run > 0.0) {
+    if (upto > rest) atomicMin(&s_first, c);
+    atomicMax(&s_turn, c);
+  }
+  __syncthreads();
+  if (c == (s_first != 0x7fffffff ? s_first : s_turn)) {
+    double cum = upto - run;
+    int token = -1;
+    bool done = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      cum += ws[i];
+      if (!done && ws[i] > 0.0) {
+        token = at + (int)threadIdx.x * PER + i;
+        done = cum > rest;
       }
-      s_token = token;
-      s_goal = goal - before;
     }
-    __syncthreads();
-    if (s_token >= 0) break;
-    goal = s_goal;
-    __syncthreads();
+    out[first] = token;
   }
-  if (threadIdx.x == 0) out[first] = s_token >= 0 ? s_token : d.best;
 }
 
-int64_t chunks_of(int32_t vocab) { return ((int64_t)vocab + kChunk - 1) / kChunk; }
+constexpr int kMaxVocab = kThreads * kThreads * 32;  // a chunk a thread
 
-template <typename T>
+// Columns of a thread: 32, or 8 where the rows' chunks would leave CUs without one (a row's chunk of 8,192 columns takes one 4 us).
+int per_of(int64_t num_rows, int64_t vocab) {
+  const bool few = num_rows * ((vocab + kThreads * 32 - 1) / (kThreads * 32)) < 512;
+  return few && vocab <= kThreads * kThreads * 8 ? 8 : 32;
+}
+
+int64_t chunks_of(int64_t num_rows, int64_t vocab) {
+  const int64_t chunk = (int64_t)kThreads * per_of(num_rows, vocab);
+  return (vocab + chunk - 1) / chunk;
+}
+
+template <typename T, int PER>
 tq_status launch(const VerifyArgs& a, hipStream_t stream) {
   const int64_t rows = a.num_rows > a.num_seqs ? a.num_rows : a.num_seqs;
   const int64_t stats = rows * a.chunks, draw = (int64_t)a.num_seqs * a.chunks;
   if (stats > 0x7fffffffLL || draw > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((verify_stats_kernel<T>), dim3((unsigned)stats), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((verify_stats_kernel<T, PER>), dim3((unsigned)stats), dim3(kThreads), 0, stream, a);
   const tq_status st = check_launch();
   if (st != TQ_OK) return st;
-  hipLaunchKernelGGL((verify_draw_kernel<T>), dim3((unsigned)draw), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((verify_draw_kernel<T, PER>), dim3((unsigned)draw), dim3(kThreads), 0, stream, a);
   return check_launch();
+}
+
+template <typename T>
+tq_status launch(const VerifyArgs& a, hipStream_t stream) {
+  return per_of(a.num_rows, a.vocab) == 8 ? launch<T, 8>(a, stream) : launch<T, 32>(a, stream);
 }
 
 }  // namespace
@@ -381,8 +458,8 @@ tq_status launch(const VerifyArgs& a, hipStream_t stream) {
 
 extern "C" size_t tq_verify_drafts_workspace_size(int32_t num_seqs, int32_t num_rows, int32_t vocab) {
   using namespace tq;
-  if (num_seqs < 1 || num_rows < 0 || vocab < 1) return 0;
-  const size_t chunks = (size_t)chunks_of(vocab);
+  if (num_seqs < 1 || num_rows < 0 || vocab < 1 || vocab > kMaxVocab) return 0;
+  const size_t chunks = (size_t)chunks_of(num_rows, vocab);
   return num_rows * chunks * sizeof(Stat) + num_seqs * chunks * sizeof(double) + num_seqs * sizeof(uint32_t);
 }
 
@@ -394,7 +471,7 @@ extern "C" tq_status tq_verify_drafts(int64_t* tokens, int32_t* accepted, const 
                                       size_t workspace_bytes, int32_t* d_error, void* stream) {
   using namespace tq;
   if (num_seqs < 0 || num_rows < 0 || max_query_len < 0 || vocab < 1) return TQ_ERR_INVALID_ARGUMENT;
-  if ((dtype != TQ_F32 && dtype != TQ_F16 && dtype != TQ_BF16) || vocab > 1 << 30) return TQ_ERR_UNSUPPORTED;
+  if ((dtype != TQ_F32 && dtype != TQ_F16 && dtype != TQ_BF16) || vocab > kMaxVocab) return TQ_ERR_UNSUPPORTED;
   if (num_seqs == 0) return TQ_OK;
   if (max_query_len < 1 || tokens == nullptr || accepted == nullptr || cu_seqlens_q == nullptr ||
       temperature == nullptr || (num_rows > 0 && (logits == nullptr || draft_tokens == nullptr || uniforms == nullptr)) ||
@@ -417,7 +494,7 @@ extern "C" tq_status tq_verify_drafts(int64_t* tokens, int32_t* accepted, const 
   a.num_rows = num_rows;
   a.max_rows = max_query_len;
   a.vocab = vocab;
-  a.chunks = (int32_t)chunks_of(vocab);
+  a.chunks = (int32_t)chunks_of(num_rows, vocab);
   a.stats = static_cast<Stat*>(workspace);
   a.sums = reinterpret_cast<double*>(a.stats + (size_t)num_rows * a.chunks);
   a.arrived = reinterpret_cast<uint32_t*>(a.sums + (size_t)num_seqs * a.chunks);

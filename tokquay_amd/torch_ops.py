@@ -344,8 +344,8 @@ def _fake_verify_drafts(tokens, accepted, logits, draft_probs, draft_tokens, uni
         _fail(op, "logits must be a float32, float16 or bfloat16 [rows, vocab] tensor on a HIP device")
     rows, vocab = logits.shape
     n = temperature.numel()
-    if not 1 <= vocab <= 1 << 30:
-        _fail(op, "sizes out of range")
+    if not 1 <= vocab <= 1 << 21:
+        _fail(op, "logits must have 1 to 2097152 columns")
 
     def vocab_rows(name, t):
         if not (t.dim() == 2 and tuple(t.shape) == (rows, vocab) and (vocab <= 1 or t.stride(1) == 1)):
