@@ -54,23 +54,21 @@ struct VerifyArgs {
   int32_t chunks;
 };
 
-// 2^t for t <= 0: 2^k 2^f with k the nearest integer (read off the low bits of t + 1.5 2^52), the second factor by its Taylor
-// series (|f ln 2| < 0.35: the first term left out is below 3e-13). Below -1000, and for NaN: 2^-1000, which no sum of theirs
-// notices.
+// 2^t for t <= 0: 2^k 2^f with k the nearest integer (read off the low bits of t + 1.5 2^52), the second factor by the polynomial
+// that meets 2^f at 0 and at the 8 Chebyshev points of [-1/2, 1/2]; off by at most 2.2e-12, and 1 for 0, so that equal logits
+// have equal, whole weights. Below -1000, and for NaN: 2^-1000, which no sum of theirs notices.
 __device__ __forceinline__ double exp2_neg(double t) {
   t = __builtin_fmax(t, -1000.0);
   const double shifted = t + 0x1.8p52;
   const double f = t - (shifted - 0x1.8p52);
-  double r = 7.054911620801121e-09;  // ln(2)^10 / 10!
-  r = __builtin_fma(r, f, 1.0178086009239696e-07);
-  r = __builtin_fma(r, f, 1.3215486790144305e-06);
-  r = __builtin_fma(r, f, 1.525273380405984e-05);
-  r = __builtin_fma(r, f, 1.540353039338161e-04);
-  r = __builtin_fma(r, f, 1.3333558146428441e-03);
-  r = __builtin_fma(r, f, 9.618129107628477e-03);
-  r = __builtin_fma(r, f, 5.5504108664821576e-02);
-  r = __builtin_fma(r, f, 2.402265069591007e-01);
-  r = __builtin_fma(r, f, 6.931471805599453e-01);
+  double r = 1.3250805512080399e-06;
+  r = __builtin_fma(r, f, 1.5303700711214572e-05);
+  r = __builtin_fma(r, f, 1.5403475186561525e-04);
+  r = __builtin_fma(r, f, 1.333347847368613e-03);
+  r = __builtin_fma(r, f, 9.618129135236088e-03);
+  r = __builtin_fma(r, f, 5.550410906325866e-02);
+  r = __builtin_fma(r, f, 2.4022650695888503e-01);
+  r = __builtin_fma(r, f, 6.931471805568324e-01);
   r = __builtin_fma(r, f, 1.0);
   const uint64_t bits = __builtin_bit_cast(uint64_t, r);
   const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, shifted);
@@ -103,27 +101,35 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-// PER columns of a chunk as floats, columns past n as -inf. Thread t has the 16-byte pieces t, t + 256, .. (RUNS false) or
-// PER columns in a row (true), in order. Rows start at any element.
-template <typename T, int PER, bool RUNS, typename F>
-__device__ __forceinline__ void columns(const void* row, int base, int n, F&& put) {
-  constexpr int kVec = __is_same(T, float) ? 4 : 8;
+template <typename T>
+constexpr int kVec = __is_same(T, float) ? 4 : 8;  // logits in 16 bytes
+
+// Thread t's column i of a chunk: pieces of VEC columns t, t + 256, .., or (RUNS) PER columns in a row.
+template <int VEC, int PER, bool RUNS>
+__device__ __forceinline__ int column_of(int i) {
+  return RUNS ? (int)threadIdx.x * PER + i : (i / VEC * kThreads + (int)threadIdx.x) * VEC + i % VEC;
+}
+
+// Those columns of a row of T as floats, columns past n as -inf. Rows start at any element.
+template <typename T, int VEC, int PER, bool RUNS>
+__device__ __forceinline__ void columns(const void* row, int base, int n, float (&x)[PER]) {
+  constexpr int kSize = __is_same(T, float) ? 4 : 2;
 #pragma unroll
-  for (int v = 0; v < PER / kVec; ++v) {
-    const int at = RUNS ? (int)threadIdx.x * PER + v * kVec : (v * kThreads + (int)threadIdx.x) * kVec;
-    if (at + kVec <= n) {
-      u32x4 w;
-      __builtin_memcpy(&w, static_cast<const char*>(row) + (int64_t)(base + at) * (16 / kVec), 16);
+  for (int v = 0; v < PER; v += VEC) {
+    const int at = column_of<VEC, PER, RUNS>(v);
+    if (at + VEC <= n) {
+      u32x4 w[VEC * kSize / 16];
+      __builtin_memcpy(w, static_cast<const char*>(row) + (int64_t)(base + at) * kSize, VEC * kSize);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
+      for (int e = 0; e < VEC; ++e) {
         if constexpr (__is_same(T, float))
-          put(v * kVec + e, at + e, __uint_as_float(w[e]));
+          x[v + e] = __uint_as_float(w[e / 4][e % 4]);
         else
-          put(v * kVec + e, at + e, T::load((uint16_t)(w[e / 2] >> (16 * (e & 1)))));
+          x[v + e] = T::load((uint16_t)(w[e / 8][e % 8 / 2] >> (16 * (e & 1))));
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) put(v * kVec + e, at + e, at + e < n ? logit_at<T>(row, base + at + e) : -INFINITY);
+      for (int e = 0; e < VEC; ++e) x[v + e] = at + e < n ? logit_at<T>(row, base + at + e) : -INFINITY;
     }
   }
 }
@@ -155,7 +161,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs
   const int base = chunk * kThreads * PER, n = min(kThreads * PER, a.vocab - base);
   float x[PER], top = -INFINITY;
   const void* lp = row_of<T>(a, row);
-  columns<T, PER, false>(lp, base, n, [&](int i, int, float v) { x[i] = v; });
+  columns<T, kVec<T>, PER, false>(lp, base, n, x);
   const float temp = a.temperature[sequence_of(a, row)];
 #pragma unroll
   for (int i = 0; i < PER; ++i) top = __builtin_elementwise_maximum(top, x[i]);  // NaN, if any is
@@ -175,11 +181,10 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs
     sum = wave_sum(sum);
     if (lane == 0) s_sum[wave] = sum;
   } else {  // no distribution, or none needed: the first column that holds the maximum
-    constexpr int kVec = __is_same(T, float) ? 4 : 8;
     int mine = 0x7fffffff;
 #pragma unroll
     for (int i = PER - 1; i >= 0; --i) {
-      const int at = (i / kVec * kThreads + (int)threadIdx.x) * kVec + i % kVec;
+      const int at = column_of<kVec<T>, PER, false>(i);
       if (at < n && (top != top ? x[i] != x[i] : x[i] == top)) mine = at;
     }
     atomicMin(&s_col, mine);
@@ -245,18 +250,22 @@ __device__ __forceinline__ double weight_of(const Dist& d, float logit, double q
   return w > 0.0 ? w : 0.0;
 }
 
-// The weights of PER columns of a chunk.
+// The weights of a thread's columns of a chunk.
 template <typename T, int PER, bool RUNS, typename F>
 __device__ __forceinline__ void weights(const Dist& d, const void* row, const float* qrow, int64_t draft, int mode,
                                         int base, int n, F&& put) {
-  float x[PER];
-  columns<T, PER, RUNS>(row, base, n, [&](int i, int, float v) { x[i] = v; });
-  constexpr int kVec = __is_same(T, float) ? 4 : 8;
+  float x[PER], q[PER];
+  columns<T, kVec<T>, PER, RUNS>(row, base, n, x);
+  if (mode == kLess) {
+    columns<float, kVec<T>, PER, RUNS>(qrow, base, n, q);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) q[i] = 0.f;
+  }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int at = RUNS ? (int)threadIdx.x * PER + i : (i / kVec * kThreads + (int)threadIdx.x) * kVec + i % kVec;
-    const double q = mode == kLess && at < n ? (double)qrow[base + at] : 0.0;
-    put(i, at < n ? weight_of(d, x[i], q, draft, mode, base + at) : 0.0);
+    const int at = column_of<kVec<T>, PER, RUNS>(i);
+    put(i, at < n ? weight_of(d, x[i], (double)q[i], draft, mode, base + at) : 0.0);
   }
 }
 
