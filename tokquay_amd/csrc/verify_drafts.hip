@@ -95,10 +95,42 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
 }
 
+// Reductions of a wave, through DPP in rows of 16 lanes and lanes 0, 16, 32, 48 (a 64-bit shuffle through LDS takes five times as
+// long, and they lie on the path of a small call). Every lane gets the result; all orders of the lanes give the same.
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_move64(uint64_t v) {
+  const uint32_t lo = __float_as_uint(dpp_move<CTRL>(__uint_as_float((uint32_t)v)));
+  const uint32_t hi = __float_as_uint(dpp_move<CTRL>(__uint_as_float((uint32_t)(v >> 32))));
+  return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (uint64_t)hi << 32 | lo;
+}
+template <typename F>
+__device__ __forceinline__ uint64_t wave_reduce(uint64_t v, F&& join) {
+  v = join(v, dpp_move64<kDppQuadXor1>(v));
+  v = join(v, dpp_move64<kDppQuadXor2>(v));
+  v = join(v, dpp_move64<kDppRowHalfMirror>(v));
+  v = join(v, dpp_move64<kDppRowMirror>(v));
+  return join(join(lane_of(v, 0), lane_of(v, 16)), join(lane_of(v, 32), lane_of(v, 48)));
+}
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off);
-  return v;
+  return __builtin_bit_cast(double, wave_reduce(__builtin_bit_cast(uint64_t, v), [](uint64_t a, uint64_t b) {
+                              return __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, a) + __builtin_bit_cast(double, b));
+                            }));
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+  return wave_reduce(v, [](uint64_t a, uint64_t b) { return max_u64(a, b); });
+}
+__device__ __forceinline__ float wave_maximum(float v) {  // NaN, if any is
+  v = __builtin_elementwise_maximum(v, dpp_move<kDppQuadXor1>(v));
+  v = __builtin_elementwise_maximum(v, dpp_move<kDppQuadXor2>(v));
+  v = __builtin_elementwise_maximum(v, dpp_move<kDppRowHalfMirror>(v));
+  v = __builtin_elementwise_maximum(v, dpp_move<kDppRowMirror>(v));
+  auto lane = [&](int l) { return __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(v), l)); };
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(lane(0), lane(16)),
+                                       __builtin_elementwise_maximum(lane(32), lane(48)));
 }
 
 template <typename T>
@@ -165,8 +197,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs
   const float temp = a.temperature[sequence_of(a, row)];
 #pragma unroll
   for (int i = 0; i < PER; ++i) top = __builtin_elementwise_maximum(top, x[i]);  // NaN, if any is
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, off));
+  top = wave_maximum(top);
   if (lane == 0) s_top[wave] = top;
   if (threadIdx.x == 0) s_col = 0x7fffffff;
   __syncthreads();
@@ -214,8 +245,7 @@ __device__ __forceinline__ Dist dist_of(const VerifyArgs& a, int row, float temp
   const int lane = threadIdx.x & (kWave - 1);
   uint64_t key = 0;
   for (int c = lane; c < a.chunks; c += kWave) key = max_u64(key, st[c].key);
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) key = max_u64(key, __shfl_xor(key, off));
+  key = wave_max(key);
   Dist d;
   d.top = key_value(key);
   d.best = argmax_key_column(key);
@@ -288,7 +318,8 @@ __device__ __forceinline__ double scan(double v, double* s_part) {
 template <typename T, int PER>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs a) {
   __shared__ int s_first, s_bad, s_turn;
-  __shared__ Dist s_dist;
+  constexpr int kDists = 16;  // rows whose distributions are kept
+  __shared__ Dist s_dist[kDists];
   __shared__ double s_part[kWaves], s_goal;
   constexpr int kChunk = kThreads * PER;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -312,26 +343,45 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs 
     s_bad = drafts + 1;
   }
   __syncthreads();
-  // The first drafted token that does not stand: a wave a row. (Rows behind one that does not are left out.)
-  for (int i = wave; i <= drafts && i <= *(volatile int*)&s_first; i += kWaves) {
-    const Dist d = dist_of(a, lo + i, temp);
-    if (d.peak && temp > 0.f && lane == 0) atomicMin(&s_bad, i);
-    if (i == drafts) break;
-    const int64_t x = a.drafts[lo + i];
-    bool stands = false;
-    if (x >= 0 && x < a.vocab) {
-      const double p = d.peak ? (x == d.best ? 1.0 : 0.0) : mass_of(d, logit_at<T>(row_of<T>(a, lo + i), x), x) / d.sum;
-      const double q = a.probs == nullptr ? 1.0 : (double)a.probs[(int64_t)(lo + i) * a.probs_stride + x];
-      stands = (double)a.uniforms[lo + i] * q < p;
+  // The first drafted token that does not stand: a wave a row, after a lane a row has fetched what it needs of 64 rows. (Rows
+  // behind one that does not stand are left out.)
+  for (int i0 = 0; i0 <= drafts && i0 <= *(volatile int*)&s_first; i0 += kWave) {
+    float lx = 0.f, qx = 1.f, ux = 0.f;
+    bool in = false;
+    int64_t x = 0;
+    if (i0 + lane < drafts) {
+      x = a.drafts[lo + i0 + lane];
+      ux = a.uniforms[lo + i0 + lane];
+      in = x >= 0 && x < a.vocab;
+      if (in) {
+        lx = logit_at<T>(row_of<T>(a, lo + i0 + lane), x);
+        if (a.probs != nullptr) qx = a.probs[(int64_t)(lo + i0 + lane) * a.probs_stride + x];
+      }
     }
-    if (!stands && lane == 0) atomicMin(&s_first, i);
+    for (int i = i0 + wave; i <= drafts && i < i0 + kWave && i <= *(volatile int*)&s_first; i += kWaves) {
+      const Dist d = dist_of(a, lo + i, temp);
+      if (lane == 0 && i < kDists) s_dist[i] = d;
+      if (d.peak && temp > 0.f && lane == 0) atomicMin(&s_bad, i);
+      if (lane == i - i0 && i < drafts) {
+        bool stands = false;
+        if (in) {
+          const double p = d.peak ? (x == d.best ? 1.0 : 0.0) : mass_of(d, lx, x) / d.sum;
+          stands = (double)ux * (double)qx < p;
+        }
+        if (!stands) atomicMin(&s_first, i);
+      }
+    }
   }
   __syncthreads();
   const int first = s_first, row = lo + first;
-  if (wave == 0) {
-    const Dist d = dist_of(a, row, temp);
-    if (lane == 0) s_dist = d;
+  if (first >= kDists) {  // uniform
+    if (wave == 0) {
+      const Dist d = dist_of(a, row, temp);
+      if (lane == 0) s_dist[0] = d;
+    }
+    __syncthreads();
   }
+  const Dist d = s_dist[first < kDists ? first : 0];
   if (lead) {
     for (int i = threadIdx.x; i < a.max_rows; i += kThreads)
       if (i != first) out[i] = i < first ? a.drafts[lo + i] : -1;
@@ -341,8 +391,6 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs 
       if (first < drafts && (a.drafts[row] < 0 || a.drafts[row] >= a.vocab)) flag_error(a.d_error, TQ_DEVERR_TOKEN);
     }
   }
-  __syncthreads();
-  const Dist d = s_dist;
   const void* lp = row_of<T>(a, row);
   const float* qrow = a.probs == nullptr ? nullptr : a.probs + (int64_t)row * a.probs_stride;
   const int64_t draft = first < drafts ? a.drafts[row] : -1;
