@@ -404,8 +404,13 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs 
   double* sums = a.sums + (int64_t)b * a.chunks;
   if (threadIdx.x == 0) {
     for (int v = 1; v < kWaves; ++v) w += s_part[v];
+    // The sums are all that workgroups hand each other, by accesses of agent scope, which are done where all XCDs meet: the
+    // count has to follow the store, which has ended after the wait. (Release and acquire of everything else would write this
+    // XCD's L2 back and drop it.)
     __hip_atomic_store(&sums[chunk], w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_turn = (int)__hip_atomic_fetch_add(&a.arrived[b], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    s_turn = (int)__hip_atomic_fetch_add(&a.arrived[b], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (s_turn != a.chunks - 1) return;
