@@ -17,7 +17,7 @@
 //    stand and sums its chunk's weights of that row; the last workgroup of a sequence to finish finds the chunk the draw
 //    falls in, and the column in it.
 
-#include <float.h>
+#include <type_traits>
 
 #include "half_types.h"
 
@@ -44,7 +44,8 @@ struct VerifyArgs {
   const float* temperature;
   const int32_t* cu;
   Stat* stats;        // [num_rows][chunks]
-  double* sums;       // [num_seqs][chunks]
+  struct Decision* decisions;  // [num_seqs]
+  double* sums;       // [num_seqs][draw_chunks]
   uint32_t* arrived;  // [num_seqs]
   int32_t* d_error;
   int32_t num_seqs;
@@ -52,6 +53,7 @@ struct VerifyArgs {
   int32_t max_rows;
   int32_t vocab;
   int32_t chunks;
+  int32_t draw_chunks;
 };
 
 // 2^t for t <= 0: 2^k 2^f with k the nearest integer (read off the low bits of t + 1.5 2^52), the second factor by the polynomial
@@ -302,50 +304,86 @@ __device__ __forceinline__ void weights(const Dist& d, const void* row, const fl
 // Inclusive sums over the workgroup's threads, in order; s_part: a word a wave.
 __device__ __forceinline__ double scan(double v, double* s_part) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  auto up = [&](auto ctrl) {  // from a lane further down in the row of 16; 0 past its start
+    return __builtin_bit_cast(double, dpp_move64<decltype(ctrl)::value>(__builtin_bit_cast(uint64_t, v)));
+  };
+  v += up(std::integral_constant<int, 0x111>());  // row_shr:1, 2, 4, 8
+  v += up(std::integral_constant<int, 0x112>());
+  v += up(std::integral_constant<int, 0x114>());
+  v += up(std::integral_constant<int, 0x118>());
+  double before = 0.0;  // the rows before this one
 #pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const double up = __shfl_up(v, off);
-    if (lane >= off) v += up;
+  for (int r = 1; r < kWave / 16; ++r) {
+    const double row = __builtin_bit_cast(double, lane_of(__builtin_bit_cast(uint64_t, v), 16 * r - 1));
+    before += lane >= 16 * r ? row : 0.0;
   }
+  v += before;
   if (lane == kWave - 1) s_part[wave] = v;
   __syncthreads();
-  double before = 0.0;
-  for (int u = 0; u < wave; ++u) before += s_part[u];
+  before = 0.0;
+#pragma unroll
+  for (int u = 0; u < kWaves - 1; ++u) before += u < wave ? s_part[u] : 0.0;
   __syncthreads();
   return before + v;
 }
 
-template <typename T, int PER>
-__global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs a) {
-  __shared__ int s_first, s_bad, s_turn;
-  constexpr int kDists = 16;  // rows whose distributions are kept
-  __shared__ Dist s_dist[kDists];
-  __shared__ double s_part[kWaves], s_goal;
-  constexpr int kChunk = kThreads * PER;
+// The first thread with `over`, or the last with `has` where there is none; -1: none either. s_pick: two words a wave.
+__device__ __forceinline__ int pick(bool over, bool has, int (*s_pick)[2]) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int chunk = blockIdx.x % a.chunks, b = blockIdx.x / a.chunks;
+  const uint64_t overs = __builtin_amdgcn_ballot_w64(over), those = __builtin_amdgcn_ballot_w64(has);
+  if (lane == 0) {
+    s_pick[wave][0] = overs != 0 ? wave * kWave + __builtin_ctzll(overs) : 0x7fffffff;
+    s_pick[wave][1] = those != 0 ? wave * kWave + 63 - __builtin_clzll(those) : -1;
+  }
+  __syncthreads();
+  int first = 0x7fffffff, last = -1;
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) {
+    first = min(first, s_pick[v][0]);
+    last = max(last, s_pick[v][1]);
+  }
+  __syncthreads();
+  return first != 0x7fffffff ? first : last;
+}
+
+// What became of a sequence's drafts: how many stand, and the distribution of the row that the next token is drawn from.
+struct Decision {
+  Dist dist;
+  int first;  // -1: the sequence has no rows (or does not fit)
+};
+
+constexpr int kDists = 16;  // rows whose distributions are kept in LDS
+struct DecideShared {
+  Dist dist[kDists];
+  int first, bad;
+};
+
+// By one workgroup. `lead`: it also writes the tokens that stand, and the flags.
+template <typename T>
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, int b, bool lead, DecideShared& sh) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int lo = a.cu[b];
-  const int64_t rows64 = (int64_t)a.cu[b + 1] - lo;
+  const int64_t rows = (int64_t)a.cu[b + 1] - lo;
   int64_t* out = a.tokens + (int64_t)b * a.max_rows;
-  const bool lead = chunk == 0;
-  if (lo < 0 || rows64 <= 0 || lo + rows64 > a.num_rows || rows64 > a.max_rows) {
+  Decision r;
+  if (lo < 0 || rows <= 0 || lo + rows > a.num_rows || rows > a.max_rows) {
     if (lead) {
-      if (rows64 != 0 && threadIdx.x == 0) flag_error(a.d_error, TQ_DEVERR_LENGTH);
+      if (rows != 0 && threadIdx.x == 0) flag_error(a.d_error, TQ_DEVERR_LENGTH);
       for (int i = threadIdx.x; i < a.max_rows; i += kThreads) out[i] = -1;
       if (threadIdx.x == 0) a.accepted[b] = 0;
     }
-    return;
+    r.first = -1;
+    return r;
   }
-  const int drafts = (int)rows64 - 1;
+  const int drafts = (int)rows - 1;
   const float temp = a.temperature[b];
   if (threadIdx.x == 0) {
-    s_first = drafts;
-    s_bad = drafts + 1;
+    sh.first = drafts;
+    sh.bad = drafts + 1;
   }
   __syncthreads();
-  // The first drafted token that does not stand: a wave a row, after a lane a row has fetched what it needs of 64 rows. (Rows
-  // behind one that does not stand are left out.)
-  for (int i0 = 0; i0 <= drafts && i0 <= *(volatile int*)&s_first; i0 += kWave) {
+  // A wave a row, after a lane a row has fetched what it needs of 64 rows. (Rows behind one that does not stand are left out.)
+  for (int i0 = 0; i0 <= drafts && i0 <= *(volatile int*)&sh.first; i0 += kWave) {
     float lx = 0.f, qx = 1.f, ux = 0.f;
     bool in = false;
     int64_t x = 0;
@@ -358,52 +396,87 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs 
         if (a.probs != nullptr) qx = a.probs[(int64_t)(lo + i0 + lane) * a.probs_stride + x];
       }
     }
-    for (int i = i0 + wave; i <= drafts && i < i0 + kWave && i <= *(volatile int*)&s_first; i += kWaves) {
+    for (int i = i0 + wave; i <= drafts && i < i0 + kWave && i <= *(volatile int*)&sh.first; i += kWaves) {
       const Dist d = dist_of(a, lo + i, temp);
-      if (lane == 0 && i < kDists) s_dist[i] = d;
-      if (d.peak && temp > 0.f && lane == 0) atomicMin(&s_bad, i);
+      if (lane == 0 && i < kDists) sh.dist[i] = d;
+      if (d.peak && temp > 0.f && lane == 0) atomicMin(&sh.bad, i);
       if (lane == i - i0 && i < drafts) {
         bool stands = false;
         if (in) {
           const double p = d.peak ? (x == d.best ? 1.0 : 0.0) : mass_of(d, lx, x) / d.sum;
           stands = (double)ux * (double)qx < p;
         }
-        if (!stands) atomicMin(&s_first, i);
+        if (!stands) atomicMin(&sh.first, i);
       }
     }
   }
   __syncthreads();
-  const int first = s_first, row = lo + first;
-  if (first >= kDists) {  // uniform
+  r.first = sh.first;
+  if (r.first >= kDists) {  // uniform
     if (wave == 0) {
-      const Dist d = dist_of(a, row, temp);
-      if (lane == 0) s_dist[0] = d;
+      const Dist d = dist_of(a, lo + r.first, temp);
+      if (lane == 0) sh.dist[0] = d;
     }
     __syncthreads();
   }
-  const Dist d = s_dist[first < kDists ? first : 0];
+  r.dist = sh.dist[r.first < kDists ? r.first : 0];
   if (lead) {
     for (int i = threadIdx.x; i < a.max_rows; i += kThreads)
-      if (i != first) out[i] = i < first ? a.drafts[lo + i] : -1;
+      if (i != r.first) out[i] = i < r.first ? a.drafts[lo + i] : -1;
     if (threadIdx.x == 0) {
-      a.accepted[b] = first;
-      if (s_bad <= first) flag_error(a.d_error, TQ_DEVERR_VALUE);
-      if (first < drafts && (a.drafts[row] < 0 || a.drafts[row] >= a.vocab)) flag_error(a.d_error, TQ_DEVERR_TOKEN);
+      a.accepted[b] = r.first;
+      if (sh.bad <= r.first) flag_error(a.d_error, TQ_DEVERR_VALUE);
+      if (r.first < drafts && (a.drafts[lo + r.first] < 0 || a.drafts[lo + r.first] >= a.vocab))
+        flag_error(a.d_error, TQ_DEVERR_TOKEN);
     }
   }
+  return r;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void verify_decide_kernel(const VerifyArgs a) {
+  __shared__ DecideShared s_decide;
+  const Decision r = decide<T>(a, blockIdx.x, true, s_decide);
+  if (threadIdx.x == 0) a.decisions[blockIdx.x] = r;
+}
+
+// DECIDED: by verify_decide_kernel; else each workgroup decides for itself.
+template <typename T, int PER, bool DECIDED>
+__global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs a) {
+  __shared__ int s_turn, s_pick[kWaves][2];
+  __shared__ double s_part[kWaves], s_goal;
+  constexpr int kChunk = kThreads * PER;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int chunk = blockIdx.x % a.draw_chunks, b = blockIdx.x / a.draw_chunks;
+  Decision r;
+  if constexpr (DECIDED) {
+    r = a.decisions[b];
+  } else {
+    __shared__ DecideShared s_decide;
+    r = decide<T>(a, b, chunk == 0, s_decide);
+  }
+  if (r.first < 0) return;
+  const Dist d = r.dist;
+  const int lo = a.cu[b], drafts = a.cu[b + 1] - lo - 1, first = r.first, row = lo + first;
   const void* lp = row_of<T>(a, row);
   const float* qrow = a.probs == nullptr ? nullptr : a.probs + (int64_t)row * a.probs_stride;
   const int64_t draft = first < drafts ? a.drafts[row] : -1;
   int mode = first == drafts ? kAll : qrow != nullptr ? kLess : kWithout;
-  const int base = chunk * kChunk, n = min(kChunk, a.vocab - base);
-  double w = 0.0;
-  weights<T, PER, false>(d, lp, qrow, draft, mode, base, n, [&](int, double v) { w += v; });
-  w = wave_sum(w);
-  if (lane == 0) s_part[wave] = w;
-  __syncthreads();
-  double* sums = a.sums + (int64_t)b * a.chunks;
+  auto chunk_sum = [&](int c) {  // of this workgroup's waves, in thread 0
+    double w = 0.0;
+    weights<T, PER, false>(d, lp, qrow, draft, mode, c * kChunk, min(kChunk, a.vocab - c * kChunk),
+                           [&](int, double v) { w += v; });
+    w = wave_sum(w);
+    if (lane == 0) s_part[wave] = w;
+    __syncthreads();
+    w = 0.0;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) w += s_part[v];
+    return w;
+  };
+  const double w = chunk_sum(chunk);
+  double* sums = a.sums + (int64_t)b * a.draw_chunks;
   if (threadIdx.x == 0) {
-    for (int v = 1; v < kWaves; ++v) w += s_part[v];
     // The sums are all that workgroups hand each other, by accesses of agent scope, which are done where all XCDs meet: the
     // count has to follow the store, which has ended after the wait. (Release and acquire of everything else would write this
     // XCD's L2 back and drop it.)
@@ -413,63 +486,47 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs 
     s_turn = (int)__hip_atomic_fetch_add(&a.arrived[b], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  if (s_turn != a.chunks - 1) return;
+  if (s_turn != a.draw_chunks - 1) return;
 
   // The last workgroup of the sequence: the chunk that the draw falls in (the last one with weight where rounding
   // leaves none above the goal), a chunk a thread.
   const int c = threadIdx.x;
-  double mine = c < a.chunks ? __hip_atomic_load(&sums[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+  const double u = (double)a.uniforms[lo + drafts];
+  double mine = c < a.draw_chunks ? __hip_atomic_load(&sums[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
   double upto = scan(mine, s_part);
   if (c == kThreads - 1) s_goal = upto;
   __syncthreads();
   if (!(s_goal > 0.0)) {
-    // Nothing left where q covers p (to rounding): the draw is from p itself, whose chunks' sums the statistics have.
+    // Nothing left where q covers p (to rounding): the draw is from p itself.
     mode = kAll;
     mine = 0.0;
-    if (c < a.chunks) {
-      const Stat st = a.stats[(int64_t)row * a.chunks + c];
-      const float m = key_value(st.key);
-      if (d.peak)
-        mine = c == (int)(d.best / kChunk) ? 1.0 : 0.0;
-      else if (m > -INFINITY)
-        mine = st.sum * exp2_neg(((double)m - (double)d.top) * d.c);
+    __syncthreads();
+    for (int k = 0; k < a.draw_chunks; ++k) {
+      const double sum = chunk_sum(k);
+      mine = c == k ? sum : mine;
+      __syncthreads();
     }
     upto = scan(mine, s_part);
     if (c == kThreads - 1) s_goal = upto;
     __syncthreads();
   }
-  const double goal = (double)a.uniforms[lo + drafts] * s_goal;
-  if (c == 0) s_first = 0x7fffffff, s_turn = -1;
-  __syncthreads();
-  if (mine > 0.0) {
-    if (upto > goal) atomicMin(&s_first, c);
-    atomicMax(&s_turn, c);
-  }
-  __syncthreads();
-  const int chosen = s_first != 0x7fffffff ? s_first : s_turn;
+  const double goal = u * s_goal;
+  const int chosen = pick(mine > 0.0 && upto > goal, mine > 0.0, s_pick);
   if (chosen < 0) {  // no weight anywhere: draft probabilities that are not numbers
-    if (c == 0) out[first] = d.best;
+    if (c == 0) a.tokens[(int64_t)b * a.max_rows + first] = d.best;
     return;
   }
   if (c == chosen) s_goal = goal - (upto - mine);
-  __syncthreads();
-  const double rest = s_goal;
   // The column in it: runs of PER columns a thread.
-  const int at = chosen * kChunk, m = min(kChunk, a.vocab - at);
+  const int at = chosen * kChunk;
   double ws[PER], run = 0.0;
-  weights<T, PER, true>(d, lp, qrow, draft, mode, at, m, [&](int i, double v) {
+  weights<T, PER, true>(d, lp, qrow, draft, mode, at, min(kChunk, a.vocab - at), [&](int i, double v) {
     ws[i] = v;
     run += v;
   });
   upto = scan(run, s_part);
-  if (c == 0) s_first = 0x7fffffff, s_turn = -1;
-  __syncthreads();
-  if (run > 0.0) {
-    if (upto > rest) atomicMin(&s_first, c);
-    atomicMax(&s_turn, c);
-  }
-  __syncthreads();
-  if (c == (s_first != 0x7fffffff ? s_first : s_turn)) {
+  const double rest = s_goal;
+  if (c == pick(run > 0.0 && upto > rest, run > 0.0, s_pick)) {
     double cum = upto - run;
     int token = -1;
     bool done = false;
@@ -477,42 +534,74 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs 
     for (int i = 0; i < PER; ++i) {
       cum += ws[i];
       if (!done && ws[i] > 0.0) {
-        token = at + (int)threadIdx.x * PER + i;
+        token = at + c * PER + i;
         done = cum > rest;
       }
     }
-    out[first] = token;
+    a.tokens[(int64_t)b * a.max_rows + first] = token;
   }
 }
 
 constexpr int kMaxVocab = kThreads * kThreads * 32;  // a chunk a thread
+constexpr int kFewDraws = 1024;
+constexpr int kDecideFrom = 512;  // workgroups of the draw from which one decision a sequence is worth its launch
 
-// Columns of a thread: 32, or 8 where the rows' chunks would leave CUs without one (a row's chunk of 8,192 columns takes one 4 us).
-int per_of(int64_t num_rows, int64_t vocab) {
-  const bool few = num_rows * ((vocab + kThreads * 32 - 1) / (kThreads * 32)) < 512;
-  return few && vocab <= kThreads * kThreads * 8 ? 8 : 32;
-}
+// How a call is split, and its workspace.
+struct Plan {
+  int per, draw_per;  // columns of a thread in the two launches: 8 or 32
+  int chunks, draw_chunks;
+  bool decide;  // a launch between them
+  size_t stats, decisions, sums, arrived, bytes;  // offsets
+};
 
-int64_t chunks_of(int64_t num_rows, int64_t vocab) {
-  const int64_t chunk = (int64_t)kThreads * per_of(num_rows, vocab);
-  return (vocab + chunk - 1) / chunk;
+Plan plan_of(int32_t num_seqs, int32_t num_rows, int32_t vocab) {
+  Plan p;
+  auto chunks = [&](int per) { return (vocab + kThreads * per - 1) / (kThreads * per); };
+  // 32 columns a thread keep the loads of a row in flight; 8 spread few rows over more CUs.
+  p.per = (int64_t)num_rows * chunks(32) < 512 && chunks(8) <= kThreads ? 8 : 32;
+  p.draw_per = chunks(8) <= kThreads && (int64_t)num_seqs * chunks(8) <= kFewDraws ? 8 : chunks(16) <= kThreads ? 16 : 32;
+  p.chunks = chunks(p.per);
+  p.draw_chunks = chunks(p.draw_per);
+  p.decide = (int64_t)num_seqs * p.draw_chunks > kDecideFrom;
+  p.stats = 0;
+  p.decisions = p.stats + (size_t)num_rows * p.chunks * sizeof(Stat);
+  p.sums = p.decisions + (size_t)num_seqs * sizeof(Decision);
+  p.arrived = p.sums + (size_t)num_seqs * p.draw_chunks * sizeof(double);
+  p.bytes = p.arrived + (size_t)num_seqs * sizeof(uint32_t);
+  return p;
 }
 
 template <typename T, int PER>
-tq_status launch(const VerifyArgs& a, hipStream_t stream) {
-  const int64_t rows = a.num_rows > a.num_seqs ? a.num_rows : a.num_seqs;
-  const int64_t stats = rows * a.chunks, draw = (int64_t)a.num_seqs * a.chunks;
-  if (stats > 0x7fffffffLL || draw > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((verify_stats_kernel<T, PER>), dim3((unsigned)stats), dim3(kThreads), 0, stream, a);
-  const tq_status st = check_launch();
-  if (st != TQ_OK) return st;
-  hipLaunchKernelGGL((verify_draw_kernel<T, PER>), dim3((unsigned)draw), dim3(kThreads), 0, stream, a);
+tq_status launch_draw(const VerifyArgs& a, bool decided, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)a.num_seqs * a.draw_chunks));
+  if (decided)
+    hipLaunchKernelGGL((verify_draw_kernel<T, PER, true>), grid, dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((verify_draw_kernel<T, PER, false>), grid, dim3(kThreads), 0, stream, a);
   return check_launch();
 }
 
 template <typename T>
-tq_status launch(const VerifyArgs& a, hipStream_t stream) {
-  return per_of(a.num_rows, a.vocab) == 8 ? launch<T, 8>(a, stream) : launch<T, 32>(a, stream);
+tq_status launch(const VerifyArgs& a, const Plan& p, hipStream_t stream) {
+  const int64_t rows = a.num_rows > a.num_seqs ? a.num_rows : a.num_seqs;
+  const int64_t stats = rows * a.chunks;
+  if (stats > 0x7fffffffLL || (int64_t)a.num_seqs * a.draw_chunks > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
+  if (p.per == 8)
+    hipLaunchKernelGGL((verify_stats_kernel<T, 8>), dim3((unsigned)stats), dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((verify_stats_kernel<T, 32>), dim3((unsigned)stats), dim3(kThreads), 0, stream, a);
+  tq_status st = check_launch();
+  if (st != TQ_OK) return st;
+  if (p.decide) {
+    hipLaunchKernelGGL((verify_decide_kernel<T>), dim3((unsigned)a.num_seqs), dim3(kThreads), 0, stream, a);
+    st = check_launch();
+    if (st != TQ_OK) return st;
+  }
+  switch (p.draw_per) {
+    case 8: return launch_draw<T, 8>(a, p.decide, stream);
+    case 16: return launch_draw<T, 16>(a, p.decide, stream);
+    default: return launch_draw<T, 32>(a, p.decide, stream);
+  }
 }
 
 }  // namespace
@@ -521,8 +610,7 @@ tq_status launch(const VerifyArgs& a, hipStream_t stream) {
 extern "C" size_t tq_verify_drafts_workspace_size(int32_t num_seqs, int32_t num_rows, int32_t vocab) {
   using namespace tq;
   if (num_seqs < 1 || num_rows < 0 || vocab < 1 || vocab > kMaxVocab) return 0;
-  const size_t chunks = (size_t)chunks_of(num_rows, vocab);
-  return num_rows * chunks * sizeof(Stat) + num_seqs * chunks * sizeof(double) + num_seqs * sizeof(uint32_t);
+  return plan_of(num_seqs, num_rows, vocab).bytes;
 }
 
 extern "C" tq_status tq_verify_drafts(int64_t* tokens, int32_t* accepted, const void* logits,
@@ -539,8 +627,8 @@ extern "C" tq_status tq_verify_drafts(int64_t* tokens, int32_t* accepted, const 
       temperature == nullptr || (num_rows > 0 && (logits == nullptr || draft_tokens == nullptr || uniforms == nullptr)) ||
       (num_rows > 1 && (logits_row_stride < vocab || (draft_probs != nullptr && probs_row_stride < vocab))))
     return TQ_ERR_INVALID_ARGUMENT;
-  const size_t need = tq_verify_drafts_workspace_size(num_seqs, num_rows, vocab);
-  if (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 16 != 0) return TQ_ERR_WORKSPACE;
+  const Plan p = plan_of(num_seqs, num_rows, vocab);
+  if (workspace == nullptr || workspace_bytes < p.bytes || (uintptr_t)workspace % 16 != 0) return TQ_ERR_WORKSPACE;
   VerifyArgs a;
   a.tokens = tokens;
   a.accepted = accepted;
@@ -556,12 +644,15 @@ extern "C" tq_status tq_verify_drafts(int64_t* tokens, int32_t* accepted, const 
   a.num_rows = num_rows;
   a.max_rows = max_query_len;
   a.vocab = vocab;
-  a.chunks = (int32_t)chunks_of(num_rows, vocab);
-  a.stats = static_cast<Stat*>(workspace);
-  a.sums = reinterpret_cast<double*>(a.stats + (size_t)num_rows * a.chunks);
-  a.arrived = reinterpret_cast<uint32_t*>(a.sums + (size_t)num_seqs * a.chunks);
+  a.chunks = p.chunks;
+  a.draw_chunks = p.draw_chunks;
+  char* ws = static_cast<char*>(workspace);
+  a.stats = reinterpret_cast<Stat*>(ws + p.stats);
+  a.decisions = reinterpret_cast<Decision*>(ws + p.decisions);
+  a.sums = reinterpret_cast<double*>(ws + p.sums);
+  a.arrived = reinterpret_cast<uint32_t*>(ws + p.arrived);
   a.d_error = d_error;
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == TQ_F32) return launch<float>(a, st);
-  return dtype == TQ_BF16 ? launch<Bf16>(a, st) : launch<Fp16>(a, st);
+  if (dtype == TQ_F32) return launch<float>(a, p, st);
+  return dtype == TQ_BF16 ? launch<Bf16>(a, p, st) : launch<Fp16>(a, p, st);
 }
