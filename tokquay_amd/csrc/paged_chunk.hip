@@ -998,7 +998,7 @@ constexpr int kCus = 256;
 constexpr int kTilesNt = 2;   // 16-row tiles of a wave of chunk_tiles_kernel
 constexpr int kTilesPerCu = 2;
 
-Plan plan_of(int num_seqs, int kv_heads, int group, int max_query_len, int max_context) {
+Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int max_query_len, int max_context) {
   Plan p;
   const int64_t rows = (int64_t)max_query_len * group;
   p.tiles = rows > 64;
@@ -1007,9 +1007,9 @@ Plan plan_of(int num_seqs, int kv_heads, int group, int max_query_len, int max_c
   constexpr int kStep = kWaves * kTileKeys;
   const int64_t steps = ((int64_t)max_context + kStep - 1) / kStep;
   const int64_t groups = (int64_t)num_seqs * kv_heads * p.row_tiles;
-  const int64_t want = p.tiles ? kTilesPerCu * kCus : kCus;
-  int64_t parts = (want + groups - 1) / groups;
-  if (parts > steps) parts = steps;
+  const int64_t want = p.tiles ? kTilesPerCu * kCus : kCus * (head_dim == 64 ? 2 : 1);
+  int64_t parts = want / groups;  // no second round for a few
+  parts = parts < 1 ? 1 : parts > steps ? steps : parts;
   const int64_t per = (steps + parts - 1) / parts;
   p.part_tokens = (int)(per * kStep > 0x7fffffff - kStep ? 0x7fffffff / kStep * kStep : per * kStep);
   p.parts = (int)((steps + per - 1) / per);
@@ -1066,7 +1066,7 @@ extern "C" size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_he
       num_seqs == 0 || num_q_rows == 0 || max_query_len == 0 || max_context_len == 0)
     return 0;
   const int32_t group = num_heads / num_kv_heads;
-  return workspace_of(plan_of(num_seqs, num_kv_heads, group, max_query_len, max_context_len), num_seqs, num_q_rows,
+  return workspace_of(plan_of(num_seqs, num_kv_heads, group, head_dim, max_query_len, max_context_len), num_seqs, num_q_rows,
                       num_heads, group, head_dim);
 }
 
@@ -1098,7 +1098,7 @@ extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const voi
   if ((int64_t)max_query_len * num_heads > 0x7fffffffLL - 65536) return TQ_ERR_UNSUPPORTED;
 
   const int32_t group = num_heads / num_kv_heads;
-  const Plan p = plan_of(num_seqs, num_kv_heads, group, max_query_len, max_context_len);
+  const Plan p = plan_of(num_seqs, num_kv_heads, group, head_dim, max_query_len, max_context_len);
   const size_t need = workspace_of(p, num_seqs, num_q_rows, num_heads, group, head_dim);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 16 != 0))
     return TQ_ERR_WORKSPACE;

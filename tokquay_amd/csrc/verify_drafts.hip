@@ -170,17 +170,14 @@ __device__ __forceinline__ void columns(const void* row, int base, int n, float 
 
 constexpr double kLog2e = 1.4426950408889634;
 
-// The sequence that a row belongs to: the last with cu[b] <= row (empty sequences hold no row).
-__device__ __forceinline__ int sequence_of(const VerifyArgs& a, int row) {
-  int lo = 0, hi = a.num_seqs;  // cu[lo] <= row < cu[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (a.cu[mid] <= row)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return lo;
+// The temperature of the sequence that a row belongs to: the last one with cu[b] <= row (empty sequences hold no row), counted 64
+// at a time. Asked for before the logits, it arrives before them.
+__device__ __forceinline__ float temperature_of(const VerifyArgs& a, int row) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int b = -1;
+  for (int b0 = 0; b0 < a.num_seqs; b0 += kWave)
+    b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b0 + lane < a.num_seqs && a.cu[b0 + lane] <= row));
+  return a.temperature[max(b, 0)];
 }
 
 template <typename T, int PER>
@@ -194,9 +191,8 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int base = chunk * kThreads * PER, n = min(kThreads * PER, a.vocab - base);
   float x[PER], top = -INFINITY;
-  const void* lp = row_of<T>(a, row);
-  columns<T, kVec<T>, PER, false>(lp, base, n, x);
-  const float temp = a.temperature[sequence_of(a, row)];
+  const float temp = temperature_of(a, row);
+  columns<T, kVec<T>, PER, false>(row_of<T>(a, row), base, n, x);
 #pragma unroll
   for (int i = 0; i < PER; ++i) top = __builtin_elementwise_maximum(top, x[i]);  // NaN, if any is
   top = wave_maximum(top);
