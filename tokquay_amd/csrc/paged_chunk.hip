@@ -997,6 +997,10 @@ struct Plan {
 constexpr int kCus = 256;
 constexpr int kTilesNt = 2;   // 16-row tiles of a wave of chunk_tiles_kernel
 constexpr int kTilesPerCu = 2;
+// Row tiles of contexts up to this differ too little for the queue and its launch (direct -> queue): 16 prompts of 17-1,023 tokens
+// 31 -> 38 us, 16 x 512 behind 512 151 -> 165, 4 x 2,048 168 -> 173; but 16 of 100-1,900 behind up to 2,000 224 -> 199, 64 of
+// 100-500 behind up to 2,000 325 -> 267, 4 x 2,048 behind up to 6,144 696 -> 535.
+constexpr int kQueueFrom = 2048;
 
 Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int max_query_len, int max_context) {
   Plan p;
@@ -1013,7 +1017,7 @@ Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int max_query_
   const int64_t per = (steps + parts - 1) / parts;
   p.part_tokens = (int)(per * kStep > 0x7fffffff - kStep ? 0x7fffffff / kStep * kStep : per * kStep);
   p.parts = (int)((steps + per - 1) / per);
-  p.queue = p.tiles && p.parts == 1 && groups > want;
+  p.queue = p.tiles && p.parts == 1 && groups > want && max_context >= kQueueFrom;
   return p;
 }
 
