@@ -191,9 +191,9 @@ struct Cursor {
   __device__ __forceinline__ void place(const ChunkArgs& a, int local, int& entry, int& slot) const {
     const bool in = kt < stop;
     const uint32_t x = (uint32_t)((in ? r : end_r) + min(local, in ? stop - 1 - kt : 0));
-    const int b = (int)(__umul24(x, a.inv_block) >> 21);
-    entry = (in ? q : end_q) + b;
-    slot = (int)x - b * a.block_size;
+    const uint32_t b = __umul24(x, a.inv_block) >> 21;
+    entry = (in ? q : end_q) + (int)b;
+    slot = (int)(x - __umul24(b, a.block_size));
   }
 };
 
@@ -250,15 +250,15 @@ struct Loader {
   }
   // `id`, `slot`: block and slot of this lane's own_key.
   __device__ __forceinline__ void aim(const ChunkArgs& a, const uint16_t* head_base, int first, int32_t id, int slot) {
-    aim_each(a, head_base, first, (uint64_t)(uint32_t)id * a.block_stride + slot * D, std::make_integer_sequence<int, J>());
+    const uint64_t row = (uint64_t)head_base + ((uint64_t)(uint32_t)id * (2 * a.block_stride) + (uint32_t)slot * (2 * D));
+    aim_each(first, row, std::make_integer_sequence<int, J>());
   }
   template <int... j>
-  __device__ __forceinline__ void aim_each(const ChunkArgs& a, const uint16_t* head_base, int first, uint64_t row,
-                                           std::integer_sequence<int, j...>) {
+  __device__ __forceinline__ void aim_each(int first, uint64_t row, std::integer_sequence<int, j...>) {
     const int lane = threadIdx.x & (kWave - 1);
-    ((src[j] = head_base +
-               ((uint64_t)broadcast<j>((uint32_t)(row >> 32)) << 32 | broadcast<j>((uint32_t)row)) +
-               8 * ((lane % kLanes) ^ swizzle<D>(first + j * kKeys + lane / kLanes))),
+    ((src[j] = reinterpret_cast<const uint16_t*>(
+          ((uint64_t)broadcast<j>((uint32_t)(row >> 32)) << 32 | broadcast<j>((uint32_t)row)) +
+          16 * (uint32_t)((lane % kLanes) ^ swizzle<D>(first + j * kKeys + lane / kLanes)))),
      ...);
   }
 
@@ -674,31 +674,31 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
   Loader<D, J> load;
   const int first = wave * (kKeys / kWaves);
   const int at = first * D;
-  Cursor c, ahead;  // the tile to aim at, and the one to fetch block ids of
+  Cursor c;  // the tile to fetch block ids of
   c.init(a, kbeg, kstop, kKeys);
-  ahead = c;
-  auto fetch_ids = [&] {
-    int entry, slot;
-    ahead.place(a, Loader<D, J>::own_key(first), entry, slot);
-    ahead.next(a, kKeys);
-    return bt[entry];
+  struct Place {
+    int32_t id;
+    int slot;
   };
-  auto aim = [&](int32_t id) {
-    int entry, slot;
-    c.place(a, Loader<D, J>::own_key(first), entry, slot);
-    load.aim(a, head_base, first, checked(a, id), slot);
+  auto fetch = [&] {
+    int entry;
+    Place at;
+    c.place(a, Loader<D, J>::own_key(first), entry, at.slot);
     c.next(a, kKeys);
+    at.id = bt[entry];
+    return at;
   };
+  auto aim = [&](const Place& at) { load.aim(a, head_base, first, checked(a, at.id), at.slot); };
   // Tiles past the last one repeat its last key.
-  int32_t id2, id3;
+  Place at2, at3;
   {
-    const int32_t id0 = fetch_ids(), id1 = fetch_ids();
-    id2 = fetch_ids();
-    id3 = fetch_ids();
-    aim(id0);
+    const Place at0 = fetch(), at1 = fetch();
+    at2 = fetch();
+    at3 = fetch();
+    aim(at0);
     load.start(s_k0 + at, 0);
     load.start(s_v0 + at, a.kv_stride);
-    aim(id1);
+    aim(at1);
     load.start(s_k1 + at, 0);
   }
   w.flip(a.q_sign);
@@ -720,10 +720,10 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
     if (kt + kKeys - 1 > lo && clean_values<T>(v_this + at, kTileElems / 8 / kWaves)) s_dirty = 1;
     barrier();
     load.start(v_free + at, a.kv_stride);
-    aim(id2);
+    aim(at2);
     load.start(k_free + at, 0);
-    id2 = id3;
-    id3 = fetch_ids();
+    at2 = at3;
+    at3 = fetch();
     if (has_rows && kt <= w.hi) {
       u32x4 kf[2][D / 32];
       R::read_k(k_next, 0, kf[0]);
