@@ -516,7 +516,7 @@ tq_status tq_rope_cache_write(void* q_out, int64_t q_out_row_stride, const void*
  *
  * cu_seqlens_q has num_seqs + 1 entries and is non-decreasing; sequences may be empty, and rows of q and out
  * outside every sequence are left alone. max_query_len >= every n_b and max_context_len >= every
- * q_start[b] + n_b size the launch: a sequence past them, past num_q_rows or past its block table sets
+ * q_start[b] + n_b (at most 2^30) size the launch: a sequence past them, past num_q_rows or past its block table sets
  * TQ_DEVERR_LENGTH and gets no output. Bad block ids set TQ_DEVERR_BLOCK_ID (that sequence's output is undefined).
  * q and pool 16-byte aligned, out 8-byte, q_row_stride a multiple of 8 elements, out_row_stride of 4. out
  * must not overlap q.

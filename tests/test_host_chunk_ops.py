@@ -170,7 +170,7 @@ def rope_call(q_out=P, qs=256, q=P, k=P, v=P, kvs=128, pool=P, nb=8, layers=2, h
     (INVALID, dict(n=-1)), (INVALID, dict(nb=0)), (INVALID, dict(layer=2)), (INVALID, dict(heads=0)), (INVALID, dict(kv=0)),
     (INVALID, dict(bs=0)), (INVALID, dict(rotary=0)), (INVALID, dict(rotary=80)), (INVALID, dict(inter=2)),
     (INVALID, dict(eps=-1.0)), (INVALID, dict(eps=math.nan)), (UNSUPPORTED, dict(d=96)), (UNSUPPORTED, dict(bs=1025)),
-    (UNSUPPORTED, dict(rotary=24)), (UNSUPPORTED, dict(dtype=3)), (UNSUPPORTED, dict(dtype=-1)), (OK, dict(n=0)),
+    (UNSUPPORTED, dict(rotary=24)), (UNSUPPORTED, dict(nb=1 << 32)), (UNSUPPORTED, dict(n=1 << 32)), (UNSUPPORTED, dict(dtype=3)), (UNSUPPORTED, dict(dtype=-1)), (OK, dict(n=0)),
     (INVALID, dict(q=None)), (INVALID, dict(q_out=None)), (INVALID, dict(pool=None)), (INVALID, dict(slots=None)),
     (INVALID, dict(pos=None)), (INVALID, dict(table=None)), (INVALID, dict(qs=248)), (INVALID, dict(kvs=120)),
     (INVALID, dict(q=P + 8)), (INVALID, dict(table=P + 4)), (INVALID, dict(qn=P + 2)), (INVALID, dict(qs=260)),
@@ -189,7 +189,8 @@ def chunk_call(out=P, os=256, q=P, qs=256, pool=P, nb=8, layers=2, heads=4, kv=2
     (INVALID, dict(seqs=-1)), (INVALID, dict(rows=-1)), (INVALID, dict(mq=-1)), (INVALID, dict(mc=-1)),
     (INVALID, dict(heads=5)), (INVALID, dict(kv=0)), (INVALID, dict(nb=0)), (INVALID, dict(layer=-1)),
     (INVALID, dict(scale=math.inf)), (INVALID, dict(scale=math.nan)), (UNSUPPORTED, dict(d=96)),
-    (UNSUPPORTED, dict(bs=1025)), (UNSUPPORTED, dict(dtype=0)), (OK, dict(seqs=0)), (OK, dict(rows=0)), (OK, dict(mq=0)),
+    (UNSUPPORTED, dict(bs=1025)), (UNSUPPORTED, dict(dtype=0)),
+    (UNSUPPORTED, dict(mc=(1 << 30) + 1)), (OK, dict(seqs=0)), (OK, dict(rows=0)), (OK, dict(mq=0)),
     (INVALID, dict(out=None)), (INVALID, dict(q=None)), (INVALID, dict(pool=None)), (INVALID, dict(tables=None)),
     (INVALID, dict(cu=None)), (INVALID, dict(start=None)), (INVALID, dict(ts=3)), (INVALID, dict(os=255)),
     (INVALID, dict(qs=248)), (INVALID, dict(mc=0)), (INVALID, dict(q=P + 8)), (INVALID, dict(out=P + 4)),

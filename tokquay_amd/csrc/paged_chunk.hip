@@ -647,6 +647,9 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
 // in LDS, each loading a quarter. The scores of tile t + 1 are computed beside the weights of tile t (matrix and
 // vector instructions of one iteration do not depend on each other), so one barrier a tile is enough: behind it K of t + 1
 // and V of t are in LDS, and the buffers of K of t and V of t - 1 are free for K of t + 2 and V of t + 1.
+// Workgroups of a CU: as many as have the registers (168 a wave at D = 64, 256 at 128).
+constexpr int tiles_per_cu(int head_dim) { return head_dim == 64 ? 3 : 2; }
+
 template <int D, int NT, typename T>
 __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b, int tile, int kvh, int part,
                                          uint16_t* s_k0, uint16_t* s_v0, uint16_t* s_k1, uint16_t* s_v1, int& s_dirty) {
@@ -799,7 +802,7 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
 // One workgroup a (sequence, K/V head, part, row tile). The last row tiles see the most keys and go first. Tiles of one K/V
 // head and part follow each other every 8th workgroup, so on one XCD, where these are a multiple of 8.
 template <int D, int NT, typename T>
-__global__ __launch_bounds__(kWave* kWaves, 2) void chunk_tiles_kernel(const ChunkArgs a) {
+__global__ __launch_bounds__(kWave* kWaves, tiles_per_cu(D)) void chunk_tiles_kernel(const ChunkArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t s_k0[64 * D], s_v0[64 * D], s_k1[64 * D], s_v1[64 * D];
   __shared__ int s_dirty;
   int idx = blockIdx.x;
@@ -893,7 +896,7 @@ __global__ __launch_bounds__(kOrderThreads) void chunk_order_kernel(const ChunkA
 // Item f is pair f / kv_heads with K/V head f % kv_heads. XCD x takes the items f % 8 = x (with a multiple of 8 heads, heads of
 // its own), then those that others left.
 template <int D, int NT, typename T>
-__global__ __launch_bounds__(kWave* kWaves, 2) void chunk_queue_kernel(const ChunkArgs a) {
+__global__ __launch_bounds__(kWave* kWaves, tiles_per_cu(D)) void chunk_queue_kernel(const ChunkArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t s_k0[64 * D], s_v0[64 * D], s_k1[64 * D], s_v1[64 * D];
   __shared__ int s_dirty;
   __shared__ int64_t s_item;
@@ -995,8 +998,8 @@ struct Plan {
 };
 
 constexpr int kCus = 256;
+constexpr int kMaxContext = 1 << 30;  // positions a few tiles past it are still ints
 constexpr int kTilesNt = 2;   // 16-row tiles of a wave of chunk_tiles_kernel
-constexpr int kTilesPerCu = 2;
 // Row tiles of contexts up to this differ too little for the queue and its launch (direct -> queue): 16 prompts of 17-1,023 tokens
 // 31 -> 38 us, 16 x 512 behind 512 151 -> 165, 4 x 2,048 168 -> 173; but 16 of 100-1,900 behind up to 2,000 224 -> 199, 64 of
 // 100-500 behind up to 2,000 325 -> 267, 4 x 2,048 behind up to 6,144 696 -> 535.
@@ -1011,7 +1014,7 @@ Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int max_query_
   constexpr int kStep = kWaves * kTileKeys;
   const int64_t steps = ((int64_t)max_context + kStep - 1) / kStep;
   const int64_t groups = (int64_t)num_seqs * kv_heads * p.row_tiles;
-  const int64_t want = p.tiles ? kTilesPerCu * kCus : kCus * (head_dim == 64 ? 2 : 1);
+  const int64_t want = kCus * (p.tiles ? tiles_per_cu(head_dim) : head_dim == 64 ? 2 : 1);
   int64_t parts = want / groups;  // no second round for a few
   parts = parts < 1 ? 1 : parts > steps ? steps : parts;
   const int64_t per = (steps + parts - 1) / parts;
@@ -1043,7 +1046,7 @@ tq_status launch(const ChunkArgs& a, const Plan& p, hipStream_t stream) {
     hipLaunchKernelGGL(chunk_order_kernel, dim3(1), dim3(kOrderThreads), 0, stream, a, p.rows);
     const tq_status st = check_launch();
     if (st != TQ_OK) return st;
-    hipLaunchKernelGGL((chunk_queue_kernel<D, kTilesNt, T>), dim3(kTilesPerCu * kCus), t, 0, stream, a);
+    hipLaunchKernelGGL((chunk_queue_kernel<D, kTilesNt, T>), dim3(tiles_per_cu(D) * kCus), t, 0, stream, a);
   } else if (p.tiles)
     hipLaunchKernelGGL((chunk_tiles_kernel<D, kTilesNt, T>), g, t, 0, stream, a);
   else
@@ -1067,7 +1070,7 @@ extern "C" size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_he
                                                 int32_t max_context_len) {
   using namespace tq;
   if (!sizes_ok(num_seqs, num_heads, num_kv_heads, head_dim, num_q_rows, max_query_len, max_context_len) ||
-      num_seqs == 0 || num_q_rows == 0 || max_query_len == 0 || max_context_len == 0)
+      num_seqs == 0 || num_q_rows == 0 || max_query_len == 0 || max_context_len == 0 || max_context_len > kMaxContext)
     return 0;
   const int32_t group = num_heads / num_kv_heads;
   return workspace_of(plan_of(num_seqs, num_kv_heads, group, head_dim, max_query_len, max_context_len), num_seqs, num_q_rows,
@@ -1087,7 +1090,8 @@ extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const voi
       num_blocks < 1 || num_blocks > 0x7fffffffLL || num_layers < 1 || block_size < 1 || layer < 0 ||
       layer >= num_layers || max_blocks_per_seq < 0 || !(scale - scale == 0.f))
     return TQ_ERR_INVALID_ARGUMENT;
-  if ((head_dim != 64 && head_dim != 128) || block_size > kMaxBlockSize || (dtype != TQ_F16 && dtype != TQ_BF16))
+  if ((head_dim != 64 && head_dim != 128) || block_size > kMaxBlockSize || (dtype != TQ_F16 && dtype != TQ_BF16) ||
+      max_context_len > kMaxContext)
     return TQ_ERR_UNSUPPORTED;
   if (num_seqs == 0 || num_q_rows == 0 || max_query_len == 0) return TQ_OK;
   const int64_t width = (int64_t)num_heads * head_dim;

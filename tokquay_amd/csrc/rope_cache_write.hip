@@ -108,11 +108,11 @@ __device__ __forceinline__ float head_sum(float v) {
 template <int D, typename T, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rope_cache_write_kernel(const RopeArgs a) {
   constexpr int kLanes = D / 16;  // threads of a head
-  const int head_rows = a.heads + 2 * a.kv_heads;
-  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes;
+  const uint32_t head_rows = a.heads + 2 * a.kv_heads;
+  const uint32_t unit = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;  // below 2^32: 64-bit divisions are slow
   const int64_t n = unit / head_rows;
   if (n >= a.num_tokens) return;  // whole heads: the lanes that trade sums end together
-  const int hr = (int)(unit - n * head_rows), t = threadIdx.x % kLanes;
+  const int hr = (int)(unit - (uint32_t)n * head_rows), t = threadIdx.x % kLanes;
   const int64_t slot = a.slot_mapping[n], pos = a.positions[n];
   if (pos < 0 || pos >= a.num_positions) {
     if (hr == 0 && t == 0) flag_error(a.d_error, TQ_DEVERR_POSITION);
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256) void rope_cache_write_kernel(const RopeArgs a)
   }
   if (slot >= a.num_slots && hr == 0 && t == 0) flag_error(a.d_error, TQ_DEVERR_SLOT);
   const bool cached = slot >= 0 && slot < a.num_slots;
-  const int64_t blk = cached ? slot / a.block_size : 0;
+  const int64_t blk = cached ? (uint32_t)slot / (uint32_t)a.block_size : 0;
   const int64_t at = blk * a.block_stride + (slot - blk * a.block_size) * D;
   const int half = a.rotary / 2;
   const bool turned = 16 * t < a.rotary;
@@ -189,8 +189,10 @@ __global__ __launch_bounds__(256) void rope_cache_write_kernel(const RopeArgs a)
 
 template <int D, typename T>
 tq_status launch(const RopeArgs& a, bool interleaved, hipStream_t stream) {
-  const int64_t grid = (a.num_tokens * (a.heads + 2 * a.kv_heads) * (D / 16) + 255) / 256;
-  if (grid > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
+  constexpr int kUnits = 256 / (D / 16);  // heads of a workgroup
+  const int64_t head_rows = a.heads + 2LL * a.kv_heads;
+  if (a.num_tokens > 0xffff0000LL / head_rows) return TQ_ERR_UNSUPPORTED;
+  const int64_t grid = (a.num_tokens * head_rows + kUnits - 1) / kUnits;
   if (interleaved)
     hipLaunchKernelGGL((rope_cache_write_kernel<D, T, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   else
@@ -220,6 +222,7 @@ extern "C" tq_status tq_rope_cache_write(void* q_out, int64_t q_out_row_stride, 
       rotary_dim > head_dim || (interleaved != 0 && interleaved != 1) || !(eps >= 0.f))
     return TQ_ERR_INVALID_ARGUMENT;
   if ((head_dim != 64 && head_dim != 128) || block_size > kMaxBlockSize || rotary_dim % 16 != 0 ||
+      num_blocks > 0xffffffffLL / block_size || num_heads > 1 << 20 || num_kv_heads > 1 << 20 ||
       (dtype != TQ_F32 && dtype != TQ_F16 && dtype != TQ_BF16))
     return TQ_ERR_UNSUPPORTED;
   if (num_tokens == 0) return TQ_OK;
