@@ -20,9 +20,15 @@
 // the same one (two transposing LDS reads of 4 keys each). Rounding p to the cache's type costs each weight half a
 // step, about as much as the rounding of the output; the rounded weights are summed, so equal values come out exactly.
 //
-// K and V come in 32-key tiles straight from HBM into LDS (16 bytes a lane, no registers), a tile ahead
-// of the products. 16-byte pieces are permuted inside a row as they arrive (swizzled), so that the 16 keys
-// that one LDS read takes lie in different banks.
+// K and V come in tiles straight from HBM into LDS (16 bytes a lane, no registers), a tile ahead of the products.
+// 16-byte pieces are permuted inside a row as they arrive (swizzled), so that what an LDS read takes in a clock
+// lies in different banks.
+//
+// Two kernels. Up to 64 rows a K/V head (tokens, drafted tokens) the bytes of K and V bound it: chunk_rows_kernel streams them,
+// each wave its own keys (128 tokens at 511-4,094 positions, 8 heads of 128: 1.21 GB in 218 us, 5.5 TB/s, where a device copy
+// moves 5.07). More rows share tiles (chunk_tiles_kernel; chunk_queue_kernel over long contexts), and the matrix cores beside
+// the exponentials bound it: 4 x 2,048 tokens behind 768-5,376 cached ones run 550 GFLOP in 525 us (1,047 TFLOP/s; a large
+// bf16 library product reaches 1,370), with the matrix cores busy for 55 % of the cycles and the vector units for 53 %.
 #include <float.h>
 
 #include <utility>
@@ -504,8 +510,10 @@ __device__ __forceinline__ void barrier() {
 // Few rows: a workgroup takes 16 NT rows and one part of the keys; its waves take every fourth tile of the
 // part, each with its own two K and two V buffers in LDS and no barrier, and join their sums in LDS at the end.
 //
-// K and V of the next tile and V of this one are on their way while a tile's scores are computed: 24 KB a wave,
-// 96 KB a CU (D = 128), which covers the latency of HBM at its full rate.
+// K and V of the next tile and V of this one are on their way while a tile's scores are computed: 24 KB a wave, 96 KB a CU
+// (12 KB and two workgroups at D = 64), which covers the latency of HBM at its full rate. With the tile loaded only when the one
+// before was done: 128 tokens at 511-4,094 positions 557 us instead of 218. Tiles of 64 keys at D = 64 changed nothing on average
+// (32 x 5 drafted tokens 39.7 -> 39.2 us, 64 tokens of 12 heads 38 -> 42, 16 x 4 of 28 heads 32 -> 28).
 template <int D, int NT, typename T>
 __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkArgs a) {
   constexpr int kTileElems = kTileKeys * D;
@@ -647,7 +655,8 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
 // in LDS, each loading a quarter. The scores of tile t + 1 are computed beside the weights of tile t (matrix and
 // vector instructions of one iteration do not depend on each other), so one barrier a tile is enough: behind it K of t + 1
 // and V of t are in LDS, and the buffers of K of t and V of t - 1 are free for K of t + 2 and V of t + 1.
-// Workgroups of a CU: as many as have the registers (168 a wave at D = 64, 256 at 128).
+// Workgroups of a CU: as many as have the registers (168 a wave at D = 64, 256 at 128). A third at D = 64: 64 chunks of 100-300
+// tokens 85 -> 78 us, 8 x 1,024 behind 4,000-8,000 293 -> 279.
 constexpr int tiles_per_cu(int head_dim) { return head_dim == 64 ? 3 : 2; }
 
 template <int D, int NT, typename T>
@@ -999,7 +1008,8 @@ struct Plan {
 
 constexpr int kCus = 256;
 constexpr int kMaxContext = 1 << 30;  // positions a few tiles past it are still ints
-constexpr int kTilesNt = 2;   // 16-row tiles of a wave of chunk_tiles_kernel
+// 16-row tiles of a wave of chunk_tiles_kernel. Three spill at D = 128 and are slower at 64 (16 x 100-1,900 tokens 190 -> 198 us).
+constexpr int kTilesNt = 2;
 // Row tiles of contexts up to this differ too little for the queue and its launch (direct -> queue): 16 prompts of 17-1,023 tokens
 // 31 -> 38 us, 16 x 512 behind 512 151 -> 165, 4 x 2,048 168 -> 173; but 16 of 100-1,900 behind up to 2,000 224 -> 199, 64 of
 // 100-500 behind up to 2,000 325 -> 267, 4 x 2,048 behind up to 6,144 696 -> 535.
@@ -1015,7 +1025,7 @@ Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int max_query_
   const int64_t steps = ((int64_t)max_context + kStep - 1) / kStep;
   const int64_t groups = (int64_t)num_seqs * kv_heads * p.row_tiles;
   const int64_t want = kCus * (p.tiles ? tiles_per_cu(head_dim) : head_dim == 64 ? 2 : 1);
-  int64_t parts = want / groups;  // no second round for a few
+  int64_t parts = want / groups;  // no second round for a few (259 tokens behind 32,500: 8 parts 220 us, 7 175)
   parts = parts < 1 ? 1 : parts > steps ? steps : parts;
   const int64_t per = (steps + parts - 1) / parts;
   p.part_tokens = (int)(per * kStep > 0x7fffffff - kStep ? 0x7fffffff / kStep * kStep : per * kStep);

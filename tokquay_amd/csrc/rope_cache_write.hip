@@ -8,7 +8,8 @@
 // with cos and sin from the caller's fp32 table, so their angles are as exact as the caller made them; all
 // arithmetic is fp32, rounded once to the rows' type.
 //
-// HBM bound: every element is read once and written once. A thread holds 16 elements of one head, the two
+// HBM bound: every element is read once and written once (8,192 tokens of 32 + 8 + 8 heads of 128, normed: 206 MB in 45 us, 4.5
+// TB/s, where a device copy moves 5.07). A thread holds 16 elements of one head, the two
 // octets that the rotation pairs (8 t .. and R / 2 + 8 t .., or 16 t ..), so both are moved by 16-byte accesses
 // and the pairs meet in registers; the D / 16 threads of a head share its sum of squares by lane permutations.
 

@@ -12,10 +12,12 @@
 // not matter. Two launches:
 //
 // 1. stats: one workgroup per row and chunk of columns keeps its logits in registers and leaves their maximum and their
-//    sum of exponentials. The logits are read once: HBM bound.
+//    sum of exponentials. The logits are read once, 21 vector instructions each, which take about as long as their
+//    bytes: 640 rows of 128,000 fp32 logits 71 us (4.6 TB/s), 288 of 50,257 bf16 ones 17 us.
 // 2. draw: one workgroup per sequence and chunk joins the rows' statistics, finds the first token that does not
 //    stand and sums its chunk's weights of that row; the last workgroup of a sequence to finish finds the chunk the draw
-//    falls in, and the column in it.
+//    falls in, and the column in it (one sequence of 4 drafts: 11 us, dependent steps of 1-2 us). With many sequences the
+//    decision is a launch of its own between the two (128 of 4 drafts over 128,000 columns: draw 73 -> 6 + 47 us).
 
 #include <type_traits>
 
@@ -72,9 +74,9 @@ __device__ __forceinline__ double exp2_neg(double t) {
   r = __builtin_fma(r, f, 2.4022650695888503e-01);
   r = __builtin_fma(r, f, 6.931471805568324e-01);
   r = __builtin_fma(r, f, 1.0);
-  const uint64_t bits = __builtin_bit_cast(uint64_t, r);
-  const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, shifted);
-  return __builtin_bit_cast(double, bits + ((uint64_t)k << 52));
+  u32x2 bits = __builtin_bit_cast(u32x2, r);
+  bits[1] += __builtin_bit_cast(u32x2, shifted)[0] << 20;
+  return __builtin_bit_cast(double, bits);
 }
 
 template <typename T>
@@ -539,8 +541,8 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs 
 }
 
 constexpr int kMaxVocab = kThreads * kThreads * 32;  // a chunk a thread
-constexpr int kFewDraws = 1024;
-constexpr int kDecideFrom = 512;  // workgroups of the draw from which one decision a sequence is worth its launch
+constexpr int kFewDraws = 1024;   // workgroups of the draw up to which 2,048 columns each end sooner than 4,096
+constexpr int kDecideFrom = 512;  // and from which one decision a sequence is worth its launch (64 sequences: 42 -> 39 us in all)
 
 // How a call is split, and its workspace.
 struct Plan {
