@@ -259,3 +259,19 @@ def test_refusals():
             ops.verify_drafts(**{**good, name: value})
     with pytest.raises(ValueError, match="tokens must be"):
         ops.verify_drafts(**good, tokens=torch.zeros(2, 4, dtype=torch.int64, device="cuda"))
+
+
+@pytest.mark.parametrize("sequences", [3, 200])
+def test_a_draft_of_any_weight_is_left_out(sequences):
+    # Drafts with between a thousandth of the weight and all but a millionth of it, none of which stands.
+    c = Case([2] * sequences, 20000, torch.float32, False, seed=17)
+    rows = torch.arange(0, 2 * sequences, 2)
+    c.drafts[rows] = torch.arange(sequences) * 7919 % 20000
+    c.logits[rows, c.drafts[rows]] = -math.inf
+    others = torch.logsumexp(c.logits[rows], -1)
+    c.logits[rows, c.drafts[rows]] = others + torch.linspace(-7.0, 14.0, sequences)
+    c.uniforms[rows] = 1 - 2.0**-24
+    assert c.check() == 0
+    tokens, accepted = c.run()
+    assert bool((accepted == 0).all())
+    assert bool((tokens[:, 0] != c.drafts[rows]).all())

@@ -9,15 +9,16 @@
 //
 // Which side of a border of that running sum u_last falls on decides a token, and 100,000 borders lie
 // close: exponentials and sums are fp64 (fp64 FMAs run at the fp32 rate here), which also makes the order of a sum
-// not matter. Two launches:
+// not matter.
 //
 // 1. stats: one workgroup per row and chunk of columns keeps its logits in registers and leaves their maximum and their
 //    sum of exponentials. The logits are read once, 21 vector instructions each, which take about as long as their
-//    bytes: 640 rows of 128,000 fp32 logits 71 us (4.6 TB/s), 288 of 50,257 bf16 ones 17 us.
-// 2. draw: one workgroup per sequence and chunk joins the rows' statistics, finds the first token that does not
-//    stand and sums its chunk's weights of that row; the last workgroup of a sequence to finish finds the chunk the draw
-//    falls in, and the column in it (one sequence of 4 drafts: 11 us, dependent steps of 1-2 us). With many sequences the
-//    decision is a launch of its own between the two (128 of 4 drafts over 128,000 columns: draw 73 -> 6 + 47 us).
+//    bytes in fp32, twice as long in 16 bits: 640 rows of 128,000 fp32 logits 72 us (4.6 TB/s), 288 of 50,257 bf16 ones 16 us.
+// 2. decide: one workgroup per sequence joins the rows' statistics, finds the first token that does not stand and, but for draws
+//    from max(p - q, 0), the chunk the next token falls in, from the statistics again, and the column in that.
+// 3. draw, where q is given: one workgroup per sequence and chunk sums its chunk of max(p - q, 0); the last workgroup of a
+//    sequence to finish finds chunk and column. A few sequences do without 2: each workgroup decides, all draw (one sequence of
+//    4 drafts: 10 us, dependent steps of 1-2 us).
 
 #include <type_traits>
 
@@ -140,19 +141,19 @@ __device__ __forceinline__ float wave_maximum(float v) {  // NaN, if any is
 template <typename T>
 constexpr int kVec = __is_same(T, float) ? 4 : 8;  // logits in 16 bytes
 
-// Thread t's column i of a chunk: pieces of VEC columns t, t + 256, .., or (RUNS) PER columns in a row.
-template <int VEC, int PER, bool RUNS>
+// Thread t's column i of a chunk: pieces of VEC columns t, t + N, .. (of N threads), or (RUNS) PER columns in a row.
+template <int VEC, int N, int PER, bool RUNS>
 __device__ __forceinline__ int column_of(int i) {
-  return RUNS ? (int)threadIdx.x * PER + i : (i / VEC * kThreads + (int)threadIdx.x) * VEC + i % VEC;
+  return RUNS ? (int)threadIdx.x * PER + i : (i / VEC * N + (int)threadIdx.x) * VEC + i % VEC;
 }
 
 // Those columns of a row of T as floats, columns past n as -inf. Rows start at any element.
-template <typename T, int VEC, int PER, bool RUNS>
+template <typename T, int VEC, int N, int PER, bool RUNS>
 __device__ __forceinline__ void columns(const void* row, int base, int n, float (&x)[PER]) {
   constexpr int kSize = __is_same(T, float) ? 4 : 2;
 #pragma unroll
   for (int v = 0; v < PER; v += VEC) {
-    const int at = column_of<VEC, PER, RUNS>(v);
+    const int at = column_of<VEC, N, PER, RUNS>(v);
     if (at + VEC <= n) {
       u32x4 w[VEC * kSize / 16];
       __builtin_memcpy(w, static_cast<const char*>(row) + (int64_t)(base + at) * kSize, VEC * kSize);
@@ -172,14 +173,20 @@ __device__ __forceinline__ void columns(const void* row, int base, int n, float 
 
 constexpr double kLog2e = 1.4426950408889634;
 
-// The temperature of the sequence that a row belongs to: the last one with cu[b] <= row (empty sequences hold no row), counted 64
-// at a time. Asked for before the logits, it arrives before them.
+// The temperature of the sequence that a row belongs to: the last one with cu[b] <= row (empty sequences hold no row), among 64
+// parts at a time. Asked for before the logits, it arrives before them. (Counted through all 1,024 sequences of 5 rows, 50,257 bf16
+// logits each, the call took 328 us instead of 259.)
 __device__ __forceinline__ float temperature_of(const VerifyArgs& a, int row) {
   const int lane = threadIdx.x & (kWave - 1);
-  int b = -1;
-  for (int b0 = 0; b0 < a.num_seqs; b0 += kWave)
-    b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b0 + lane < a.num_seqs && a.cu[b0 + lane] <= row));
-  return a.temperature[max(b, 0)];
+  int64_t b = 0, n = a.num_seqs;
+  while (n > 1) {
+    const int64_t step = (n + kWave - 1) / kWave, at = b + lane * step;
+    const int k = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane * step < n && a.cu[at] <= row));
+    const int64_t skip = max(k - 1, 0) * step;
+    b += skip;
+    n = min(step, n - skip);
+  }
+  return a.temperature[b];
 }
 
 template <typename T, int PER>
@@ -194,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs
   const int base = chunk * kThreads * PER, n = min(kThreads * PER, a.vocab - base);
   float x[PER], top = -INFINITY;
   const float temp = temperature_of(a, row);
-  columns<T, kVec<T>, PER, false>(row_of<T>(a, row), base, n, x);
+  columns<T, kVec<T>, kThreads, PER, false>(row_of<T>(a, row), base, n, x);
 #pragma unroll
   for (int i = 0; i < PER; ++i) top = __builtin_elementwise_maximum(top, x[i]);  // NaN, if any is
   top = wave_maximum(top);
@@ -215,7 +222,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs
     int mine = 0x7fffffff;
 #pragma unroll
     for (int i = PER - 1; i >= 0; --i) {
-      const int at = column_of<kVec<T>, PER, false>(i);
+      const int at = column_of<kVec<T>, kThreads, PER, false>(i);
       if (at < n && (top != top ? x[i] != x[i] : x[i] == top)) mine = at;
     }
     atomicMin(&s_col, mine);
@@ -262,9 +269,8 @@ __device__ __forceinline__ Dist dist_of(const VerifyArgs& a, int row, float temp
   return d;
 }
 
-// p of a column, times sum (the draw needs no division). A logit of -inf has none.
-__device__ __forceinline__ double mass_of(const Dist& d, float logit, int64_t col) {
-  if (d.peak) return col == d.best ? 1.0 : 0.0;
+// p of a column times sum (the draw needs no division), of a distribution without peak. A logit of -inf has none.
+__device__ __forceinline__ double mass_of(const Dist& d, float logit) {
   const double t = ((double)logit - (double)d.top) * d.c;
   return t >= -1000.0 ? exp2_neg(t) : 0.0;
 }
@@ -273,33 +279,34 @@ enum Mode { kAll, kLess, kWithout };  // the draw is from p, from p - q where po
 
 // The draw's weight of a column, times sum.
 __device__ __forceinline__ double weight_of(const Dist& d, float logit, double q, int64_t draft, int mode, int64_t col) {
-  const double p = mass_of(d, logit, col);
+  const double p = mass_of(d, logit);
   if (mode == kAll) return p;
   if (mode == kWithout) return col == draft ? 0.0 : p;
-  const double w = p - (d.peak ? q : q * d.sum);
+  const double w = p - q * d.sum;
   return w > 0.0 ? w : 0.0;
 }
 
 // The weights of a thread's columns of a chunk.
-template <typename T, int PER, bool RUNS, typename F>
+template <typename T, int N, int PER, bool RUNS, typename F>
 __device__ __forceinline__ void weights(const Dist& d, const void* row, const float* qrow, int64_t draft, int mode,
                                         int base, int n, F&& put) {
   float x[PER], q[PER];
-  columns<T, kVec<T>, PER, RUNS>(row, base, n, x);
+  columns<T, kVec<T>, N, PER, RUNS>(row, base, n, x);
   if (mode == kLess) {
-    columns<float, kVec<T>, PER, RUNS>(qrow, base, n, q);
+    columns<float, kVec<T>, N, PER, RUNS>(qrow, base, n, q);
   } else {
 #pragma unroll
     for (int i = 0; i < PER; ++i) q[i] = 0.f;
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int at = column_of<kVec<T>, PER, RUNS>(i);
+    const int at = column_of<kVec<T>, N, PER, RUNS>(i);
     put(i, at < n ? weight_of(d, x[i], (double)q[i], draft, mode, base + at) : 0.0);
   }
 }
 
-// Inclusive sums over the workgroup's threads, in order; s_part: a word a wave.
+// Inclusive sums over the workgroup's N threads, in order; s_part: a word a wave.
+template <int N>
 __device__ __forceinline__ double scan(double v, double* s_part) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   auto up = [&](auto ctrl) {  // from a lane further down in the row of 16; 0 past its start
@@ -320,12 +327,13 @@ __device__ __forceinline__ double scan(double v, double* s_part) {
   __syncthreads();
   before = 0.0;
 #pragma unroll
-  for (int u = 0; u < kWaves - 1; ++u) before += u < wave ? s_part[u] : 0.0;
+  for (int u = 0; u < N / kWave - 1; ++u) before += u < wave ? s_part[u] : 0.0;
   __syncthreads();
   return before + v;
 }
 
 // The first thread with `over`, or the last with `has` where there is none; -1: none either. s_pick: two words a wave.
+template <int N>
 __device__ __forceinline__ int pick(bool over, bool has, int (*s_pick)[2]) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const uint64_t overs = __builtin_amdgcn_ballot_w64(over), those = __builtin_amdgcn_ballot_w64(has);
@@ -336,7 +344,7 @@ __device__ __forceinline__ int pick(bool over, bool has, int (*s_pick)[2]) {
   __syncthreads();
   int first = 0x7fffffff, last = -1;
 #pragma unroll
-  for (int v = 0; v < kWaves; ++v) {
+  for (int v = 0; v < N / kWave; ++v) {
     first = min(first, s_pick[v][0]);
     last = max(last, s_pick[v][1]);
   }
@@ -356,8 +364,8 @@ struct DecideShared {
   int first, bad;
 };
 
-// By one workgroup. `lead`: it also writes the tokens that stand, and the flags.
-template <typename T>
+// By one workgroup of N threads. `lead`: it also writes the tokens that stand, and the flags.
+template <typename T, int N>
 __device__ __forceinline__ Decision decide(const VerifyArgs& a, int b, bool lead, DecideShared& sh) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int lo = a.cu[b];
@@ -367,7 +375,7 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, int b, bool lead
   if (lo < 0 || rows <= 0 || lo + rows > a.num_rows || rows > a.max_rows) {
     if (lead) {
       if (rows != 0 && threadIdx.x == 0) flag_error(a.d_error, TQ_DEVERR_LENGTH);
-      for (int i = threadIdx.x; i < a.max_rows; i += kThreads) out[i] = -1;
+      for (int i = threadIdx.x; i < a.max_rows; i += N) out[i] = -1;
       if (threadIdx.x == 0) a.accepted[b] = 0;
     }
     r.first = -1;
@@ -394,14 +402,14 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, int b, bool lead
         if (a.probs != nullptr) qx = a.probs[(int64_t)(lo + i0 + lane) * a.probs_stride + x];
       }
     }
-    for (int i = i0 + wave; i <= drafts && i < i0 + kWave && i <= *(volatile int*)&sh.first; i += kWaves) {
+    for (int i = i0 + wave; i <= drafts && i < i0 + kWave && i <= *(volatile int*)&sh.first; i += N / kWave) {
       const Dist d = dist_of(a, lo + i, temp);
       if (lane == 0 && i < kDists) sh.dist[i] = d;
       if (d.peak && temp > 0.f && lane == 0) atomicMin(&sh.bad, i);
       if (lane == i - i0 && i < drafts) {
         bool stands = false;
         if (in) {
-          const double p = d.peak ? (x == d.best ? 1.0 : 0.0) : mass_of(d, lx, x) / d.sum;
+          const double p = d.peak ? (x == d.best ? 1.0 : 0.0) : mass_of(d, lx) / d.sum;
           stands = (double)ux * (double)qx < p;
         }
         if (!stands) atomicMin(&sh.first, i);
@@ -419,7 +427,7 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, int b, bool lead
   }
   r.dist = sh.dist[r.first < kDists ? r.first : 0];
   if (lead) {
-    for (int i = threadIdx.x; i < a.max_rows; i += kThreads)
+    for (int i = threadIdx.x; i < a.max_rows; i += N)
       if (i != r.first) out[i] = i < r.first ? a.drafts[lo + i] : -1;
     if (threadIdx.x == 0) {
       a.accepted[b] = r.first;
@@ -431,48 +439,149 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, int b, bool lead
   return r;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_decide_kernel(const VerifyArgs a) {
-  __shared__ DecideShared s_decide;
-  const Decision r = decide<T>(a, blockIdx.x, true, s_decide);
-  if (threadIdx.x == 0) a.decisions[blockIdx.x] = r;
+template <int N>
+struct DrawShared {
+  double part[N / kWave], goal;
+  int turn, pick[N / kWave][2];
+};
+
+// The sum of a chunk's weights, by the workgroup.
+template <typename T, int N, int PER>
+__device__ __forceinline__ double chunk_sum(const VerifyArgs& a, const Dist& d, const void* row, const float* qrow,
+                                            int64_t draft, int mode, int chunk, DrawShared<N>& sh) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, at = chunk * N * PER;
+  double w = 0.0;
+  weights<T, N, PER, false>(d, row, qrow, draft, mode, at, min(N * PER, a.vocab - at), [&](int, double v) { w += v; });
+  w = wave_sum(w);
+  if (lane == 0) sh.part[wave] = w;
+  __syncthreads();
+  w = 0.0;
+#pragma unroll
+  for (int v = 0; v < N / kWave; ++v) w += sh.part[v];
+  __syncthreads();
+  return w;
 }
 
-// DECIDED: by verify_decide_kernel; else each workgroup decides for itself.
+// The workgroup's sum of mine, in all of its threads; upto: up to this one.
+template <int N>
+__device__ __forceinline__ double total_of(double mine, double& upto, DrawShared<N>& sh) {
+  upto = scan<N>(mine, sh.part);
+  if (threadIdx.x == N - 1) sh.goal = upto;
+  __syncthreads();
+  return sh.goal;
+}
+
+// The draw, from the chunks' sums (thread c's: of chunk c, and up to it): the chunk it falls in, the last one with weight where
+// rounding leaves none above the goal, and the column in that.
+template <typename T, int N, int PER>
+__device__ __forceinline__ void draw(const VerifyArgs& a, const Dist& d, const void* row, const float* qrow, int64_t draft,
+                                     int mode, double mine, double upto, double goal, int64_t* token, DrawShared<N>& sh) {
+  const int c = threadIdx.x;
+  const int chosen = pick<N>(mine > 0.0 && upto > goal, mine > 0.0, sh.pick);
+  if (chosen < 0) {  // no weight anywhere: draft probabilities that are not numbers
+    if (c == 0) *token = d.best;
+    return;
+  }
+  if (c == chosen) sh.goal = goal - (upto - mine);
+  // Runs of PER columns a thread.
+  const int at = chosen * N * PER;
+  double ws[PER], run = 0.0;
+  weights<T, N, PER, true>(d, row, qrow, draft, mode, at, min(N * PER, a.vocab - at), [&](int i, double v) {
+    ws[i] = v;
+    run += v;
+  });
+  upto = scan<N>(run, sh.part);
+  const double rest = sh.goal;
+  if (c == pick<N>(run > 0.0 && upto > rest, run > 0.0, sh.pick)) {
+    double cum = upto - run;
+    int col = -1;
+    bool done = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      cum += ws[i];
+      if (!done && ws[i] > 0.0) {
+        col = at + c * PER + i;
+        done = cum > rest;
+      }
+    }
+    *token = col;
+  }
+}
+
+// One workgroup a sequence. Where the draw is not from a difference, the statistics hold its chunks' sums already, less the draft
+// (whose chunk is summed again without it: the rest may be far below it; only doing so where it has more than half of the weight
+// saves nothing), and the sequence ends here; the others' decisions are left for verify_draw_kernel. A chunk of the statistics
+// is 8 columns a thread: 64 sequences of 50,257 columns 13.8 us with 1,024 threads, 19.2 with 256 of 32 columns.
+template <typename T, int N>
+__global__ __launch_bounds__(N) void verify_decide_kernel(const VerifyArgs a) {
+  __shared__ DecideShared s_decide;
+  __shared__ DrawShared<N> sh;
+  constexpr int kPer = 8;  // columns of a thread in a chunk of the statistics
+  const int b = blockIdx.x, c = threadIdx.x;
+  Decision r = decide<T, N>(a, b, true, s_decide);
+  const int lo = a.cu[b], drafts = a.cu[b + 1] - lo - 1, row = lo + r.first;
+  const bool less = r.first >= 0 && r.first < drafts && a.probs != nullptr && !r.dist.peak;
+  if (a.probs != nullptr && c == 0) {
+    a.decisions[b] = r;
+    if (!less) a.decisions[b].first = -1;
+  }
+  if (r.first < 0 || less) return;
+  const Dist d = r.dist;
+  int64_t* token = a.tokens + (int64_t)b * a.max_rows + r.first;
+  if (d.peak) {  // whatever q is
+    if (c == 0) *token = d.best;
+    return;
+  }
+  const Stat* st = a.stats + (int64_t)row * a.chunks;
+  const void* lp = row_of<T>(a, row);
+  const double u = (double)a.uniforms[lo + drafts];
+  const int64_t draft = r.first < drafts ? a.drafts[row] : -1;
+  double all = 0.0;
+  if (c < a.chunks) {
+    const double t = ((double)key_value(st[c].key) - (double)d.top) * d.c;
+    if (t >= -1000.0) all = st[c].sum * exp2_neg(t);  // else no column of it has weight
+  }
+  double mine = all, upto;
+  int mode = kAll;
+  if (draft >= 0 && draft < a.vocab) {
+    mode = kWithout;
+    const int skip = (int)draft / (N * kPer);
+    const double sum = chunk_sum<T, N, kPer>(a, d, lp, nullptr, draft, mode, skip, sh);
+    if (c == skip) mine = sum;
+  }
+  double total = total_of<N>(mine, upto, sh);
+  if (!(total > 0.0)) {  // p is all on the draft (to rounding): the draw is from p itself
+    mode = kAll;
+    mine = all;
+    total = total_of<N>(mine, upto, sh);
+  }
+  draw<T, N, kPer>(a, d, lp, nullptr, draft, mode, mine, upto, u * total, token, sh);
+}
+
+// One workgroup a sequence and chunk. DECIDED: by verify_decide_kernel; else each decides for itself.
 template <typename T, int PER, bool DECIDED>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs a) {
-  __shared__ int s_turn, s_pick[kWaves][2];
-  __shared__ double s_part[kWaves], s_goal;
-  constexpr int kChunk = kThreads * PER;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  __shared__ DrawShared<kThreads> sh;
   const int chunk = blockIdx.x % a.draw_chunks, b = blockIdx.x / a.draw_chunks;
   Decision r;
   if constexpr (DECIDED) {
     r = a.decisions[b];
   } else {
     __shared__ DecideShared s_decide;
-    r = decide<T>(a, b, chunk == 0, s_decide);
+    r = decide<T, kThreads>(a, b, chunk == 0, s_decide);
   }
   if (r.first < 0) return;
   const Dist d = r.dist;
-  const int lo = a.cu[b], drafts = a.cu[b + 1] - lo - 1, first = r.first, row = lo + first;
+  const int lo = a.cu[b], drafts = a.cu[b + 1] - lo - 1, row = lo + r.first;
   const void* lp = row_of<T>(a, row);
-  const float* qrow = a.probs == nullptr ? nullptr : a.probs + (int64_t)row * a.probs_stride;
-  const int64_t draft = first < drafts ? a.drafts[row] : -1;
-  int mode = first == drafts ? kAll : qrow != nullptr ? kLess : kWithout;
-  auto chunk_sum = [&](int c) {  // of this workgroup's waves, in thread 0
-    double w = 0.0;
-    weights<T, PER, false>(d, lp, qrow, draft, mode, c * kChunk, min(kChunk, a.vocab - c * kChunk),
-                           [&](int, double v) { w += v; });
-    w = wave_sum(w);
-    if (lane == 0) s_part[wave] = w;
-    __syncthreads();
-    w = 0.0;
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v) w += s_part[v];
-    return w;
-  };
-  const double w = chunk_sum(chunk);
+  const float* qrow = a.probs + (int64_t)row * a.probs_stride;
+  int64_t* token = a.tokens + (int64_t)b * a.max_rows + r.first;
+  if (!DECIDED && d.peak) {
+    if (chunk == 0 && threadIdx.x == 0) *token = d.best;
+    return;
+  }
+  int mode = r.first == drafts ? kAll : kLess;
+  const double w = chunk_sum<T, kThreads, PER>(a, d, lp, qrow, -1, mode, chunk, sh);
   double* sums = a.sums + (int64_t)b * a.draw_chunks;
   if (threadIdx.x == 0) {
     // The sums are all that workgroups hand each other, by accesses of agent scope, which are done where all XCDs meet: the
@@ -481,86 +590,55 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs 
     __hip_atomic_store(&sums[chunk], w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    s_turn = (int)__hip_atomic_fetch_add(&a.arrived[b], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sh.turn = (int)__hip_atomic_fetch_add(&a.arrived[b], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  if (s_turn != a.draw_chunks - 1) return;
+  if (sh.turn != a.draw_chunks - 1) return;
 
-  // The last workgroup of the sequence: the chunk that the draw falls in (the last one with weight where rounding
-  // leaves none above the goal), a chunk a thread.
+  // The last workgroup of the sequence, a chunk a thread.
   const int c = threadIdx.x;
-  const double u = (double)a.uniforms[lo + drafts];
-  double mine = c < a.draw_chunks ? __hip_atomic_load(&sums[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
-  double upto = scan(mine, s_part);
-  if (c == kThreads - 1) s_goal = upto;
-  __syncthreads();
-  if (!(s_goal > 0.0)) {
+  double mine = c < a.draw_chunks ? __hip_atomic_load(&sums[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0, upto;
+  double total = total_of<kThreads>(mine, upto, sh);
+  if (!(total > 0.0)) {
     // Nothing left where q covers p (to rounding): the draw is from p itself.
     mode = kAll;
     mine = 0.0;
     __syncthreads();
     for (int k = 0; k < a.draw_chunks; ++k) {
-      const double sum = chunk_sum(k);
+      const double sum = chunk_sum<T, kThreads, PER>(a, d, lp, qrow, -1, mode, k, sh);
       mine = c == k ? sum : mine;
-      __syncthreads();
     }
-    upto = scan(mine, s_part);
-    if (c == kThreads - 1) s_goal = upto;
-    __syncthreads();
+    total = total_of<kThreads>(mine, upto, sh);
   }
-  const double goal = u * s_goal;
-  const int chosen = pick(mine > 0.0 && upto > goal, mine > 0.0, s_pick);
-  if (chosen < 0) {  // no weight anywhere: draft probabilities that are not numbers
-    if (c == 0) a.tokens[(int64_t)b * a.max_rows + first] = d.best;
-    return;
-  }
-  if (c == chosen) s_goal = goal - (upto - mine);
-  // The column in it: runs of PER columns a thread.
-  const int at = chosen * kChunk;
-  double ws[PER], run = 0.0;
-  weights<T, PER, true>(d, lp, qrow, draft, mode, at, min(kChunk, a.vocab - at), [&](int i, double v) {
-    ws[i] = v;
-    run += v;
-  });
-  upto = scan(run, s_part);
-  const double rest = s_goal;
-  if (c == pick(run > 0.0 && upto > rest, run > 0.0, s_pick)) {
-    double cum = upto - run;
-    int token = -1;
-    bool done = false;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      cum += ws[i];
-      if (!done && ws[i] > 0.0) {
-        token = at + c * PER + i;
-        done = cum > rest;
-      }
-    }
-    a.tokens[(int64_t)b * a.max_rows + first] = token;
-  }
+  draw<T, kThreads, PER>(a, d, lp, qrow, -1, mode, mine, upto, (double)a.uniforms[lo + drafts] * total, token, sh);
 }
 
 constexpr int kMaxVocab = kThreads * kThreads * 32;  // a chunk a thread
-constexpr int kFewDraws = 1024;   // workgroups of the draw up to which 2,048 columns each end sooner than 4,096
-constexpr int kDecideFrom = 512;  // and from which one decision a sequence is worth its launch (64 sequences: 42 -> 39 us in all)
+// Workgroups of the draw up to which 2,048 columns each end sooner than 4,096 (sequences of 4 drafts with q, both launches: 8 over
+// 50,257 bf16 columns 15.6 and 17.3 us, 16 20.3 and 20.6, 32 26.8 and 24.8; 8,192 columns 23.2, 25.3, 29.1), and from which a
+// decision launch pays (32 over 128,000 fp32 columns 47 us with, 42 without; 128 over 50,257 55 and 55; 64 over 128,000 63 and 69;
+// 128 108 and 133).
+constexpr int kFewDraws = 400;
+constexpr int kDecideFrom = 1664;
 
 // How a call is split, and its workspace.
 struct Plan {
-  int per, draw_per;  // columns of a thread in the two launches: 8 or 32
+  int per, draw_per;  // columns of a thread in stats (8 or 32) and draw (8, 16, or 32 where 256 chunks ask for it)
   int chunks, draw_chunks;
-  bool decide;  // a launch between them
+  bool decide;  // a launch between them, where q is given
   size_t stats, decisions, sums, arrived, bytes;  // offsets
 };
 
 Plan plan_of(int32_t num_seqs, int32_t num_rows, int32_t vocab) {
   Plan p;
   auto chunks = [&](int per) { return (vocab + kThreads * per - 1) / (kThreads * per); };
-  // 32 columns a thread keep the loads of a row in flight; 8 spread few rows over more CUs.
+  // 32 columns a thread keep the loads of a row in flight (640 rows of 128,000 fp32 logits 73 us, with 16 82, with 8 95); 8 spread
+  // few rows over more CUs (5 rows of 50,257: 3.6 us, with 16 4.0).
   p.per = (int64_t)num_rows * chunks(32) < 512 && chunks(8) <= kThreads ? 8 : 32;
   p.draw_per = chunks(8) <= kThreads && (int64_t)num_seqs * chunks(8) <= kFewDraws ? 8 : chunks(16) <= kThreads ? 16 : 32;
   p.chunks = chunks(p.per);
   p.draw_chunks = chunks(p.draw_per);
-  p.decide = (int64_t)num_seqs * p.draw_chunks > kDecideFrom;
+  p.decide = (int64_t)num_seqs * p.draw_chunks >= kDecideFrom;
   p.stats = 0;
   p.decisions = p.stats + (size_t)num_rows * p.chunks * sizeof(Stat);
   p.sums = p.decisions + (size_t)num_seqs * sizeof(Decision);
@@ -590,15 +668,19 @@ tq_status launch(const VerifyArgs& a, const Plan& p, hipStream_t stream) {
     hipLaunchKernelGGL((verify_stats_kernel<T, 32>), dim3((unsigned)stats), dim3(kThreads), 0, stream, a);
   tq_status st = check_launch();
   if (st != TQ_OK) return st;
-  if (p.decide) {
-    hipLaunchKernelGGL((verify_decide_kernel<T>), dim3((unsigned)a.num_seqs), dim3(kThreads), 0, stream, a);
+  const bool decided = p.decide || a.probs == nullptr;
+  if (decided) {
+    if (p.per == 8)
+      hipLaunchKernelGGL((verify_decide_kernel<T, kThreads>), dim3((unsigned)a.num_seqs), dim3(kThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL((verify_decide_kernel<T, 4 * kThreads>), dim3((unsigned)a.num_seqs), dim3(4 * kThreads), 0, stream, a);
     st = check_launch();
-    if (st != TQ_OK) return st;
+    if (st != TQ_OK || a.probs == nullptr) return st;
   }
   switch (p.draw_per) {
-    case 8: return launch_draw<T, 8>(a, p.decide, stream);
-    case 16: return launch_draw<T, 16>(a, p.decide, stream);
-    default: return launch_draw<T, 32>(a, p.decide, stream);
+    case 8: return launch_draw<T, 8>(a, decided, stream);
+    case 16: return launch_draw<T, 16>(a, decided, stream);
+    default: return launch_draw<T, 32>(a, decided, stream);
   }
 }
 
