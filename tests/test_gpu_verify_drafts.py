@@ -275,3 +275,31 @@ def test_a_draft_of_any_weight_is_left_out(sequences):
     tokens, accepted = c.run()
     assert bool((accepted == 0).all())
     assert bool((tokens[:, 0] != c.drafts[rows]).all())
+
+
+@pytest.mark.parametrize("probs", [True, False])
+def test_thousands_of_sequences_each_by_its_temperature(probs):
+    g = torch.Generator().manual_seed(23)
+    rows = torch.randint(0, 3, (5000,), generator=g).tolist()
+    assert Case(rows, 11, torch.float32, probs, temps=(0.5, 0.0, 1.0, 2.0, 0.25), seed=24).check() == 0
+
+
+@pytest.mark.parametrize("probs", [True, False])
+def test_a_captured_batch_replays(probs):
+    # 130 sequences of 13 chunks of 4,096 columns: the decision is a launch of its own, with probabilities too.
+    a, b = (Case([2] * 130, 50257, torch.bfloat16, probs, seed=s) for s in (25, 26))
+    put = [None if t is None else t.cuda() for t in (a.logits, a.drafts, a.uniforms, a.cu, a.temperature, a.probs)]
+    wants = [verified(c.logits, c.drafts, c.uniforms, c.cu, 2, c.temperature, c.probs) for c in (a, b)]
+    l, d, u, cu, t, p = put
+    ops.verify_drafts(l, d, u, cu, 2, t, p)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tokens, accepted = ops.verify_drafts(l, d, u, cu, 2, t, p)
+    for i in (0, 1, 0, 1):
+        c = (a, b)[i]
+        for to, x in zip(put, (c.logits, c.drafts, c.uniforms, c.cu, c.temperature, c.probs)):
+            if to is not None:
+                to.copy_(x)
+        tokens.zero_()
+        graph.replay()
+        assert torch.equal(tokens.cpu(), wants[i][0]) and torch.equal(accepted.cpu(), wants[i][1])
