@@ -938,46 +938,57 @@ __global__ __launch_bounds__(kWave* kWaves, tiles_per_cu(D)) void chunk_queue_ke
   }
 }
 
-// Joins the parts of each (row, head): one wave a pair. A lane first takes a part's maximum and weight sum, then D / 64 dims
-// of all parts, whose loads do not depend on each other.
+// Joins the parts of each (row, head). A lane first takes a part's maximum and weight sum, then some dims of all parts, whose loads
+// do not depend on each other. 16 lanes a pair at D = 64, a wave at 128, where the pair's place is worked out once a wave (4 x 256
+// rows of 12 heads of 64 in two parts: whole launch 24.6 us, with a wave a pair 35.5; 512 rows of 32 heads of 128: 21.7, with 32
+// lanes a pair 25.6).
+template <int D>
+constexpr int kJoinLanes = D == 64 ? 16 : kWave;
+template <int D>
+constexpr int kJoinPairs = 256 / kJoinLanes<D>;
+
 template <int D, typename T>
 __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkArgs a) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const int tiles = (a.max_query_len * a.num_heads + 3) / 4;
+  constexpr int kLanes = kJoinLanes<D>, kDims = D / kLanes;
+  typedef float Dims __attribute__((ext_vector_type(kDims)));
+  const int lane = threadIdx.x % kLanes;
+  const int tiles = (a.max_query_len * a.num_heads + kJoinPairs<D> - 1) / kJoinPairs<D>;
   const int b = blockIdx.x / tiles;
-  const int pair = __builtin_amdgcn_readfirstlane((blockIdx.x - b * tiles) * 4 + threadIdx.x / kWave);
+  int pair = (blockIdx.x - b * tiles) * kJoinPairs<D> + threadIdx.x / kLanes;
+  if constexpr (kLanes == kWave) pair = __builtin_amdgcn_readfirstlane(pair);
   Seq s;
   if (!seq_of(a, b, false, s)) return;
   const int t = pair / a.num_heads, h = pair - t * a.num_heads;
   if (t >= s.nq) return;
   const int parts = (s.start + t) / a.part_tokens + 1;  // parts that the row sees
   const int64_t at = ((int64_t)(s.row0 + t) * a.num_heads + h) * a.parts;
-  constexpr int kDims = D / kWave;
-  float top = -FLT_MAX, l = 0.f, o[kDims] = {};
-  for (int p0 = 0; p0 < parts; p0 += kWave) {
-    const int n = min(kWave, parts - p0);
+  float top = -FLT_MAX, l = 0.f;
+  Dims o = {};
+  for (int p0 = 0; p0 < parts; p0 += kLanes) {
+    const int n = min(kLanes, parts - p0);
     const f32x2 ml = lane < n ? *reinterpret_cast<const f32x2*>(a.part_ml + (at + p0 + lane) * 2) : f32x2{-FLT_MAX, 0.f};
     float most = ml[0];
 #pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off));
+    for (int off = kLanes / 2; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off));
     const float next = fmaxf(top, most), f = __builtin_amdgcn_exp2f(top - next);
     const float fp = lane < n ? __builtin_amdgcn_exp2f(ml[0] - next) : 0.f;
     float sum = lane < n ? fp * ml[1] : 0.f;
 #pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+    for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
     l = fmaf(l, f, sum);
     top = next;
 #pragma unroll
     for (int k = 0; k < kDims; ++k) o[k] *= f;
+    auto weight = [&](int p) {
+      if constexpr (kLanes == kWave) return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, fp), p));
+      return __shfl(fp, p, kLanes);
+    };
     const float* op = a.part_o + (at + p0) * D + lane * kDims;
-    auto weight = [&](int p) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, fp), p)); };
     int p = 0;
     for (; p + 8 <= n; p += 8) {
-      float x[8][kDims];
+      Dims x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int k = 0; k < kDims; ++k) x[e][k] = op[(int64_t)(p + e) * D + k];
+      for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const Dims*>(op + (int64_t)(p + e) * D);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float w = weight(p + e);
@@ -987,16 +998,15 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkArgs a) {
     }
     for (; p < n; ++p) {
       const float w = weight(p);
+      const Dims x = *reinterpret_cast<const Dims*>(op + (int64_t)p * D);
 #pragma unroll
-      for (int k = 0; k < kDims; ++k) o[k] = fmaf(w, op[(int64_t)p * D + k], o[k]);
+      for (int k = 0; k < kDims; ++k) o[k] = fmaf(w, x[k], o[k]);
     }
   }
   const float inv = 1.f / l;
   uint16_t* to = a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + lane * kDims;
-  if constexpr (kDims == 2)
-    *reinterpret_cast<uint32_t*>(to) = pack2<T>(o[0] * inv, o[1] * inv);
-  else
-    *to = (uint16_t)pack2<T>(o[0] * inv, 0.f);
+#pragma unroll
+  for (int k = 0; k < kDims; k += 2) reinterpret_cast<uint32_t*>(to)[k / 2] = pack2<T>(o[k] * inv, o[k + 1] * inv);
 }
 
 // How a call is split: row tiles of `rows` rows per (sequence, K/V head), key parts of part_tokens.
@@ -1015,7 +1025,7 @@ constexpr int kTilesNt = 2;
 // 100-500 behind up to 2,000 325 -> 267, 4 x 2,048 behind up to 6,144 696 -> 535.
 constexpr int kQueueFrom = 2048;
 
-Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int max_query_len, int max_context) {
+Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int num_q_rows, int max_query_len, int max_context) {
   Plan p;
   const int64_t rows = (int64_t)max_query_len * group;
   p.tiles = rows > 64;
@@ -1025,8 +1035,17 @@ Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int max_query_
   const int64_t steps = ((int64_t)max_context + kStep - 1) / kStep;
   const int64_t groups = (int64_t)num_seqs * kv_heads * p.row_tiles;
   const int64_t want = kCus * (p.tiles ? tiles_per_cu(head_dim) : head_dim == 64 ? 2 : 1);
-  int64_t parts = want / groups;  // no second round for a few (259 tokens behind 32,500: 8 parts 220 us, 7 175)
+  // No second round for a few (259 tokens behind 32,500: 8 parts 220 us, 7 175), and no more parts than pay: steps go on beside
+  // each other, but a launch is added and every pair of row and head has its sums written and read a part (us: measured on this
+  // card). 16 x 256 tokens of 12 heads of 64 in one part 12 us, in two 25; 4 x 1,023 23 and 32; one token at 300 8.9 and 10.7; but
+  // 300 tokens at 4,000 66 in one part, 23 in eight; one token at 4,000 30 in one, 12 in 32.
+  const float step = (p.tiles ? 2.0f : 0.6f) * (head_dim == 64 ? 1.f : 1.3f), launch = 4.5f;
+  const float pairs = 2e-6f * head_dim * num_q_rows * kv_heads * group;
+  const float best = __builtin_sqrtf(steps * step / __builtin_fmaxf(pairs, 1e-6f));
+  int64_t parts = want / groups;
+  if ((float)parts > best) parts = (int64_t)best;
   parts = parts < 1 ? 1 : parts > steps ? steps : parts;
+  if (steps * step <= (float)((steps + parts - 1) / parts) * step + launch + pairs * parts) parts = 1;
   const int64_t per = (steps + parts - 1) / parts;
   p.part_tokens = (int)(per * kStep > 0x7fffffff - kStep ? 0x7fffffff / kStep * kStep : per * kStep);
   p.parts = (int)((steps + per - 1) / per);
@@ -1049,7 +1068,7 @@ size_t workspace_of(const Plan& p, int32_t num_seqs, int32_t num_q_rows, int32_t
 template <int D, typename T>
 tq_status launch(const ChunkArgs& a, const Plan& p, hipStream_t stream) {
   const int64_t grid = (int64_t)a.num_seqs * a.kv_heads * a.row_tiles * a.parts;
-  const int64_t join = (int64_t)a.num_seqs * (((int64_t)a.max_query_len * a.num_heads + 3) / 4);
+  const int64_t join = (int64_t)a.num_seqs * (((int64_t)a.max_query_len * a.num_heads + kJoinPairs<D> - 1) / kJoinPairs<D>);
   if (grid > 0x7fffffffLL || (a.parts > 1 && join > 0x7fffffffLL)) return TQ_ERR_UNSUPPORTED;
   const dim3 g((unsigned)grid), t(kWave * kWaves);
   if (p.queue) {
@@ -1083,7 +1102,7 @@ extern "C" size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_he
       num_seqs == 0 || num_q_rows == 0 || max_query_len == 0 || max_context_len == 0 || max_context_len > kMaxContext)
     return 0;
   const int32_t group = num_heads / num_kv_heads;
-  return workspace_of(plan_of(num_seqs, num_kv_heads, group, head_dim, max_query_len, max_context_len), num_seqs, num_q_rows,
+  return workspace_of(plan_of(num_seqs, num_kv_heads, group, head_dim, num_q_rows, max_query_len, max_context_len), num_seqs, num_q_rows,
                       num_heads, group, head_dim);
 }
 
@@ -1116,7 +1135,7 @@ extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const voi
   if ((int64_t)max_query_len * num_heads > 0x7fffffffLL - 65536) return TQ_ERR_UNSUPPORTED;
 
   const int32_t group = num_heads / num_kv_heads;
-  const Plan p = plan_of(num_seqs, num_kv_heads, group, head_dim, max_query_len, max_context_len);
+  const Plan p = plan_of(num_seqs, num_kv_heads, group, head_dim, num_q_rows, max_query_len, max_context_len);
   const size_t need = workspace_of(p, num_seqs, num_q_rows, num_heads, group, head_dim);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 16 != 0))
     return TQ_ERR_WORKSPACE;
