@@ -72,6 +72,30 @@ def test_long_contexts_in_parts(seqs, dim, dtype):
     check(c)
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (12, 12), (7, 1), (16, 2), (40, 2)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_head_layouts_in_parts(heads, kv_heads, dim):
+    # 257 positions end a part of 128 or 256 keys one key behind its border.
+    c = Chunk([(1200, 3), (2060, 40), (255, 1), (256, 1), (257, 0)], heads, kv_heads, dim, FP16, 16, seed=23)
+    assert ops.chunk_workspace_bytes(5, heads, kv_heads, dim, c.q.size(0), c.max_new, c.max_context) > 0
+    check(c)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_places_in_parts_that_no_row_sees(dim, bad):
+    c = Chunk([(1500, 200), (2100, 3)], 4, 1, dim, BF16, 16, seed=24, garbage=bad)
+    assert ops.chunk_workspace_bytes(2, 4, 1, dim, c.q.size(0), c.max_new, c.max_context) > 0
+    check(c)
+
+
+@pytest.mark.parametrize("seqs", [[(0, 256)] * 16, [(300, 1)] * 8, [(0, 1023)] * 2])
+def test_short_contexts_stay_in_one_part(seqs):
+    c = Chunk(seqs, 12, 12, 64, FP16, 16, seed=25)
+    assert ops.chunk_workspace_bytes(len(seqs), 12, 12, 64, c.q.size(0), c.max_new, c.max_context) == 0
+    check(c)
+
+
 @pytest.mark.parametrize("group", [1, 4])
 def test_many_rows(group):
     check(Chunk([(300, 500), (0, 1029)], 2 * group, 2, 128, BF16, 16, seed=5))
