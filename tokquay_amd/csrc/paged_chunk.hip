@@ -41,6 +41,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;  // log2 units a score may exceed the running maximum by
 constexpr int kTileKeys = 32;  // keys of a tile
+constexpr int kCus = 256, kXcds = 8;
 constexpr int kTileRows = 16;  // rows of a tile
 constexpr int kWaves = 4;
 
@@ -810,11 +811,18 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
 
 // One workgroup a (sequence, K/V head, part, row tile). The last row tiles see the most keys and go first. Tiles of one K/V
 // head and part follow each other every 8th workgroup, so on one XCD, where these are a multiple of 8.
+//
+// Workgroups go to CUs in turn, so every other 256 of them are dealt backwards on each XCD: the CU with the longest gets
+// the shortest of those beside it (8 x 1,023 tokens of 12 heads of 64 30.0 -> 28.3 us, 8 x 100-1,900 44 -> 42, 2 x 2,000 of
+// 32 heads of 128 84 -> 81; 4 x 1,023 of these 55 -> 57).
 template <int D, int NT, typename T>
 __global__ __launch_bounds__(kWave* kWaves, tiles_per_cu(D)) void chunk_tiles_kernel(const ChunkArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t s_k0[64 * D], s_v0[64 * D], s_k1[64 * D], s_v1[64 * D];
   __shared__ int s_dirty;
   int idx = blockIdx.x;
+  const int turn = idx / kCus;
+  if (turn % 2 == 1 && (turn + 1) * kCus <= (int)gridDim.x)
+    idx = turn * kCus + (kCus / kXcds - 1 - idx % kCus / kXcds) * kXcds + idx % kXcds;
   const int units = a.num_seqs * a.kv_heads * a.parts;
   const int tile = a.row_tiles - 1 - idx / units;
   idx %= units;
@@ -829,7 +837,6 @@ __global__ __launch_bounds__(kWave* kWaves, tiles_per_cu(D)) void chunk_tiles_ke
 // With more row tiles than run at once, workgroups that stay and take them from a queue, the most keys first: dispatched
 // workgroups go to an XCD's CUs in turn, and one that has to wait for its CU holds up those behind it (4 x 2,048 tokens behind 768
 // to 5,376: 330 of 512 workgroups at work on average).
-constexpr int kXcds = 8;
 constexpr int kQueueLine = 32;                           // words between counters: a 128-byte line each
 constexpr int kQueueHead = (kXcds + 1) * kQueueLine;     // [0] pairs, then the counter of each XCD's share
 constexpr int kOrderThreads = 1024, kBuckets = 2048;
@@ -1016,7 +1023,6 @@ struct Plan {
   bool queue;
 };
 
-constexpr int kCus = 256;
 constexpr int kMaxContext = 1 << 30;  // positions a few tiles past it are still ints
 // 16-row tiles of a wave of chunk_tiles_kernel. Three spill at D = 128 and are slower at 64 (16 x 100-1,900 tokens 190 -> 198 us).
 constexpr int kTilesNt = 2;
@@ -1102,8 +1108,8 @@ extern "C" size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_he
       num_seqs == 0 || num_q_rows == 0 || max_query_len == 0 || max_context_len == 0 || max_context_len > kMaxContext)
     return 0;
   const int32_t group = num_heads / num_kv_heads;
-  return workspace_of(plan_of(num_seqs, num_kv_heads, group, head_dim, num_q_rows, max_query_len, max_context_len), num_seqs, num_q_rows,
-                      num_heads, group, head_dim);
+  const Plan p = plan_of(num_seqs, num_kv_heads, group, head_dim, num_q_rows, max_query_len, max_context_len);
+  return workspace_of(p, num_seqs, num_q_rows, num_heads, group, head_dim);
 }
 
 extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
