@@ -510,8 +510,9 @@ tq_status tq_rope_cache_write(void* q_out, int64_t q_out_row_stride, const void*
  *   out[row, h] = softmax_{j <= q_start[b] + i}(scale * q[row, h] . K_b[h / G][j]) @ V_b[h / G][j],  G = num_heads / num_kv_heads
  *
  * pool[num_blocks][num_layers][2][num_kv_heads][block_size][head_dim], q and out are of dtype (TQ_F16 or TQ_BF16),
- * head_dim 64 or 128. Scores, weights and sums are fp32; each weight is rounded to dtype before it meets V, and the
- * output once. What the pool holds behind a sequence's last position, or at positions a row does not see, never
+ * head_dim 64 or 128. Scores, weights and sums are fp32; each weight is rounded to dtype before it meets V (in TQ_F16,
+ * those below 2^-21 of the row's largest by up to 2^-32 of that one), and the output once. Scores stay below 2^27 in
+ * magnitude. What the pool holds behind a sequence's last position, or at positions a row does not see, never
  * reaches that row, infinities and NaN included. scale is any finite number.
  *
  * cu_seqlens_q has num_seqs + 1 entries and is non-decreasing; sequences may be empty, and rows of q and out

@@ -3,8 +3,8 @@
 //
 //   out[t, h] = sum_j p_j V[j, h / G] / sum_j p_j,   p_j = 2^(c (q[t, h] . K[j, h / G]) - m),   j <= q_start + t
 //
-// with c = scale log2(e) and m a running maximum (any m gives the same quotient; it is raised when a score
-// passes it by more than kSlack, so p stays below 2^8 and the sums are rescaled rarely). The G heads of a
+// with c = scale log2(e) and m a running maximum less kLift (any m gives the same quotient; it is raised when a score
+// passes the maximum by more than kSlack, so p stays below 2^(kLift + kSlack) and the sums are rescaled rarely). The G heads of a
 // token read the same keys, so (token, head of the group) pairs are the rows of one matrix product: row r
 // is token r / G, head r % G of the group, and a 16-row tile holds 16 / G tokens.
 //
@@ -18,7 +18,10 @@
 // is taken in the lane and across four lanes) and are, rounded to 16 bits, the B operand
 // of the second product with no exchange: that product may take the keys in any order, and V^T is read in
 // the same one (two transposing LDS reads of 4 keys each). Rounding p to the cache's type costs each weight half a
-// step, about as much as the rounding of the output; the rounded weights are summed, so equal values come out exactly.
+// step, about as much as the rounding of the output; the rounded weights are summed, so equal values come out exactly. float16
+// has no full step below 2^-14, so its weights are lifted by 2^7: those below 2^-21 of the row's largest are off by up to 2^-32 of
+// that one, where half a step would be less (without the lift 2^-25: 4,000 equal keys 17 nats below one without value came
+// out 44 % too heavy, and not at all at 17.4).
 //
 // K and V come in tiles straight from HBM into LDS (16 bytes a lane, no registers), a tile ahead of the products.
 // 16-byte pieces are permuted inside a row as they arrive (swizzled), so that what an LDS read takes in a clock
@@ -39,7 +42,6 @@ namespace tq {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.f;  // log2 units a score may exceed the running maximum by
 constexpr int kTileKeys = 32;  // keys of a tile
 constexpr int kCus = 256, kXcds = 8;
 constexpr int kTileRows = 16;  // rows of a tile
@@ -285,7 +287,7 @@ struct Rows {
   u32x4 q[NT][D / 32];
   f32x4 o[NT][D / 16];
   f32x4 l[NT];  // sum of the weights, four times
-  float m[NT], mthr[NT];
+  float m[NT];
   int qpos[NT];
   int lo, hi;  // positions of the first and last row (uniform)
 
@@ -305,7 +307,6 @@ struct Rows {
       for (int d = 0; d < D / 16; ++d) o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
       qpos[n] = s.start + t;
       m[n] = -FLT_MAX;
-      mthr[n] = -FLT_MAX;
       l[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     lo = __builtin_amdgcn_readfirstlane(s.start + min(r0, last) / a.group);
@@ -381,17 +382,18 @@ struct Rows {
       for (int h = 1; h < 2 * KS; ++h)
         top = max2(max2(max2(top, s[h][n][0]), s[h][n][1]), max2(s[h][n][2], s[h][n][3]));
       top *= a.c;
-      if (__builtin_amdgcn_ballot_w64(top > mthr[n]) != 0) {
+      // By the difference, which is exact where it is near: a limit of its own would be rounded, at scores from 2^24 on past
+      // what a float16 weight holds.
+      if (__builtin_amdgcn_ballot_w64(top - m[n] > T::kLift + T::kSlack) != 0) {
         top = max2(top, __shfl_xor(top, 16));
         top = max2(top, __shfl_xor(top, 32));
-        const bool grow = top > mthr[n];
-        const float next = grow ? top : m[n];
+        const bool grow = top - m[n] > T::kLift + T::kSlack;
+        const float next = grow ? top - T::kLift : m[n];
         const float corr = grow ? __builtin_amdgcn_exp2f(m[n] - next) : 1.f;
         l[n] *= corr;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) o[n][d] *= corr;
         m[n] = next;
-        mthr[n] = next + kSlack;
       }
     }
   }
