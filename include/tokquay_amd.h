@@ -561,8 +561,8 @@ size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_heads, int32_
  * fp32 [num_rows, vocab], row stride probs_row_stride (rows of no drafted token, the last ones, are not read).
  * A row of a sequence with a temperature that holds a NaN or +inf, or nothing above -inf, has no distribution: it is
  * taken greedily and sets TQ_DEVERR_VALUE if the sequence came to it. A drafted token outside [0, vocab) sets
- * TQ_DEVERR_TOKEN and does not stand. A sequence that does not fit num_rows or max_query_len sets
- * TQ_DEVERR_LENGTH and is treated as one of no rows. tokens is int64 [num_seqs, max_query_len], accepted int32 [num_seqs].
+ * TQ_DEVERR_TOKEN and does not stand. cu_seqlens_q is non-decreasing. A sequence that does not fit num_rows or max_query_len sets
+ * TQ_DEVERR_LENGTH and is treated as one of no rows; so may others be where the offsets fall. tokens is int64 [num_seqs, max_query_len], accepted int32 [num_seqs].
  *
  * Needs tq_verify_drafts_workspace_size(...) bytes of workspace (16-byte aligned, any contents; calls that may
  * run at the same time need one each). No counterpart in the reference; it stands beside Engine._sample

@@ -303,3 +303,22 @@ def test_a_captured_batch_replays(probs):
         tokens.zero_()
         graph.replay()
         assert torch.equal(tokens.cpu(), wants[i][0]) and torch.equal(accepted.cpu(), wants[i][1])
+
+
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("cu", [[0, 99, 5, 9], [0, 5, -3, 9], [0, 5, 2, 7], [0, 3, 99, 9], [4, 0, 5, 9], [0, 2**31 - 1, 3, 9]])
+@pytest.mark.parametrize("temps", [(1.0, 0.0, 0.8), (0.0, 1.0, 0.7), (0.9, 0.9, 0.9)])
+def test_offsets_that_fall(cu, temps, probs):
+    # A sequence beside one that does not fit gets its own result or is taken as one of no rows, never another's.
+    c = Case([3, 2, 4], 600, torch.float32, probs, temps=temps, seed=16)
+    c.cu = torch.tensor(cu, dtype=torch.int32)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    tokens, accepted = c.run(err=err, max_rows=5)
+    assert int(err) == _lib.DEVERR_LENGTH
+    for b in range(3):
+        fits = 0 <= cu[b] < cu[b + 1] <= 9 and cu[b + 1] - cu[b] <= 5
+        if fits and not (int(accepted[b]) == 0 and bool((tokens[b] == -1).all())):
+            want, count = verified(c.logits, c.drafts, c.uniforms, c.cu[b : b + 2], 5, c.temperature[b : b + 1], c.probs)
+            assert torch.equal(tokens[b], want[0]) and int(accepted[b]) == int(count[0])
+        else:
+            assert bool((tokens[b] == -1).all()) and int(accepted[b]) == 0

@@ -173,10 +173,11 @@ __device__ __forceinline__ void columns(const void* row, int base, int n, float 
 
 constexpr double kLog2e = 1.4426950408889634;
 
-// The temperature of the sequence that a row belongs to: the last one with cu[b] <= row (empty sequences hold no row), among 64
-// parts at a time. Asked for before the logits, it arrives before them. (Counted through all 1,024 sequences of 5 rows, 50,257 bf16
-// logits each, the call took 328 us instead of 259.)
-__device__ __forceinline__ float temperature_of(const VerifyArgs& a, int row) {
+// The sequence that a row belongs to: the last one with cu[b] <= row (empty sequences hold no row), among 64 parts at a time.
+// Its temperature, asked for before the logits, arrives before them. (Counted through all 1,024 sequences of 5 rows, 50,257 bf16
+// logits each, the call took 328 us instead of 259.) Where cu falls somewhere this may be another one, still below num_seqs; every
+// count grows with the row, so if it is b for two rows it is for those between them.
+__device__ __forceinline__ int64_t owner_of(const VerifyArgs& a, int row) {
   const int lane = threadIdx.x & (kWave - 1);
   int64_t b = 0, n = a.num_seqs;
   while (n > 1) {
@@ -186,7 +187,7 @@ __device__ __forceinline__ float temperature_of(const VerifyArgs& a, int row) {
     b += skip;
     n = min(step, n - skip);
   }
-  return a.temperature[b];
+  return b;
 }
 
 template <typename T, int PER>
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int base = chunk * kThreads * PER, n = min(kThreads * PER, a.vocab - base);
   float x[PER], top = -INFINITY;
-  const float temp = temperature_of(a, row);
+  const float temp = a.temperature[owner_of(a, row)];
   columns<T, kVec<T>, kThreads, PER, false>(row_of<T>(a, row), base, n, x);
 #pragma unroll
   for (int i = 0; i < PER; ++i) top = __builtin_elementwise_maximum(top, x[i]);  // NaN, if any is
@@ -355,13 +356,14 @@ __device__ __forceinline__ int pick(bool over, bool has, int (*s_pick)[2]) {
 // What became of a sequence's drafts: how many stand, and the distribution of the row that the next token is drawn from.
 struct Decision {
   Dist dist;
-  int first;  // -1: the sequence has no rows (or does not fit)
+  int first;  // -1: the sequence has no rows (or is refused)
 };
 
 constexpr int kDists = 16;  // rows whose distributions are kept in LDS
 struct DecideShared {
   Dist dist[kDists];
   int first, bad;
+  bool refused;
 };
 
 // By one workgroup of N threads. `lead`: it also writes the tokens that stand, and the flags.
@@ -372,22 +374,19 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, int b, bool lead
   const int64_t rows = (int64_t)a.cu[b + 1] - lo;
   int64_t* out = a.tokens + (int64_t)b * a.max_rows;
   Decision r;
-  if (lo < 0 || rows <= 0 || lo + rows > a.num_rows || rows > a.max_rows) {
-    if (lead) {
-      if (rows != 0 && threadIdx.x == 0) flag_error(a.d_error, TQ_DEVERR_LENGTH);
-      for (int i = threadIdx.x; i < a.max_rows; i += N) out[i] = -1;
-      if (threadIdx.x == 0) a.accepted[b] = 0;
-    }
-    r.first = -1;
-    return r;
-  }
-  const int drafts = (int)rows - 1;
+  const bool fits = lo >= 0 && rows > 0 && lo + rows <= a.num_rows && rows <= a.max_rows;
+  const int drafts = fits ? (int)rows - 1 : -1;
   const float temp = a.temperature[b];
   if (threadIdx.x == 0) {
     sh.first = drafts;
     sh.bad = drafts + 1;
   }
   __syncthreads();
+  // Rows that another sequence claims too may have statistics of its temperature. The last wave has the fewest rows.
+  if (wave == N / kWave - 1) {
+    const bool refused = !fits || owner_of(a, lo) != b || owner_of(a, lo + drafts) != b;
+    if (lane == 0) sh.refused = refused;
+  }
   // A wave a row, after a lane a row has fetched what it needs of 64 rows. (Rows behind one that does not stand are left out.)
   for (int i0 = 0; i0 <= drafts && i0 <= *(volatile int*)&sh.first; i0 += kWave) {
     float lx = 0.f, qx = 1.f, ux = 0.f;
@@ -417,6 +416,15 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, int b, bool lead
     }
   }
   __syncthreads();
+  if (sh.refused) {
+    if (lead) {
+      if (rows != 0 && threadIdx.x == 0) flag_error(a.d_error, TQ_DEVERR_LENGTH);
+      for (int i = threadIdx.x; i < a.max_rows; i += N) out[i] = -1;
+      if (threadIdx.x == 0) a.accepted[b] = 0;
+    }
+    r.first = -1;
+    return r;
+  }
   r.first = sh.first;
   if (r.first >= kDists) {  // uniform
     if (wave == 0) {
