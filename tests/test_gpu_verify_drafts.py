@@ -322,3 +322,15 @@ def test_offsets_that_fall(cu, temps, probs):
             assert torch.equal(tokens[b], want[0]) and int(accepted[b]) == int(count[0])
         else:
             assert bool((tokens[b] == -1).all()) and int(accepted[b]) == 0
+
+
+# draw of 16 columns a thread without a decision launch (the first four); of 32, without and with one; vocabularies whose
+# statistics always take 32 columns a thread.
+@pytest.mark.parametrize("sequences,vocab,dtype", [
+    (64, 50257, torch.float32), (64, 50257, torch.bfloat16), (32, 128000, torch.float32), (17, 60001, torch.float16),
+    (2, 1048577, torch.float32), (3, 2097152, torch.bfloat16), (13, 1100003, torch.float16), (2, 600011, torch.bfloat16),
+])  # fmt: skip
+@pytest.mark.parametrize("probs", [True, False])
+def test_batches_and_vocabularies_of_every_draw(sequences, vocab, dtype, probs):
+    rows = [(3 if vocab < 10**6 else 2) if b % 3 else 1 for b in range(sequences)]
+    assert Case(rows, vocab, dtype, probs, temps=(1.0, 0.0, 0.8), seed=27).check() == 0
