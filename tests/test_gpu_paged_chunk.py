@@ -314,3 +314,15 @@ def test_refusals():
         ops.paged_chunk(torch.empty_like(long.q, device="cuda"), long.q.cuda(), long.pool.cuda(), LAYER,
                         long.tables.cuda(), long.cu.cuda(), long.start.cuda(), 1, 3001,
                         workspace=torch.empty(64, dtype=torch.uint8, device="cuda"))  # fmt: skip
+
+
+def test_refusals_of_values():
+    c = Chunk([(70, 3), (0, 40)], 4, 2, 64, BF16, 16, seed=21)
+    good = dict(out=torch.empty_like(c.q, device="cuda"), q=c.q.cuda(), pool=c.pool.cuda(), layer=LAYER,
+                block_tables=c.tables.cuda(), cu_seqlens_q=c.cu.cuda(), q_start=c.start.cuda(), max_query_len=40,
+                max_context_len=73)  # fmt: skip
+    for name, value in [("scale", math.inf), ("scale", math.nan), ("scale", 1e300), ("max_context_len", 2**30 + 1),
+                        ("max_context_len", 0), ("max_query_len", 2**30), ("block_tables", c.tables.cuda()[:, :0])]:  # fmt: skip
+        with pytest.raises(ValueError, match="paged_chunk"):
+            ops.paged_chunk(**{**good, name: value})
+    ops.paged_chunk(**{**good, "max_query_len": 0, "max_context_len": 0, "block_tables": c.tables.cuda()[:, :0]})

@@ -208,3 +208,13 @@ def test_refusals():
                         ("k_norm", c.k_norm.cuda()[:32]), ("eps", -1.0), ("eps", math.nan)]:  # fmt: skip
         with pytest.raises((ValueError, _lib.KernelError), match="rope_cache_write"):
             ops.rope_cache_write(**{**good, name: value})
+
+
+def test_refusals_of_values():
+    c = Case(12, 4, 2, 64, BF16, 64, norm=True, seed=15)
+    good = c.args()
+    for name, value in [("eps", -1.0), ("eps", math.nan), ("table", c.table.cuda()[:0])]:
+        with pytest.raises(ValueError, match="rope_cache_write"):
+            ops.rope_cache_write(**{**good, name: value})
+    none = {n: good[n][:0] for n in ("q_out", "q", "k", "v", "slot_mapping", "positions", "table")}
+    ops.rope_cache_write(**{**good, **none})

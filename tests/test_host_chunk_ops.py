@@ -227,3 +227,58 @@ def test_workspace_sizes():
     assert size(0, 32, 8, 128, 0, 0, 0) == 0 and size(1, 32, 7, 128, 1, 1, 4000) == 0
     assert _lib.lib().tq_verify_drafts_workspace_size(2, 10, 50257) > _lib.lib().tq_verify_drafts_workspace_size(2, 5, 50257) > 0
     assert _lib.lib().tq_verify_drafts_workspace_size(0, 0, 50257) == 0
+
+
+# What depends on values rather than tensors: the fakes refuse it as the operators do.
+UNFIT = {
+    "rope_cache_write": [("eps", -1.0), ("eps", math.nan), ("table", lambda t: t[:0]),
+                         ("pool", lambda t: t.new_empty(1 << 23, 1, 2, 2, 1024, 64)), ("tokens", 1 << 30)],
+    "paged_chunk": [("scale", math.inf), ("scale", -math.inf), ("scale", math.nan), ("scale", 1e300), ("max_context_len", (1 << 30) + 1),
+                    ("max_context_len", 0), ("max_query_len", 1 << 30), ("block_tables", lambda t: t[:, :0]),
+                    ("pool", lambda t: t.new_empty(1, 1 << 14, 2, 2, 1024, 64)),
+                    ("pool", lambda t: t.new_empty(1 << 31, 1, 2, 2, 1, 64))],
+    "verify_drafts": [("rows", 1 << 31), ("tokens", lambda t: t.new_empty(2, 1 << 31))],
+}  # fmt: skip
+
+
+@pytest.mark.parametrize("op,name,i", [(op, name, i) for op, all_ in UNFIT.items() for i, (name, _) in enumerate(all_)],
+                         ids=lambda v: str(v))  # fmt: skip
+def test_fakes_refuse_unfit_values(op, name, i):
+    with FakeTensorMode():
+        args, value = ARGS[op](), UNFIT[op][i][1]
+        more = lambda t, n: t.new_empty(n, *t.shape[1:])  # noqa: E731
+        if op == "rope_cache_write":
+            args["layer"] = 0
+        if name in ("tokens", "rows") and not callable(value):
+            for n in {"tokens": ("q_out", "q", "k", "v", "slot_mapping", "positions"),
+                      "rows": ("logits", "draft_probs", "draft_tokens", "uniforms")}[name]:  # fmt: skip
+                args[n] = more(args[n], value)
+        else:
+            args[name] = value(args[name]) if callable(value) else value
+        with pytest.raises(RuntimeError, match=f"tokquay_amd::{op}: "):
+            getattr(torch_ops.load(), op)(*args.values())
+
+
+def test_fakes_refuse_short_workspaces():
+    with FakeTensorMode():
+        args = chunk_args()
+        args["max_context_len"], args["block_tables"] = 4000, torch.empty(3, 400, dtype=torch.int32, device="cuda")
+        need = ops.chunk_workspace_bytes(3, 4, 2, 64, 7, 4, 4000)
+        for bad in (torch.empty(need - 1, dtype=torch.uint8, device="cuda"), torch.empty(need + 8, dtype=torch.uint8, device="cuda")[8:]):
+            args["workspace"] = bad
+            with pytest.raises(RuntimeError, match="tq_paged_chunk failed: workspace"):
+                torch_ops.load().paged_chunk(*args.values())
+            with pytest.raises(_lib.KernelError, match="tq_paged_chunk failed: workspace"):
+                ops.paged_chunk(**args)
+        args["workspace"] = torch.empty(need, dtype=torch.uint8, device="cuda")
+        ops.paged_chunk(**args)
+
+
+def test_calls_without_work_need_no_lengths():
+    with FakeTensorMode():
+        args = chunk_args()
+        ops.paged_chunk(**{**args, "max_query_len": 0, "max_context_len": 0, "block_tables": args["block_tables"][:, :0]})
+        args = rope_args()
+        for n in ("q_out", "q", "k", "v", "slot_mapping", "positions", "table"):
+            args[n] = args[n][:0]
+        ops.rope_cache_write(**args)

@@ -15,6 +15,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <cmath>
 #include <string>
 #include <utility>
 #include <vector>
@@ -401,6 +402,10 @@ void rope_cache_write(at::Tensor q_out, const at::Tensor& q, const at::Tensor& k
               p.head_dim);
   norm_of(op, "q_norm", q_norm, pool, p);
   norm_of(op, "k_norm", k_norm, pool, p);
+  TORCH_CHECK(eps >= 0, op, ": eps must not be negative, got ", eps);
+  TORCH_CHECK(p.blocks <= UINT32_MAX / p.block_size, op, ": pool has more than 2^32 - 1 slots");
+  TORCH_CHECK(n <= 0xffff0000LL / (heads + 2 * kv_heads), op, ": too many rows for their heads");
+  TORCH_CHECK(n == 0 || table.size(0) >= 1, op, ": table has no positions");
   error_word_of(op, d_error, p);
   check(tq_rope_cache_write(q_out.data_ptr(), os, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
                             pool.data_ptr(), p.blocks, p.layers, (int32_t)heads, p.heads, p.block_size, p.head_dim,
@@ -431,7 +436,14 @@ void paged_chunk(at::Tensor out, const at::Tensor& q, const at::Tensor& pool, in
   const int64_t ts = tables_of(op, "block_tables", block_tables, n, p);
   TORCH_CHECK(block_tables.size(1) <= INT32_MAX, op, ": block_tables has too many columns");
   TORCH_CHECK(max_query_len >= 0 && max_query_len <= INT32_MAX && max_context_len >= 0 &&
-                  max_context_len <= INT32_MAX, op, ": max_query_len and max_context_len must be lengths");
+                  max_context_len <= 1 << 30, op, ": max_query_len and max_context_len must be lengths, contexts up to 2^30");
+  TORCH_CHECK(std::isfinite((float)scale), op, ": scale must be a finite float32, got ", scale);
+  if (n > 0 && rows > 0 && max_query_len > 0) {
+    TORCH_CHECK(max_query_len <= (INT32_MAX - 65536) / heads, op, ": max_query_len is too long for ", heads, " heads");
+    TORCH_CHECK(max_context_len >= 1 && block_tables.size(1) >= 1, op,
+                ": max_context_len and block_tables must have room for the sequences");
+    TORCH_CHECK(pool.numel() / p.blocks <= INT32_MAX, op, ": a block of the pool has too many elements");
+  }
   error_word_of(op, d_error, p);
   size_t ws = workspace_of(op, workspace, p);
   const size_t need = tq_paged_chunk_workspace_size((int32_t)n, (int32_t)heads, p.heads, p.head_dim, (int32_t)rows,

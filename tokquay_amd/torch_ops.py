@@ -6,7 +6,7 @@ HIP stream. This module loads that library and registers the operators' fake (sh
 implementations, so programs that record torch calls (``make_fx``, FX graphs on fake tensors)
 see the kernels as single operators. Both the operators and their fakes refuse, before any launch,
 every tensor a kernel would read or write past: wrong device, dtype or inner layout, too few rows
-or entries, overlapping rows:
+or entries, overlapping rows; the last three also refuse every number out of its range:
 
 * ``cache_write(pool!, layer, k, v, slot_mapping, d_error!?)``
 * ``paged_decode(out!, q, pool, layer, block_tables, context_lens, max_context_len, scale,
@@ -38,6 +38,7 @@ import os
 
 import torch
 
+from tokquay_amd import _lib
 from tokquay_amd.build import TORCH_OPS_PATH
 
 OPS = ("cache_write", "paged_decode", "paged_decode_write", "paged_prefill", "paged_mixed", "paged_gather",
@@ -255,7 +256,8 @@ def _typed_pool_of(op, pool, layer, float32):
         _fail(op, f"only d_head 64 and 128 are supported, got {pool.size(5)}")
     if not 0 <= layer < pool.size(1):
         _fail(op, f"layer {layer} out of range [0, {pool.size(1)})")
-    if not (pool.size(0) >= 1 and 1 <= pool.size(3) <= 65535 and 1 <= pool.size(4) <= 1024):
+    if not (1 <= pool.size(0) < 2**31 and pool.size(1) < 2**31 and 1 <= pool.size(3) <= 65535
+            and 1 <= pool.size(4) <= 1024):  # fmt: skip
         _fail(op, "pool must hold blocks and heads, in blocks of at most 1024 slots")
 
 
@@ -314,6 +316,14 @@ def _fake_rope_cache_write(q_out, q, k, v, pool, layer, slot_mapping, positions,
                   f"{pool.size(5)}")  # fmt: skip
     _norm_of(op, "q_norm", q_norm, pool)
     _norm_of(op, "k_norm", k_norm, pool)
+    if not eps >= 0:
+        _fail(op, f"eps must not be negative, got {eps}")
+    if pool.size(0) > (2**32 - 1) // pool.size(4):
+        _fail(op, "pool has more than 2^32 - 1 slots")
+    if n > 0xFFFF0000 // (heads + 2 * pool.size(3)):
+        _fail(op, "too many rows for their heads")
+    if n > 0 and table.size(0) < 1:
+        _fail(op, "table has no positions")
     _error_word(op, d_error, pool)
 
 
@@ -326,15 +336,36 @@ def _fake_paged_chunk(out, q, pool, layer, block_tables, cu_seqlens_q, q_start, 
     _vector_of(op, "cu_seqlens_q", cu_seqlens_q, torch.int32, n + 1, pool)
     if cu_seqlens_q.numel() != n + 1:
         _fail(op, "cu_seqlens_q must have num_seqs + 1 entries")
-    heads = _typed_rows_of(op, "q", q, q.size(0) if q.dim() else 0, 0, pool, 16)
-    _typed_rows_of(op, "out", out, q.size(0), heads, pool, 8)
+    if n >= 2**31:
+        _fail(op, "too many sequences")
+    if not (q.dim() >= 1 and q.size(0) < 2**31):
+        _fail(op, "q has too many rows")
+    rows = q.size(0)
+    heads = _typed_rows_of(op, "q", q, rows, 0, pool, 16)
+    _typed_rows_of(op, "out", out, rows, heads, pool, 8)
     if heads % pool.size(3):
         _fail(op, f"{heads} query heads are no multiple of the pool's {pool.size(3)}")
     _tables_of(op, "block_tables", block_tables, n, pool)
-    if not (0 <= max_query_len < 2**31 and 0 <= max_context_len < 2**31):
-        _fail(op, "max_query_len and max_context_len must be lengths")
+    if block_tables.size(1) >= 2**31:
+        _fail(op, "block_tables has too many columns")
+    if not (0 <= max_query_len < 2**31 and 0 <= max_context_len <= 2**30):
+        _fail(op, "max_query_len and max_context_len must be lengths, contexts up to 2^30")
+    if not abs(scale) < 2.0**128 - 2.0**103:  # rounds to a finite float32
+        _fail(op, f"scale must be a finite float32, got {scale}")
+    if n > 0 and rows > 0 and max_query_len > 0:
+        if max_query_len > (2**31 - 1 - 65536) // heads:
+            _fail(op, f"max_query_len is too long for {heads} heads")
+        if not (max_context_len >= 1 and block_tables.size(1) >= 1):
+            _fail(op, "max_context_len and block_tables must have room for the sequences")
+        if pool.numel() // pool.size(0) >= 2**31:
+            _fail(op, "a block of the pool has too many elements")
     _error_word(op, d_error, pool)
     _workspace(op, workspace, pool)
+    if workspace is not None:
+        need = _lib.lib().tq_paged_chunk_workspace_size(n, heads, pool.size(3), pool.size(5), rows, max_query_len, max_context_len)
+        size = workspace.element_size()
+        if need > 0 and (workspace.numel() * size < need or workspace.storage_offset() * size % 16):
+            raise RuntimeError(f"tq_paged_chunk failed: {_lib.STATUS_NAMES[3]}")
 
 
 def _fake_verify_drafts(tokens, accepted, logits, draft_probs, draft_tokens, uniforms, temperature, cu_seqlens_q,
@@ -344,7 +375,7 @@ def _fake_verify_drafts(tokens, accepted, logits, draft_probs, draft_tokens, uni
         _fail(op, "logits must be a float32, float16 or bfloat16 [rows, vocab] tensor on a HIP device")
     rows, vocab = logits.shape
     n = temperature.numel()
-    if not 1 <= vocab <= 1 << 21:
+    if not (rows < 2**31 and 1 <= vocab <= 1 << 21 and n < 2**31):
         _fail(op, "logits must have 1 to 2097152 columns")
 
     def vocab_rows(name, t):
@@ -366,7 +397,7 @@ def _fake_verify_drafts(tokens, accepted, logits, draft_probs, draft_tokens, uni
     if d_error is not None:
         vector("d_error", d_error, torch.int32, 1)
     if not (tokens.device == logits.device and tokens.dtype == torch.int64 and tokens.dim() == 2
-            and tokens.size(0) == n and tokens.size(1) >= 1 and tokens.is_contiguous()):  # fmt: skip
+            and tokens.size(0) == n and 1 <= tokens.size(1) < 2**31 and tokens.is_contiguous()):  # fmt: skip
         _fail(op, f"tokens must be a contiguous int64 [{n}, max_query_len] tensor on the logits' device")
     if draft_probs is not None:
         if draft_probs.device != logits.device or draft_probs.dtype != torch.float32:
