@@ -628,6 +628,7 @@ constexpr int kMaxVocab = kThreads * kThreads * 32;  // a chunk a thread
 // 128 108 and 133).
 constexpr int kFewDraws = 400;
 constexpr int kDecideFrom = 1664;
+static_assert(kFewDraws < kDecideFrom, "draws of 8 columns a thread have no decision launch");
 
 // How a call is split, and its workspace.
 struct Plan {
@@ -658,10 +659,13 @@ Plan plan_of(int32_t num_seqs, int32_t num_rows, int32_t vocab) {
 template <typename T, int PER>
 tq_status launch_draw(const VerifyArgs& a, bool decided, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.num_seqs * a.draw_chunks));
-  if (decided)
-    hipLaunchKernelGGL((verify_draw_kernel<T, PER, true>), grid, dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((verify_draw_kernel<T, PER, false>), grid, dim3(kThreads), 0, stream, a);
+  if constexpr (PER > 8) {
+    if (decided) {
+      hipLaunchKernelGGL((verify_draw_kernel<T, PER, true>), grid, dim3(kThreads), 0, stream, a);
+      return check_launch();
+    }
+  }
+  hipLaunchKernelGGL((verify_draw_kernel<T, PER, false>), grid, dim3(kThreads), 0, stream, a);
   return check_launch();
 }
 
