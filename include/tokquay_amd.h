@@ -522,6 +522,10 @@ tq_status tq_rope_cache_write(void* q_out, int64_t q_out_row_stride, const void*
  * q and pool 16-byte aligned, out 8-byte, q_row_stride a multiple of 8 elements, out_row_stride of 4. out
  * must not overlap q.
  *
+ * The sequences of a call are split alike, as max_query_len and max_context_len ask for: a few tokens over long contexts take
+ * less time in a call of their own than beside a long chunk (4 at 32,768 positions and a prompt of 512, 32 / 8 heads of 128: 596 us
+ * in one call, 99 and 19 in two).
+ *
  * Keys are split into parts where the rows alone do not fill the GPU; the parts' sums are joined by a second
  * launch, in a fixed order, and kept in tq_paged_chunk_workspace_size(...) bytes of workspace (16-byte aligned, any
  * contents; calls that may run at the same time need one each).
@@ -554,8 +558,8 @@ size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_heads, int32_
  *   tokens[b] = x_0 .. x_{r-1}, next, -1, -1 ..                (max_query_len entries)
  *
  * The draw from weights w is the lowest j with w_0 + .. + w_j > u (w_0 + w_1 + ..), u = uniforms[last row] (the last
- * j with w_j > 0 where rounding leaves none). Weights and sums are fp64. With
- * independent uniform numbers and drafts drawn from q the tokens are distributed as the target's own. A sequence of no rows gets r = 0 and only -1.
+ * j with w_j > 0 where rounding leaves none). Weights and sums are fp64, of exponentials off by at most 2.2e-12: p and the
+ * running sums are right to 1e-11, and so is what the uniform numbers decide. With independent uniform numbers and drafts drawn from q the tokens are distributed as the target's own. A sequence of no rows gets r = 0 and only -1.
  *
  * logits: [num_rows, vocab] of dtype (tq_dtype), vocab at most 2^21, row stride logits_row_stride; -inf masks a token. draft_probs:
  * fp32 [num_rows, vocab], row stride probs_row_stride (rows of no drafted token, the last ones, are not read).

@@ -30,8 +30,10 @@
 // Two kernels. Up to 64 rows a K/V head (tokens, drafted tokens) the bytes of K and V bound it: chunk_rows_kernel streams them,
 // each wave its own keys (128 tokens at 511-4,094 positions, 8 heads of 128: 1.21 GB in 218 us, 5.5 TB/s, where a device copy
 // moves 5.07). More rows share tiles (chunk_tiles_kernel; chunk_queue_kernel over long contexts), and the matrix cores beside
-// the exponentials bound it: 4 x 2,048 tokens behind 768-5,376 cached ones run 550 GFLOP in 510 us (1,079 TFLOP/s; a large
-// bf16 library product reaches 1,370), with the matrix cores busy for 57 % of the time and the vector units for 55.
+// the exponentials bound it: 4 x 2,048 tokens behind 768-5,376 cached ones run 550 GFLOP in 495-540 us (1,020-1,110 TFLOP/s from
+// card to card; a large bf16 library product reaches 1,370), with the matrix cores busy for 57 % of the time and the vector units
+// for 55. The longest sequence decides for all (plan_of): beside 259 tokens behind 32,500, three single tokens at 300 take 818 us
+// with them, where the two calls take 175 and 9.
 #include <float.h>
 
 #include <utility>

@@ -575,7 +575,8 @@ def paged_chunk(
     whose K/V heads each serve ``n_head / n_kv_head`` neighbouring query heads: ``paged_prefill`` and ``paged_decode`` (rows of one
     token) for such pools, heads of 64 or 128 dims. The rows' own K/V must be in the pool already
     (``rope_cache_write``). ``max_query_len`` and ``max_context_len`` (the longest ``q_start[b] + n_b``) size the launch; in a captured graph,
-    which replays with other lengths, give the largest. Rows of no sequence are left alone."""
+    which replays with other lengths, give the largest. All sequences are split alike, by those two: a few tokens over long contexts
+    are faster in a call of their own than beside a long chunk. Rows of no sequence are left alone."""
     if scale is None:
         scale = 1.0 / math.sqrt(pool.size(-1))
     _checked_op("paged_chunk", out, q, pool, layer, block_tables, cu_seqlens_q, q_start, max_query_len, max_context_len,
