@@ -362,7 +362,8 @@ def _fake_paged_chunk(out, q, pool, layer, block_tables, cu_seqlens_q, q_start, 
     _error_word(op, d_error, pool)
     _workspace(op, workspace, pool)
     if workspace is not None:
-        need = _lib.lib().tq_paged_chunk_workspace_size(n, heads, pool.size(3), pool.size(5), rows, max_query_len, max_context_len)
+        sizes = (n, heads, pool.size(3), pool.size(5), rows, max_query_len, max_context_len)
+        need = _lib.lib().tq_paged_chunk_workspace_size(*map(int, sizes))  # (sizes of a dynamic trace become numbers)
         size = workspace.element_size()
         if need > 0 and (workspace.numel() * size < need or workspace.storage_offset() * size % 16):
             raise RuntimeError(f"tq_paged_chunk failed: {_lib.STATUS_NAMES[3]}")
