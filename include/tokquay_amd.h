@@ -559,14 +559,17 @@ size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_heads, int32_
  *
  * The draw from weights w is the lowest j with w_0 + .. + w_j > u (w_0 + w_1 + ..), u = uniforms[last row] (the last
  * j with w_j > 0 where rounding leaves none). Weights and sums are fp64, of exponentials off by at most 2.2e-12: p and the
- * running sums are right to 1e-11, and so is what the uniform numbers decide. With independent uniform numbers and drafts drawn from q the tokens are distributed as the target's own. A sequence of no rows gets r = 0 and only -1.
+ * running sums of p are right to 1e-11 of them, those of p - q to 1e-11 of 1, and a token may differ from the exact rule's where
+ * its uniform number meets a border that closely. With independent uniform numbers and drafts drawn from q the tokens are
+ * distributed as the target's own. A sequence of no rows gets r = 0 and only -1.
  *
  * logits: [num_rows, vocab] of dtype (tq_dtype), vocab at most 2^21, row stride logits_row_stride; -inf masks a token. draft_probs:
  * fp32 [num_rows, vocab], row stride probs_row_stride (rows of no drafted token, the last ones, are not read).
  * A row of a sequence with a temperature that holds a NaN or +inf, or nothing above -inf, has no distribution: it is
  * taken greedily and sets TQ_DEVERR_VALUE if the sequence came to it. A drafted token outside [0, vocab) sets
  * TQ_DEVERR_TOKEN and does not stand. cu_seqlens_q is non-decreasing. A sequence that does not fit num_rows or max_query_len sets
- * TQ_DEVERR_LENGTH and is treated as one of no rows; so may others be where the offsets fall. tokens is int64 [num_seqs, max_query_len], accepted int32 [num_seqs].
+ * TQ_DEVERR_LENGTH and is treated as one of no rows; so may others be where the offsets fall. tokens is int64
+ * [num_seqs, max_query_len], accepted int32 [num_seqs].
  *
  * Needs tq_verify_drafts_workspace_size(...) bytes of workspace (16-byte aligned, any contents; calls that may
  * run at the same time need one each). No counterpart in the reference; it stands beside Engine._sample

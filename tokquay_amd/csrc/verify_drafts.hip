@@ -9,8 +9,9 @@
 //
 // Which side of a border of that running sum u_last falls on decides a token, and 100,000 borders lie
 // close: sums are fp64, of exponentials that are off by at most 2.2e-12 (fp64 FMAs run at the fp32 rate here). A chunk's sum
-// is made of two of them, its columns' to its maximum and that one's to the row's, so borders and p are right to 1e-11; whether
-// a draft stands or which token is drawn can differ from the exact rule where a uniform is that close, for every order of a sum.
+// is made of two of them, its columns' to its maximum and that one's to the row's, so p and its running sums are right to 1e-11 of
+// them (those of p - q to 1e-11 of 1). Whether a draft stands and which token is drawn can differ from the exact rule only where a
+// uniform is that close, for every order of a sum.
 //
 // 1. stats: one workgroup per row and chunk of columns keeps its logits in registers and leaves their maximum and their
 //    sum of exponentials. The logits are read once, 21 vector instructions each, which take about as long as their
