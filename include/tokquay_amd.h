@@ -21,6 +21,14 @@
  *   tq_paged_chunk    causal attention of chunks of new tokens (from one on) straight off a 16-bit pool
  *   tq_verify_drafts  drafted tokens against the target's logits, and the token drawn after them
  *
+ * five for trees of drafted tokens, sampling and the pool's blocks:
+ *
+ *   tq_tree_layout    positions and masks of trees, from their nodes' parents
+ *   tq_paged_tree     attention of trees straight off a 16-bit pool
+ *   tq_sample_tokens  a token of each logit row by temperature, top-k, top-p and min-p
+ *   tq_accept_tree    the path of a tree that the sampled tokens take, and its cache rows moved together
+ *   tq_copy_blocks    copies of blocks of the pool
+ *
  * plus two kernels of the model step around them:
  *
  *   tq_argmax_rows    index of each logit row's maximum (greedy sampling)
@@ -52,8 +60,8 @@
  *     out-of-range block id, slot or length. Such an entry is skipped (the
  *     kernel never reads or writes outside the pool), so the result for that
  *     row is undefined but the launch is memory safe.
- *   - Only head_dim == 64 is supported (GPT-2 family), and 64 and 128 by tq_rope_cache_write and
- *     tq_paged_chunk. block_size may be any value in [1, 1024].
+ *   - Only head_dim == 64 is supported (GPT-2 family), and 64 and 128 by tq_rope_cache_write,
+ *     tq_paged_chunk, tq_paged_tree, tq_accept_tree and tq_copy_blocks. block_size may be any value in [1, 1024].
  *   - Calls are not thread safe with respect to the same pool: the caller
  *     (one engine thread) orders them on one stream.
  */
@@ -83,8 +91,11 @@ typedef enum tq_status {
 #define TQ_DEVERR_POSITION 16  /* a position outside the rotation table */
 #define TQ_DEVERR_TOKEN 32     /* a drafted token outside [0, vocab) */
 #define TQ_DEVERR_VALUE 64     /* a logit row that has no distribution (a NaN or +inf, or nothing above -inf) */
+#define TQ_DEVERR_PARENT 128   /* a tree node whose parent does not come before it */
+#define TQ_DEVERR_OVERLAP 256  /* a block copied to that another copy of the call reads or writes */
 
-/* Element types of the entry points that take one (tq_paged_chunk, tq_rope_cache_write, tq_verify_drafts). */
+/* Element types of the entry points that take one (tq_paged_chunk, tq_paged_tree, tq_rope_cache_write, tq_verify_drafts,
+ * tq_sample_tokens, tq_accept_tree, tq_copy_blocks). */
 typedef enum tq_dtype { TQ_F32 = 0, TQ_F16 = 1, TQ_BF16 = 2 } tq_dtype;
 
 /* Human-readable name of a status code (static storage, never NULL). */
@@ -583,6 +594,102 @@ tq_status tq_verify_drafts(int64_t* tokens, int32_t* accepted, const void* logit
 
 /* Bytes of workspace tq_verify_drafts needs for these sizes. */
 size_t tq_verify_drafts_workspace_size(int32_t num_seqs, int32_t num_rows, int32_t vocab);
+
+/*
+ * The layout of trees of drafted tokens. Sequence b's nodes are rows lo = cu_seqlens_q[b] .. cu_seqlens_q[b+1] - 1; parents[lo + i] is
+ * the index among them of node i's parent, below i, or -1 for a node without one (node 0, the last known token, and any other that
+ * follows the cached tokens directly). With A(i) node i and its ancestors:
+ *
+ *   positions[lo + i] = q_start[b] + |A(i)| - 1       (what the node's rotation takes; its slot is that of position q_start[b] + i)
+ *   masks[lo + i] = bits A(i): bit j % 64 of word j / 64                (mask_words words a row)
+ *
+ * positions is int64 [num_rows], masks int64 [num_rows, mask_words] with 64 mask_words >= max_query_len. Rows of no sequence get
+ * position 0 and no bits. A parent out of its range sets TQ_DEVERR_PARENT and counts as -1; a sequence past num_rows or
+ * max_query_len, or with a negative start, sets TQ_DEVERR_LENGTH and its rows are left alone. cu_seqlens_q is non-decreasing.
+ * No counterpart in the reference.
+ */
+tq_status tq_tree_layout(int64_t* positions, int64_t* masks, int64_t mask_words, const int32_t* parents,
+                         const int32_t* cu_seqlens_q, const int32_t* q_start, int32_t num_seqs, int32_t num_rows,
+                         int32_t max_query_len, int32_t* d_error, void* stream);
+
+/*
+ * tq_paged_chunk for trees of drafted tokens: the keys and values of sequence b's new rows, its nodes, lie at positions
+ * q_start[b] + i, and row i sees every key before q_start[b] and, of the new ones, key q_start[b] + j where j <= i and bit
+ * j % 64 of masks[row][j / 64] is set (tq_tree_layout, or any other mask). A row that sees nothing (no cached keys and no bits) gets
+ * zeros. masks is int64 [num_q_rows, mask_words] with 64 mask_words >= max_query_len. All else, the workspace too
+ * (tq_paged_chunk_workspace_size), is tq_paged_chunk's. No counterpart in the reference.
+ */
+tq_status tq_paged_tree(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                        const void* pool, int64_t num_blocks, int32_t num_layers, int32_t num_heads,
+                        int32_t num_kv_heads, int32_t block_size, int32_t head_dim, int32_t layer,
+                        const int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks_per_seq,
+                        const int32_t* cu_seqlens_q, const int32_t* q_start, const int64_t* masks, int64_t mask_words,
+                        int32_t num_seqs, int32_t num_q_rows, int32_t max_query_len, int32_t max_context_len,
+                        float scale, int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* d_error,
+                        void* stream);
+
+/*
+ * A token of each row of logits, drawn from a given random number. The columns of a row are ranked by logit, largest first, equal ones
+ * (-0 and 0 too) by column; with T the row's temperature and w_j = exp((logit_j - largest) / T):
+ *
+ *   top_k leaves the first k ranks (all where k <= 0);
+ *   top_p of these each rank with less than p of their summed weight before it, the first always (all where p >= 1 or is NaN);
+ *   min_p of these the columns with w_j >= min(p, 1) (all where p <= 0 or is NaN);
+ *   tokens[row] = the lowest column j that is left with  w_0 + .. + w_j > uniforms[row] (w_0 + w_1 + ..)  over those left,
+ *                 the last one with weight where rounding leaves none.
+ *
+ * Where T is not above 0 the token is tq_argmax_rows' column. A row that holds a NaN or +inf, or nothing above -inf, has no
+ * distribution: it is taken greedily, and sets TQ_DEVERR_VALUE where T is above 0. -inf masks a token.
+ *
+ * temperature, top_k, top_p and min_p (the last three: or null) have an entry a row, or, where cu_seqlens_q (num_seqs + 1
+ * entries, non-decreasing) is given, an entry a sequence, for its rows; rows of no sequence are left alone. Without cu_seqlens_q
+ * num_seqs is num_rows. logits is [num_rows, vocab] of dtype (tq_dtype), vocab at most 2^21, rows logits_row_stride elements apart.
+ *
+ * The weights are exponentials off by at most 2.2e-12 and the draw's sums fp64. top_p's sums are whole multiples of vocab 2^-63 (of 2^-51
+ * below 4,097 columns), the largest weight being 1, and so the same for every order. A token may differ from the exact rule's only where
+ * a uniform number, or p times the sum, meets a border that closely.
+ *
+ * No counterpart in the reference's kernels; it stands beside Engine._sample (tokquay/engine.py:83-92, :189-194).
+ */
+tq_status tq_sample_tokens(int64_t* tokens, const void* logits, int64_t logits_row_stride, const float* uniforms,
+                           const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                           const int32_t* cu_seqlens_q, int32_t num_seqs, int32_t num_rows, int32_t vocab,
+                           int32_t dtype, int32_t* d_error, void* stream);
+
+/*
+ * The path of each tree that the sampled tokens take. parents and cu_seqlens_q are tq_tree_layout's, sampled[row] is the token that
+ * the target puts after node row, draft_tokens[row] the token that the node itself is. From node 0 on: path holds the node, tokens the token
+ * after it; the next node is the first of its children whose draft token that is (only those behind their parent are looked at, and none
+ * follows a negative token). counts[b] is the length of the path (0 for a sequence of no rows), at most max_path, where it ends. path
+ * (int32) and tokens (int64) are [num_seqs, max_path], -1 behind the path. The sequence goes on with its counts[b] tokens.
+ *
+ * Where pool is not null, the keys and values of position q_start[b] + path[j] then move to position q_start[b] + j, in all layers, for
+ * every j of the path, so that the cache holds the sequence's first q_start[b] + counts[b] positions. pool is
+ * [num_blocks][num_layers][2][num_kv_heads][block_size][head_dim] of dtype (tq_dtype), head_dim 64 or 128, 16-byte aligned; block_tables and
+ * q_start are tq_paged_chunk's. A block that a position is moved to must be in no other sequence's table.
+ *
+ * A sequence past num_rows (or its block table, with a pool) sets TQ_DEVERR_LENGTH and gets no path; a bad block id sets
+ * TQ_DEVERR_BLOCK_ID and that position is not moved. No counterpart in the reference.
+ */
+tq_status tq_accept_tree(int64_t* tokens, int32_t* path, int32_t* counts, int32_t max_path, const int64_t* sampled,
+                         const int64_t* draft_tokens, const int32_t* parents, const int32_t* cu_seqlens_q,
+                         int32_t num_seqs, int32_t num_rows, void* pool, int64_t num_blocks, int32_t num_layers,
+                         int32_t num_kv_heads, int32_t block_size, int32_t head_dim, int32_t dtype,
+                         const int32_t* block_tables, int64_t block_table_stride, int32_t max_blocks_per_seq,
+                         const int32_t* q_start, int32_t* d_error, void* stream);
+
+/*
+ * Copies blocks of the pool, all layers, keys and values: the first num_slots[p] slots (all block_size where num_slots is null) of block
+ * src_blocks[p] to those of block dst_blocks[p], bit exact, for every pair p. A forked sequence's last block, blocks moved together.
+ * Pairs with a negative id, with src_blocks[p] = dst_blocks[p], or of no slots do nothing. The copies run beside each other: a pair
+ * whose destination is another such pair's source, or the destination of an earlier one, sets TQ_DEVERR_OVERLAP and is left out. An id
+ * >= num_blocks sets TQ_DEVERR_BLOCK_ID, a count outside [0, block_size] TQ_DEVERR_LENGTH, and the pair is left out.
+ * pool is [num_blocks][num_layers][2][num_kv_heads][block_size][head_dim] of dtype (tq_dtype), head_dim 64 or 128, 16-byte aligned.
+ * The reference shares and frees blocks by their counts (tokquay/kv_cache.py:38-127) and copies none.
+ */
+tq_status tq_copy_blocks(void* pool, int64_t num_blocks, int32_t num_layers, int32_t num_kv_heads, int32_t block_size,
+                         int32_t head_dim, int32_t dtype, const int32_t* src_blocks, const int32_t* dst_blocks,
+                         const int32_t* num_slots, int32_t num_pairs, int32_t* d_error, void* stream);
 
 #ifdef __cplusplus
 }

@@ -26,6 +26,8 @@ DEVERR_ORDER = 8
 DEVERR_POSITION = 16
 DEVERR_TOKEN = 32
 DEVERR_VALUE = 64
+DEVERR_PARENT = 128
+DEVERR_OVERLAP = 256
 
 # name -> (restype, argtypes); the order of argtypes is the C declaration's.
 SIGNATURES: dict[str, tuple] = {
@@ -219,6 +221,57 @@ SIGNATURES: dict[str, tuple] = {
         ],
     ),
     "tq_verify_drafts_workspace_size": (ctypes.c_size_t, [ctypes.c_int32] * 3),
+    "tq_tree_layout": (
+        ctypes.c_int,
+        [
+            c_i64p, c_i64p, ctypes.c_int64, c_i32p,  # positions, masks, mask_words, parents
+            c_i32p, c_i32p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,  # cu_seqlens_q, q_start, num_seqs, num_rows, max_query_len
+            c_i32p, ctypes.c_void_p,  # d_error, stream
+        ],
+    ),
+    "tq_paged_tree": (
+        ctypes.c_int,
+        [
+            ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,  # out, stride, q, stride
+            ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,  # pool, num_blocks, num_layers, num_heads
+            ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,  # num_kv_heads, block_size, head_dim, layer
+            c_i32p, ctypes.c_int64, ctypes.c_int32,  # block_tables, block_table_stride, max_blocks_per_seq
+            c_i32p, c_i32p, c_i64p, ctypes.c_int64,  # cu_seqlens_q, q_start, masks, mask_words
+            ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,  # num_seqs, num_q_rows, max_query_len, max_context_len
+            ctypes.c_float, ctypes.c_int32,  # scale, dtype
+            ctypes.c_void_p, ctypes.c_size_t,  # workspace, workspace_bytes
+            c_i32p, ctypes.c_void_p,  # d_error, stream
+        ],
+    ),
+    "tq_sample_tokens": (
+        ctypes.c_int,
+        [
+            c_i64p, ctypes.c_void_p, ctypes.c_int64, c_f32p, c_f32p,  # tokens, logits, logits_row_stride, uniforms, temperature
+            c_i32p, c_f32p, c_f32p, c_i32p,  # top_k, top_p, min_p, cu_seqlens_q
+            ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,  # num_seqs, num_rows, vocab, dtype
+            c_i32p, ctypes.c_void_p,  # d_error, stream
+        ],
+    ),
+    "tq_accept_tree": (
+        ctypes.c_int,
+        [
+            c_i64p, c_i32p, c_i32p, ctypes.c_int32,  # tokens, path, counts, max_path
+            c_i64p, c_i64p, c_i32p, c_i32p,  # sampled, draft_tokens, parents, cu_seqlens_q
+            ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64,  # num_seqs, num_rows, pool, num_blocks
+            ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,  # num_layers, num_kv_heads, block_size, head_dim
+            ctypes.c_int32, c_i32p, ctypes.c_int64, ctypes.c_int32,  # dtype, block_tables, stride, max_blocks_per_seq
+            c_i32p, c_i32p, ctypes.c_void_p,  # q_start, d_error, stream
+        ],
+    ),
+    "tq_copy_blocks": (
+        ctypes.c_int,
+        [
+            ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,  # pool, num_blocks, num_layers, num_kv_heads
+            ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,  # block_size, head_dim, dtype
+            c_i32p, c_i32p, c_i32p, ctypes.c_int32,  # src_blocks, dst_blocks, num_slots, num_pairs
+            c_i32p, ctypes.c_void_p,  # d_error, stream
+        ],
+    ),
     "tq_argmax_rows": (
         ctypes.c_int,
         [c_i64p, c_f32p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p],  # out, logits, rows, cols, row_stride, stream

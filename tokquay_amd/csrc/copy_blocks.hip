@@ -1,0 +1,113 @@
+// Copies of whole or partly filled blocks of the pool, all layers at once.
+//
+// A block is num_layers * 2 * num_kv_heads slabs of block_size slots; the first n slots of each are copied. The copies of one call
+// run beside each other, so none may read what another writes: a pair whose destination is another pair's source, or the
+// destination of an earlier one, is left out and flagged, which every workgroup of the pair finds out by itself.
+#include "tq_internal.h"
+
+namespace tq {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr int kPer = 4;  // pieces of a thread
+
+struct CopyArgs {
+  char* pool;
+  const int32_t* src;
+  const int32_t* dst;
+  const int32_t* num_slots;  // or null: whole blocks
+  int32_t* d_error;
+  int64_t block_bytes;
+  int64_t slab_bytes;
+  int32_t slot_pieces;  // 16-byte pieces of a slot in a slab
+  int32_t slabs;
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t pairs;
+  int32_t slices;
+};
+
+__global__ __launch_bounds__(kThreads) void copy_blocks_kernel(const CopyArgs a) {
+  __shared__ int s_clash;
+  const int slice = blockIdx.x % a.slices, pair = blockIdx.x / a.slices;
+  const int32_t src = a.src[pair], dst = a.dst[pair];
+  const int32_t n = a.num_slots != nullptr ? a.num_slots[pair] : a.block_size;
+  if (src < 0 || dst < 0 || src == dst || n == 0) return;
+  const bool lead = slice == 0 && threadIdx.x == 0;
+  if (src >= a.num_blocks || dst >= a.num_blocks) {
+    if (lead) flag_error(a.d_error, TQ_DEVERR_BLOCK_ID);
+    return;
+  }
+  if (n < 0 || n > a.block_size) {
+    if (lead) flag_error(a.d_error, TQ_DEVERR_LENGTH);
+    return;
+  }
+  if (threadIdx.x == 0) s_clash = 0;
+  __syncthreads();
+  bool clash = false;
+  for (int p = threadIdx.x; p < a.pairs; p += kThreads) {
+    const int32_t s = a.src[p], d = a.dst[p];
+    const bool copies = s >= 0 && d >= 0 && s != d && (a.num_slots == nullptr || a.num_slots[p] != 0);
+    clash |= copies && (s == dst || (d == dst && p < pair));
+  }
+  if (clash) s_clash = 1;
+  __syncthreads();
+  if (s_clash != 0) {
+    if (lead) flag_error(a.d_error, TQ_DEVERR_OVERLAP);
+    return;
+  }
+  const char* from = a.pool + src * a.block_bytes;
+  char* to = a.pool + dst * a.block_bytes;
+  const int64_t run = (int64_t)n * a.slot_pieces, all = run * a.slabs;  // pieces of a slab, of the block
+  const int64_t first = (int64_t)slice * kThreads * kPer + threadIdx.x;
+  u32x4 v[kPer];
+  int64_t at[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int64_t i = first + j * kThreads;
+    at[j] = i / run * a.slab_bytes + i % run * 16;
+    if (i < all) v[j] = *reinterpret_cast<const u32x4*>(from + at[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (first + j * kThreads < all) *reinterpret_cast<u32x4*>(to + at[j]) = v[j];
+}
+
+}  // namespace
+}  // namespace tq
+
+extern "C" tq_status tq_copy_blocks(void* pool, int64_t num_blocks, int32_t num_layers, int32_t num_kv_heads,
+                                    int32_t block_size, int32_t head_dim, int32_t dtype, const int32_t* src_blocks,
+                                    const int32_t* dst_blocks, const int32_t* num_slots, int32_t num_pairs,
+                                    int32_t* d_error, void* stream) {
+  using namespace tq;
+  if (num_pairs < 0 || num_blocks < 1 || num_blocks > 0x7fffffffLL || num_layers < 1 || num_kv_heads < 1 || block_size < 1)
+    return TQ_ERR_INVALID_ARGUMENT;
+  if ((head_dim != 64 && head_dim != 128) || block_size > kMaxBlockSize ||
+      (dtype != TQ_F32 && dtype != TQ_F16 && dtype != TQ_BF16))
+    return TQ_ERR_UNSUPPORTED;
+  if (num_pairs == 0) return TQ_OK;
+  if (pool == nullptr || src_blocks == nullptr || dst_blocks == nullptr || (uintptr_t)pool % 16 != 0)
+    return TQ_ERR_INVALID_ARGUMENT;
+  const int64_t slot = (int64_t)head_dim * (dtype == TQ_F32 ? 4 : 2), slabs = 2LL * num_layers * num_kv_heads;
+  CopyArgs a;
+  a.pool = static_cast<char*>(pool);
+  a.src = src_blocks;
+  a.dst = dst_blocks;
+  a.num_slots = num_slots;
+  a.d_error = d_error;
+  a.slab_bytes = slot * block_size;
+  a.block_bytes = slabs * a.slab_bytes;
+  const int64_t slices = (a.block_bytes / 16 + kThreads * kPer - 1) / (kThreads * kPer);
+  if (slabs > 0x7fffffffLL || slices * num_pairs > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
+  a.slot_pieces = (int32_t)(slot / 16);
+  a.slabs = (int32_t)slabs;
+  a.num_blocks = (int32_t)num_blocks;
+  a.block_size = block_size;
+  a.pairs = num_pairs;
+  a.slices = (int32_t)slices;
+  hipLaunchKernelGGL(copy_blocks_kernel, dim3((unsigned)(slices * num_pairs)), dim3(kThreads), 0, (hipStream_t)stream, a);
+  return check_launch();
+}

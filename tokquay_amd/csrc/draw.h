@@ -1,0 +1,169 @@
+// What the kernels that draw tokens from rows of logits share: exponentials and their sums in fp64, reductions and scans.
+#pragma once
+
+#include <type_traits>
+
+#include "half_types.h"
+
+namespace tq {
+namespace {
+
+// 2^t for t <= 0: 2^k 2^f with k the nearest integer (read off the low bits of t + 1.5 2^52), the second factor by the polynomial
+// that meets 2^f at 0 and at the 8 Chebyshev points of [-1/2, 1/2]; off by at most 2.2e-12, and 1 for 0, so that equal logits
+// have equal, whole weights. Below -1000, and for NaN: 2^-1000, which no sum of theirs notices.
+__device__ __forceinline__ double exp2_neg(double t) {
+  t = __builtin_fmax(t, -1000.0);
+  const double shifted = t + 0x1.8p52;
+  const double f = t - (shifted - 0x1.8p52);
+  double r = 1.3250805512080399e-06;
+  r = __builtin_fma(r, f, 1.5303700711214572e-05);
+  r = __builtin_fma(r, f, 1.5403475186561525e-04);
+  r = __builtin_fma(r, f, 1.333347847368613e-03);
+  r = __builtin_fma(r, f, 9.618129135236088e-03);
+  r = __builtin_fma(r, f, 5.550410906325866e-02);
+  r = __builtin_fma(r, f, 2.4022650695888503e-01);
+  r = __builtin_fma(r, f, 6.931471805568324e-01);
+  r = __builtin_fma(r, f, 1.0);
+  u32x2 bits = __builtin_bit_cast(u32x2, r);
+  bits[1] += __builtin_bit_cast(u32x2, shifted)[0] << 20;
+  return __builtin_bit_cast(double, bits);
+}
+
+template <typename T>
+__device__ __forceinline__ float logit_at(const void* row, int64_t j) {
+  if constexpr (__is_same(T, float))
+    return static_cast<const float*>(row)[j];
+  else
+    return T::load(static_cast<const uint16_t*>(row)[j]);
+}
+
+// The value an argmax_key stands for (NaN: every NaN).
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  if (u == 0xFFFFFFFFu) return __builtin_nanf("");
+  return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+}
+
+// Reductions of a wave, through DPP in rows of 16 lanes and lanes 0, 16, 32, 48 (a 64-bit shuffle through LDS takes five times as
+// long, and they lie on the path of a small call). Every lane gets the result; all orders of the lanes give the same.
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_move64(uint64_t v) {
+  const uint32_t lo = __float_as_uint(dpp_move<CTRL>(__uint_as_float((uint32_t)v)));
+  const uint32_t hi = __float_as_uint(dpp_move<CTRL>(__uint_as_float((uint32_t)(v >> 32))));
+  return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (uint64_t)hi << 32 | lo;
+}
+template <typename F>
+__device__ __forceinline__ uint64_t wave_reduce(uint64_t v, F&& join) {
+  v = join(v, dpp_move64<kDppQuadXor1>(v));
+  v = join(v, dpp_move64<kDppQuadXor2>(v));
+  v = join(v, dpp_move64<kDppRowHalfMirror>(v));
+  v = join(v, dpp_move64<kDppRowMirror>(v));
+  return join(join(lane_of(v, 0), lane_of(v, 16)), join(lane_of(v, 32), lane_of(v, 48)));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+  return __builtin_bit_cast(double, wave_reduce(__builtin_bit_cast(uint64_t, v), [](uint64_t a, uint64_t b) {
+                              return __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, a) + __builtin_bit_cast(double, b));
+                            }));
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+  return wave_reduce(v, [](uint64_t a, uint64_t b) { return max_u64(a, b); });
+}
+__device__ __forceinline__ float wave_maximum(float v) {  // NaN, if any is
+  v = __builtin_elementwise_maximum(v, dpp_move<kDppQuadXor1>(v));
+  v = __builtin_elementwise_maximum(v, dpp_move<kDppQuadXor2>(v));
+  v = __builtin_elementwise_maximum(v, dpp_move<kDppRowHalfMirror>(v));
+  v = __builtin_elementwise_maximum(v, dpp_move<kDppRowMirror>(v));
+  auto lane = [&](int l) { return __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(v), l)); };
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(lane(0), lane(16)),
+                                       __builtin_elementwise_maximum(lane(32), lane(48)));
+}
+
+template <typename T>
+constexpr int kVec = __is_same(T, float) ? 4 : 8;  // logits in 16 bytes
+
+// Thread t's column i of a chunk: pieces of VEC columns t, t + N, .. (of N threads), or (RUNS) PER columns in a row.
+template <int VEC, int N, int PER, bool RUNS>
+__device__ __forceinline__ int column_of(int i) {
+  return RUNS ? (int)threadIdx.x * PER + i : (i / VEC * N + (int)threadIdx.x) * VEC + i % VEC;
+}
+
+// Those columns of a row of T as floats, columns past n as -inf. Rows start at any element.
+template <typename T, int VEC, int N, int PER, bool RUNS>
+__device__ __forceinline__ void columns(const void* row, int base, int n, float (&x)[PER]) {
+  constexpr int kSize = __is_same(T, float) ? 4 : 2;
+#pragma unroll
+  for (int v = 0; v < PER; v += VEC) {
+    const int at = column_of<VEC, N, PER, RUNS>(v);
+    if (at + VEC <= n) {
+      u32x4 w[VEC * kSize / 16];
+      __builtin_memcpy(w, static_cast<const char*>(row) + (int64_t)(base + at) * kSize, VEC * kSize);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if constexpr (__is_same(T, float))
+          x[v + e] = __uint_as_float(w[e / 4][e % 4]);
+        else
+          x[v + e] = T::load((uint16_t)(w[e / 8][e % 8 / 2] >> (16 * (e & 1))));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[v + e] = at + e < n ? logit_at<T>(row, base + at + e) : -INFINITY;
+    }
+  }
+}
+
+constexpr double kLog2e = 1.4426950408889634;
+
+// Inclusive sums (of doubles or 64-bit integers) over the workgroup's N threads, in order; s_part: a word a wave.
+template <int N, typename V>
+__device__ __forceinline__ V scan(V v, V* s_part) {
+  static_assert(sizeof(V) == 8, "moved as 64 bits");
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  auto up = [&](auto ctrl) {  // from a lane further down in the row of 16; 0 past its start
+    return __builtin_bit_cast(V, dpp_move64<decltype(ctrl)::value>(__builtin_bit_cast(uint64_t, v)));
+  };
+  v += up(std::integral_constant<int, 0x111>());  // row_shr:1, 2, 4, 8
+  v += up(std::integral_constant<int, 0x112>());
+  v += up(std::integral_constant<int, 0x114>());
+  v += up(std::integral_constant<int, 0x118>());
+  V before = 0;  // the rows before this one
+#pragma unroll
+  for (int r = 1; r < kWave / 16; ++r) {
+    const V row = __builtin_bit_cast(V, lane_of(__builtin_bit_cast(uint64_t, v), 16 * r - 1));
+    before += lane >= 16 * r ? row : 0;
+  }
+  v += before;
+  if (lane == kWave - 1) s_part[wave] = v;
+  __syncthreads();
+  before = 0;
+#pragma unroll
+  for (int u = 0; u < N / kWave - 1; ++u) before += u < wave ? s_part[u] : 0;
+  __syncthreads();
+  return before + v;
+}
+
+// The first thread with `over`, or the last with `has` where there is none; -1: none either. s_pick: two words a wave.
+template <int N>
+__device__ __forceinline__ int pick(bool over, bool has, int (*s_pick)[2]) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const uint64_t overs = __builtin_amdgcn_ballot_w64(over), those = __builtin_amdgcn_ballot_w64(has);
+  if (lane == 0) {
+    s_pick[wave][0] = overs != 0 ? wave * kWave + __builtin_ctzll(overs) : 0x7fffffff;
+    s_pick[wave][1] = those != 0 ? wave * kWave + 63 - __builtin_clzll(those) : -1;
+  }
+  __syncthreads();
+  int first = 0x7fffffff, last = -1;
+#pragma unroll
+  for (int v = 0; v < N / kWave; ++v) {
+    first = min(first, s_pick[v][0]);
+    last = max(last, s_pick[v][1]);
+  }
+  __syncthreads();
+  return first != 0x7fffffff ? first : last;
+}
+
+}  // namespace
+}  // namespace tq

@@ -62,6 +62,8 @@ struct ChunkArgs {
   int64_t bt_stride;
   const int32_t* cu_q;
   const int32_t* q_start;
+  const uint32_t* masks;  // tq_paged_tree: row r's bits from masks + r mask_words on
+  int64_t mask_words;
   float* part_o;   // [num_q_rows][num_heads][parts][D] sums of each part, or null: one part
   float* part_ml;  // [num_q_rows][num_heads][parts][2] maximum and weight sum
   int32_t* queue;  // kQueueHead words, then (sequence, row tile) pairs: chunk_order_kernel; or null
@@ -142,13 +144,24 @@ __device__ __forceinline__ bool clean_values(uint16_t* s_v, int pieces) {
   return __builtin_amdgcn_ballot_w64(any) != 0;
 }
 
+// Which of the keys from .. from + 31 a tree's row at position qpos sees: every key before `start`, of those from there on the ones
+// its mask names, none behind its own.
+__device__ __forceinline__ uint32_t seen_bits(const ChunkArgs& a, int64_t row, int start, int qpos, int from) {
+  const uint32_t* m = a.masks + row * a.mask_words;
+  const int rel = from - start, w = rel >> 5, own = qpos - from;
+  auto word = [&](int i) { return i < 0 ? ~0u : i < a.mask_words ? m[i] : 0u; };
+  const uint32_t bits = __builtin_amdgcn_alignbit(word(w + 1), word(w), rel & 31);
+  return own >= 31 ? bits : own < 0 ? 0u : bits & ((2u << own) - 1u);
+}
+
 // Values of four dims of a row that the products left out, added to `o`: those of keys from..to - 1 (to: past the row's last
-// key) that are infinities or NaN. head_base is at the first of the dims in the K slab.
-template <typename T>
+// key) that are infinities or NaN. head_base is at the first of the dims in the K slab. TREE: of those the row sees.
+template <typename T, bool TREE>
 __device__ __forceinline__ void add_left_out(const ChunkArgs& a, const int32_t* bt, const uint16_t* head_base, int D,
-                                             int from, int to, f32x4& o) {
+                                             int from, int to, const Seq& s, int t, f32x4& o) {
 #pragma unroll 1
   for (int key = from; key < to; ++key) {
+    if (TREE && !(seen_bits(a, s.row0 + t, s.start, s.start + t, key) & 1u)) continue;
     const int ti = key / a.block_size;
     const int32_t blk = bt[ti];
     if ((uint32_t)blk >= (uint32_t)a.num_blocks) continue;  // flagged by the loads
@@ -284,14 +297,16 @@ struct Loader {
 };
 
 // The rows of one wave: queries, sums, running maxima. KS: 32-key steps of a tile.
-template <int D, int NT, int KS, typename T>
+template <int D, int NT, int KS, typename T, bool TREE>
 struct Rows {
   u32x4 q[NT][D / 32];
   f32x4 o[NT][D / 16];
   f32x4 l[NT];  // sum of the weights, four times
   float m[NT];
   int qpos[NT];
-  int lo, hi;  // positions of the first and last row (uniform)
+  int lo, hi;  // every row sees the keys up to lo, none those past hi (uniform)
+  int start;   // of the sequence, with TREE
+  int64_t row_at;  // a row at position p is row p + row_at of the call, with TREE
 
   typedef f32x4 Scores[2 * KS][NT];  // of keys 16 h + 4 g + 0..3 with row i of row tile n
   typedef u32x4 Weights[KS][NT];     // rounded: of keys 32 k + 4 g + 0..3 and 32 k + 16 + 4 g + 0..3
@@ -311,7 +326,11 @@ struct Rows {
       m[n] = -FLT_MAX;
       l[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    lo = __builtin_amdgcn_readfirstlane(s.start + min(r0, last) / a.group);
+    lo = TREE ? s.start - 1 : __builtin_amdgcn_readfirstlane(s.start + min(r0, last) / a.group);
+    if constexpr (TREE) {
+      start = s.start;
+      row_at = (int64_t)s.row0 - s.start;
+    }
     hi = __builtin_amdgcn_readfirstlane(s.start + min(r0 + kTileRows * NT - 1, last) / a.group);
   }
 
@@ -368,7 +387,18 @@ struct Rows {
   // Masks the scores of the tile of keys kt .. and raises the running maxima where they are passed.
   __device__ __forceinline__ void maxima(const ChunkArgs& a, int kt, Scores& s) {
     const int g = (threadIdx.x & (kWave - 1)) >> 4;
-    if (masked(kt)) {
+    if (TREE && masked(kt)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const uint32_t bits = seen_bits(a, qpos[n] + row_at, start, qpos[n], kt + 32 * k) >> (4 * g);
+#pragma unroll
+          for (int h = 2 * k; h < 2 * k + 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[h][n][e] = bits >> (16 * (h % 2) + e) & 1u ? s[h][n][e] : -INFINITY;
+        }
+    } else if (masked(kt)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -512,6 +542,12 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
+// One over a row's sum of weights; 0 for a tree's row that sees nothing, whose output is zero.
+template <bool TREE>
+__device__ __forceinline__ float inverse(float l) {
+  return TREE && l == 0.f ? 0.f : 1.f / l;
+}
+
 // Few rows: a workgroup takes 16 NT rows and one part of the keys; its waves take every fourth tile of the
 // part, each with its own two K and two V buffers in LDS and no barrier, and join their sums in LDS at the end.
 //
@@ -519,7 +555,7 @@ __device__ __forceinline__ void barrier() {
 // (12 KB and two workgroups at D = 64), which covers the latency of HBM at its full rate. With the tile loaded only when the one
 // before was done: 128 tokens at 511-4,094 positions 557 us instead of 218. Tiles of 64 keys at D = 64 changed nothing on average
 // (32 x 5 drafted tokens 39.7 -> 39.2 us, 64 tokens of 12 heads 38 -> 42, 16 x 4 of 28 heads 32 -> 28).
-template <int D, int NT, typename T>
+template <int D, int NT, typename T, bool TREE>
 __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkArgs a) {
   constexpr int kTileElems = kTileKeys * D;
   __shared__ __attribute__((aligned(16))) uint16_t s_k0[kWaves * kTileElems], s_v0[kWaves * kTileElems],
@@ -547,7 +583,7 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
   const uint16_t* head_base = a.pool_layer + (int64_t)kvh * a.head_stride;
   constexpr int kStep = kWaves * kTileKeys;
   constexpr int J = kTileElems * 2 / 1024;
-  typedef Rows<D, NT, 1, T> R;
+  typedef Rows<D, NT, 1, T, TREE> R;
   R w;
   Loader<D, J> load;
   uint16_t *k0 = s_k0 + wave * kTileElems, *v0 = s_v0 + wave * kTileElems, *k1 = s_k1 + wave * kTileElems,
@@ -643,9 +679,10 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
     }
     const int t = (r0 + r) / a.group, h = kvh * a.group + (r0 + r) - t * a.group;
     if (dirty)
-      add_left_out<T>(a, bt, head_base + d, D, max(kbeg, (w.lo + 1) / kTileKeys * kTileKeys), min(kstop, s.start + t + 1), o);
+      add_left_out<T, TREE>(a, bt, head_base + d, D, max(kbeg, (w.lo + 1) / kTileKeys * kTileKeys), min(kstop, s.start + t + 1),
+                            s, t, o);
     if (a.parts == 1) {
-      const float inv = 1.f / l;
+      const float inv = inverse<TREE>(l);
       *reinterpret_cast<u32x2*>(a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + d) =
           u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
     } else {
@@ -664,7 +701,7 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
 // tokens 85 -> 78 us, 8 x 1,024 behind 4,000-8,000 293 -> 279.
 constexpr int tiles_per_cu(int head_dim) { return head_dim == 64 ? 3 : 2; }
 
-template <int D, int NT, typename T>
+template <int D, int NT, typename T, bool TREE>
 __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b, int tile, int kvh, int part,
                                          uint16_t* s_k0, uint16_t* s_v0, uint16_t* s_k1, uint16_t* s_v1, int& s_dirty) {
   constexpr int kKeys = 64, kTileElems = kKeys * D;
@@ -681,12 +718,12 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
 
   const int32_t* bt = a.block_tables + (int64_t)b * a.bt_stride;
   const uint16_t* head_base = a.pool_layer + (int64_t)kvh * a.head_stride;
-  typedef Rows<D, NT, 2, T> R;
+  typedef Rows<D, NT, 2, T, TREE> R;
   R w;
   const int wr0 = r0 + wave * kRows;  // the wave's first row; from total on: it only loads
   w.init(a, s, kvh, wr0);
   const bool has_rows = wr0 < total;
-  const int lo = s.start + r0 / a.group;  // the workgroup's first position
+  const int lo = TREE ? s.start - 1 : s.start + r0 / a.group;  // every row of the workgroup sees the keys up to it
   if (threadIdx.x == 0) s_dirty = 0;
   Loader<D, J> load;
   const int first = wave * (kKeys / kWaves);
@@ -774,7 +811,7 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
     if (r >= total) continue;
     const int t = r / a.group, h = kvh * a.group + r - t * a.group;
     if (a.parts == 1) {
-      const float inv = 1.f / l;
+      const float inv = inverse<TREE>(l);
       uint16_t* op = a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + 4 * g;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d)
@@ -798,7 +835,7 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
 #pragma unroll 1
     for (int d = 4 * g; d < D; d += 16) {
       f32x4 more = {0.f, 0.f, 0.f, 0.f};
-      add_left_out<T>(a, bt, head_base + d, D, from, min(kstop, s.start + t + 1), more);
+      add_left_out<T, TREE>(a, bt, head_base + d, D, from, min(kstop, s.start + t + 1), s, t, more);
       if (a.parts == 1) {
         uint16_t* op = a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + d;
 #pragma unroll
@@ -819,7 +856,7 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
 // Workgroups go to CUs in turn, so every other 256 of them are dealt backwards on each XCD: the CU with the longest gets
 // the shortest of those beside it (8 x 1,023 tokens of 12 heads of 64 30.0 -> 28.3 us, 8 x 100-1,900 44 -> 42, 2 x 2,000 of
 // 32 heads of 128 84 -> 81; 4 x 1,023 of these 55 -> 57).
-template <int D, int NT, typename T>
+template <int D, int NT, typename T, bool TREE>
 __global__ __launch_bounds__(kWave* kWaves, tiles_per_cu(D)) void chunk_tiles_kernel(const ChunkArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t s_k0[64 * D], s_v0[64 * D], s_k1[64 * D], s_v1[64 * D];
   __shared__ int s_dirty;
@@ -835,7 +872,7 @@ __global__ __launch_bounds__(kWave* kWaves, tiles_per_cu(D)) void chunk_tiles_ke
   const int part = idx % a.parts, b = idx / a.parts;
   Seq s;
   if (!seq_of(a, b, part == 0 && tile == 0 && kvh == 0, s)) return;
-  row_tile<D, NT, T>(a, s, b, tile, kvh, part, s_k0, s_v0, s_k1, s_v1, s_dirty);
+  row_tile<D, NT, T, TREE>(a, s, b, tile, kvh, part, s_k0, s_v0, s_k1, s_v1, s_dirty);
 }
 
 // With more row tiles than run at once, workgroups that stay and take them from a queue, the most keys first: dispatched
@@ -915,7 +952,7 @@ __global__ __launch_bounds__(kOrderThreads) void chunk_order_kernel(const ChunkA
 
 // Item f is pair f / kv_heads with K/V head f % kv_heads. XCD x takes the items f % 8 = x (with a multiple of 8 heads, heads of
 // its own), then those that others left.
-template <int D, int NT, typename T>
+template <int D, int NT, typename T, bool TREE>
 __global__ __launch_bounds__(kWave* kWaves, tiles_per_cu(D)) void chunk_queue_kernel(const ChunkArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t s_k0[64 * D], s_v0[64 * D], s_k1[64 * D], s_v1[64 * D];
   __shared__ int s_dirty;
@@ -944,7 +981,7 @@ __global__ __launch_bounds__(kWave* kWaves, tiles_per_cu(D)) void chunk_queue_ke
     const int tile = __builtin_amdgcn_readfirstlane(a.queue[kQueueHead + 2 * (int64_t)pair + 1]);
     Seq s;
     seq_of(a, b, false, s);
-    row_tile<D, NT, T>(a, s, b, tile, kvh, 0, s_k0, s_v0, s_k1, s_v1, s_dirty);
+    row_tile<D, NT, T, TREE>(a, s, b, tile, kvh, 0, s_k0, s_v0, s_k1, s_v1, s_dirty);
     __syncthreads();  // the buffers and s_item are free
   }
 }
@@ -958,7 +995,7 @@ constexpr int kJoinLanes = D == 64 ? 16 : kWave;
 template <int D>
 constexpr int kJoinPairs = 256 / kJoinLanes<D>;
 
-template <int D, typename T>
+template <int D, typename T, bool TREE>
 __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkArgs a) {
   constexpr int kLanes = kJoinLanes<D>, kDims = D / kLanes;
   typedef float Dims __attribute__((ext_vector_type(kDims)));
@@ -1014,7 +1051,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkArgs a) {
       for (int k = 0; k < kDims; ++k) o[k] = fmaf(w, x[k], o[k]);
     }
   }
-  const float inv = 1.f / l;
+  const float inv = inverse<TREE>(l);
   uint16_t* to = a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + lane * kDims;
 #pragma unroll
   for (int k = 0; k < kDims; k += 2) reinterpret_cast<uint32_t*>(to)[k / 2] = pack2<T>(o[k] * inv, o[k + 1] * inv);
@@ -1075,7 +1112,7 @@ size_t workspace_of(const Plan& p, int32_t num_seqs, int32_t num_q_rows, int32_t
   return p.parts <= 1 ? 0 : (size_t)num_q_rows * num_heads * p.parts * (head_dim + 2) * sizeof(float);
 }
 
-template <int D, typename T>
+template <int D, typename T, bool TREE>
 tq_status launch(const ChunkArgs& a, const Plan& p, hipStream_t stream) {
   const int64_t grid = (int64_t)a.num_seqs * a.kv_heads * a.row_tiles * a.parts;
   const int64_t join = (int64_t)a.num_seqs * (((int64_t)a.max_query_len * a.num_heads + kJoinPairs<D> - 1) / kJoinPairs<D>);
@@ -1085,46 +1122,29 @@ tq_status launch(const ChunkArgs& a, const Plan& p, hipStream_t stream) {
     hipLaunchKernelGGL(chunk_order_kernel, dim3(1), dim3(kOrderThreads), 0, stream, a, p.rows);
     const tq_status st = check_launch();
     if (st != TQ_OK) return st;
-    hipLaunchKernelGGL((chunk_queue_kernel<D, kTilesNt, T>), dim3(tiles_per_cu(D) * kCus), t, 0, stream, a);
+    hipLaunchKernelGGL((chunk_queue_kernel<D, kTilesNt, T, TREE>), dim3(tiles_per_cu(D) * kCus), t, 0, stream, a);
   } else if (p.tiles)
-    hipLaunchKernelGGL((chunk_tiles_kernel<D, kTilesNt, T>), g, t, 0, stream, a);
+    hipLaunchKernelGGL((chunk_tiles_kernel<D, kTilesNt, T, TREE>), g, t, 0, stream, a);
   else
     switch (p.rows) {
-      case 16: hipLaunchKernelGGL((chunk_rows_kernel<D, 1, T>), g, t, 0, stream, a); break;
-      case 32: hipLaunchKernelGGL((chunk_rows_kernel<D, 2, T>), g, t, 0, stream, a); break;
-      case 48: hipLaunchKernelGGL((chunk_rows_kernel<D, 3, T>), g, t, 0, stream, a); break;
-      default: hipLaunchKernelGGL((chunk_rows_kernel<D, 4, T>), g, t, 0, stream, a); break;
+      case 16: hipLaunchKernelGGL((chunk_rows_kernel<D, 1, T, TREE>), g, t, 0, stream, a); break;
+      case 32: hipLaunchKernelGGL((chunk_rows_kernel<D, 2, T, TREE>), g, t, 0, stream, a); break;
+      case 48: hipLaunchKernelGGL((chunk_rows_kernel<D, 3, T, TREE>), g, t, 0, stream, a); break;
+      default: hipLaunchKernelGGL((chunk_rows_kernel<D, 4, T, TREE>), g, t, 0, stream, a); break;
     }
   tq_status st = check_launch();
   if (st != TQ_OK || a.parts == 1) return st;
-  hipLaunchKernelGGL((chunk_join_kernel<D, T>), dim3((unsigned)join), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((chunk_join_kernel<D, T, TREE>), dim3((unsigned)join), dim3(256), 0, stream, a);
   return check_launch();
 }
 
-}  // namespace
-}  // namespace tq
-
-extern "C" size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
-                                                int32_t head_dim, int32_t num_q_rows, int32_t max_query_len,
-                                                int32_t max_context_len) {
-  using namespace tq;
-  if (!sizes_ok(num_seqs, num_heads, num_kv_heads, head_dim, num_q_rows, max_query_len, max_context_len) ||
-      num_seqs == 0 || num_q_rows == 0 || max_query_len == 0 || max_context_len == 0 || max_context_len > kMaxContext)
-    return 0;
-  const int32_t group = num_heads / num_kv_heads;
-  const Plan p = plan_of(num_seqs, num_kv_heads, group, head_dim, num_q_rows, max_query_len, max_context_len);
-  return workspace_of(p, num_seqs, num_q_rows, num_heads, group, head_dim);
-}
-
-extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
-                                    const void* pool, int64_t num_blocks, int32_t num_layers, int32_t num_heads,
-                                    int32_t num_kv_heads, int32_t block_size, int32_t head_dim, int32_t layer,
-                                    const int32_t* block_tables, int64_t block_table_stride,
-                                    int32_t max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start,
-                                    int32_t num_seqs, int32_t num_q_rows, int32_t max_query_len,
-                                    int32_t max_context_len, float scale, int32_t dtype, void* workspace,
-                                    size_t workspace_bytes, int32_t* d_error, void* stream) {
-  using namespace tq;
+template <bool TREE>
+tq_status attend(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride, const void* pool,
+                 int64_t num_blocks, int32_t num_layers, int32_t num_heads, int32_t num_kv_heads, int32_t block_size,
+                 int32_t head_dim, int32_t layer, const int32_t* block_tables, int64_t block_table_stride,
+                 int32_t max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start, const int64_t* masks,
+                 int64_t mask_words, int32_t num_seqs, int32_t num_q_rows, int32_t max_query_len, int32_t max_context_len,
+                 float scale, int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* d_error, void* stream) {
   if (!sizes_ok(num_seqs, num_heads, num_kv_heads, head_dim, num_q_rows, max_query_len, max_context_len) ||
       num_blocks < 1 || num_blocks > 0x7fffffffLL || num_layers < 1 || block_size < 1 || layer < 0 ||
       layer >= num_layers || max_blocks_per_seq < 0 || !(scale - scale == 0.f))
@@ -1138,6 +1158,7 @@ extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const voi
       q_start == nullptr || block_table_stride < max_blocks_per_seq || out_row_stride < width ||
       q_row_stride < width || max_context_len < 1)
     return TQ_ERR_INVALID_ARGUMENT;
+  if (TREE && (masks == nullptr || mask_words > 0x3fffffffLL || mask_words * 64 < max_query_len)) return TQ_ERR_INVALID_ARGUMENT;
   // 16-byte loads of q and the pool, 8-byte stores of out.
   if (((uintptr_t)q | (uintptr_t)pool) % 16 != 0 || (uintptr_t)out % 8 != 0 || q_row_stride % 8 != 0 ||
       out_row_stride % 4 != 0)
@@ -1165,6 +1186,8 @@ extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const voi
   a.bt_stride = block_table_stride;
   a.cu_q = cu_seqlens_q;
   a.q_start = q_start;
+  a.masks = reinterpret_cast<const uint32_t*>(masks);
+  a.mask_words = 2 * mask_words;
   a.queue = p.queue ? static_cast<int32_t*>(workspace) : nullptr;
   a.part_o = p.parts > 1 ? static_cast<float*>(workspace) : nullptr;
   a.part_ml = a.part_o == nullptr ? nullptr : a.part_o + (size_t)num_q_rows * num_heads * p.parts * head_dim;
@@ -1190,6 +1213,50 @@ extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const voi
   a.part_tokens = p.part_tokens;
   const hipStream_t st = (hipStream_t)stream;
   if (head_dim == 64)
-    return dtype == TQ_BF16 ? launch<64, Bf16>(a, p, st) : launch<64, Fp16>(a, p, st);
-  return dtype == TQ_BF16 ? launch<128, Bf16>(a, p, st) : launch<128, Fp16>(a, p, st);
+    return dtype == TQ_BF16 ? launch<64, Bf16, TREE>(a, p, st) : launch<64, Fp16, TREE>(a, p, st);
+  return dtype == TQ_BF16 ? launch<128, Bf16, TREE>(a, p, st) : launch<128, Fp16, TREE>(a, p, st);
+}
+
+}  // namespace
+}  // namespace tq
+
+extern "C" size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                                int32_t head_dim, int32_t num_q_rows, int32_t max_query_len,
+                                                int32_t max_context_len) {
+  using namespace tq;
+  if (!sizes_ok(num_seqs, num_heads, num_kv_heads, head_dim, num_q_rows, max_query_len, max_context_len) ||
+      num_seqs == 0 || num_q_rows == 0 || max_query_len == 0 || max_context_len == 0 || max_context_len > kMaxContext)
+    return 0;
+  const int32_t group = num_heads / num_kv_heads;
+  const Plan p = plan_of(num_seqs, num_kv_heads, group, head_dim, num_q_rows, max_query_len, max_context_len);
+  return workspace_of(p, num_seqs, num_q_rows, num_heads, group, head_dim);
+}
+
+extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                                    const void* pool, int64_t num_blocks, int32_t num_layers, int32_t num_heads,
+                                    int32_t num_kv_heads, int32_t block_size, int32_t head_dim, int32_t layer,
+                                    const int32_t* block_tables, int64_t block_table_stride,
+                                    int32_t max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start,
+                                    int32_t num_seqs, int32_t num_q_rows, int32_t max_query_len,
+                                    int32_t max_context_len, float scale, int32_t dtype, void* workspace,
+                                    size_t workspace_bytes, int32_t* d_error, void* stream) {
+  return tq::attend<false>(out, out_row_stride, q, q_row_stride, pool, num_blocks, num_layers, num_heads, num_kv_heads, block_size,
+                           head_dim, layer, block_tables, block_table_stride, max_blocks_per_seq, cu_seqlens_q, q_start, nullptr, 0,
+                           num_seqs, num_q_rows, max_query_len, max_context_len, scale, dtype, workspace, workspace_bytes,
+                           d_error, stream);
+}
+
+extern "C" tq_status tq_paged_tree(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                                    const void* pool, int64_t num_blocks, int32_t num_layers, int32_t num_heads,
+                                    int32_t num_kv_heads, int32_t block_size, int32_t head_dim, int32_t layer,
+                                    const int32_t* block_tables, int64_t block_table_stride,
+                                    int32_t max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* q_start,
+                                    const int64_t* masks, int64_t mask_words,
+                                    int32_t num_seqs, int32_t num_q_rows, int32_t max_query_len,
+                                    int32_t max_context_len, float scale, int32_t dtype, void* workspace,
+                                    size_t workspace_bytes, int32_t* d_error, void* stream) {
+  return tq::attend<true>(out, out_row_stride, q, q_row_stride, pool, num_blocks, num_layers, num_heads, num_kv_heads, block_size,
+                          head_dim, layer, block_tables, block_table_stride, max_blocks_per_seq, cu_seqlens_q, q_start, masks, mask_words,
+                          num_seqs, num_q_rows, max_query_len, max_context_len, scale, dtype, workspace, workspace_bytes,
+                          d_error, stream);
 }

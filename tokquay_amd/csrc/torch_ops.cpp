@@ -416,11 +416,19 @@ void rope_cache_write(at::Tensor q_out, const at::Tensor& q, const at::Tensor& k
         "tq_rope_cache_write");
 }
 
-void paged_chunk(at::Tensor out, const at::Tensor& q, const at::Tensor& pool, int64_t layer,
-                 const at::Tensor& block_tables, const at::Tensor& cu_seqlens_q, const at::Tensor& q_start,
-                 int64_t max_query_len, int64_t max_context_len, double scale,
-                 const c10::optional<at::Tensor>& workspace, const c10::optional<at::Tensor>& d_error) {
-  const char* op = "tokquay_amd::paged_chunk";
+// An int64 [rows, words] tensor of masks of max_query_len bits.
+void masks_of(const char* op, const at::Tensor& t, int64_t rows, int64_t max_query_len, at::Device device) {
+  TORCH_CHECK(t.device() == device && t.scalar_type() == at::kLong && t.dim() == 2 && t.size(0) == rows &&
+                  t.is_contiguous() && t.size(1) <= 0x3fffffff && t.size(1) >= (max_query_len + 63) / 64,
+              op, ": masks must be a contiguous int64 [", rows, ", words] tensor of at least ", max_query_len,
+              " bits a row on ", device);
+}
+
+// paged_chunk, or paged_tree where there are masks.
+void attend(const char* op, at::Tensor& out, const at::Tensor& q, const at::Tensor& pool, int64_t layer,
+            const at::Tensor& block_tables, const at::Tensor& cu_seqlens_q, const at::Tensor& q_start,
+            const at::Tensor* masks, int64_t max_query_len, int64_t max_context_len, double scale,
+            const c10::optional<at::Tensor>& workspace, const c10::optional<at::Tensor>& d_error) {
   const Pool p = typed_pool_of(op, pool, layer, false);
   vector_of(op, "q_start", q_start, at::kInt, 0, p);
   const int64_t n = q_start.numel();
@@ -444,6 +452,7 @@ void paged_chunk(at::Tensor out, const at::Tensor& q, const at::Tensor& pool, in
                 ": max_context_len and block_tables must have room for the sequences");
     TORCH_CHECK(pool.numel() / p.blocks <= INT32_MAX, op, ": a block of the pool has too many elements");
   }
+  if (masks != nullptr) masks_of(op, *masks, rows, max_query_len, q.device());
   error_word_of(op, d_error, p);
   size_t ws = workspace_of(op, workspace, p);
   const size_t need = tq_paged_chunk_workspace_size((int32_t)n, (int32_t)heads, p.heads, p.head_dim, (int32_t)rows,
@@ -455,12 +464,37 @@ void paged_chunk(at::Tensor out, const at::Tensor& q, const at::Tensor& pool, in
     at_ws = own.data_ptr();
     ws = need;
   }
-  check(tq_paged_chunk(out.data_ptr(), os, q.data_ptr(), qs, pool.data_ptr(), p.blocks, p.layers, (int32_t)heads,
-                       p.heads, p.block_size, p.head_dim, (int32_t)layer, block_tables.data_ptr<int32_t>(), ts,
-                       (int32_t)block_tables.size(1), cu_seqlens_q.data_ptr<int32_t>(), q_start.data_ptr<int32_t>(),
-                       (int32_t)n, (int32_t)rows, (int32_t)max_query_len, (int32_t)max_context_len, (float)scale,
-                       dtype_of(pool.scalar_type()), at_ws, ws, ptr<int32_t>(d_error), stream_of(pool)),
-        "tq_paged_chunk");
+  if (masks != nullptr)
+    check(tq_paged_tree(out.data_ptr(), os, q.data_ptr(), qs, pool.data_ptr(), p.blocks, p.layers, (int32_t)heads,
+                        p.heads, p.block_size, p.head_dim, (int32_t)layer, block_tables.data_ptr<int32_t>(), ts,
+                        (int32_t)block_tables.size(1), cu_seqlens_q.data_ptr<int32_t>(), q_start.data_ptr<int32_t>(),
+                        masks->data_ptr<int64_t>(), masks->size(1), (int32_t)n, (int32_t)rows, (int32_t)max_query_len,
+                        (int32_t)max_context_len, (float)scale, dtype_of(pool.scalar_type()), at_ws, ws,
+                        ptr<int32_t>(d_error), stream_of(pool)),
+          "tq_paged_tree");
+  else
+    check(tq_paged_chunk(out.data_ptr(), os, q.data_ptr(), qs, pool.data_ptr(), p.blocks, p.layers, (int32_t)heads,
+                         p.heads, p.block_size, p.head_dim, (int32_t)layer, block_tables.data_ptr<int32_t>(), ts,
+                         (int32_t)block_tables.size(1), cu_seqlens_q.data_ptr<int32_t>(), q_start.data_ptr<int32_t>(),
+                         (int32_t)n, (int32_t)rows, (int32_t)max_query_len, (int32_t)max_context_len, (float)scale,
+                         dtype_of(pool.scalar_type()), at_ws, ws, ptr<int32_t>(d_error), stream_of(pool)),
+          "tq_paged_chunk");
+}
+
+void paged_chunk(at::Tensor out, const at::Tensor& q, const at::Tensor& pool, int64_t layer,
+                 const at::Tensor& block_tables, const at::Tensor& cu_seqlens_q, const at::Tensor& q_start,
+                 int64_t max_query_len, int64_t max_context_len, double scale,
+                 const c10::optional<at::Tensor>& workspace, const c10::optional<at::Tensor>& d_error) {
+  attend("tokquay_amd::paged_chunk", out, q, pool, layer, block_tables, cu_seqlens_q, q_start, nullptr, max_query_len,
+         max_context_len, scale, workspace, d_error);
+}
+
+void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& pool, int64_t layer,
+                const at::Tensor& block_tables, const at::Tensor& cu_seqlens_q, const at::Tensor& q_start,
+                const at::Tensor& masks, int64_t max_query_len, int64_t max_context_len, double scale,
+                const c10::optional<at::Tensor>& workspace, const c10::optional<at::Tensor>& d_error) {
+  attend("tokquay_amd::paged_tree", out, q, pool, layer, block_tables, cu_seqlens_q, q_start, &masks, max_query_len,
+         max_context_len, scale, workspace, d_error);
 }
 
 // A [rows, vocab] tensor with contiguous rows on p's device; its row stride.
@@ -513,6 +547,127 @@ void verify_drafts(at::Tensor tokens, at::Tensor accepted, const at::Tensor& log
         "tq_verify_drafts");
 }
 
+// ---- trees of drafted tokens, sampling, copies of blocks
+
+// A pool whose slots are copied: a block's places of one slot number fit 31 bits, its address 16 bytes.
+void slots_of(const char* op, const at::Tensor& pool) {
+  TORCH_CHECK((uintptr_t)pool.data_ptr() % 16 == 0, op, ": pool must be 16-byte aligned");
+  TORCH_CHECK(pool.numel() / (pool.size(0) * pool.size(4)) <= 1 << 30, op, ": a slot of the pool has too many elements");
+}
+
+// A contiguous vector with `entries` entries (any number: -1) on `device`.
+void exactly(const char* op, const char* name, const at::Tensor& t, at::ScalarType type, int64_t entries, at::Device device) {
+  TORCH_CHECK(t.device() == device && t.scalar_type() == type && t.dim() == 1 && t.is_contiguous() &&
+                  (entries < 0 || t.numel() == entries) && t.numel() <= INT32_MAX,
+              op, ": ", name, " must be a contiguous ", type, " [", entries < 0 ? std::string("N") : std::to_string(entries),
+              "] tensor on ", device);
+}
+
+void tree_layout(at::Tensor positions, at::Tensor masks, const at::Tensor& parents, const at::Tensor& cu_seqlens_q,
+                 const at::Tensor& q_start, int64_t max_query_len, const c10::optional<at::Tensor>& d_error) {
+  const char* op = "tokquay_amd::tree_layout";
+  const at::Device device = parents.device();
+  TORCH_CHECK(parents.is_cuda(), op, ": parents must be on a HIP device");
+  exactly(op, "parents", parents, at::kInt, -1, device);
+  exactly(op, "q_start", q_start, at::kInt, -1, device);
+  const int64_t rows = parents.numel(), n = q_start.numel();
+  exactly(op, "cu_seqlens_q", cu_seqlens_q, at::kInt, n + 1, device);
+  exactly(op, "positions", positions, at::kLong, rows, device);
+  TORCH_CHECK(max_query_len >= 0 && max_query_len <= INT32_MAX, op, ": max_query_len must be a length");
+  masks_of(op, masks, rows, max_query_len, device);
+  if (d_error.has_value()) exactly(op, "d_error", *d_error, at::kInt, 1, device);
+  check(tq_tree_layout(positions.data_ptr<int64_t>(), masks.data_ptr<int64_t>(), masks.size(1),
+                       parents.data_ptr<int32_t>(), cu_seqlens_q.data_ptr<int32_t>(), q_start.data_ptr<int32_t>(),
+                       (int32_t)n, (int32_t)rows, (int32_t)max_query_len, ptr<int32_t>(d_error), stream_of(parents)),
+        "tq_tree_layout");
+}
+
+void sample_tokens(at::Tensor tokens, const at::Tensor& logits, const at::Tensor& uniforms, const at::Tensor& temperature,
+                   const c10::optional<at::Tensor>& top_k, const c10::optional<at::Tensor>& top_p,
+                   const c10::optional<at::Tensor>& min_p, const c10::optional<at::Tensor>& cu_seqlens_q,
+                   const c10::optional<at::Tensor>& d_error) {
+  const char* op = "tokquay_amd::sample_tokens";
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && dtype_of(logits.scalar_type()) >= 0, op,
+              ": logits must be a float32, float16 or bfloat16 [rows, vocab] tensor on a HIP device");
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  const at::Device device = logits.device();
+  TORCH_CHECK(rows <= INT32_MAX && vocab >= 1 && vocab <= 1 << 21, op, ": logits must have 1 to 2097152 columns");
+  const int64_t ls = vocab_rows_of(op, "logits", logits, rows, vocab);
+  exactly(op, "temperature", temperature, at::kFloat, cu_seqlens_q.has_value() ? -1 : rows, device);
+  const int64_t n = temperature.numel();
+  if (cu_seqlens_q.has_value()) exactly(op, "cu_seqlens_q", *cu_seqlens_q, at::kInt, n + 1, device);
+  if (top_k.has_value()) exactly(op, "top_k", *top_k, at::kInt, n, device);
+  if (top_p.has_value()) exactly(op, "top_p", *top_p, at::kFloat, n, device);
+  if (min_p.has_value()) exactly(op, "min_p", *min_p, at::kFloat, n, device);
+  exactly(op, "uniforms", uniforms, at::kFloat, rows, device);
+  exactly(op, "tokens", tokens, at::kLong, rows, device);
+  if (d_error.has_value()) exactly(op, "d_error", *d_error, at::kInt, 1, device);
+  check(tq_sample_tokens(tokens.data_ptr<int64_t>(), logits.data_ptr(), ls, uniforms.data_ptr<float>(),
+                         temperature.data_ptr<float>(), ptr<int32_t>(top_k), ptr<float>(top_p), ptr<float>(min_p),
+                         ptr<int32_t>(cu_seqlens_q), (int32_t)n, (int32_t)rows, (int32_t)vocab,
+                         dtype_of(logits.scalar_type()), ptr<int32_t>(d_error), stream_of(logits)),
+        "tq_sample_tokens");
+}
+
+void accept_tree(at::Tensor tokens, at::Tensor path, at::Tensor counts, const at::Tensor& sampled,
+                 const at::Tensor& draft_tokens, const at::Tensor& parents, const at::Tensor& cu_seqlens_q,
+                 const c10::optional<at::Tensor>& pool, const c10::optional<at::Tensor>& block_tables,
+                 const c10::optional<at::Tensor>& q_start, const c10::optional<at::Tensor>& d_error) {
+  const char* op = "tokquay_amd::accept_tree";
+  const at::Device device = sampled.device();
+  TORCH_CHECK(sampled.is_cuda(), op, ": sampled must be on a HIP device");
+  exactly(op, "sampled", sampled, at::kLong, -1, device);
+  exactly(op, "counts", counts, at::kInt, -1, device);
+  const int64_t rows = sampled.numel(), n = counts.numel();
+  exactly(op, "draft_tokens", draft_tokens, at::kLong, rows, device);
+  exactly(op, "parents", parents, at::kInt, rows, device);
+  exactly(op, "cu_seqlens_q", cu_seqlens_q, at::kInt, n + 1, device);
+  const auto per_seq = [&](const char* name, const at::Tensor& t, at::ScalarType type, int64_t columns) {
+    TORCH_CHECK(t.device() == device && t.scalar_type() == type && t.dim() == 2 && t.size(0) == n && t.size(1) >= 1 &&
+                    (columns < 0 || t.size(1) == columns) && t.size(1) <= INT32_MAX && t.is_contiguous(),
+                op, ": ", name, " must be a contiguous ", type, " [", n, ", max_path] tensor on ", device);
+  };
+  per_seq("tokens", tokens, at::kLong, -1);
+  per_seq("path", path, at::kInt, tokens.size(1));
+  if (d_error.has_value()) exactly(op, "d_error", *d_error, at::kInt, 1, device);
+  TORCH_CHECK(pool.has_value() == block_tables.has_value() && pool.has_value() == q_start.has_value(), op,
+              ": pool, block_tables and q_start go together");
+  Pool p{1, 1, 1, 1, 64, device};
+  int64_t ts = 0;
+  if (pool.has_value()) {
+    p = typed_pool_of(op, *pool, 0, true);
+    TORCH_CHECK(p.device == device, op, ": pool is on ", p.device, ", sampled on ", device);
+    slots_of(op, *pool);
+    ts = tables_of(op, "block_tables", *block_tables, n, p);
+    TORCH_CHECK(block_tables->size(1) <= INT32_MAX, op, ": block_tables has too many columns");
+    exactly(op, "q_start", *q_start, at::kInt, n, device);
+  }
+  check(tq_accept_tree(tokens.data_ptr<int64_t>(), path.data_ptr<int32_t>(), counts.data_ptr<int32_t>(),
+                       (int32_t)tokens.size(1), sampled.data_ptr<int64_t>(), draft_tokens.data_ptr<int64_t>(),
+                       parents.data_ptr<int32_t>(), cu_seqlens_q.data_ptr<int32_t>(), (int32_t)n, (int32_t)rows,
+                       ptr<void>(pool), p.blocks, p.layers, p.heads, p.block_size, p.head_dim,
+                       pool.has_value() ? dtype_of(pool->scalar_type()) : TQ_F32, ptr<int32_t>(block_tables), ts,
+                       block_tables.has_value() ? (int32_t)block_tables->size(1) : 0, ptr<int32_t>(q_start),
+                       ptr<int32_t>(d_error), stream_of(sampled)),
+        "tq_accept_tree");
+}
+
+void copy_blocks(at::Tensor pool, const at::Tensor& src_blocks, const at::Tensor& dst_blocks,
+                 const c10::optional<at::Tensor>& num_slots, const c10::optional<at::Tensor>& d_error) {
+  const char* op = "tokquay_amd::copy_blocks";
+  const Pool p = typed_pool_of(op, pool, 0, true);
+  slots_of(op, pool);
+  exactly(op, "src_blocks", src_blocks, at::kInt, -1, p.device);
+  const int64_t n = src_blocks.numel();
+  exactly(op, "dst_blocks", dst_blocks, at::kInt, n, p.device);
+  if (num_slots.has_value()) exactly(op, "num_slots", *num_slots, at::kInt, n, p.device);
+  if (d_error.has_value()) exactly(op, "d_error", *d_error, at::kInt, 1, p.device);
+  check(tq_copy_blocks(pool.data_ptr(), p.blocks, p.layers, p.heads, p.block_size, p.head_dim,
+                       dtype_of(pool.scalar_type()), src_blocks.data_ptr<int32_t>(), dst_blocks.data_ptr<int32_t>(),
+                       ptr<int32_t>(num_slots), (int32_t)n, ptr<int32_t>(d_error), stream_of(pool)),
+        "tq_copy_blocks");
+}
+
 }  // namespace
 
 TORCH_LIBRARY(tokquay_amd, m) {
@@ -541,6 +696,17 @@ TORCH_LIBRARY(tokquay_amd, m) {
         "Tensor(c!)? d_error) -> ()");
   m.def("verify_drafts(Tensor(a!) tokens, Tensor(b!) accepted, Tensor logits, Tensor? draft_probs, "
         "Tensor draft_tokens, Tensor uniforms, Tensor temperature, Tensor cu_seqlens_q, Tensor(c!)? d_error) -> ()");
+  m.def("tree_layout(Tensor(a!) positions, Tensor(b!) masks, Tensor parents, Tensor cu_seqlens_q, Tensor q_start, "
+        "int max_query_len, Tensor(c!)? d_error) -> ()");
+  m.def("paged_tree(Tensor(a!) out, Tensor q, Tensor pool, int layer, Tensor block_tables, Tensor cu_seqlens_q, "
+        "Tensor q_start, Tensor masks, int max_query_len, int max_context_len, float scale, Tensor(b!)? workspace, "
+        "Tensor(c!)? d_error) -> ()");
+  m.def("sample_tokens(Tensor(a!) tokens, Tensor logits, Tensor uniforms, Tensor temperature, Tensor? top_k, "
+        "Tensor? top_p, Tensor? min_p, Tensor? cu_seqlens_q, Tensor(b!)? d_error) -> ()");
+  m.def("accept_tree(Tensor(a!) tokens, Tensor(b!) path, Tensor(c!) counts, Tensor sampled, Tensor draft_tokens, "
+        "Tensor parents, Tensor cu_seqlens_q, Tensor(d!)? pool, Tensor? block_tables, Tensor? q_start, "
+        "Tensor(e!)? d_error) -> ()");
+  m.def("copy_blocks(Tensor(a!) pool, Tensor src_blocks, Tensor dst_blocks, Tensor? num_slots, Tensor(b!)? d_error) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(tokquay_amd, CUDA, m) {
@@ -555,4 +721,9 @@ TORCH_LIBRARY_IMPL(tokquay_amd, CUDA, m) {
   m.impl("rope_cache_write", &rope_cache_write);
   m.impl("paged_chunk", &paged_chunk);
   m.impl("verify_drafts", &verify_drafts);
+  m.impl("tree_layout", &tree_layout);
+  m.impl("paged_tree", &paged_tree);
+  m.impl("sample_tokens", &sample_tokens);
+  m.impl("accept_tree", &accept_tree);
+  m.impl("copy_blocks", &copy_blocks);
 }

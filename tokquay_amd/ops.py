@@ -615,6 +615,128 @@ def verify_drafts(
     return tokens, accepted
 
 
+# ------------------------------------------------------- trees of drafted tokens, sampling, copies of blocks
+def tree_layout(
+    parents: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    q_start: torch.Tensor,
+    max_query_len: int,
+    d_error: torch.Tensor | None = None,
+    positions: torch.Tensor | None = None,
+    masks: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(positions, masks)`` of trees of drafted tokens, int64 ``[N]`` and int64 ``[N, words]``, from each node's parent.
+
+    Sequence b's nodes are its rows by ``cu_seqlens_q`` (``paged_chunk``'s), node 0 its last known token; ``parents`` (int32
+    ``[N]``) counts inside the sequence: below the node itself, -1 for none. A node's position is ``q_start[b]`` plus
+    its number of ancestors, what ``rope_cache_write`` rotates by, while its slot is that of position ``q_start[b] + i``. Its mask has a bit for
+    itself and for each ancestor, node j's in word ``j // 64``: what ``paged_tree`` takes. Rows of no sequence get zeros. For all layers of a step
+    one call is enough."""
+    n = parents.numel()
+    if positions is None:
+        positions = torch.empty(n, dtype=torch.int64, device=parents.device)
+    if masks is None:
+        masks = torch.empty(n, -(-max_query_len // 64), dtype=torch.int64, device=parents.device)
+    _checked_op("tree_layout", positions, masks, parents, cu_seqlens_q, q_start, max_query_len, d_error)
+    return positions, masks
+
+
+def paged_tree(
+    out: torch.Tensor,
+    q: torch.Tensor,
+    pool: torch.Tensor,
+    layer: int,
+    block_tables: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    q_start: torch.Tensor,
+    masks: torch.Tensor,
+    max_query_len: int,
+    max_context_len: int,
+    scale: float | None = None,
+    workspace: torch.Tensor | None = None,
+    d_error: torch.Tensor | None = None,
+) -> None:
+    """``paged_chunk`` for trees of drafted tokens: row i of sequence b sees every key before ``q_start[b]`` and, of the sequence's new
+    ones, the keys ``q_start[b] + j``, ``j <= i``, whose bit j of the row's mask is set. ``masks`` is ``tree_layout``'s, or any
+    other int64 ``[N, words]``. A row that sees nothing gets zeros. A line of drafts takes the same time in ``paged_chunk``, which
+    needs no masks. The workspace is ``paged_chunk``'s (``chunk_workspace_bytes``)."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(pool.size(-1))
+    _checked_op("paged_tree", out, q, pool, layer, block_tables, cu_seqlens_q, q_start, masks, max_query_len, max_context_len,
+                scale, workspace, d_error)  # fmt: skip
+
+
+def sample_tokens(
+    logits: torch.Tensor,
+    uniforms: torch.Tensor,
+    temperature: torch.Tensor,
+    top_k: torch.Tensor | None = None,
+    top_p: torch.Tensor | None = None,
+    min_p: torch.Tensor | None = None,
+    cu_seqlens_q: torch.Tensor | None = None,
+    d_error: torch.Tensor | None = None,
+    tokens: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """A token of each row of ``logits`` (``[N, vocab]``, float32, float16 or bfloat16), int64 ``[N]``, drawn with the row's number of
+    ``uniforms`` (float32 in [0, 1)).
+
+    Each row's settings: ``temperature`` (float32; 0 is greedy: ``argmax_rows``), ``top_k`` (int32; 0: off), then of those columns
+    ``top_p`` (float32; 1: off), then ``min_p`` (float32, of the largest probability; 0: off). Equal logits rank by column, the lowest
+    first, so exactly k are left. The draw is the lowest column whose running sum of what is left passes the uniform number's share.
+    With ``cu_seqlens_q`` (``paged_chunk``'s) the settings have an entry a sequence, for all of its rows, and rows of no sequence keep
+    their token. Mask tokens with -inf logits."""
+    if tokens is None:
+        tokens = torch.empty(logits.size(0), dtype=torch.int64, device=logits.device)
+    _checked_op("sample_tokens", tokens, logits, uniforms, temperature, top_k, top_p, min_p, cu_seqlens_q, d_error)
+    return tokens
+
+
+def accept_tree(
+    sampled: torch.Tensor,
+    draft_tokens: torch.Tensor,
+    parents: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    max_path: int,
+    pool: torch.Tensor | None = None,
+    block_tables: torch.Tensor | None = None,
+    q_start: torch.Tensor | None = None,
+    d_error: torch.Tensor | None = None,
+    tokens: torch.Tensor | None = None,
+    path: torch.Tensor | None = None,
+    counts: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The path of each tree that the sampled tokens take: ``(tokens, path, counts)``, int64 and int32 ``[B, max_path]`` (-1 behind
+    the path) and int32 ``[B]``.
+
+    ``sampled`` (int64 ``[N]``, ``sample_tokens`` over the nodes' logits) is the token after each node, ``draft_tokens`` (int64 ``[N]``) the one that
+    each node is; ``parents`` and ``cu_seqlens_q`` are ``tree_layout``'s. The path begins at node 0 and goes on to the first child that is the
+    token after its last node, for at most ``max_path`` nodes (the tree's depth + 1 is enough). ``tokens`` are those after the path's nodes: the sequence
+    goes on with ``tokens[b, : counts[b]]``, which are distributed as the target's own.
+
+    With ``pool`` (float32, float16 or bfloat16), ``block_tables`` and ``q_start`` the path's keys and values move together: those of
+    position ``q_start[b] + path[b, j]`` to ``q_start[b] + j``, in all layers, in the same launch. The cache then holds the sequence's first
+    ``q_start[b] + counts[b]`` positions."""
+    if counts is None:
+        counts = torch.empty(cu_seqlens_q.numel() - 1, dtype=torch.int32, device=sampled.device)
+    if tokens is None:
+        tokens = torch.empty(counts.numel(), max_path, dtype=torch.int64, device=sampled.device)
+    if path is None:
+        path = torch.empty(counts.numel(), max_path, dtype=torch.int32, device=sampled.device)
+    if tokens.dim() != 2 or tokens.size(1) != max_path:
+        raise ValueError(f"tokens must be [{counts.numel()}, {max_path}]")
+    _checked_op("accept_tree", tokens, path, counts, sampled, draft_tokens, parents, cu_seqlens_q, pool, block_tables, q_start,
+                d_error)  # fmt: skip
+    return tokens, path, counts
+
+
+def copy_blocks(pool: torch.Tensor, src_blocks: torch.Tensor, dst_blocks: torch.Tensor, num_slots: torch.Tensor | None = None,
+                d_error: torch.Tensor | None = None) -> None:
+    """Copies the first ``num_slots[p]`` slots (default: all) of block ``src_blocks[p]`` of ``pool`` (float32, float16 or bfloat16) to block
+    ``dst_blocks[p]``, all layers, keys and values, for every pair p (int32 ``[P]``; a negative id: no copy). The copies run beside each other:
+    a pair that writes to a block which another reads, or which an earlier one writes to, is flagged and left out."""
+    _checked_op("copy_blocks", pool, src_blocks, dst_blocks, num_slots, d_error)
+
+
 # ------------------------------------------------------------------------------ library GEMMs
 # hipBLASLt's default fp32 kernel for a given shape depends on the operand layout. Measured on the
 # device (a spin kernel holding the stream while ten calls per layout queue behind it, best of three

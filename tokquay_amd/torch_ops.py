@@ -6,7 +6,7 @@ HIP stream. This module loads that library and registers the operators' fake (sh
 implementations, so programs that record torch calls (``make_fx``, FX graphs on fake tensors)
 see the kernels as single operators. Both the operators and their fakes refuse, before any launch,
 every tensor a kernel would read or write past: wrong device, dtype or inner layout, too few rows
-or entries, overlapping rows; the last three also refuse every number out of its range:
+or entries, overlapping rows; the last eight also refuse every number out of its range:
 
 * ``cache_write(pool!, layer, k, v, slot_mapping, d_error!?)``
 * ``paged_decode(out!, q, pool, layer, block_tables, context_lens, max_context_len, scale,
@@ -27,6 +27,13 @@ or entries, overlapping rows; the last three also refuse every number out of its
   scale, workspace!?, d_error!?)``
 * ``verify_drafts(tokens!, accepted!, logits, draft_probs?, draft_tokens, uniforms, temperature,
   cu_seqlens_q, d_error!?)``
+* ``tree_layout(positions!, masks!, parents, cu_seqlens_q, q_start, max_query_len, d_error!?)``
+* ``paged_tree(out!, q, pool, layer, block_tables, cu_seqlens_q, q_start, masks, max_query_len, max_context_len,
+  scale, workspace!?, d_error!?)``
+* ``sample_tokens(tokens!, logits, uniforms, temperature, top_k?, top_p?, min_p?, cu_seqlens_q?, d_error!?)``
+* ``accept_tree(tokens!, path!, counts!, sampled, draft_tokens, parents, cu_seqlens_q, pool!?, block_tables?,
+  q_start?, d_error!?)``
+* ``copy_blocks(pool!, src_blocks, dst_blocks, num_slots?, d_error!?)``
 
 (``!``: written in place.) ``tokquay_amd.ops`` checks the tensors with the reference's messages
 and calls these operators; there is no fallback when the library is missing.
@@ -42,7 +49,8 @@ from tokquay_amd import _lib
 from tokquay_amd.build import TORCH_OPS_PATH
 
 OPS = ("cache_write", "paged_decode", "paged_decode_write", "paged_prefill", "paged_mixed", "paged_gather",
-       "argmax_rows", "linear", "rope_cache_write", "paged_chunk", "verify_drafts")
+       "argmax_rows", "linear", "rope_cache_write", "paged_chunk", "verify_drafts", "tree_layout", "paged_tree",
+       "sample_tokens", "accept_tree", "copy_blocks")
 
 _loaded = False
 
@@ -327,9 +335,26 @@ def _fake_rope_cache_write(q_out, q, k, v, pool, layer, slot_mapping, positions,
     _error_word(op, d_error, pool)
 
 
+def _masks_of(op, t, rows, max_query_len, device):
+    if not (t.device == device and t.dtype == torch.int64 and t.dim() == 2 and t.size(0) == rows and t.is_contiguous()
+            and t.size(1) <= 0x3FFFFFFF and t.size(1) >= (max_query_len + 63) // 64):  # fmt: skip
+        _fail(op, f"masks must be a contiguous int64 [{rows}, words] tensor of at least {max_query_len} bits a row on {device}")
+
+
 def _fake_paged_chunk(out, q, pool, layer, block_tables, cu_seqlens_q, q_start, max_query_len, max_context_len, scale,
                       workspace, d_error):  # fmt: skip
-    op = "paged_chunk"
+    _attend("paged_chunk", out, q, pool, layer, block_tables, cu_seqlens_q, q_start, None, max_query_len, max_context_len,
+            scale, workspace, d_error)  # fmt: skip
+
+
+def _fake_paged_tree(out, q, pool, layer, block_tables, cu_seqlens_q, q_start, masks, max_query_len, max_context_len, scale,
+                     workspace, d_error):  # fmt: skip
+    _attend("paged_tree", out, q, pool, layer, block_tables, cu_seqlens_q, q_start, masks, max_query_len, max_context_len,
+            scale, workspace, d_error)  # fmt: skip
+
+
+def _attend(op, out, q, pool, layer, block_tables, cu_seqlens_q, q_start, masks, max_query_len, max_context_len, scale,
+            workspace, d_error):  # fmt: skip
     _typed_pool_of(op, pool, layer, False)
     _vector_of(op, "q_start", q_start, torch.int32, 0, pool)
     n = q_start.numel()
@@ -359,6 +384,8 @@ def _fake_paged_chunk(out, q, pool, layer, block_tables, cu_seqlens_q, q_start, 
             _fail(op, "max_context_len and block_tables must have room for the sequences")
         if pool.numel() // pool.size(0) >= 2**31:
             _fail(op, "a block of the pool has too many elements")
+    if masks is not None:
+        _masks_of(op, masks, rows, max_query_len, q.device)
     _error_word(op, d_error, pool)
     _workspace(op, workspace, pool)
     if workspace is not None:
@@ -366,7 +393,7 @@ def _fake_paged_chunk(out, q, pool, layer, block_tables, cu_seqlens_q, q_start, 
         need = _lib.lib().tq_paged_chunk_workspace_size(*map(int, sizes))  # (sizes of a dynamic trace become numbers)
         size = workspace.element_size()
         if need > 0 and (workspace.numel() * size < need or workspace.storage_offset() * size % 16):
-            raise RuntimeError(f"tq_paged_chunk failed: {_lib.STATUS_NAMES[3]}")
+            raise RuntimeError(f"tq_{op} failed: {_lib.STATUS_NAMES[3]}")
 
 
 def _fake_verify_drafts(tokens, accepted, logits, draft_probs, draft_tokens, uniforms, temperature, cu_seqlens_q,
@@ -404,6 +431,98 @@ def _fake_verify_drafts(tokens, accepted, logits, draft_probs, draft_tokens, uni
         if draft_probs.device != logits.device or draft_probs.dtype != torch.float32:
             _fail(op, "draft_probs must be a float32 tensor on the logits' device")
         vocab_rows("draft_probs", draft_probs)
+
+
+def _exactly(op, name, t, dtype, entries, device):
+    if not (t.device == device and t.dtype == dtype and t.dim() == 1 and t.is_contiguous()
+            and (entries < 0 or t.numel() == entries) and t.numel() < 2**31):  # fmt: skip
+        _fail(op, f"{name} must be a contiguous {dtype} [{'N' if entries < 0 else entries}] tensor on {device}")
+
+
+def _slots_of(op, pool):
+    if pool.storage_offset() * pool.element_size() % 16:
+        _fail(op, "pool must be 16-byte aligned")
+    if pool.numel() // (pool.size(0) * pool.size(4)) > 1 << 30:
+        _fail(op, "a slot of the pool has too many elements")
+
+
+def _fake_tree_layout(positions, masks, parents, cu_seqlens_q, q_start, max_query_len, d_error):
+    op, device = "tree_layout", parents.device
+    if not parents.is_cuda:
+        _fail(op, "parents must be on a HIP device")
+    _exactly(op, "parents", parents, torch.int32, -1, device)
+    _exactly(op, "q_start", q_start, torch.int32, -1, device)
+    rows, n = parents.numel(), q_start.numel()
+    _exactly(op, "cu_seqlens_q", cu_seqlens_q, torch.int32, n + 1, device)
+    _exactly(op, "positions", positions, torch.int64, rows, device)
+    if not 0 <= max_query_len < 2**31:
+        _fail(op, "max_query_len must be a length")
+    _masks_of(op, masks, rows, max_query_len, device)
+    if d_error is not None:
+        _exactly(op, "d_error", d_error, torch.int32, 1, device)
+
+
+def _fake_sample_tokens(tokens, logits, uniforms, temperature, top_k, top_p, min_p, cu_seqlens_q, d_error):
+    op, device = "sample_tokens", logits.device
+    if not (logits.is_cuda and logits.dim() == 2 and logits.dtype in _TYPES):
+        _fail(op, "logits must be a float32, float16 or bfloat16 [rows, vocab] tensor on a HIP device")
+    rows, vocab = logits.shape
+    if not (rows < 2**31 and 1 <= vocab <= 1 << 21):
+        _fail(op, "logits must have 1 to 2097152 columns")
+    if vocab > 1 and logits.stride(1) != 1:
+        _fail(op, f"logits must be [{rows}, {vocab}] with contiguous rows")
+    if rows > 1 and logits.stride(0) < vocab:
+        _fail(op, "logits's rows overlap")
+    _exactly(op, "temperature", temperature, torch.float32, rows if cu_seqlens_q is None else -1, device)
+    n = temperature.numel()
+    for name, t, dtype, entries in (("cu_seqlens_q", cu_seqlens_q, torch.int32, n + 1), ("top_k", top_k, torch.int32, n),
+                                    ("top_p", top_p, torch.float32, n), ("min_p", min_p, torch.float32, n),
+                                    ("uniforms", uniforms, torch.float32, rows), ("tokens", tokens, torch.int64, rows),
+                                    ("d_error", d_error, torch.int32, 1)):  # fmt: skip
+        if t is not None:
+            _exactly(op, name, t, dtype, entries, device)
+
+
+def _fake_accept_tree(tokens, path, counts, sampled, draft_tokens, parents, cu_seqlens_q, pool, block_tables, q_start, d_error):
+    op, device = "accept_tree", sampled.device
+    if not sampled.is_cuda:
+        _fail(op, "sampled must be on a HIP device")
+    _exactly(op, "sampled", sampled, torch.int64, -1, device)
+    _exactly(op, "counts", counts, torch.int32, -1, device)
+    rows, n = sampled.numel(), counts.numel()
+    _exactly(op, "draft_tokens", draft_tokens, torch.int64, rows, device)
+    _exactly(op, "parents", parents, torch.int32, rows, device)
+    _exactly(op, "cu_seqlens_q", cu_seqlens_q, torch.int32, n + 1, device)
+    for name, t, dtype, columns in (("tokens", tokens, torch.int64, -1), ("path", path, torch.int32, tokens.size(-1))):
+        if not (t.device == device and t.dtype == dtype and t.dim() == 2 and t.size(0) == n and 1 <= t.size(1) < 2**31
+                and (columns < 0 or t.size(1) == columns) and t.is_contiguous()):  # fmt: skip
+            _fail(op, f"{name} must be a contiguous {dtype} [{n}, max_path] tensor on {device}")
+    if d_error is not None:
+        _exactly(op, "d_error", d_error, torch.int32, 1, device)
+    if not (pool is None) == (block_tables is None) == (q_start is None):
+        _fail(op, "pool, block_tables and q_start go together")
+    if pool is not None:
+        _typed_pool_of(op, pool, 0, True)
+        if pool.device != device:
+            _fail(op, f"pool is on {pool.device}, sampled on {device}")
+        _slots_of(op, pool)
+        _tables_of(op, "block_tables", block_tables, n, pool)
+        if block_tables.size(1) >= 2**31:
+            _fail(op, "block_tables has too many columns")
+        _exactly(op, "q_start", q_start, torch.int32, n, device)
+
+
+def _fake_copy_blocks(pool, src_blocks, dst_blocks, num_slots, d_error):
+    op = "copy_blocks"
+    _typed_pool_of(op, pool, 0, True)
+    _slots_of(op, pool)
+    _exactly(op, "src_blocks", src_blocks, torch.int32, -1, pool.device)
+    n = src_blocks.numel()
+    _exactly(op, "dst_blocks", dst_blocks, torch.int32, n, pool.device)
+    if num_slots is not None:
+        _exactly(op, "num_slots", num_slots, torch.int32, n, pool.device)
+    if d_error is not None:
+        _exactly(op, "d_error", d_error, torch.int32, 1, pool.device)
 
 
 FAKES = {name: globals()[f"_fake_{name}"] for name in OPS}
