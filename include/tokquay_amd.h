@@ -649,12 +649,17 @@ tq_status tq_paged_tree(void* out, int64_t out_row_stride, const void* q, int64_
  * below 4,097 columns), the largest weight being 1, and so the same for every order. A token may differ from the exact rule's only where
  * a uniform number, or p times the sum, meets a border that closely.
  *
- * No counterpart in the reference's kernels; it stands beside Engine._sample (tokquay/engine.py:83-92, :189-194).
+ * Needs tq_sample_tokens_workspace_size(...) bytes of workspace (16-byte aligned, any contents; calls that may run at the
+ * same time need one each). No counterpart in the reference's kernels; it stands beside Engine._sample
+ * (tokquay/engine.py:83-92, :189-194).
  */
 tq_status tq_sample_tokens(int64_t* tokens, const void* logits, int64_t logits_row_stride, const float* uniforms,
                            const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                            const int32_t* cu_seqlens_q, int32_t num_seqs, int32_t num_rows, int32_t vocab,
-                           int32_t dtype, int32_t* d_error, void* stream);
+                           int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* d_error, void* stream);
+
+/* Bytes of workspace tq_sample_tokens needs for these sizes. */
+size_t tq_sample_tokens_workspace_size(int32_t num_rows, int32_t vocab);
 
 /*
  * The path of each tree that the sampled tokens take. parents and cu_seqlens_q are tq_tree_layout's, sampled[row] is the token that

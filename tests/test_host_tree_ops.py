@@ -241,14 +241,15 @@ def test_copy_blocks_c_refusals(status, more):
     assert copy_call(**more) == status
 
 
-def sample_call(tokens=P, logits=P, ls=90, u=P, t=P, k=P, p=P, m=P, cu=None, seqs=5, rows=5, vocab=90, dtype=0):
-    return _lib.lib().tq_sample_tokens(tokens, logits, ls, u, t, k, p, m, cu, seqs, rows, vocab, dtype, None, None)
+def sample_call(tokens=P, logits=P, ls=90, u=P, t=P, k=P, p=P, m=P, cu=None, seqs=5, rows=5, vocab=90, dtype=0, ws=P, wb=1 << 20):
+    return _lib.lib().tq_sample_tokens(tokens, logits, ls, u, t, k, p, m, cu, seqs, rows, vocab, dtype, ws, wb, None, None)
 
 
 @pytest.mark.parametrize("status,more", [
     (INVALID, dict(seqs=-1)), (INVALID, dict(rows=-1)), (INVALID, dict(vocab=0)), (UNSUPPORTED, dict(vocab=(1 << 21) + 1)),
     (UNSUPPORTED, dict(dtype=3)), (OK, dict(rows=0)), (INVALID, dict(tokens=None)), (INVALID, dict(logits=None)),
     (INVALID, dict(u=None)), (INVALID, dict(t=None)), (INVALID, dict(seqs=4)), (INVALID, dict(ls=89)), (OK, dict(seqs=0, cu=P)),
+    (WORKSPACE, dict(ws=None)), (WORKSPACE, dict(wb=8)), (WORKSPACE, dict(ws=P + 8)),
 ])  # fmt: skip
 def test_sample_tokens_c_refusals(status, more):
     assert sample_call(**more) == status

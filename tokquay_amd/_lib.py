@@ -249,9 +249,10 @@ SIGNATURES: dict[str, tuple] = {
             c_i64p, ctypes.c_void_p, ctypes.c_int64, c_f32p, c_f32p,  # tokens, logits, logits_row_stride, uniforms, temperature
             c_i32p, c_f32p, c_f32p, c_i32p,  # top_k, top_p, min_p, cu_seqlens_q
             ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,  # num_seqs, num_rows, vocab, dtype
-            c_i32p, ctypes.c_void_p,  # d_error, stream
+            ctypes.c_void_p, ctypes.c_size_t, c_i32p, ctypes.c_void_p,  # workspace, workspace_bytes, d_error, stream
         ],
     ),
+    "tq_sample_tokens_workspace_size": (ctypes.c_size_t, [ctypes.c_int32] * 2),
     "tq_accept_tree": (
         ctypes.c_int,
         [

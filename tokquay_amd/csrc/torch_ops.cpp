@@ -602,10 +602,14 @@ void sample_tokens(at::Tensor tokens, const at::Tensor& logits, const at::Tensor
   exactly(op, "uniforms", uniforms, at::kFloat, rows, device);
   exactly(op, "tokens", tokens, at::kLong, rows, device);
   if (d_error.has_value()) exactly(op, "d_error", *d_error, at::kInt, 1, device);
+  const size_t need = tq_sample_tokens_workspace_size((int32_t)rows, (int32_t)vocab);
+  at::Tensor workspace;
+  if (need > 0) workspace = at::empty({(int64_t)need}, logits.options().dtype(at::kByte));
   check(tq_sample_tokens(tokens.data_ptr<int64_t>(), logits.data_ptr(), ls, uniforms.data_ptr<float>(),
                          temperature.data_ptr<float>(), ptr<int32_t>(top_k), ptr<float>(top_p), ptr<float>(min_p),
                          ptr<int32_t>(cu_seqlens_q), (int32_t)n, (int32_t)rows, (int32_t)vocab,
-                         dtype_of(logits.scalar_type()), ptr<int32_t>(d_error), stream_of(logits)),
+                         dtype_of(logits.scalar_type()), need > 0 ? workspace.data_ptr() : nullptr, need,
+                         ptr<int32_t>(d_error), stream_of(logits)),
         "tq_sample_tokens");
 }
 

@@ -28,12 +28,6 @@ namespace tq {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
-
-struct Stat {  // of one row's chunk
-  double sum;      // of exp((logit - max) / T); 0 at T = 0
-  uint64_t key;    // argmax_key of its largest logit (the column: where T = 0 or the maximum is not finite)
-};
 
 struct VerifyArgs {
   int64_t* tokens;
@@ -64,70 +58,17 @@ __device__ __forceinline__ const void* row_of(const VerifyArgs& a, int64_t row) 
   return static_cast<const char*>(a.logits) + row * a.logits_stride * (__is_same(T, float) ? 4 : 2);
 }
 
-// The sequence that a row belongs to: the last one with cu[b] <= row (empty sequences hold no row), among 64 parts at a time.
-// Its temperature, asked for before the logits, arrives before them. (Counted through all 1,024 sequences of 5 rows, 50,257 bf16
-// logits each, the call took 328 us instead of 259.) Where cu falls somewhere this may be another one, still below num_seqs; every
-// count grows with the row, so if it is b for two rows it is for those between them.
-__device__ __forceinline__ int64_t owner_of(const VerifyArgs& a, int row) {
-  const int lane = threadIdx.x & (kWave - 1);
-  int64_t b = 0, n = a.num_seqs;
-  while (n > 1) {
-    const int64_t step = (n + kWave - 1) / kWave, at = b + lane * step;
-    const int k = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane * step < n && a.cu[at] <= row));
-    const int64_t skip = max(k - 1, 0) * step;
-    b += skip;
-    n = min(step, n - skip);
-  }
-  return b;
-}
-
 template <typename T, int PER>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(const VerifyArgs a) {
-  __shared__ float s_top[kWaves];
-  __shared__ double s_sum[kWaves];
-  __shared__ int s_col;
+  __shared__ StatShared<kThreads> sh;
   const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks;
   if (row < a.num_seqs && chunk == 0 && threadIdx.x == 0) a.arrived[row] = 0;  // for the second launch
   if (row >= a.num_rows) return;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int base = chunk * kThreads * PER, n = min(kThreads * PER, a.vocab - base);
-  float x[PER], top = -INFINITY;
-  const float temp = a.temperature[owner_of(a, row)];
+  float x[PER];
+  const float temp = a.temperature[owner_of(a.cu, a.num_seqs, row)];
   columns<T, kVec<T>, kThreads, PER, false>(row_of<T>(a, row), base, n, x);
-#pragma unroll
-  for (int i = 0; i < PER; ++i) top = __builtin_elementwise_maximum(top, x[i]);  // NaN, if any is
-  top = wave_maximum(top);
-  if (lane == 0) s_top[wave] = top;
-  if (threadIdx.x == 0) s_col = 0x7fffffff;
-  __syncthreads();
-#pragma unroll
-  for (int v = 0; v < kWaves; ++v) top = __builtin_elementwise_maximum(top, s_top[v]);
-  double sum = 0.0;
-  int col = 0;
-  if (temp > 0.f && top > -INFINITY && top < INFINITY) {  // uniform
-    const double c = kLog2e / (double)temp, t0 = (double)top;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) sum += exp2_neg(((double)x[i] - t0) * c);
-    sum = wave_sum(sum);
-    if (lane == 0) s_sum[wave] = sum;
-  } else {  // no distribution, or none needed: the first column that holds the maximum
-    int mine = 0x7fffffff;
-#pragma unroll
-    for (int i = PER - 1; i >= 0; --i) {
-      const int at = column_of<kVec<T>, kThreads, PER, false>(i);
-      if (at < n && (top != top ? x[i] != x[i] : x[i] == top)) mine = at;
-    }
-    atomicMin(&s_col, mine);
-    if (lane == 0) s_sum[wave] = 0.0;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    sum = s_sum[0];
-#pragma unroll
-    for (int v = 1; v < kWaves; ++v) sum += s_sum[v];
-    if (s_col != 0x7fffffff) col = s_col;
-    a.stats[(int64_t)row * a.chunks + chunk] = Stat{sum, argmax_key(top, base + col)};
-  }
+  chunk_stat<T>(x, temp, true, base, n, a.stats + (int64_t)row * a.chunks + chunk, sh);
 }
 
 // A row's distribution: 2^((logit - top) c) / sum, or all of it on column best.
@@ -228,7 +169,7 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, int b, bool lead
   __syncthreads();
   // Rows that another sequence claims too may have statistics of its temperature. The last wave has the fewest rows.
   if (wave == N / kWave - 1) {
-    const bool refused = !fits || owner_of(a, lo) != b || owner_of(a, lo + drafts) != b;
+    const bool refused = !fits || owner_of(a.cu, a.num_seqs, lo) != b || owner_of(a.cu, a.num_seqs, lo + drafts) != b;
     if (lane == 0) sh.refused = refused;
   }
   // A wave a row, after a lane a row has fetched what it needs of 64 rows. (Rows behind one that does not stand are left out.)
