@@ -27,9 +27,12 @@ constexpr int kPick = 1024;         // threads of a row's workgroup
 constexpr int kPickWaves = kPick / kWave;
 constexpr int kBins = 2 * kPick;
 constexpr int kListed = 8192;       // columns that are kept in LDS; rows of which more matter are read again
+constexpr int kRanked = 1024;       // of them, those that are ranked by comparing each with each; at most kPick
 constexpr int kSelected = 4096;     // groups whose columns are listed; if more reach the limit, all are looked at
 constexpr int kMaxVocab = 1 << 21;
-constexpr int kMaxRounds = kMaxVocab / (4 * kPick);
+constexpr int kRound = 4 * kPick;
+constexpr int kMaxRounds = kMaxVocab / kRound;
+static_assert(kMaxRounds <= kPick && kRanked <= kPick && kMaxVocab / kGroup <= 1 << 16, "an entry a thread, groups in 16 bits");
 
 struct SampleArgs {
   int64_t* tokens;
@@ -123,27 +126,25 @@ __global__ __launch_bounds__(kThreads) void sample_stats_kernel(const SampleArgs
 struct PickShared {
   uint32_t n[kBins];
   uint64_t m[kBins];
-  uint64_t part[kPickWaves], part_m[kPickWaves];
+  uint64_t part[kPickWaves];
   double sum[kPickWaves], goal;
   double round[kMaxRounds];
-  uint32_t distance[kListed], column[kListed];  // the columns that matter
-  uint16_t group[kSelected];                    // the groups that they lie in
+  alignas(16) uint32_t distance[kListed + 4], column[kListed];  // the columns that matter
+  uint16_t group[kSelected];                                    // the groups that they lie in
   uint64_t before_n, before_m, bin_n;
   uint32_t member;
   int found, pick[kPickWaves][2], last;
 };
 
-// Where the count of columns, or their weight, first reaches a goal: at distance lo .. hi, with n columns of weight m before.
-struct Cut {
-  uint32_t lo, hi;
-  uint64_t n, m, ties;  // ties: columns in the interval
-  bool found;
-};
+// What is gone through, four items in a row a thread, a round of all threads at a time: the maxima of the groups, the columns of the
+// selected groups, those of the row (or of one chunk), those listed in LDS.
+enum Source { kMaxima, kGroups, kColumns, kList };
 
+// One code for all steps and sources, none of it unrolled over rounds: a row's workgroup runs most of it once, and is held up by the
+// fetching of instructions (unrolled over several rounds it took twice as long).
 template <typename T>
 __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) {
   __shared__ PickShared sh;
-  constexpr int V = kVec<T>, L = kTeam<T>, kRound = kPick * V;
   // Keys of different values of the type are at least this far apart.
   constexpr uint32_t kApart = __is_same(T, float) ? 1u : __is_same(T, Bf16) ? 1u << 16 : 1u << 13;
   constexpr uint32_t kNone = 0xffffffffu;  // no column's distance
@@ -151,7 +152,9 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
   const Settings s = settings_of(a, row);
   if (s.none) return;
   const char* at = row_of<T>(a, row);
+  const float* maxima = a.maxima + (int64_t)row * a.groups;
   const Stat* st = a.stats + (int64_t)row * a.chunks;
+  const double u = (double)a.uniforms[row];
 
   // The row's largest logit, each wave by itself.
   uint64_t best = 0;
@@ -176,142 +179,49 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
   auto fixed = [&](double w) {  // w below 2^(52 - mass_bits)
     return __builtin_bit_cast(uint64_t, __builtin_fma(w, unit, 0x1p52)) & 0xfffffffffffffull;
   };
-  const double u = (double)a.uniforms[row];
 
-  // The columns at hand: those from `first` to `end`, or the list's, V in a row a thread, a round at a time.
-  int first = 0, end = a.vocab, listed = -1, rounds = (a.vocab + kRound - 1) / kRound;
-  uint32_t limit = kNone - 1;  // no column past this distance is among the first ranks
-  uint32_t d[V];
-  auto load = [&](int r) {
-    const int i0 = r * kRound + tid * V;
-    if (listed >= 0) {
+  Source source = kColumns;
+  int first = 0, items = a.vocab;  // of the source; columns from `first` on
+  auto column = [&](Source from, int i) {
+    return from == kList ? (int)sh.column[i] : from == kGroups ? sh.group[i / kGroup] * kGroup + i % kGroup : first + i;
+  };
+  // The distances of items i .. i + 3 of `many`.
+  auto fetch = [&](Source from, int i, int many, uint32_t (&d)[4]) {
+    if (from == kList) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(&sh.distance[min(i, kListed)]);
 #pragma unroll
-      for (int e = 0; e < V; ++e) d[e] = i0 + e < listed ? sh.distance[i0 + e] : kNone;
+      for (int e = 0; e < 4; ++e) d[e] = i + e < many ? v[e] : kNone;
+      return;
+    }
+    float x[4];
+    const bool wide = __is_same(T, float) || from == kMaxima;
+    int j = i, end = many;  // places in the array
+    if (from == kGroups) {
+      j = column(kGroups, min(i, many - 1));
+      end = i < many ? a.vocab : j;
+    } else if (from == kColumns) {
+      j += first;
+      end += first;
+    }
+    const char* p = from == kMaxima ? reinterpret_cast<const char*>(maxima) : at;
+    if (j + 4 <= end) {
+      if (wide) {
+        u32x4 v;
+        __builtin_memcpy(&v, p + 4 * (int64_t)j, 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(v[e]);
+      } else if constexpr (!__is_same(T, float)) {
+        u32x2 v;
+        __builtin_memcpy(&v, p + 2 * (int64_t)j, 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = T::load((uint16_t)(v[e / 2] >> (16 * (e & 1))));
+      }
     } else {
-      float x[V];
-      columns<T, V, kPick, V, true>(at, first + r * kRound, end - first - r * kRound, x);
 #pragma unroll
-      for (int e = 0; e < V; ++e) d[e] = first + i0 + e < end ? distance_of(x[e]) : kNone;
+      for (int e = 0; e < 4; ++e) x[e] = j + e < end ? wide ? reinterpret_cast<const float*>(p)[j + e] : logit_at<T>(p, j + e) : 0.f;
     }
-  };
-  auto column = [&](int r, int e) {
-    const int i = r * kRound + tid * V + e;
-    return listed >= 0 ? (int)sh.column[min(i, kListed - 1)] : first + i;
-  };
-  auto each_column = [&](auto&& use) {
-    for (int r = 0; r < rounds; ++r) {
-      load(r);
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (d[e] <= limit) use(d[e]);
-    }
-  };
-  const float* maxima = a.maxima + (int64_t)row * a.groups;
-  auto each_maximum = [&](auto&& use) {
-    for (int i = tid; i < a.groups; i += kPick) use(distance_of(maxima[i]));
-  };
-  // Lists the columns within the limit, in order, if there is room; those of the `many` selected groups, or (-1) of all.
-  auto list = [&](int many) {
-    const int groups = many >= 0 ? many : a.groups;
-    int count = 0;
-    for (int g0 = 0; g0 < groups && count <= kListed; g0 += kPick / L) {
-      const int slot = g0 + tid / L;
-      const int col = (slot < groups ? many >= 0 ? (int)sh.group[slot] : slot : 0) * kGroup + tid % L * V;
-      float x[V];
-      uint32_t near[V];
-      columns<T, V, kPick, V, true>(at, col - tid * V, slot < groups ? a.vocab - col + tid * V : 0, x);
-      int mine = 0;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        near[e] = slot < groups && col + e < a.vocab ? distance_of(x[e]) : kNone;
-        mine += near[e] <= limit;
-      }
-      const int upto = (int)scan<kPick>((uint64_t)mine, sh.part);
-      int place = count + upto - mine;
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (near[e] <= limit) {
-          if (place < kListed) {
-            sh.distance[place] = near[e];
-            sh.column[place] = col + e;
-          }
-          ++place;
-        }
-      if (tid == kPick - 1) sh.found = upto;
-      __syncthreads();
-      count += sh.found;
-      __syncthreads();
-    }
-    if (count <= kListed) {
-      listed = count;
-      rounds = (count + kRound - 1) / kRound;
-    }
-  };
-
-  // `apart`: the interval is narrowed down until its columns have one value; 0: as it was found.
-  auto find = [&](auto&& each, bool weigh, bool by_mass, double goal, uint32_t apart) {
-    Cut r = {0, 0, 0, 0, 0, false};
-    int shift = 14;
-    for (;;) {
-      for (int i = tid; i < kBins; i += kPick) {
-        sh.n[i] = 0;
-        sh.m[i] = 0;
-      }
-      if (tid == 0) sh.found = -1;
-      __syncthreads();
-      each([&](uint32_t v) {
-        const uint32_t b = (v - r.lo) >> shift;
-        if (v >= r.lo && b < kBins) {
-          atomicAdd(&sh.n[b], 1u);
-          if (weigh) atomicAdd((unsigned long long*)&sh.m[b], (unsigned long long)fixed(weight(v)));
-        }
-      });
-      __syncthreads();
-      const uint64_t na = sh.n[2 * tid], nb = sh.n[2 * tid + 1], ma = sh.m[2 * tid], mb = sh.m[2 * tid + 1];
-      const uint64_t n = r.n + scan<kPick>(na + nb, sh.part), m = weigh ? r.m + scan<kPick>(ma + mb, sh.part_m) : 0;
-      auto reaches = [&](uint64_t n, uint64_t m) { return by_mass ? (double)m >= goal : (double)n >= goal; };
-      const uint64_t n1 = n - na - nb, m1 = m - ma - mb;  // before this thread's
-      if (reaches(n, m) && (tid == 0 || !reaches(n1, m1))) {
-        const bool one = reaches(n1 + na, m1 + ma);
-        sh.found = 2 * tid + (one ? 0 : 1);
-        sh.before_n = one ? n1 : n1 + na;
-        sh.before_m = one ? m1 : m1 + ma;
-        sh.bin_n = one ? na : nb;
-      } else if (tid == kPick - 1 && !reaches(n, m)) {
-        sh.before_n = n;
-        sh.before_m = m;
-      }
-      __syncthreads();
-      const int found = sh.found;
-      r.n = sh.before_n;
-      r.m = sh.before_m;
-      if (found < 0) {
-        if (shift == 21) return r;
-        r.lo += (uint32_t)kBins << shift;
-        shift = 21;
-        __syncthreads();
-        continue;
-      }
-      r.found = true;
-      r.ties = sh.bin_n;
-      r.lo += (uint32_t)found << shift;
-      r.hi = r.lo + ((1u << shift) - 1);
-      __syncthreads();
-      if (apart == 0) return r;
-      if (listed < 0 && r.n + r.ties <= kListed) {
-        limit = r.hi;
-        list(-1);
-      }
-      if (r.ties == 1 || (1u << shift) <= apart) {
-        each([&](uint32_t v) {
-          if (v >= r.lo && v <= r.hi) sh.member = v;
-        });
-        __syncthreads();
-        r.lo = r.hi = sh.member;
-        return r;
-      }
-      shift = shift == 14 ? 3 : shift == 21 ? 10 : 0;
-    }
+    for (int e = 0; e < 4; ++e) d[e] = j + e < end ? distance_of(x[e]) : kNone;
   };
 
   // The sum of the row's weights, and for draws from all of them the chunk that the token falls in.
@@ -333,83 +243,230 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
       __syncthreads();
       rest = sh.goal;
       first = chosen * a.chunk_columns;
-      end = min(first + a.chunk_columns, a.vocab);
-      rounds = (end - first + kRound - 1) / kRound;
+      items = min(a.chunk_columns, a.vocab - first);
     }
   }
 
-  // A limit from the groups' maxima, and the groups that reach it.
-  if (!s.all()) {
-    if (s.k > 0) {
-      if (s.k <= a.groups) {
-        const Cut cut = find(each_maximum, false, false, (double)s.k, 0);
-        if (cut.found) limit = cut.hi;
-      }
-    } else if (s.nucleus()) {
-      const Cut cut = find(each_maximum, true, true, (s.p > 0.f ? (double)s.p : 0.0) * (total * unit), 0);
-      if (cut.found) limit = cut.hi;
-    } else {
+  // 0: a limit from the maxima, past which no column is among the first ranks, and a list of those up to it. 1: top-k, 2: top-p: columns with
+  // distance below `cut`, and the first `ties` of those at it.
+  uint32_t limit = kNone - 1, cut = kNone - 1;
+  uint64_t ties = 0, cut_m = 0;
+  bool some = false;  // whether `ties` is less than there are
+  double whole = total * unit;
+#pragma unroll 1
+  for (int job = s.all() ? 3 : 0; job < 3; ++job) {
+    bool run = job == 0 ? s.k > 0 ? s.k <= a.groups : s.nucleus() : job == 1 ? s.k > 0 : s.nucleus();
+    const bool by_mass = job == 0 ? s.k == 0 : job == 2, weigh = by_mass || (job == 1 && s.nucleus());
+    if (job == 2 && s.k > 0) whole = (double)(cut_m + ties * fixed(weight(cut)));
+    const double goal = by_mass ? (s.p > 0.f ? (double)s.p : 0.0) * whole : (double)s.k;
+    int make = -1;  // the source to be listed
+    if (job == 0 && !run && s.k == 0) {
       // Where the weight is `least`, and a little further: the columns are weighed again.
       const double edge = t0 + ((double)__builtin_amdgcn_logf(s.least) - 1e-4) / c;
       const float low = (float)(edge - 1e-6 * __builtin_fabs(edge));
-      if (low > -INFINITY) limit = distance_of(low);
-    }
-    if (limit < kNone - 1) {
-      int many = 0;
-      for (int i0 = 0; i0 < a.groups; i0 += kPick) {
-        const bool in = i0 + tid < a.groups && distance_of(maxima[i0 + tid]) <= limit;
-        const uint64_t those = __builtin_amdgcn_ballot_w64(in);
-        if (lane == 0) sh.pick[wave][0] = __builtin_popcountll(those);
-        __syncthreads();
-        int place = many + __builtin_popcountll(those & ((1ull << lane) - 1));
-        for (int v = 0; v < kPickWaves; ++v) {
-          place += v < wave ? sh.pick[v][0] : 0;
-          many += sh.pick[v][0];
-        }
-        if (in && place < kSelected) sh.group[place] = (uint16_t)(i0 + tid);
-        __syncthreads();
+      if (low > -INFINITY) {
+        limit = distance_of(low);
+        make = kMaxima;
       }
-      list(many <= kSelected ? many : -1);
+    }
+    uint32_t lo = 0;
+    uint64_t n0 = 0, m0 = 0;  // before lo
+    int shift = 14;
+#pragma unroll 1
+    while (run || make >= 0) {
+      if (make >= 0) {
+        // Items up to the limit, in order.
+        const Source from = (Source)make;
+        const int many = from == kMaxima ? a.groups : from == kGroups ? items * kGroup : a.vocab;
+        int count = 0;
+#pragma unroll 1
+        for (int i0 = 0; i0 < many && count <= kListed; i0 += kRound) {
+          const int i = i0 + 4 * tid;
+          uint32_t d[4];
+          fetch(from, i, many, d);
+          int mine = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mine += d[e] <= limit;
+          const int upto = (int)scan<kPick>((uint64_t)mine, sh.part);
+          int place = count + upto - mine;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d[e] <= limit) {
+              if (from == kMaxima) {
+                if (place < kSelected) sh.group[place] = (uint16_t)(i + e);
+              } else if (place < kListed) {
+                sh.distance[place] = d[e];
+                sh.column[place] = column(from, i + e);
+              }
+              ++place;
+            }
+          if (tid == kPick - 1) sh.found = upto;
+          __syncthreads();
+          count += sh.found;
+          __syncthreads();
+        }
+        if (from == kMaxima) {
+          make = count <= kSelected ? kGroups : kColumns;
+          items = count <= kSelected ? count : items;
+        } else {
+          make = -1;
+          source = count <= kListed ? kList : kColumns;
+          items = count <= kListed ? count : a.vocab;
+        }
+        continue;
+      }
+      const Source from = job == 0 ? kMaxima : source;
+      const int many = job == 0 ? a.groups : items;
+      for (int i = tid; i < kBins; i += kPick) {
+        sh.n[i] = 0;
+        sh.m[i] = 0;
+      }
+      if (tid == 0) sh.found = -1;
+      __syncthreads();
+#pragma unroll 1
+      for (int i = 4 * tid; i < many; i += kRound) {
+        uint32_t d[4];
+        fetch(from, i, many, d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t b = (d[e] - lo) >> shift;
+          if (d[e] >= lo && d[e] <= limit && b < kBins) {
+            atomicAdd(&sh.n[b], 1u);
+            if (weigh) atomicAdd((unsigned long long*)&sh.m[b], (unsigned long long)fixed(weight(d[e])));
+          }
+        }
+      }
+      __syncthreads();
+      const uint64_t na = sh.n[2 * tid], nb = sh.n[2 * tid + 1], ma = sh.m[2 * tid], mb = sh.m[2 * tid + 1];
+      const uint64_t n = n0 + scan<kPick>(na + nb, sh.part), m = m0 + scan<kPick>(ma + mb, sh.part);
+      auto reaches = [&](uint64_t n, uint64_t m) { return by_mass ? (double)m >= goal : (double)n >= goal; };
+      const uint64_t n1 = n - na - nb, m1 = m - ma - mb;  // before this thread's
+      if (reaches(n, m) && (tid == 0 || !reaches(n1, m1))) {
+        const bool one = reaches(n1 + na, m1 + ma);
+        sh.found = 2 * tid + (one ? 0 : 1);
+        sh.before_n = one ? n1 : n1 + na;
+        sh.before_m = one ? m1 : m1 + ma;
+        sh.bin_n = one ? na : nb;
+      } else if (tid == kPick - 1 && !reaches(n, m)) {
+        sh.before_n = n;
+        sh.before_m = m;
+      }
+      __syncthreads();
+      const int found = sh.found;
+      n0 = sh.before_n;
+      m0 = sh.before_m;
+      const uint64_t there = sh.bin_n;
+      __syncthreads();
+      if (found < 0) {
+        run = shift != 21;
+        lo += (uint32_t)kBins << shift;
+        shift = 21;
+        continue;
+      }
+      lo += (uint32_t)found << shift;
+      const uint32_t hi = lo + ((1u << shift) - 1);
+      if (job == 0) {
+        limit = hi;
+        make = kMaxima;
+        run = false;
+        continue;
+      }
+      if (source == kColumns && n0 + there <= kListed) {
+        limit = hi;
+        make = kColumns;
+      }
+      if (there > 1 && (1u << shift) > kApart) {
+        shift = shift == 14 ? 3 : shift == 21 ? 10 : 0;
+        continue;
+      }
+      // The interval holds one value.
+#pragma unroll 1
+      for (int i = 4 * tid; i < many; i += kRound) {
+        uint32_t d[4];
+        fetch(from, i, many, d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d[e] >= lo && d[e] <= hi) sh.member = d[e];
+      }
+      __syncthreads();
+      const uint32_t value = sh.member;
+      uint64_t want = there;
+      if (job == 1) {
+        want = s.k - n0;
+      } else {
+        const double each = (double)fixed(weight(value)), need = __builtin_ceil((goal - (double)m0) / each);
+        want = need >= 1.0 && need < (double)there ? (uint64_t)need : need < 1.0 ? 1 : there;
+        if (s.k > 0 && value == cut && want > ties) want = ties;
+      }
+      cut = value;
+      cut_m = m0;
+      ties = want;
+      some = want < there;
+      run = false;
+    }
+
+    // Few: each column's rank is counted, and the ranks are weighed in their order.
+    if (job == 0 && source == kList && items <= kRanked) {
+      // Up to 16 neighbouring lanes take a column, each every so many-th four of the others.
+      if (tid < 4) sh.distance[items + tid] = kNone;
+      __syncthreads();
+      int lanes = 1;
+      while (lanes < 16 && 2 * lanes * items <= kPick) lanes *= 2;
+      const int of = tid / lanes;
+      if (of < items) {
+        const uint32_t its = sh.distance[of];
+        float count = 0.f;
+#pragma unroll 2
+        for (int i = 4 * (tid % lanes); i < items; i += 4 * lanes) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(&sh.distance[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) count += v[e] < its + (i + e < of ? 1u : 0u) ? 1.f : 0.f;
+        }
+        if (lanes > 1) count += dpp_move<kDppQuadXor1>(count);
+        if (lanes > 2) count += dpp_move<kDppQuadXor2>(count);
+        if (lanes > 4) count += dpp_move<kDppRowHalfMirror>(count);
+        if (lanes > 8) count += dpp_move<kDppRowMirror>(count);
+        if (tid % lanes == 0) sh.n[of] = (uint32_t)count;
+      }
+      __syncthreads();
+      const int rank = tid < items ? (int)sh.n[tid] : 0;
+      const double w = tid < items ? weight(sh.distance[tid]) : 0.0;
+      if (tid < items) sh.m[rank] = fixed(w);
+      __syncthreads();
+      const int k = s.k > 0 ? s.k : items;
+      const uint64_t m = tid < min(k, items) ? sh.m[tid] : 0, upto = scan<kPick>(m, sh.part);
+      if (tid == kPick - 1) sh.before_m = upto;
+      __syncthreads();
+      const double edge = (s.p > 0.f ? (double)s.p : 0.0) * (s.k > 0 ? (double)sh.before_m : whole);
+      sh.n[tid] = tid == 0 || (tid < k && (!s.nucleus() || (double)(upto - m) < edge));
+      __syncthreads();
+      const double kept = tid < items && sh.n[rank] != 0 && w >= (double)s.least ? w : 0.0;
+      const double cum = scan<kPick>(kept, sh.sum);
+      if (tid == kPick - 1) sh.goal = u * cum;
+      __syncthreads();
+      if (tid == pick<kPick>(kept > 0.0 && cum > sh.goal, kept > 0.0, sh.pick)) a.tokens[row] = sh.column[tid];
+      return;
     }
   }
 
-  // The first ranks: columns with distance below cut.lo, and the first `ties` of those at it.
-  Cut cut = {kNone - 1, kNone - 1, 0, 0, 0, false};
-  uint64_t ties = 0;
-  bool some = false;  // whether `ties` is less than there are
-  if (s.k > 0) {
-    cut = find(each_column, s.nucleus(), false, (double)s.k, kApart);
-    ties = s.k - cut.n;
-    some = cut.found && ties < cut.ties;
-  }
-  if (s.nucleus()) {
-    const double whole = s.k > 0 ? (double)(cut.m + ties * fixed(weight(cut.lo))) : total * unit;
-    const double goal = (s.p > 0.f ? (double)s.p : 0.0) * whole;
-    const Cut nucleus = find(each_column, true, true, goal, kApart);
-    if (nucleus.found) {
-      const double each = (double)fixed(weight(nucleus.lo)), need = __builtin_ceil((goal - (double)nucleus.m) / each);
-      uint64_t want = need >= 1.0 && need < (double)nucleus.ties ? (uint64_t)need : need < 1.0 ? 1 : nucleus.ties;
-      if (s.k > 0 && nucleus.lo == cut.lo && want > ties) want = ties;
-      cut = nucleus;
-      ties = want;
-      some = ties < cut.ties;
-    }
-  }
+  const int rounds = (items + kRound - 1) / kRound;
   // The column of the last tie that is kept.
   int last = 0x7fffffff;
   if (some) {
     uint64_t before = 0;
-    for (int r = 0; r < rounds && before < ties; ++r) {
-      load(r);
+#pragma unroll 1
+    for (int i0 = 0; i0 < items && before < ties; i0 += kRound) {
+      uint32_t d[4];
+      fetch(source, i0 + 4 * tid, items, d);
       uint64_t mine = 0;
 #pragma unroll
-      for (int e = 0; e < V; ++e) mine += d[e] == cut.lo;
+      for (int e = 0; e < 4; ++e) mine += d[e] == cut;
       const uint64_t upto = before + scan<kPick>(mine, sh.part);
       if (upto >= ties && upto - mine < ties) {
         uint64_t left = ties - (upto - mine);
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (d[e] == cut.lo && left-- == 1) sh.last = column(r, e);
+        for (int e = 0; e < 4; ++e)
+          if (d[e] == cut && left-- == 1) sh.last = column(source, i0 + 4 * tid + e);
       }
       if (tid == kPick - 1) sh.before_n = upto;
       __syncthreads();
@@ -420,36 +477,33 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
   }
 
   // The draw: the round, then the column.
-  const double least = (double)s.least;
-  double w[V];
-  auto weigh = [&](int r) {
-    load(r);
-    double sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      w[e] = 0.0;
-      if (d[e] < cut.lo || (d[e] == cut.lo && column(r, e) <= last)) {
-        const double v = weight(d[e]);
-        w[e] = v >= least ? v : 0.0;
-      }
-      sum += w[e];
-    }
-    return sum;
-  };
+  double mine = 0.0, upto = 0.0, w[4];
   int r = 0;
-  double mine = 0.0, upto = 0.0;
-  if (rounds > 1) {
-    for (r = 0; r < rounds; ++r) {
-      const double sum = wave_sum(weigh(r));
-      if (lane == 0) sh.sum[wave] = sum;
-      __syncthreads();
-      if (tid == 0) {
-        double all = 0.0;
-        for (int v = 0; v < kPickWaves; ++v) all += sh.sum[v];
-        sh.round[r] = all;
-      }
-      __syncthreads();
+  bool found = rounds == 1;
+#pragma unroll 1
+  for (;;) {
+    const int i = r * kRound + 4 * tid;
+    uint32_t d[4];
+    fetch(source, i, items, d);
+    mine = 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = 0.0;
+      if (d[e] < cut || (d[e] == cut && column(source, min(i + e, items - 1)) <= last)) w[e] = weight(d[e]);
+      w[e] = w[e] >= (double)s.least ? w[e] : 0.0;
+      mine += w[e];
     }
+    if (found) break;
+    const double sum = wave_sum(mine);
+    if (lane == 0) sh.sum[wave] = sum;
+    __syncthreads();
+    if (tid == 0) {
+      double all = 0.0;
+      for (int v = 0; v < kPickWaves; ++v) all += sh.sum[v];
+      sh.round[r] = all;
+    }
+    __syncthreads();
+    if (++r < rounds) continue;
     mine = tid < rounds ? sh.round[tid] : 0.0;
     upto = scan<kPick>(mine, sh.sum);
     if (tid == kPick - 1) sh.goal = upto;
@@ -459,8 +513,8 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
     if (tid == r) sh.goal = goal - (upto - mine);
     __syncthreads();
     rest = sh.goal;
+    found = true;
   }
-  mine = weigh(r);
   upto = scan<kPick>(mine, sh.sum);
   if (rest < 0.0) {
     if (tid == kPick - 1) sh.goal = upto;
@@ -469,17 +523,17 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
   }
   if (tid == pick<kPick>(mine > 0.0 && upto > rest, mine > 0.0, sh.pick)) {
     double cum = upto - mine;
-    int col = -1;
+    int at_item = -1;
     bool done = false;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
+    for (int e = 0; e < 4; ++e) {
       cum += w[e];
       if (!done && w[e] > 0.0) {
-        col = column(r, e);
+        at_item = r * kRound + 4 * tid + e;
         done = cum > rest;
       }
     }
-    a.tokens[row] = col;
+    a.tokens[row] = column(source, at_item);
   }
 }
 
