@@ -180,6 +180,15 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
     return __builtin_bit_cast(uint64_t, __builtin_fma(w, unit, 0x1p52)) & 0xfffffffffffffull;
   };
 
+  // The same nearly, for a search that is made again with exact ones where it ends: by an exponential that is off by 2e-6 (of
+  // exponents up to 30), in units of 2^-31; `slack` is more than both.
+  const float cf = fminf((float)c, 1e30f);
+  auto nearly = [&](uint32_t d) {
+    const float w = __builtin_amdgcn_exp2f((key_value((uint64_t)(key - d) << 32) - top) * cf);
+    return (uint64_t)(uint32_t)(w * 0x1p31f) << (a.mass_bits - 31);
+  };
+  const double slack = 1.0 + 1e-4 + a.vocab * 0x1p-31;
+
   Source source = kColumns;
   int first = 0, items = a.vocab;  // of the source; columns from `first` on
   auto column = [&](Source from, int i) {
@@ -222,6 +231,40 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) d[e] = j + e < end ? distance_of(x[e]) : kNone;
+  };
+
+  // The same of N rounds, whose loads are on their way together.
+  auto fetch_rounds = [&](Source from, int i0, int many, auto& d) {
+    constexpr int N = sizeof(d) / sizeof(d[0]);
+    typedef typename std::conditional<__is_same(T, float), u32x4, u32x2>::type Raw;
+    if (N == 1 || from == kMaxima || from == kList) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) fetch(from, i0 + j * kRound, many, d[j]);
+      return;
+    }
+    Raw v[N];
+    bool full[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = i0 + j * kRound, col = column(from, min(i, many - 4));
+      full[j] = i + 4 <= many && col + 4 <= a.vocab;
+      const char* p = full[j] ? at + (int64_t)col * (sizeof(Raw) / 4) : reinterpret_cast<const char*>(a.stats);
+      __builtin_memcpy(&v[j], p, sizeof(Raw));
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (full[j]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (__is_same(T, float))
+            d[j][e] = distance_of(__uint_as_float(v[j][e]));
+          else
+            d[j][e] = distance_of(T::load((uint16_t)(v[j][e / 2] >> (16 * (e & 1)))));
+        }
+      } else {
+        fetch(from, i0 + j * kRound, many, d[j]);
+      }
+    }
   };
 
   // The sum of the row's weights, and for draws from all of them the chunk that the token falls in.
@@ -269,42 +312,72 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
         make = kMaxima;
       }
     }
+    bool scouted = false;
     uint32_t lo = 0;
     uint64_t n0 = 0, m0 = 0;  // before lo
     int shift = 14;
 #pragma unroll 1
     while (run || make >= 0) {
       if (make >= 0) {
-        // Items up to the limit, in order.
+        // Items up to the limit, in order: the waves count theirs, and each adds up all counts.
         const Source from = (Source)make;
         const int many = from == kMaxima ? a.groups : from == kGroups ? items * kGroup : a.vocab;
-        int count = 0;
-#pragma unroll 1
-        for (int i0 = 0; i0 < many && count <= kListed; i0 += kRound) {
-          const int i = i0 + 4 * tid;
-          uint32_t d[4];
-          fetch(from, i, many, d);
-          int mine = 0;
+        const int room = from == kMaxima ? kSelected : kListed;
+        int count = 0, turn = 0;
+        auto take = [&](int i0, auto& d) {
+          constexpr int N = sizeof(d) / sizeof(d[0]);
+          fetch_rounds(from, i0 + 4 * tid, many, d);
+          int place[N];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mine += d[e] <= limit;
-          const int upto = (int)scan<kPick>((uint64_t)mine, sh.part);
-          int place = count + upto - mine;
+          for (int j = 0; j < N; ++j) {
+            int all = 0;
+            place[j] = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (d[e] <= limit) {
-              if (from == kMaxima) {
-                if (place < kSelected) sh.group[place] = (uint16_t)(i + e);
-              } else if (place < kListed) {
-                sh.distance[place] = d[e];
-                sh.column[place] = column(from, i + e);
-              }
-              ++place;
+            for (int e = 0; e < 4; ++e) {
+              const uint64_t those = __builtin_amdgcn_ballot_w64(d[j][e] <= limit);
+              all += __builtin_popcountll(those);
+              place[j] += __builtin_popcountll(those & ((1ull << lane) - 1));
             }
-          if (tid == kPick - 1) sh.found = upto;
+            if (lane == 0) sh.n[turn * kWave + j * kPickWaves + wave] = all;
+          }
+          static_assert(4 * kPickWaves == kWave, "a count a lane");
           __syncthreads();
-          count += sh.found;
-          __syncthreads();
-        }
+          const int mine = lane < N * kPickWaves ? sh.n[turn * kWave + lane] : 0;
+          int upto = mine;
+          auto up = [&](auto ctrl) { return __builtin_amdgcn_update_dpp(0, upto, decltype(ctrl)::value, 0xF, 0xF, true); };
+          upto += up(std::integral_constant<int, 0x111>());  // in rows of 16: row_shr:1, 2, 4, 8
+          upto += up(std::integral_constant<int, 0x112>());
+          upto += up(std::integral_constant<int, 0x114>());
+          upto += up(std::integral_constant<int, 0x118>());
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            static_assert(kPickWaves == 16, "a round a row of lanes");
+            int to = count + place[j] + __builtin_amdgcn_readlane(upto - mine, j * kPickWaves + wave);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (d[j][e] <= limit) {
+                const int i = i0 + j * kRound + 4 * tid + e;
+                if (to < room) {
+                  if (from == kMaxima) {
+                    sh.group[to] = (uint16_t)i;
+                  } else {
+                    sh.distance[to] = d[j][e];
+                    sh.column[to] = column(from, i);
+                  }
+                }
+                ++to;
+              }
+            count += __builtin_amdgcn_readlane(upto, j * kPickWaves + kPickWaves - 1);
+          }
+          turn ^= 1;
+        };
+        int i0 = 0;
+        uint32_t one[1][4], four[4][4];
+#pragma unroll 1
+        for (; i0 + 2 * kRound < many && count <= room; i0 += 4 * kRound) take(i0, four);
+#pragma unroll 1
+        for (; i0 < many && count <= room; i0 += kRound) take(i0, one);
+        __syncthreads();
         if (from == kMaxima) {
           make = count <= kSelected ? kGroups : kColumns;
           items = count <= kSelected ? count : items;
@@ -323,23 +396,35 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
       }
       if (tid == 0) sh.found = -1;
       __syncthreads();
-#pragma unroll 1
-      for (int i = 4 * tid; i < many; i += kRound) {
-        uint32_t d[4];
-        fetch(from, i, many, d);
+      const bool scout = from == kColumns && !scouted;
+      auto tally = [&](int i0, auto& d) {
+        constexpr int N = sizeof(d) / sizeof(d[0]);
+        fetch_rounds(from, i0 + 4 * tid, many, d);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t b = (d[e] - lo) >> shift;
-          if (d[e] >= lo && d[e] <= limit && b < kBins) {
-            atomicAdd(&sh.n[b], 1u);
-            if (weigh) atomicAdd((unsigned long long*)&sh.m[b], (unsigned long long)fixed(weight(d[e])));
+        for (int j = 0; j < N; ++j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t v = d[j][e], b = (v - lo) >> shift;
+            if (v >= lo && v <= limit && b < kBins) {
+              atomicAdd(&sh.n[b], 1u);
+              if (scout ? by_mass : weigh)
+                atomicAdd((unsigned long long*)&sh.m[b], (unsigned long long)(scout ? nearly(v) : fixed(weight(v))));
+            }
           }
         }
-      }
+      };
+      int i0 = 0;
+      uint32_t one[1][4], four[4][4];
+      if (from == kColumns)
+#pragma unroll 1
+        for (; i0 + 2 * kRound < many; i0 += 4 * kRound) tally(i0, four);
+#pragma unroll 1
+      for (; i0 < many; i0 += kRound) tally(i0, one);
       __syncthreads();
       const uint64_t na = sh.n[2 * tid], nb = sh.n[2 * tid + 1], ma = sh.m[2 * tid], mb = sh.m[2 * tid + 1];
       const uint64_t n = n0 + scan<kPick>(na + nb, sh.part), m = m0 + scan<kPick>(ma + mb, sh.part);
-      auto reaches = [&](uint64_t n, uint64_t m) { return by_mass ? (double)m >= goal : (double)n >= goal; };
+      const double aim = scout && by_mass ? goal * slack : goal;
+      auto reaches = [&](uint64_t n, uint64_t m) { return (double)(by_mass ? m : n) >= aim; };
       const uint64_t n1 = n - na - nb, m1 = m - ma - mb;  // before this thread's
       if (reaches(n, m) && (tid == 0 || !reaches(n1, m1))) {
         const bool one = reaches(n1 + na, m1 + ma);
@@ -357,6 +442,20 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
       m0 = sh.before_m;
       const uint64_t there = sh.bin_n;
       __syncthreads();
+      if (scout) {
+        // Few enough up to the interval: the search begins again among them; else with all, and exact weights.
+        if (found >= 0 && n0 + there <= kListed) {
+          limit = lo + ((uint32_t)(found + 1) << shift) - 1;
+          make = kColumns;
+        }
+        if (found >= 0 || shift == 21) {
+          scouted = true;
+          lo = 0;
+          n0 = m0 = 0;
+          shift = 14;
+          continue;
+        }
+      }
       if (found < 0) {
         run = shift != 21;
         lo += (uint32_t)kBins << shift;
@@ -370,10 +469,6 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
         make = kMaxima;
         run = false;
         continue;
-      }
-      if (source == kColumns && n0 + there <= kListed) {
-        limit = hi;
-        make = kColumns;
       }
       if (there > 1 && (1u << shift) > kApart) {
         shift = shift == 14 ? 3 : shift == 21 ? 10 : 0;
