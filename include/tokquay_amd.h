@@ -616,8 +616,8 @@ tq_status tq_tree_layout(int64_t* positions, int64_t* masks, int64_t mask_words,
  * tq_paged_chunk for trees of drafted tokens: the keys and values of sequence b's new rows, its nodes, lie at positions
  * q_start[b] + i, and row i sees every key before q_start[b] and, of the new ones, key q_start[b] + j where j <= i and bit
  * j % 64 of masks[row][j / 64] is set (tq_tree_layout, or any other mask). A row that sees nothing (no cached keys and no bits) gets
- * zeros. masks is int64 [num_q_rows, mask_words] with 64 mask_words >= max_query_len. All else, the workspace too
- * (tq_paged_chunk_workspace_size), is tq_paged_chunk's. No counterpart in the reference.
+ * zeros. masks is int64 [num_q_rows, mask_words] with 64 mask_words >= max_query_len. The workspace is of
+ * tq_paged_tree_workspace_size(...) bytes; all else is tq_paged_chunk's. No counterpart in the reference.
  */
 tq_status tq_paged_tree(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
                         const void* pool, int64_t num_blocks, int32_t num_layers, int32_t num_heads,
@@ -627,6 +627,10 @@ tq_status tq_paged_tree(void* out, int64_t out_row_stride, const void* q, int64_
                         int32_t num_seqs, int32_t num_q_rows, int32_t max_query_len, int32_t max_context_len,
                         float scale, int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* d_error,
                         void* stream);
+
+/* Bytes of workspace tq_paged_tree needs for these sizes (0 if none). */
+size_t tq_paged_tree_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                    int32_t num_q_rows, int32_t max_query_len, int32_t max_context_len);
 
 /*
  * A token of each row of logits, drawn from a given random number. The columns of a row are ranked by logit, largest first, equal ones

@@ -85,21 +85,21 @@ def test_row_counts_a_kv_head(group):
 @pytest.mark.parametrize("dim,dtype", [(64, FP16), (128, BF16)])
 def test_long_contexts_in_parts(lengths, dim, dtype):
     c = Tree(trees(*lengths), 8, 2, dim, dtype, 16, seed=6)
-    assert ops.chunk_workspace_bytes(len(lengths), 8, 2, dim, c.q.size(0), c.max_new, c.max_context) > 0
+    assert ops.tree_workspace_bytes(len(lengths), 8, 2, dim, c.q.size(0), c.max_new, c.max_context) > 0
     check(c)
 
 
 def test_parts_of_which_a_row_sees_nothing():
     # Every node a root: the 600 rows see a short context and, each in its own part, themselves.
     c = Tree([(100, [-1] * 600)], 1, 1, 64, BF16, 16, seed=7)
-    assert ops.chunk_workspace_bytes(1, 1, 1, 64, 600, 600, 700) > 0
+    assert ops.tree_workspace_bytes(1, 1, 1, 64, 600, 600, 700) > 0
     check(c)
     check(Tree([(0, [-1] * 600)], 1, 1, 64, FP16, 16, seed=7))
 
 
 def test_from_the_queue():
     c = Tree(trees(*[(2100 + 3 * i, 33 + i // 2) for i in range(36)]), 32, 8, 128, BF16, 16, seed=8)
-    plan = ops.chunk_workspace_bytes(36, 32, 8, 128, c.q.size(0), c.max_new, c.max_context)
+    plan = ops.tree_workspace_bytes(36, 32, 8, 128, c.q.size(0), c.max_new, c.max_context)
     assert 0 < plan < 1 << 16  # a queue of row tiles, no sums of parts
     check(c)
 

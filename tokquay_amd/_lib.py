@@ -243,6 +243,7 @@ SIGNATURES: dict[str, tuple] = {
             c_i32p, ctypes.c_void_p,  # d_error, stream
         ],
     ),
+    "tq_paged_tree_workspace_size": (ctypes.c_size_t, [ctypes.c_int32] * 7),
     "tq_sample_tokens": (
         ctypes.c_int,
         [

@@ -1072,7 +1072,7 @@ constexpr int kTilesNt = 2;
 // 100-500 behind up to 2,000 325 -> 267, 4 x 2,048 behind up to 6,144 696 -> 535.
 constexpr int kQueueFrom = 2048;
 
-Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int num_q_rows, int max_query_len, int max_context) {
+Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int num_q_rows, int max_query_len, int max_context, bool tree) {
   Plan p;
   const int64_t rows = (int64_t)max_query_len * group;
   p.tiles = rows > 64;
@@ -1089,7 +1089,10 @@ Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int num_q_rows
   const float step = (p.tiles ? 2.0f : 0.6f) * (head_dim == 64 ? 1.f : 1.3f), launch = 4.5f;
   const float pairs = 2e-6f * head_dim * num_q_rows * kv_heads * group;
   const float best = __builtin_sqrtf(steps * step / __builtin_fmaxf(pairs, 1e-6f));
-  int64_t parts = want / groups;
+#ifndef TREE_F
+#define TREE_F 1
+#endif
+  int64_t parts = (tree ? TREE_F : 1) * want / groups;
   if ((float)parts > best) parts = (int64_t)best;
   parts = parts < 1 ? 1 : parts > steps ? steps : parts;
   if (steps * step <= (float)((steps + parts - 1) / parts) * step + launch + pairs * parts) parts = 1;
@@ -1139,6 +1142,17 @@ tq_status launch(const ChunkArgs& a, const Plan& p, hipStream_t stream) {
 }
 
 template <bool TREE>
+size_t workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t num_q_rows,
+                      int32_t max_query_len, int32_t max_context_len) {
+  if (!sizes_ok(num_seqs, num_heads, num_kv_heads, head_dim, num_q_rows, max_query_len, max_context_len) ||
+      num_seqs == 0 || num_q_rows == 0 || max_query_len == 0 || max_context_len == 0 || max_context_len > kMaxContext)
+    return 0;
+  const int32_t group = num_heads / num_kv_heads;
+  const Plan p = plan_of(num_seqs, num_kv_heads, group, head_dim, num_q_rows, max_query_len, max_context_len, TREE);
+  return workspace_of(p, num_seqs, num_q_rows, num_heads, group, head_dim);
+}
+
+template <bool TREE>
 tq_status attend(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride, const void* pool,
                  int64_t num_blocks, int32_t num_layers, int32_t num_heads, int32_t num_kv_heads, int32_t block_size,
                  int32_t head_dim, int32_t layer, const int32_t* block_tables, int64_t block_table_stride,
@@ -1166,7 +1180,7 @@ tq_status attend(void* out, int64_t out_row_stride, const void* q, int64_t q_row
   if ((int64_t)max_query_len * num_heads > 0x7fffffffLL - 65536) return TQ_ERR_UNSUPPORTED;
 
   const int32_t group = num_heads / num_kv_heads;
-  const Plan p = plan_of(num_seqs, num_kv_heads, group, head_dim, num_q_rows, max_query_len, max_context_len);
+  const Plan p = plan_of(num_seqs, num_kv_heads, group, head_dim, num_q_rows, max_query_len, max_context_len, TREE);
   const size_t need = workspace_of(p, num_seqs, num_q_rows, num_heads, group, head_dim);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 16 != 0))
     return TQ_ERR_WORKSPACE;
@@ -1223,13 +1237,13 @@ tq_status attend(void* out, int64_t out_row_stride, const void* q, int64_t q_row
 extern "C" size_t tq_paged_chunk_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
                                                 int32_t head_dim, int32_t num_q_rows, int32_t max_query_len,
                                                 int32_t max_context_len) {
-  using namespace tq;
-  if (!sizes_ok(num_seqs, num_heads, num_kv_heads, head_dim, num_q_rows, max_query_len, max_context_len) ||
-      num_seqs == 0 || num_q_rows == 0 || max_query_len == 0 || max_context_len == 0 || max_context_len > kMaxContext)
-    return 0;
-  const int32_t group = num_heads / num_kv_heads;
-  const Plan p = plan_of(num_seqs, num_kv_heads, group, head_dim, num_q_rows, max_query_len, max_context_len);
-  return workspace_of(p, num_seqs, num_q_rows, num_heads, group, head_dim);
+  return tq::workspace_size<false>(num_seqs, num_heads, num_kv_heads, head_dim, num_q_rows, max_query_len, max_context_len);
+}
+
+extern "C" size_t tq_paged_tree_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                               int32_t head_dim, int32_t num_q_rows, int32_t max_query_len,
+                                               int32_t max_context_len) {
+  return tq::workspace_size<true>(num_seqs, num_heads, num_kv_heads, head_dim, num_q_rows, max_query_len, max_context_len);
 }
 
 extern "C" tq_status tq_paged_chunk(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,

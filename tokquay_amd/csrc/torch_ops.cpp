@@ -455,8 +455,8 @@ void attend(const char* op, at::Tensor& out, const at::Tensor& q, const at::Tens
   if (masks != nullptr) masks_of(op, *masks, rows, max_query_len, q.device());
   error_word_of(op, d_error, p);
   size_t ws = workspace_of(op, workspace, p);
-  const size_t need = tq_paged_chunk_workspace_size((int32_t)n, (int32_t)heads, p.heads, p.head_dim, (int32_t)rows,
-                                                    (int32_t)max_query_len, (int32_t)max_context_len);
+  const size_t need = (masks != nullptr ? tq_paged_tree_workspace_size : tq_paged_chunk_workspace_size)(
+      (int32_t)n, (int32_t)heads, p.heads, p.head_dim, (int32_t)rows, (int32_t)max_query_len, (int32_t)max_context_len);
   at::Tensor own;  // from torch's allocator: safe on any stream and under graph capture
   void* at_ws = ptr<void>(workspace);
   if (need > 0 && !workspace.has_value()) {

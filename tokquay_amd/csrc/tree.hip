@@ -24,18 +24,19 @@ struct LayoutArgs {
   int32_t max_query_len;
 };
 
-// One wave a sequence, 64 nodes at a time: inside them the ancestors are joined in six steps, each over twice as many links as the
-// one before; what lies above comes from the mask of the one node further up that the links lead to. The last
-// workgroup clears the rows of no sequence.
-__global__ __launch_bounds__(kWave) void tree_layout_kernel(const LayoutArgs a) {
-  const int lane = threadIdx.x, b = blockIdx.x;
+// One workgroup a sequence, a wave 64 of its nodes. Inside these the ancestors are joined in six steps, each over twice as many links as
+// the one before, by all waves at once; what lies above comes, wave after wave, from the mask of the one node further up that the links
+// lead to, which LDS holds (of trees of more than kLayoutNodes nodes: the masks themselves). The last workgroup clears the rows of no
+// sequence. Bound by its latency: the loads of lengths and parents, and the stores.
+constexpr int kLayoutWaves = 8, kLayoutNodes = kWave * kLayoutWaves;
+
+__global__ __launch_bounds__(kLayoutNodes) void tree_layout_kernel(const LayoutArgs a) {
+  __shared__ uint64_t s_masks[kLayoutNodes * kLayoutWaves];  // [word][node]: of nodes below kLayoutNodes
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), b = blockIdx.x, threads = blockDim.x;
   if (b == a.num_seqs) {
     const int first = min(max(a.cu[0], 0), a.num_rows), last = min(max(a.cu[a.num_seqs], first), a.num_rows);
-    for (int64_t r = lane; r < a.num_rows; r += kWave) {
-      if (r >= first && r < last) {
-        r += (last - 1 - r) / kWave * kWave;  // over the sequences' rows
-        continue;
-      }
+    for (int64_t i = tid; i < (int64_t)first + a.num_rows - last; i += threads) {
+      const int64_t r = i < first ? i : i - first + last;
       a.positions[r] = 0;
       for (int64_t w = 0; w < a.words; ++w) a.masks[r * a.words + w] = 0;
     }
@@ -45,20 +46,21 @@ __global__ __launch_bounds__(kWave) void tree_layout_kernel(const LayoutArgs a) 
   const int64_t n = (int64_t)a.cu[b + 1] - lo;
   if (n == 0) return;
   if (n < 0 || lo < 0 || lo + n > a.num_rows || n > a.max_query_len || start < 0) {
-    if (lane == 0) flag_error(a.d_error, TQ_DEVERR_LENGTH);
+    if (tid == 0) flag_error(a.d_error, TQ_DEVERR_LENGTH);
     return;
   }
-  for (int base = 0; base < n; base += kWave) {
-    const int i = base + lane;
+  for (int base = 0; base < n; base += threads) {
+    const int i = base + tid, own = i / kWave;  // the word of this wave's nodes
     int parent = i < n ? a.parents[lo + i] : -1;
     if (parent < -1 || parent >= i) {
       if (i < n) flag_error(a.d_error, TQ_DEVERR_PARENT);
       parent = -1;
     }
     uint64_t mine = 1ull << lane;
-    int up = parent >= base ? parent - base : -1, top = lane;  // a lane; the furthest one that was reached
+    int up = parent >= own * kWave ? parent - own * kWave : -1, top = lane;  // a lane; the furthest one that was reached
 #pragma unroll
     for (int step = 0; step < 6; ++step) {
+      if (__builtin_amdgcn_ballot_w64(up >= 0) == 0) break;
       const int from = up < 0 ? lane : up;
       const uint64_t more = __shfl(mine, from);
       const int there = __shfl(top, from), next = __shfl(up, from);
@@ -68,25 +70,36 @@ __global__ __launch_bounds__(kWave) void tree_layout_kernel(const LayoutArgs a) 
         up = next;
       }
     }
-    const int above = __shfl(parent, top);  // below base
-    if (i < n) {
-      uint64_t* mask = a.masks + (int64_t)(lo + i) * a.words;
-      int depth = __builtin_popcountll(mine) - 1;
-      for (int64_t w = 0; w < a.words; ++w) {
-        uint64_t word = 0;
-        if (w == base / kWave)
-          word = mine;
-        else if (w < base / kWave && above >= 0) {
-          // Written by this wave, before.
-          word = __hip_atomic_load(a.masks + (int64_t)(lo + above) * a.words + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int above = __shfl(parent, top);  // below this wave's nodes
+    uint64_t* mask = a.masks + (int64_t)(lo + i) * a.words;
+    int depth = __builtin_popcountll(mine) - 1;
+    if (i < n && own < kLayoutWaves) s_masks[own * kLayoutNodes + i] = mine;
+    // Wave after wave: words before its own.
+    const int waves = (int)min((int64_t)threads, n - base + kWave - 1) / kWave;
+    for (int turn = 0; turn < waves; ++turn) {
+      if (tid / kWave == turn && i < n) {
+        for (int w = 0; w < own; ++w) {
+          uint64_t word = 0;
+          if (w <= above / kWave && above >= 0) {
+            if (i < kLayoutNodes)
+              word = s_masks[w * kLayoutNodes + above];
+            else  // written by this workgroup before
+              word = __hip_atomic_load(a.masks + (int64_t)(lo + above) * a.words + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
           depth += __builtin_popcountll(word);
+          if (i < kLayoutNodes) s_masks[w * kLayoutNodes + i] = word;
+          __hip_atomic_store(mask + w, word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        __hip_atomic_store(mask + w, word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(mask + own, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int64_t w = own + 1; w < a.words; ++w) mask[w] = 0;
+        a.positions[lo + i] = (int64_t)start + depth;
       }
-      a.positions[lo + i] = (int64_t)start + depth;
+      if (n > kLayoutNodes) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+      }
+      if (waves > 1 || n > threads) __syncthreads();
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   }
 }
 
@@ -147,24 +160,36 @@ __global__ __launch_bounds__(kMoveThreads) void accept_tree_kernel(const AcceptA
   const int32_t* table = a.block_tables + (int64_t)b * a.bt_stride;
   const int piece = slice * kMoveThreads + threadIdx.x;
   char* mine = a.pool + (int64_t)(piece / a.slot_pieces) * a.slab_bytes + piece % a.slot_pieces * 16;
+  // The first 64 nodes, one a lane.
+  const int there = lo + min(lane, (int)n - 1);
+  const int32_t parent = lane < n ? a.parents[there] : -2;
+  const int64_t draft = a.drafts[there], after = a.sampled[there];
   int node = 0, count = 0;
   while (node >= 0 && count < a.max_path) {
     // Up to 64 nodes of the path, one a lane.
     int here = 0, many = 0;
     int64_t token = -1;
     while (node >= 0 && many < kWave && count + many < a.max_path) {
-      const int64_t t = a.sampled[lo + node];
+      int64_t t;
+      if (node < kWave)
+        t = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(after >> 32), node) << 32 |
+                      (uint32_t)__builtin_amdgcn_readlane((int)after, node));
+      else
+        t = a.sampled[lo + node];
       if (lane == many) {
         here = node;
         token = t;
       }
       ++many;
       int next = -1;
-      for (int i0 = node + 1; i0 < n && next < 0 && t >= 0; i0 += kWave) {
-        const int i = i0 + lane;
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(i < n && a.parents[lo + min(i, (int)n - 1)] == node &&
-                                                         a.drafts[lo + min(i, (int)n - 1)] == t);
-        if (hit != 0) next = i0 + __builtin_ctzll(hit);
+      if (t >= 0) {
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(parent == node && draft == t && lane > node);
+        if (hit != 0) next = __builtin_ctzll(hit);
+        for (int i0 = max(node + 1, kWave); i0 < n && next < 0; i0 += kWave) {
+          const int i = min(i0 + lane, (int)n - 1);
+          const uint64_t more = __builtin_amdgcn_ballot_w64(i0 + lane < n && a.parents[lo + i] == node && a.drafts[lo + i] == t);
+          if (more != 0) next = i0 + __builtin_ctzll(more);
+        }
       }
       node = next;
     }
@@ -172,22 +197,41 @@ __global__ __launch_bounds__(kMoveThreads) void accept_tree_kernel(const AcceptA
       tokens[count + lane] = token;
       path[count + lane] = here;
     }
-    if (a.pool != nullptr)
-      for (int j = 0; j < many; ++j) {
-        const int from = __builtin_amdgcn_readlane(here, j), to = count + j;
-        if (from == to) continue;
-        const int sp = start + from, dp = start + to;
-        const int32_t sb = table[sp / a.block_size], db = table[dp / a.block_size];
+    if (a.pool != nullptr) {
+      // Lane j finds the places of node j of these.
+      bool moves = lane < many && here != count + lane;
+      const int sp = start + (moves ? here : 0), dp = start + (moves ? count + lane : 0);
+      int32_t sb = 0, db = 0;
+      if (moves) {
+        sb = table[sp / a.block_size];
+        db = table[dp / a.block_size];
         if ((uint32_t)sb >= (uint32_t)a.num_blocks || (uint32_t)db >= (uint32_t)a.num_blocks) {
-          if (lane == 0) flag_error(a.d_error, TQ_DEVERR_BLOCK_ID);
-          continue;
-        }
-        if (piece < a.pieces) {
-          const int64_t slot = (int64_t)a.slot_pieces * 16;
-          *reinterpret_cast<u32x4*>(mine + db * a.block_bytes + dp % a.block_size * slot) =
-              *reinterpret_cast<const u32x4*>(mine + sb * a.block_bytes + sp % a.block_size * slot);
+          if (lead) flag_error(a.d_error, TQ_DEVERR_BLOCK_ID);
+          moves = false;
         }
       }
+      const int64_t slot = (int64_t)a.slot_pieces * 16;
+      const int64_t src = sb * a.block_bytes + sp % a.block_size * slot, dst = db * a.block_bytes + dp % a.block_size * slot;
+      auto of = [&](int64_t v, int j) {
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), j) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)v, j));
+      };
+      // Four at a time: none of them is written before a later one is read from the same place (above).
+      uint64_t left = __builtin_amdgcn_ballot_w64(moves);
+      while (left != 0) {
+        u32x4 v[4];
+        int j[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          j[e] = left != 0 ? __builtin_ctzll(left) : -1;
+          left &= left - 1;
+          if (j[e] >= 0 && piece < a.pieces) v[e] = *reinterpret_cast<const u32x4*>(mine + of(src, j[e]));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j[e] >= 0 && piece < a.pieces) *reinterpret_cast<u32x4*>(mine + of(dst, j[e])) = v[e];
+      }
+    }
     count += many;
   }
   if (lead) {
@@ -221,7 +265,8 @@ extern "C" tq_status tq_tree_layout(int64_t* positions, int64_t* masks, int64_t 
   a.num_rows = num_rows;
   a.num_seqs = num_seqs;
   a.max_query_len = max_query_len;
-  hipLaunchKernelGGL(tree_layout_kernel, dim3((unsigned)num_seqs + 1), dim3(kWave), 0, (hipStream_t)stream, a);
+  const int waves = max_query_len > kLayoutNodes - kWave ? kLayoutWaves : max_query_len > kWave ? (max_query_len + kWave - 1) / kWave : 1;
+  hipLaunchKernelGGL(tree_layout_kernel, dim3((unsigned)num_seqs + 1), dim3(kWave * waves), 0, (hipStream_t)stream, a);
   return check_launch();
 }
 

@@ -641,6 +641,12 @@ def tree_layout(
     return positions, masks
 
 
+def tree_workspace_bytes(num_seqs: int, n_head: int, n_kv_head: int, d_head: int, num_q_rows: int,
+                         max_query_len: int, max_context_len: int) -> int:  # fmt: skip
+    return int(_lib.lib().tq_paged_tree_workspace_size(num_seqs, n_head, n_kv_head, d_head, num_q_rows, max_query_len,
+                                                       max_context_len))  # fmt: skip
+
+
 def paged_tree(
     out: torch.Tensor,
     q: torch.Tensor,
@@ -658,8 +664,7 @@ def paged_tree(
 ) -> None:
     """``paged_chunk`` for trees of drafted tokens: row i of sequence b sees every key before ``q_start[b]`` and, of the sequence's new
     ones, the keys ``q_start[b] + j``, ``j <= i``, whose bit j of the row's mask is set. ``masks`` is ``tree_layout``'s, or any
-    other int64 ``[N, words]``. A row that sees nothing gets zeros. A line of drafts takes the same time in ``paged_chunk``, which
-    needs no masks. The workspace is ``paged_chunk``'s (``chunk_workspace_bytes``)."""
+    other int64 ``[N, words]``. A row that sees nothing gets zeros. A line of drafts needs no masks in ``paged_chunk``."""
     if scale is None:
         scale = 1.0 / math.sqrt(pool.size(-1))
     _checked_op("paged_tree", out, q, pool, layer, block_tables, cu_seqlens_q, q_start, masks, max_query_len, max_context_len,

@@ -390,7 +390,8 @@ def _attend(op, out, q, pool, layer, block_tables, cu_seqlens_q, q_start, masks,
     _workspace(op, workspace, pool)
     if workspace is not None:
         sizes = (n, heads, pool.size(3), pool.size(5), rows, max_query_len, max_context_len)
-        need = _lib.lib().tq_paged_chunk_workspace_size(*map(int, sizes))  # (sizes of a dynamic trace become numbers)
+        size_of = getattr(_lib.lib(), f"tq_{op}_workspace_size")
+        need = size_of(*map(int, sizes))  # (sizes of a dynamic trace become numbers)
         size = workspace.element_size()
         if need > 0 and (workspace.numel() * size < need or workspace.storage_offset() * size % 16):
             raise RuntimeError(f"tq_{op} failed: {_lib.STATUS_NAMES[3]}")
