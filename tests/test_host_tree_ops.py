@@ -142,6 +142,14 @@ def test_wrappers_raise_value_errors():
             ops.accept_tree(a["sampled"], a["draft_tokens"], a["parents"], a["cu_seqlens_q"], 6, pool=a["pool"])
         with pytest.raises(ValueError, match="tokens must be"):
             ops.accept_tree(a["sampled"], a["draft_tokens"], a["parents"], a["cu_seqlens_q"], 5, tokens=a["tokens"])
+        with pytest.raises(ValueError, match="max_path be a length above 0"):
+            ops.accept_tree(a["sampled"], a["draft_tokens"], a["parents"], a["cu_seqlens_q"], 0)
+        with pytest.raises(ValueError, match="accept_tree: parents must be"):
+            ops.accept_tree(a["sampled"], a["draft_tokens"], a["parents"][:-1], a["cu_seqlens_q"], 4)
+        with pytest.raises(ValueError, match="tree_layout: max_query_len must be a length"):
+            ops.tree_layout(empty(5, dtype=I32), empty(2, dtype=I32), empty(1, dtype=I32), -1)
+        with pytest.raises(ValueError, match="sample_tokens: uniforms must be"):
+            ops.sample_tokens(empty(5, 90), empty(4), empty(5))
         with pytest.raises(ValueError, match="copy_blocks: dst_blocks must be"):
             ops.copy_blocks(copy_args()["pool"], empty(3, dtype=I32), empty(2, dtype=I32))
         with pytest.raises(ValueError, match="tree_layout: masks must be"):
@@ -163,7 +171,7 @@ def test_a_traced_step_records_the_kernels_as_operators():
         graph = make_fx(step)(empty(7, 256, dtype=BF16), c["q"], c["pool"], c["block_tables"], c["cu_seqlens_q"], c["q_start"],
                               empty(7, dtype=I32), empty(7, 50), empty(7), empty(3), empty(7, dtype=I64))  # fmt: skip
     targets = [str(n.target) for n in graph.graph.nodes if n.op == "call_function"]
-    assert all(f"tokquay_amd.{op}.default" in targets for op in ARGS)
+    assert all(any(f"tokquay_amd.{op}.{form}" in targets for form in ("default", "new")) for op in ARGS)
 
 
 def test_calls_without_work():

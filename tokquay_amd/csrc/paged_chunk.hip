@@ -1072,6 +1072,13 @@ constexpr int kTilesNt = 2;
 // 100-500 behind up to 2,000 325 -> 267, 4 x 2,048 behind up to 6,144 696 -> 535.
 constexpr int kQueueFrom = 2048;
 
+// A tree has few rows, and the sequences of a batch have contexts of all lengths: parts of the longest one are empty for most others
+// and their workgroups end at once. So trees are split into as many parts as would fit in four rounds (one round -> four: 32 trees of 9-33
+// nodes behind 1,001-8,007 tokens, 32 / 4 heads of 64, 88 -> 75 us; 16 of 20-40 behind 100-12,000, 32 / 8 of 128, 174 -> 126; but 4 of
+// 130 behind 3,000-6,000 72 -> 79). With equal lengths the parts are those that pay in both (8 of 64 nodes behind 4,000: 58). Parts
+// worked out on the device from the lengths took as long as this, and 6 us more of every call.
+constexpr int kTreeRounds = 4;
+
 Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int num_q_rows, int max_query_len, int max_context, bool tree) {
   Plan p;
   const int64_t rows = (int64_t)max_query_len * group;
@@ -1089,10 +1096,7 @@ Plan plan_of(int num_seqs, int kv_heads, int group, int head_dim, int num_q_rows
   const float step = (p.tiles ? 2.0f : 0.6f) * (head_dim == 64 ? 1.f : 1.3f), launch = 4.5f;
   const float pairs = 2e-6f * head_dim * num_q_rows * kv_heads * group;
   const float best = __builtin_sqrtf(steps * step / __builtin_fmaxf(pairs, 1e-6f));
-#ifndef TREE_F
-#define TREE_F 1
-#endif
-  int64_t parts = (tree ? TREE_F : 1) * want / groups;
+  int64_t parts = (tree ? kTreeRounds : 1) * want / groups;
   if ((float)parts > best) parts = (int64_t)best;
   parts = parts < 1 ? 1 : parts > steps ? steps : parts;
   if (steps * step <= (float)((steps + parts - 1) / parts) * step + launch + pairs * parts) parts = 1;

@@ -497,14 +497,14 @@ def embed_rows(ids: torch.Tensor, positions: torch.Tensor, wte: torch.Tensor, wp
 
 # ------------------------------------------- 16-bit pools, grouped heads, chunks of new tokens, drafts
 @functools.lru_cache(maxsize=None)
-def _overload(name: str):
-    return getattr(torch_ops.load(), name).default
+def _overload(name: str, form: str):
+    return getattr(getattr(torch_ops.load(), name), form)
 
 
-def _checked_op(name: str, *args) -> None:
+def _checked_op(name: str, *args, form: str = "default"):
     """``_op`` for operators whose arguments are checked by the operator alone: what it refuses is a ``ValueError``."""
     try:
-        _overload(name)(*args)
+        return _overload(name, form)(*args)
     except RuntimeError as e:
         first = str(e).splitlines()[0] if str(e) else ""
         if first.startswith(f"tokquay_amd::{name}: "):
@@ -632,6 +632,8 @@ def tree_layout(
     its number of ancestors, what ``rope_cache_write`` rotates by, while its slot is that of position ``q_start[b] + i``. Its mask has a bit for
     itself and for each ancestor, node j's in word ``j // 64``: what ``paged_tree`` takes. Rows of no sequence get zeros. For all layers of a step
     one call is enough."""
+    if positions is None and masks is None:
+        return _checked_op("tree_layout", parents, cu_seqlens_q, q_start, max_query_len, d_error, form="new")
     n = parents.numel()
     if positions is None:
         positions = torch.empty(n, dtype=torch.int64, device=parents.device)
@@ -691,7 +693,7 @@ def sample_tokens(
     With ``cu_seqlens_q`` (``paged_chunk``'s) the settings have an entry a sequence, for all of its rows, and rows of no sequence keep
     their token. Mask tokens with -inf logits."""
     if tokens is None:
-        tokens = torch.empty(logits.size(0), dtype=torch.int64, device=logits.device)
+        return _checked_op("sample_tokens", logits, uniforms, temperature, top_k, top_p, min_p, cu_seqlens_q, d_error, form="new")
     _checked_op("sample_tokens", tokens, logits, uniforms, temperature, top_k, top_p, min_p, cu_seqlens_q, d_error)
     return tokens
 
@@ -721,6 +723,9 @@ def accept_tree(
     With ``pool`` (float32, float16 or bfloat16), ``block_tables`` and ``q_start`` the path's keys and values move together: those of
     position ``q_start[b] + path[b, j]`` to ``q_start[b] + j``, in all layers, in the same launch. The cache then holds the sequence's first
     ``q_start[b] + counts[b]`` positions."""
+    if tokens is None and path is None and counts is None:
+        return _checked_op("accept_tree", sampled, draft_tokens, parents, cu_seqlens_q, max_path, pool, block_tables, q_start,
+                           d_error, form="new")  # fmt: skip
     if counts is None:
         counts = torch.empty(cu_seqlens_q.numel() - 1, dtype=torch.int32, device=sampled.device)
     if tokens is None:

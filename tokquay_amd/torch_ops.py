@@ -35,6 +35,9 @@ or entries, overlapping rows; the last eight also refuse every number out of its
   q_start?, d_error!?)``
 * ``copy_blocks(pool!, src_blocks, dst_blocks, num_slots?, d_error!?)``
 
+The forms ``tree_layout.new``, ``sample_tokens.new`` and ``accept_tree.new`` return outputs of their own (``accept_tree.new`` takes
+``max_path`` behind ``cu_seqlens_q``).
+
 (``!``: written in place.) ``tokquay_amd.ops`` checks the tensors with the reference's messages
 and calls these operators; there is no fallback when the library is missing.
 """
@@ -526,7 +529,35 @@ def _fake_copy_blocks(pool, src_blocks, dst_blocks, num_slots, d_error):
         _exactly(op, "d_error", d_error, torch.int32, 1, pool.device)
 
 
+def _fake_tree_layout_new(parents, cu_seqlens_q, q_start, max_query_len, d_error):
+    if not 0 <= max_query_len < 2**31:
+        _fail("tree_layout", "max_query_len must be a length")
+    n = parents.numel()
+    positions = parents.new_empty(n, dtype=torch.int64)
+    masks = parents.new_empty(n, (max_query_len + 63) // 64, dtype=torch.int64)
+    _fake_tree_layout(positions, masks, parents, cu_seqlens_q, q_start, max_query_len, d_error)
+    return positions, masks
+
+
+def _fake_sample_tokens_new(logits, uniforms, temperature, top_k, top_p, min_p, cu_seqlens_q, d_error):
+    tokens = logits.new_empty(uniforms.numel(), dtype=torch.int64)
+    _fake_sample_tokens(tokens, logits, uniforms, temperature, top_k, top_p, min_p, cu_seqlens_q, d_error)
+    return tokens
+
+
+def _fake_accept_tree_new(sampled, draft_tokens, parents, cu_seqlens_q, max_path, pool, block_tables, q_start, d_error):
+    n = cu_seqlens_q.numel() - 1
+    if not (n >= 0 and 1 <= max_path < 2**31):
+        _fail("accept_tree", "cu_seqlens_q must have num_seqs + 1 entries, and max_path be a length above 0")
+    tokens, path = sampled.new_empty(n, max_path, dtype=torch.int64), sampled.new_empty(n, max_path, dtype=torch.int32)
+    counts = sampled.new_empty(n, dtype=torch.int32)
+    _fake_accept_tree(tokens, path, counts, sampled, draft_tokens, parents, cu_seqlens_q, pool, block_tables, q_start, d_error)
+    return tokens, path, counts
+
+
 FAKES = {name: globals()[f"_fake_{name}"] for name in OPS}
+# Operators with a form that makes its own outputs.
+NEW = ("tree_layout", "sample_tokens", "accept_tree")
 
 
 def load():
@@ -538,5 +569,7 @@ def load():
         torch.ops.load_library(TORCH_OPS_PATH)
         for name in OPS:
             torch.library.register_fake(f"tokquay_amd::{name}")(FAKES[name])
+        for name in NEW:
+            torch.library.register_fake(f"tokquay_amd::{name}.new")(globals()[f"_fake_{name}_new"])
         _loaded = True
     return torch.ops.tokquay_amd
