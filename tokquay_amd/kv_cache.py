@@ -115,6 +115,56 @@ class BlockAllocator:
                 self._free.append(b)
         seq.block_table = []
 
+    def fork(self, seq: Sequence, child: Sequence, num_tokens: int | None = None) -> None:
+        """Give a block-less ``child`` the first ``num_tokens`` cached positions of ``seq`` (default: all of them), so that both
+        go on from there: whole blocks are shared, by their ref counts, and the filled part of the next one is copied into a block of
+        the child's own (``ops.copy_blocks``). Neither writes to a shared block: both are past it."""
+        n = seq.num_cached_tokens if num_tokens is None else num_tokens
+        if child.block_table:
+            raise ValueError(f"sequence {child.seq_id} already owns blocks")
+        if not 0 <= n <= seq.num_cached_tokens:
+            raise ValueError(f"sequence {seq.seq_id} has {seq.num_cached_tokens} cached tokens, not {n}")
+        full, rest = divmod(n, self.block_size)
+        own = self._take(1 if rest else 0)
+        for b in seq.block_table[:full]:
+            self.ref_counts[b] += 1
+        child.block_table = seq.block_table[:full] + own
+        child.num_cached_tokens = n
+        if rest:
+            self._copy([seq.block_table[full]], own, [rest])
+
+    def compact(self, seqs: list[Sequence]) -> int:
+        """Move the blocks in use to the lowest ids, so that the pool's end is free; returns how many moved. ``seqs`` are all
+        sequences that own blocks; those of highest id go to the lowest free ids."""
+        used = {b for s in seqs for b in s.block_table}
+        if len(used) != self.num_used_blocks:
+            raise ValueError(f"{self.num_used_blocks} blocks are in use, {len(used)} of them by these sequences")
+        n = len(used)
+        src = sorted(b for b in used if b >= n)
+        dst = sorted(set(range(n)) - used)
+        self._copy(src, dst)
+        to = dict(zip(src, dst))
+        for a, b in to.items():
+            self.ref_counts[b], self.ref_counts[a] = self.ref_counts[a], 0
+        for s in seqs:
+            s.block_table = [to.get(b, b) for b in s.block_table]
+        self._free = list(range(self.num_blocks - 1, n - 1, -1))
+        return len(src)
+
+    def _copy(self, src: list[int], dst: list[int], num_slots: list[int] | None = None) -> None:
+        if not src:
+            return
+        if self.pool.is_cuda:
+            from tokquay_amd import ops
+
+            args = [None if v is None else torch.tensor(v, dtype=torch.int32, device=self.pool.device)
+                    for v in (src, dst, num_slots)]  # fmt: skip
+            ops.copy_blocks(self.pool, *args, d_error=self.error_word)
+            return
+        for i, (a, b) in enumerate(zip(src, dst)):
+            n = self.block_size if num_slots is None else num_slots[i]
+            self.pool[b, ..., :n, :] = self.pool[a, ..., :n, :]
+
     def _take(self, n: int) -> list[int]:
         if n > len(self._free):
             raise OutOfBlocksError(f"need {n} blocks, only {len(self._free)} free")
