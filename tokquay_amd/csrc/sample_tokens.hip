@@ -123,17 +123,82 @@ __global__ __launch_bounds__(kThreads) void sample_stats_kernel(const SampleArgs
   if (member < kPieces && group < a.groups) a.maxima[(int64_t)row * a.groups + group] = mine;
 }
 
+// Inclusive sums over the row's workgroup, in order, of 32- or 64-bit values. The waves' sums are added up in a row of 16 lanes, by every
+// wave. One barrier: calls that follow each other take turns with s_part (16 words each), and so does `first_of`.
+template <int CTRL, typename V>
+__device__ __forceinline__ V dpp_of(V v) {
+  if constexpr (sizeof(V) == 4)
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+  else
+    return __builtin_bit_cast(V, dpp_move64<CTRL>(__builtin_bit_cast(uint64_t, v)));
+}
+template <typename V>
+__device__ __forceinline__ V lane_value(V v, int lane) {
+  if constexpr (sizeof(V) == 4)
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  else
+    return __builtin_bit_cast(V, lane_of(__builtin_bit_cast(uint64_t, v), lane));
+}
+template <typename V>
+__device__ __forceinline__ V row_sums(V v) {  // inclusive, in rows of 16 lanes
+  v += dpp_of<0x111>(v);  // row_shr:1, 2, 4, 8
+  v += dpp_of<0x112>(v);
+  v += dpp_of<0x114>(v);
+  v += dpp_of<0x118>(v);
+  return v;
+}
+template <typename V>
+__device__ __forceinline__ V wave_sums(V v) {
+  const int lane = threadIdx.x & (kWave - 1);
+  v = row_sums(v);
+  V before = 0;
+#pragma unroll
+  for (int r = 1; r < kWave / 16; ++r) {
+    const V row = lane_value(v, 16 * r - 1);
+    before += lane >= 16 * r ? row : 0;
+  }
+  return v + before;
+}
+// all: the sum of all threads' values.
+template <typename V>
+__device__ __forceinline__ V sums(V v, uint64_t* s_part, V& all) {
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  v = wave_sums(v);
+  V* part = reinterpret_cast<V*>(s_part);
+  if (lane == kWave - 1) part[wave] = v;
+  __syncthreads();
+  static_assert(kPickWaves == 16, "the waves' sums in a row of lanes");
+  const V mine = part[lane & 15], upto = row_sums(mine);
+  all = lane_value(upto, 15);
+  return v + lane_value(upto - mine, wave);
+}
+// The first thread with `over`, or the last with `has` where there is none; -1: none either.
+__device__ __forceinline__ int first_of(bool over, bool has, uint64_t* s_part) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const uint64_t overs = __builtin_amdgcn_ballot_w64(over), those = __builtin_amdgcn_ballot_w64(has);
+  int* part = reinterpret_cast<int*>(s_part);
+  if (lane == 0) {
+    part[2 * wave] = overs != 0 ? wave * kWave + __builtin_ctzll(overs) : -1;
+    part[2 * wave + 1] = those != 0 ? wave * kWave + 63 - __builtin_clzll(those) : -1;
+  }
+  __syncthreads();
+  const int2 mine = reinterpret_cast<const int2*>(part)[lane & 15];
+  const uint64_t first = __builtin_amdgcn_ballot_w64(mine.x >= 0) & 0xffff, last = __builtin_amdgcn_ballot_w64(mine.y >= 0) & 0xffff;
+  if (first != 0) return __builtin_amdgcn_readlane(mine.x, __builtin_ctzll(first));
+  return last != 0 ? __builtin_amdgcn_readlane(mine.y, 63 - __builtin_clzll(last)) : -1;
+}
+
 struct PickShared {
   uint32_t n[kBins];
   uint64_t m[kBins];
-  uint64_t part[kPickWaves];
+  uint64_t part[2][kPickWaves];
   double sum[kPickWaves], goal;
   double round[kMaxRounds];
   alignas(16) uint32_t distance[kListed + 4], column[kListed];  // the columns that matter
   uint16_t group[kSelected];                                    // the groups that they lie in
   uint64_t before_n, before_m, bin_n;
   uint32_t member;
-  int found, pick[kPickWaves][2], last;
+  int found, last;
 };
 
 // What is gone through, four items in a row a thread, a round of all threads at a time: the maxima of the groups, the columns of the
@@ -155,6 +220,8 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
   const float* maxima = a.maxima + (int64_t)row * a.groups;
   const Stat* st = a.stats + (int64_t)row * a.chunks;
   const double u = (double)a.uniforms[row];
+  int turn = 0;
+  auto part = [&] { return sh.part[turn ^= 1]; };
 
   // The row's largest logit, each wave by itself.
   uint64_t best = 0;
@@ -275,13 +342,10 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
       const double t = ((double)key_value(st[tid].key) - t0) * c;
       if (t >= -1000.0) mine = st[tid].sum * exp2_neg(t);
     }
-    const double upto = scan<kPick>(mine, sh.sum);
-    if (tid == kPick - 1) sh.goal = upto;
-    __syncthreads();
-    total = sh.goal;
+    const double upto = sums(mine, part(), total);
     if (s.all()) {
       const double goal = u * total;
-      const int chosen = pick<kPick>(mine > 0.0 && upto > goal, mine > 0.0, sh.pick);
+      const int chosen = first_of(mine > 0.0 && upto > goal, mine > 0.0, part());
       if (tid == chosen) sh.goal = goal - (upto - mine);
       __syncthreads();
       rest = sh.goal;
@@ -323,7 +387,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
         const Source from = (Source)make;
         const int many = from == kMaxima ? a.groups : from == kGroups ? items * kGroup : a.vocab;
         const int room = from == kMaxima ? kSelected : kListed;
-        int count = 0, turn = 0;
+        int count = 0, side = 0;
         auto take = [&](int i0, auto& d) {
           constexpr int N = sizeof(d) / sizeof(d[0]);
           fetch_rounds(from, i0 + 4 * tid, many, d);
@@ -338,11 +402,11 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
               all += __builtin_popcountll(those);
               place[j] += __builtin_popcountll(those & ((1ull << lane) - 1));
             }
-            if (lane == 0) sh.n[turn * kWave + j * kPickWaves + wave] = all;
+            if (lane == 0) sh.n[side * kWave + j * kPickWaves + wave] = all;
           }
           static_assert(4 * kPickWaves == kWave, "a count a lane");
           __syncthreads();
-          const int mine = lane < N * kPickWaves ? sh.n[turn * kWave + lane] : 0;
+          const int mine = lane < N * kPickWaves ? sh.n[side * kWave + lane] : 0;
           int upto = mine;
           auto up = [&](auto ctrl) { return __builtin_amdgcn_update_dpp(0, upto, decltype(ctrl)::value, 0xF, 0xF, true); };
           upto += up(std::integral_constant<int, 0x111>());  // in rows of 16: row_shr:1, 2, 4, 8
@@ -369,7 +433,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
               }
             count += __builtin_amdgcn_readlane(upto, j * kPickWaves + kPickWaves - 1);
           }
-          turn ^= 1;
+          side ^= 1;
         };
         int i0 = 0;
         uint32_t one[1][4], four[4][4];
@@ -421,25 +485,30 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
 #pragma unroll 1
       for (; i0 < many; i0 += kRound) tally(i0, one);
       __syncthreads();
-      const uint64_t na = sh.n[2 * tid], nb = sh.n[2 * tid + 1], ma = sh.m[2 * tid], mb = sh.m[2 * tid + 1];
-      const uint64_t n = n0 + scan<kPick>(na + nb, sh.part), m = m0 + scan<kPick>(ma + mb, sh.part);
+      const uint32_t na = sh.n[2 * tid], nb = sh.n[2 * tid + 1];
+      uint32_t all_n;
+      const uint32_t n = (uint32_t)n0 + sums(na + nb, part(), all_n);
+      uint64_t ma = 0, mb = 0, m = 0, all_m = 0;
+      if (scout ? by_mass : weigh) {
+        ma = sh.m[2 * tid];
+        mb = sh.m[2 * tid + 1];
+        m = m0 + sums(ma + mb, part(), all_m);
+      }
       const double aim = scout && by_mass ? goal * slack : goal;
-      auto reaches = [&](uint64_t n, uint64_t m) { return (double)(by_mass ? m : n) >= aim; };
-      const uint64_t n1 = n - na - nb, m1 = m - ma - mb;  // before this thread's
+      auto reaches = [&](uint32_t n, uint64_t m) { return (by_mass ? (double)m : (double)n) >= aim; };
+      const uint32_t n1 = n - na - nb;  // before this thread's
+      const uint64_t m1 = m - ma - mb;
       if (reaches(n, m) && (tid == 0 || !reaches(n1, m1))) {
         const bool one = reaches(n1 + na, m1 + ma);
         sh.found = 2 * tid + (one ? 0 : 1);
         sh.before_n = one ? n1 : n1 + na;
         sh.before_m = one ? m1 : m1 + ma;
         sh.bin_n = one ? na : nb;
-      } else if (tid == kPick - 1 && !reaches(n, m)) {
-        sh.before_n = n;
-        sh.before_m = m;
       }
       __syncthreads();
       const int found = sh.found;
-      n0 = sh.before_n;
-      m0 = sh.before_m;
+      n0 = found < 0 ? n0 + all_n : sh.before_n;
+      m0 = found < 0 ? m0 + all_m : sh.before_m;
       const uint64_t there = sh.bin_n;
       __syncthreads();
       if (scout) {
@@ -529,17 +598,16 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
       if (tid < items) sh.m[rank] = fixed(w);
       __syncthreads();
       const int k = s.k > 0 ? s.k : items;
-      const uint64_t m = tid < min(k, items) ? sh.m[tid] : 0, upto = scan<kPick>(m, sh.part);
-      if (tid == kPick - 1) sh.before_m = upto;
-      __syncthreads();
-      const double edge = (s.p > 0.f ? (double)s.p : 0.0) * (s.k > 0 ? (double)sh.before_m : whole);
+      const uint64_t m = tid < min(k, items) ? sh.m[tid] : 0;
+      uint64_t all_m;
+      const uint64_t upto = sums(m, part(), all_m);
+      const double edge = (s.p > 0.f ? (double)s.p : 0.0) * (s.k > 0 ? (double)all_m : whole);
       sh.n[tid] = tid == 0 || (tid < k && (!s.nucleus() || (double)(upto - m) < edge));
       __syncthreads();
       const double kept = tid < items && sh.n[rank] != 0 && w >= (double)s.least ? w : 0.0;
-      const double cum = scan<kPick>(kept, sh.sum);
-      if (tid == kPick - 1) sh.goal = u * cum;
-      __syncthreads();
-      if (tid == pick<kPick>(kept > 0.0 && cum > sh.goal, kept > 0.0, sh.pick)) a.tokens[row] = sh.column[tid];
+      double all;
+      const double cum = sums(kept, part(), all);
+      if (tid == first_of(kept > 0.0 && cum > u * all, kept > 0.0, part())) a.tokens[row] = sh.column[tid];
       return;
     }
   }
@@ -553,21 +621,19 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
     for (int i0 = 0; i0 < items && before < ties; i0 += kRound) {
       uint32_t d[4];
       fetch(source, i0 + 4 * tid, items, d);
-      uint64_t mine = 0;
+      uint32_t mine = 0, all;
 #pragma unroll
       for (int e = 0; e < 4; ++e) mine += d[e] == cut;
-      const uint64_t upto = before + scan<kPick>(mine, sh.part);
+      const uint64_t upto = before + sums(mine, part(), all);
       if (upto >= ties && upto - mine < ties) {
         uint64_t left = ties - (upto - mine);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (d[e] == cut && left-- == 1) sh.last = column(source, i0 + 4 * tid + e);
       }
-      if (tid == kPick - 1) sh.before_n = upto;
-      __syncthreads();
-      before = sh.before_n;
-      __syncthreads();
+      before += all;
     }
+    __syncthreads();
     if (before >= ties) last = sh.last;
   }
 
@@ -600,23 +666,19 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
     __syncthreads();
     if (++r < rounds) continue;
     mine = tid < rounds ? sh.round[tid] : 0.0;
-    upto = scan<kPick>(mine, sh.sum);
-    if (tid == kPick - 1) sh.goal = upto;
-    __syncthreads();
-    const double goal = rest < 0.0 ? u * sh.goal : rest;
-    r = max(pick<kPick>(mine > 0.0 && upto > goal, mine > 0.0, sh.pick), 0);
+    double all;
+    upto = sums(mine, part(), all);
+    const double goal = rest < 0.0 ? u * all : rest;
+    r = max(first_of(mine > 0.0 && upto > goal, mine > 0.0, part()), 0);
     if (tid == r) sh.goal = goal - (upto - mine);
     __syncthreads();
     rest = sh.goal;
     found = true;
   }
-  upto = scan<kPick>(mine, sh.sum);
-  if (rest < 0.0) {
-    if (tid == kPick - 1) sh.goal = upto;
-    __syncthreads();
-    rest = u * sh.goal;
-  }
-  if (tid == pick<kPick>(mine > 0.0 && upto > rest, mine > 0.0, sh.pick)) {
+  double all;
+  upto = sums(mine, part(), all);
+  if (rest < 0.0) rest = u * all;
+  if (tid == first_of(mine > 0.0 && upto > rest, mine > 0.0, part())) {
     double cum = upto - mine;
     int at_item = -1;
     bool done = false;
