@@ -187,7 +187,37 @@ def test_settings_of_sequences():
     want = sampled(logits[2:17], u[2:17], t[owner], k[owner], p[owner], m[owner])
     assert torch.equal(got[2:17], want) and err == 0
     assert bool((got[:2] == -7).all()) and bool((got[17:] == -7).all())
+    fresh, err = run(logits, u, t, k, p, m, cu_seqlens_q=cu)
+    assert torch.equal(fresh[2:17], want) and err == 0
+    assert bool((fresh[:2] == -1).all()) and bool((fresh[17:] == -1).all())
 
+
+def test_many_sequences_and_empty_ones():
+    g = torch.Generator().manual_seed(30)
+    counts = torch.randint(0, 3, (500,), generator=g)
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]).int()
+    rows = int(cu[-1])
+    logits, u = normal(rows, 701, BF16, seed=30), torch.rand(rows, generator=g)
+    s = settings(500, USERS)
+    owner = torch.repeat_interleave(torch.arange(500), counts)
+    got, err = run(logits, u, *s, cu_seqlens_q=cu)
+    assert torch.equal(got, sampled(logits, u, *(x[owner] for x in s))) and err == 0
+
+
+def test_calls_on_two_streams_at_once():
+    a, b = peaked(60, 50257, seed=31), normal(60, 50257, BF16, seed=32)
+    u, s = torch.rand(60), settings(60, USERS)
+    want = [sampled(x, u, *s) for x in (a, b)]
+    x = [a.cuda(), b.cuda()]
+    args = [u.cuda(), *(v.cuda() for v in s)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.sample_tokens(x[i], *args))
+    torch.cuda.synchronize()
+    assert all(torch.equal(t.cpu(), want[i]) for i in range(2) for t in got[i])
 
 def test_settings_may_be_left_out():
     logits, u = peaked(12, 5003, seed=17), torch.rand(12)

@@ -149,7 +149,11 @@ __device__ __forceinline__ bool clean_values(uint16_t* s_v, int pieces) {
 __device__ __forceinline__ uint32_t seen_bits(const ChunkArgs& a, int64_t row, int start, int qpos, int from) {
   const uint32_t* m = a.masks + row * a.mask_words;
   const int rel = from - start, w = rel >> 5, own = qpos - from;
-  auto word = [&](int i) { return i < 0 ? ~0u : i < a.mask_words ? m[i] : 0u; };
+  const int words = (int)a.mask_words;
+  auto word = [&](int i) {  // no branches: the loads of all rows are on their way together
+    const uint32_t v = m[min(max(i, 0), words - 1)];
+    return i < 0 ? ~0u : i < words ? v : 0u;
+  };
   const uint32_t bits = __builtin_amdgcn_alignbit(word(w + 1), word(w), rel & 31);
   return own >= 31 ? bits : own < 0 ? 0u : bits & ((2u << own) - 1u);
 }

@@ -676,7 +676,9 @@ at::Tensor new_sample_tokens(const at::Tensor& logits, const at::Tensor& uniform
                              const c10::optional<at::Tensor>& top_k, const c10::optional<at::Tensor>& top_p,
                              const c10::optional<at::Tensor>& min_p, const c10::optional<at::Tensor>& cu_seqlens_q,
                              const c10::optional<at::Tensor>& d_error) {
-  at::Tensor tokens = fresh(logits, at::kLong, {uniforms.numel()});
+  // Rows of no sequence, which the call leaves alone, have -1.
+  at::Tensor tokens = cu_seqlens_q.has_value() ? at::full({uniforms.numel()}, -1, logits.options().dtype(at::kLong))
+                                               : fresh(logits, at::kLong, {uniforms.numel()});
   sample_tokens(tokens, logits, uniforms, temperature, top_k, top_p, min_p, cu_seqlens_q, d_error);
   return tokens;
 }

@@ -691,7 +691,7 @@ def sample_tokens(
     ``top_p`` (float32; 1: off), then ``min_p`` (float32, of the largest probability; 0: off). Equal logits rank by column, the lowest
     first, so exactly k are left. The draw is the lowest column whose running sum of what is left passes the uniform number's share.
     With ``cu_seqlens_q`` (``paged_chunk``'s) the settings have an entry a sequence, for all of its rows, and rows of no sequence keep
-    their token. Mask tokens with -inf logits."""
+    their token (-1 where ``tokens`` is left out). Mask tokens with -inf logits."""
     if tokens is None:
         return _checked_op("sample_tokens", logits, uniforms, temperature, top_k, top_p, min_p, cu_seqlens_q, d_error, form="new")
     _checked_op("sample_tokens", tokens, logits, uniforms, temperature, top_k, top_p, min_p, cu_seqlens_q, d_error)
