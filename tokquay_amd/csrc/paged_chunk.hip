@@ -34,6 +34,11 @@
 // card to card; a large bf16 library product reaches 1,370), with the matrix cores busy for 57 % of the time and the vector units
 // for 55. The longest sequence decides for all (plan_of): beside 259 tokens behind 32,500, three single tokens at 300 take 818 us
 // with them, where the two calls take 175 and 9.
+//
+// TREE (tq_paged_tree): the new tokens are nodes of a tree of drafts, and a row sees of them those that its mask names and that are not
+// behind itself, so a part of what it would see in a line: tiles, parts and maxima are those of a line, and tiles with new keys are
+// masked by bits. A row that sees nothing has a sum of zero, and gets zeros. 64 trees of 64 nodes behind 511-4,094 tokens, 32 / 8
+// heads of 128: 0.62 GB and 155 GFLOP in 202 us (as a line 196), matrix cores busy for 46 % of the time and vector units for 47.
 #include <float.h>
 
 #include <utility>

@@ -27,7 +27,8 @@ struct LayoutArgs {
 // One workgroup a sequence, a wave 64 of its nodes. Inside these the ancestors are joined in six steps, each over twice as many links as
 // the one before, by all waves at once; what lies above comes, wave after wave, from the mask of the one node further up that the links
 // lead to, which LDS holds (of trees of more than kLayoutNodes nodes: the masks themselves). The last workgroup clears the rows of no
-// sequence. Bound by its latency: the loads of lengths and parents, and the stores.
+// sequence. Bound by its latency: the loads of lengths and parents, and the stores (one tree of 26 nodes 1.9 us, 128 of 65-256 nodes 5.3;
+// with one wave a sequence, 64 nodes after the other, 8.5).
 constexpr int kLayoutWaves = 8, kLayoutNodes = kWave * kLayoutWaves;
 
 __global__ __launch_bounds__(kLayoutNodes) void tree_layout_kernel(const LayoutArgs a) {
@@ -134,7 +135,8 @@ struct AcceptArgs {
 
 // A workgroup takes 256 16-byte pieces of the slots of one sequence. Each of its waves walks the tree by itself; a piece's
 // moves are all made by one thread, and a node's place on the path is never behind the node, so moving the path in order from the top
-// reads every source before it is written over.
+// reads every source before it is written over. Bound by its latency too: lengths, nodes, tables, rows (one tree in a pool of 12 layers
+// 4.2 us, 64 in one of 16 layers 5.8; with each node of the path looked up in memory 5.3 and 7.3).
 __global__ __launch_bounds__(kMoveThreads) void accept_tree_kernel(const AcceptArgs a) {
   const int lane = threadIdx.x & (kWave - 1);
   const int slice = blockIdx.x % a.slices, b = blockIdx.x / a.slices;
