@@ -7,6 +7,7 @@ import random
 import pytest
 import torch
 
+from tokquay_amd import kv_cache
 from tokquay_amd.generate import paged_forward
 from tokquay_amd.kv_cache import BlockAllocator
 from tokquay_amd.model import GPT2, GPT2Config
@@ -84,4 +85,19 @@ def test_a_compacted_cache_goes_on(model):
     alloc.pool[alloc.num_used_blocks :] = float("nan")
     got = paged_forward(model, alloc, live)
     assert torch.isfinite(got).all() and torch.equal(got, want)
+    alloc.check_device_errors()
+
+
+def test_many_blocks_are_moved_by_several_calls(monkeypatch):
+    monkeypatch.setattr(kv_cache, "COPY_PAIRS", 3)
+    alloc = BlockAllocator(GPT2Config(n_layer=1, n_embd=64, n_head=1), 24, 4, device="cuda")
+    alloc.pool.copy_(torch.randn(alloc.pool.shape, generator=torch.Generator().manual_seed(3)))
+    first, second = Sequence(0, [0] * 48), Sequence(1, [0] * 41)
+    for s in (first, second):
+        alloc.allocate(s)
+        s.num_cached_tokens = len(s.token_ids)
+    want = alloc.pool[second.block_table].clone()
+    alloc.free(first)
+    assert alloc.compact([second]) == 11 and sorted(second.block_table) == list(range(11))
+    assert torch.equal(alloc.pool[second.block_table], want)
     alloc.check_device_errors()

@@ -239,6 +239,15 @@ def copy_call(pool=P, nb=8, layers=2, kv=2, bs=16, d=64, dtype=2, src=P, dst=P, 
     return _lib.lib().tq_copy_blocks(pool, nb, layers, kv, bs, d, dtype, src, dst, slots, pairs, None, None)
 
 
+def test_copy_blocks_takes_at_most_2_20_pairs():
+    assert copy_call(pairs=(1 << 20) + 1) == UNSUPPORTED and copy_call(pairs=2**31 - 1) == UNSUPPORTED
+    with FakeTensorMode():
+        ids = empty((1 << 20) + 1, dtype=I32)
+        with pytest.raises(ValueError, match="more than 1048576"):
+            ops.copy_blocks(copy_args()["pool"], ids, ids)
+        ops.copy_blocks(copy_args()["pool"], ids[1:], ids[1:])
+
+
 @pytest.mark.parametrize("status,more", [
     (INVALID, dict(pairs=-1)), (INVALID, dict(nb=0)), (INVALID, dict(nb=1 << 31)), (INVALID, dict(layers=0)), (INVALID, dict(kv=0)),
     (INVALID, dict(bs=0)), (OK, dict(pairs=0)), (INVALID, dict(pool=None)), (INVALID, dict(src=None)), (INVALID, dict(dst=None)),

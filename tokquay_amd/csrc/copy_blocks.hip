@@ -16,6 +16,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kPer = 2;  // pieces of a thread at a time
+// Every workgroup goes through all pairs: the square of this takes about a second, that of a hundred times as many would seem to hang.
+constexpr int kMaxPairs = 1 << 20;
 
 struct CopyArgs {
   char* pool;
@@ -98,6 +100,7 @@ extern "C" tq_status tq_copy_blocks(void* pool, int64_t num_blocks, int32_t num_
       (dtype != TQ_F32 && dtype != TQ_F16 && dtype != TQ_BF16))
     return TQ_ERR_UNSUPPORTED;
   if (num_pairs == 0) return TQ_OK;
+  if (num_pairs > kMaxPairs) return TQ_ERR_UNSUPPORTED;
   if (pool == nullptr || src_blocks == nullptr || dst_blocks == nullptr || (uintptr_t)pool % 16 != 0)
     return TQ_ERR_INVALID_ARGUMENT;
   const int64_t slot = (int64_t)head_dim * (dtype == TQ_F32 ? 4 : 2), slabs = 2LL * num_layers * num_kv_heads;
@@ -111,7 +114,7 @@ extern "C" tq_status tq_copy_blocks(void* pool, int64_t num_blocks, int32_t num_
   a.block_bytes = slabs * a.slab_bytes;
   a.turns = (num_pairs + kThreads - 1) / kThreads;
   const int64_t turn = (int64_t)kThreads * kPer * a.turns, slices = (a.block_bytes / 16 + turn - 1) / turn;
-  if (a.block_bytes / 16 > 0x7fffffffLL || turn > 0x40000000LL || slices * num_pairs > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
+  if (a.block_bytes / 16 > 0x7fffffffLL || slices * num_pairs > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
   a.slot_pieces = (int32_t)(slot / 16);
   a.slabs = (int32_t)slabs;
   a.num_blocks = (int32_t)num_blocks;

@@ -703,6 +703,7 @@ void copy_blocks(at::Tensor pool, const at::Tensor& src_blocks, const at::Tensor
   slots_of(op, pool);
   exactly(op, "src_blocks", src_blocks, at::kInt, -1, p.device);
   const int64_t n = src_blocks.numel();
+  TORCH_CHECK(n <= 1 << 20, op, ": src_blocks has more than 1048576 entries");
   exactly(op, "dst_blocks", dst_blocks, at::kInt, n, p.device);
   if (num_slots.has_value()) exactly(op, "num_slots", *num_slots, at::kInt, n, p.device);
   if (d_error.has_value()) exactly(op, "d_error", *d_error, at::kInt, 1, p.device);

@@ -32,6 +32,8 @@ if TYPE_CHECKING:
     from tokquay_amd.model import GPT2Config
 
 HEAD_DIM = 64
+# Blocks copied by a call: each is held against all others, so the time of very many grows with their square.
+COPY_PAIRS = 1 << 16
 
 
 def cdiv(a: int, b: int) -> int:
@@ -157,9 +159,10 @@ class BlockAllocator:
         if self.pool.is_cuda:
             from tokquay_amd import ops
 
-            args = [None if v is None else torch.tensor(v, dtype=torch.int32, device=self.pool.device)
-                    for v in (src, dst, num_slots)]  # fmt: skip
-            ops.copy_blocks(self.pool, *args, d_error=self.error_word)
+            for i in range(0, len(src), COPY_PAIRS):
+                args = [None if v is None else torch.tensor(v[i : i + COPY_PAIRS], dtype=torch.int32, device=self.pool.device)
+                        for v in (src, dst, num_slots)]  # fmt: skip
+                ops.copy_blocks(self.pool, *args, d_error=self.error_word)
             return
         for i, (a, b) in enumerate(zip(src, dst)):
             n = self.block_size if num_slots is None else num_slots[i]

@@ -743,7 +743,8 @@ def copy_blocks(pool: torch.Tensor, src_blocks: torch.Tensor, dst_blocks: torch.
                 d_error: torch.Tensor | None = None) -> None:
     """Copies the first ``num_slots[p]`` slots (default: all) of block ``src_blocks[p]`` of ``pool`` (float32, float16 or bfloat16) to block
     ``dst_blocks[p]``, all layers, keys and values, for every pair p (int32 ``[P]``; a negative id: no copy). The copies run beside each other:
-    a pair that writes to a block which another reads, or which an earlier one writes to, is flagged and left out."""
+    a pair that writes to a block which another reads, or which an earlier one writes to, is flagged and left out. Each is held against
+    all others, so a call takes at most 2**20 pairs."""
     _checked_op("copy_blocks", pool, src_blocks, dst_blocks, num_slots, d_error)
 
 

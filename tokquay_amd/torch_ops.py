@@ -522,6 +522,8 @@ def _fake_copy_blocks(pool, src_blocks, dst_blocks, num_slots, d_error):
     _slots_of(op, pool)
     _exactly(op, "src_blocks", src_blocks, torch.int32, -1, pool.device)
     n = src_blocks.numel()
+    if n > 1 << 20:
+        _fail(op, "src_blocks has more than 1048576 entries")
     _exactly(op, "dst_blocks", dst_blocks, torch.int32, n, pool.device)
     if num_slots is not None:
         _exactly(op, "num_slots", num_slots, torch.int32, n, pool.device)
