@@ -16,7 +16,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kPer = 2;  // pieces of a thread at a time
-// Every workgroup goes through all pairs: the square of this takes about a second, that of a hundred times as many would seem to hang.
+// Every workgroup goes through all pairs (of 256 bytes: 4,096 28 us, 65,536 4.1 ms, 262,144 63): these take about a second, a hundred times
+// as many hours.
 constexpr int kMaxPairs = 1 << 20;
 
 struct CopyArgs {

@@ -32,8 +32,9 @@ if TYPE_CHECKING:
     from tokquay_amd.model import GPT2Config
 
 HEAD_DIM = 64
-# Blocks copied by a call: each is held against all others, so the time of very many grows with their square.
-COPY_PAIRS = 1 << 16
+# Blocks copied by a call: each is held against all others, so the time of very many grows with their square (of the smallest
+# blocks 4,096 28 us, 16,384 292, 65,536 4,100).
+COPY_PAIRS = 1 << 12
 
 
 def cdiv(a: int, b: int) -> int:
