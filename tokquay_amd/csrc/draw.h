@@ -178,7 +178,7 @@ __device__ __forceinline__ void chunk_stat(const float (&x)[PER], float temp, bo
       const int at = column_of<kVec<T>, N, PER, false>(i);
       if (at < n && (top != top ? x[i] != x[i] : x[i] == top)) mine = at;
     }
-    atomicMin(&sh.col, mine);
+    if (mine != 0x7fffffff) atomicMin(&sh.col, mine);  // one lane of the workgroup, if no others hold the maximum
     if (lane == 0) sh.sum[wave] = 0.0;
   }
   __syncthreads();
