@@ -268,15 +268,8 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
   auto column = [&](Source from, int i) {
     return from == kList ? (int)sh.column[i] : from == kGroups ? sh.group[i / kGroup] * kGroup + i % kGroup : first + i;
   };
-  // The distances of items i .. i + 3 of `many`.
-  auto fetch = [&](Source from, int i, int many, uint32_t (&d)[4]) {
-    if (from == kList) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(&sh.distance[min(i, kListed)]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) d[e] = i + e < many ? v[e] : kNone;
-      return;
-    }
-    float x[4];
+  // Items i .. i + 3 of `many`, NaN past them: no other item is. Not of kList.
+  auto load = [&](Source from, int i, int many, float (&x)[4]) {
     const bool wide = __is_same(T, float) || from == kMaxima;
     int j = i, end = many;  // places in the array
     if (from == kGroups) {
@@ -301,19 +294,17 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = j + e < end ? wide ? reinterpret_cast<const float*>(p)[j + e] : logit_at<T>(p, j + e) : 0.f;
+      for (int e = 0; e < 4; ++e)
+        x[e] = j + e < end ? wide ? reinterpret_cast<const float*>(p)[j + e] : logit_at<T>(p, j + e) : __builtin_nanf("");
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) d[e] = j + e < end ? distance_of(x[e]) : kNone;
   };
 
-  // The same of N rounds, whose loads are on their way together.
-  auto fetch_rounds = [&](Source from, int i0, int many, auto& d) {
-    constexpr int N = sizeof(d) / sizeof(d[0]);
+  // The same of N rounds, whose loads are on their way together: of columns, where N > 1.
+  auto load_rounds = [&](Source from, int i0, int many, auto& x) {
+    constexpr int N = sizeof(x) / sizeof(x[0]);
     typedef typename std::conditional<__is_same(T, float), u32x4, u32x2>::type Raw;
-    if (N == 1 || from == kMaxima || from == kList) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) fetch(from, i0 + j * kRound, many, d[j]);
+    if constexpr (N == 1) {
+      load(from, i0, many, x[0]);
       return;
     }
     Raw v[N];
@@ -331,14 +322,31 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if constexpr (__is_same(T, float))
-            d[j][e] = distance_of(__uint_as_float(v[j][e]));
+            x[j][e] = __uint_as_float(v[j][e]);
           else
-            d[j][e] = distance_of(T::load((uint16_t)(v[j][e / 2] >> (16 * (e & 1)))));
+            x[j][e] = T::load((uint16_t)(v[j][e / 2] >> (16 * (e & 1))));
         }
       } else {
-        fetch(from, i0 + j * kRound, many, d[j]);
+        load(from, i0 + j * kRound, many, x[j]);
       }
     }
+  };
+
+  // Their distances; kNone past the last.
+  auto fetch = [&](Source from, int i, int many, auto& d) {
+    constexpr int N = sizeof(d) / sizeof(d[0]);
+    if (N == 1 && from == kList) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(&sh.distance[min(i, kListed)]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[0][e] = i + e < many ? v[e] : kNone;
+      return;
+    }
+    float x[N][4];
+    load_rounds(from, i, many, x);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[j][e] = x[j][e] == x[j][e] ? distance_of(x[j][e]) : kNone;
   };
 
   // The sum of the row's weights, and for draws from all of them the chunk that the token falls in.
@@ -395,9 +403,12 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
         const int many = from == kMaxima ? a.groups : from == kGroups ? items * kGroup : a.vocab;
         const int room = from == kMaxima ? kSelected : kListed;
         int count = 0, side = 0;
-        auto take = [&](int i0, auto& d) {
-          constexpr int N = sizeof(d) / sizeof(d[0]);
-          fetch_rounds(from, i0 + 4 * tid, many, d);
+        // The least value up to the limit (past the last key: -inf).
+        float low = limit <= key ? key_value((uint64_t)(key - limit) << 32) : -INFINITY;
+        low = low == low ? low : -INFINITY;
+        auto take = [&](int i0, auto& x) {
+          constexpr int N = sizeof(x) / sizeof(x[0]);
+          load_rounds(from, i0 + 4 * tid, many, x);
           int place[N];
 #pragma unroll
           for (int j = 0; j < N; ++j) {
@@ -405,9 +416,9 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
             place[j] = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint64_t those = __builtin_amdgcn_ballot_w64(d[j][e] <= limit);
+              const uint64_t those = __builtin_amdgcn_ballot_w64(x[j][e] >= low);
               all += __builtin_popcountll(those);
-              place[j] += __builtin_popcountll(those & ((1ull << lane) - 1));
+              place[j] = __builtin_amdgcn_mbcnt_hi((uint32_t)(those >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)those, place[j]));
             }
             if (lane == 0) sh.n[side * kWave + j * kPickWaves + wave] = all;
           }
@@ -426,13 +437,13 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
             int to = count + place[j] + __builtin_amdgcn_readlane(upto - mine, j * kPickWaves + wave);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (d[j][e] <= limit) {
+              if (x[j][e] >= low) {
                 const int i = i0 + j * kRound + 4 * tid + e;
                 if (to < room) {
                   if (from == kMaxima) {
                     sh.group[to] = (uint16_t)i;
                   } else {
-                    sh.distance[to] = d[j][e];
+                    sh.distance[to] = distance_of(x[j][e]);
                     sh.column[to] = column(from, i);
                   }
                 }
@@ -443,9 +454,9 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
           side ^= 1;
         };
         int i0 = 0;
-        uint32_t one[1][4], four[4][4];
+        float one[1][4], four[4][4];
 #pragma unroll 1
-        for (; i0 + 2 * kRound < many && count <= room; i0 += 4 * kRound) take(i0, four);
+        for (; from != kMaxima && i0 + 2 * kRound < many && count <= room; i0 += 4 * kRound) take(i0, four);
 #pragma unroll 1
         for (; i0 < many && count <= room; i0 += kRound) take(i0, one);
         __syncthreads();
@@ -470,7 +481,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
       const bool scout = from == kColumns && !scouted;
       auto tally = [&](int i0, auto& d) {
         constexpr int N = sizeof(d) / sizeof(d[0]);
-        fetch_rounds(from, i0 + 4 * tid, many, d);
+        fetch(from, i0 + 4 * tid, many, d);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
 #pragma unroll
@@ -553,11 +564,11 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
       // The interval holds one value.
 #pragma unroll 1
       for (int i = 4 * tid; i < many; i += kRound) {
-        uint32_t d[4];
+        uint32_t d[1][4];
         fetch(from, i, many, d);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (d[e] >= lo && d[e] <= hi) sh.member = d[e];
+          if (d[0][e] >= lo && d[0][e] <= hi) sh.member = d[0][e];
       }
       __syncthreads();
       const uint32_t value = sh.member;
@@ -626,17 +637,17 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
     uint64_t before = 0;
 #pragma unroll 1
     for (int i0 = 0; i0 < items && before < ties; i0 += kRound) {
-      uint32_t d[4];
+      uint32_t d[1][4];
       fetch(source, i0 + 4 * tid, items, d);
       uint32_t mine = 0, all;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mine += d[e] == cut;
+      for (int e = 0; e < 4; ++e) mine += d[0][e] == cut;
       const uint64_t upto = before + sums(mine, part(), all);
       if (upto >= ties && upto - mine < ties) {
         uint64_t left = ties - (upto - mine);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (d[e] == cut && left-- == 1) sh.last = column(source, i0 + 4 * tid + e);
+          if (d[0][e] == cut && left-- == 1) sh.last = column(source, i0 + 4 * tid + e);
       }
       before += all;
     }
@@ -651,13 +662,13 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
 #pragma unroll 1
   for (;;) {
     const int i = r * kRound + 4 * tid;
-    uint32_t d[4];
+    uint32_t d[1][4];
     fetch(source, i, items, d);
     mine = 0.0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       w[e] = 0.0;
-      if (d[e] < cut || (d[e] == cut && column(source, min(i + e, items - 1)) <= last)) w[e] = weight(d[e]);
+      if (d[0][e] < cut || (d[0][e] == cut && column(source, min(i + e, items - 1)) <= last)) w[e] = weight(d[0][e]);
       w[e] = w[e] >= (double)s.least ? w[e] : 0.0;
       mine += w[e];
     }
