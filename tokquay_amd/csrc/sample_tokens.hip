@@ -18,10 +18,10 @@
 //    the least of them bounds top-p. Of the groups above the bound, a few more than k, the columns above it are listed in LDS. Where
 //    there is no bound (top-p of a flat row), the row is read again to find one.
 //
-// 1 is bound by HBM (256 rows of 128,000 fp32 logits 25 us, 5.2 TB/s, of which the sums of exponentials, where all rows need them,
-// make 31), 2 by its dependent steps of 1-3 us: one row of 50,257 with top-k 50 and top-p 11.5 us, from the temperature alone 5.7, with top-k
-// 1,000 24; 256 rows of 128,000 with settings of all kinds 25. Read and ranked by one workgroup a row in passes over all of its columns, one row
-// took 103 us and the 256 273. Top-p 0.9 of 256 x 128,000 normal logits, some 5,700 columns each, takes 100.
+// 1 is bound by HBM (256 rows of 128,000 fp32 logits 23 us, 5.6 TB/s, of which the sums of exponentials, where all rows need them,
+// make 31), 2 by its dependent steps of 1-3 us: one row of 50,257 with top-k 50 and top-p 11 us, from the temperature alone 5.6, with top-k
+// 1,000 23; 256 rows of 128,000 with settings of all kinds 24. Read and ranked by one workgroup a row in passes over all of its columns, one row
+// took 103 us and the 256 273. Top-p 0.9 of 256 x 128,000 normal logits, some 5,700 columns each, takes 96.
 #include "draw.h"
 
 namespace tq {
