@@ -178,7 +178,9 @@ __device__ __forceinline__ void chunk_stat(const float (&x)[PER], float temp, bo
       const int at = column_of<kVec<T>, N, PER, false>(i);
       if (at < n && (top != top ? x[i] != x[i] : x[i] == top)) mine = at;
     }
-    if (mine != 0x7fffffff) atomicMin(&sh.col, mine);  // one lane of the workgroup, if no others hold the maximum
+    // One lane of the workgroup, if no others hold the maximum (the atomics of all lanes go one by one: 64 greedy rows of 50,257 bf16
+    // logits 9.0 us instead of 4.6).
+    if (mine != 0x7fffffff) atomicMin(&sh.col, mine);
     if (lane == 0) sh.sum[wave] = 0.0;
   }
   __syncthreads();
