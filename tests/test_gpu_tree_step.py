@@ -87,3 +87,68 @@ def test_steps_of_drafted_trees(dtype, dim):
             c.tables = tables.cpu()
             start[2], last[2] = start[0], last[0]
     assert emitted >= 16
+
+
+def test_a_captured_step_is_replayed_on_other_trees():
+    """The whole step in one graph: other trees, lengths, starts and settings from replay to replay, rows behind the last sequence."""
+    heads, kv_heads, dim, bs, vocab, rows, max_new, max_context, layer = 8, 2, 64, 16, 5003, 96, 40, 2100, 1
+    gen = torch.Generator().manual_seed(5)
+    c = Tree([(s, grown(40, 1)) for s in (2060, 100, 700)], heads, kv_heads, dim, torch.bfloat16, bs, seed=6)
+    tables, table = c.tables.cuda(), ops.rope_table(4096, dim).cuda()
+    buffers = dict(parents=torch.zeros(rows, dtype=torch.int32), cu=torch.zeros(4, dtype=torch.int32),
+                   start=torch.zeros(3, dtype=torch.int32), slots=torch.full((rows,), -1), drafts=torch.zeros(rows, dtype=torch.int64),
+                   q=torch.zeros(rows, heads * dim, dtype=torch.bfloat16), k=torch.zeros(rows, kv_heads * dim, dtype=torch.bfloat16),
+                   v=torch.zeros(rows, kv_heads * dim, dtype=torch.bfloat16), logits=torch.zeros(rows, vocab), uniforms=torch.zeros(rows),
+                   temperature=torch.ones(3), top_k=torch.zeros(3, dtype=torch.int32), top_p=torch.ones(3), min_p=torch.zeros(3),
+                   pool=c.pool)  # fmt: skip
+    buffers = {name: x.cuda() for name, x in buffers.items()}
+    error = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def step(parents, cu, start, slots, drafts, q, k, v, logits, uniforms, temperature, top_k, top_p, min_p, pool):
+        positions, masks = ops.tree_layout(parents, cu, start, max_new, error)
+        q_out, out = torch.zeros(rows, heads, dim, dtype=q.dtype, device="cuda"), torch.zeros(rows, heads, dim, dtype=q.dtype, device="cuda")
+        ops.rope_cache_write(q_out, q, k, v, pool, layer, slots, positions, table, d_error=error)
+        ops.paged_tree(out, q_out, pool, layer, tables, cu, start, masks, max_new, max_context, d_error=error)
+        tokens = ops.sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p, cu, error)
+        return positions, masks, out, tokens, *ops.accept_tree(tokens, drafts, parents, cu, 12, pool, tables, start, error)
+
+    def refill(turn):
+        sizes, start = ([26, 1, 33], [40, 7, 40], [1, 1, 1], [0, 40, 13])[turn], ([2060, 33, 600], [0, 100, 700], [5, 0, 1], [7, 90, 650])[turn]
+        cu = [0, sizes[0], sizes[0] + sizes[1], sum(sizes)]
+        trees = [grown(n, 7 * turn + b) if n else [] for b, n in enumerate(sizes)]
+        slots, logits, drafts = torch.full((rows,), -1), torch.randn(rows, vocab, generator=gen) * 3, torch.randint(0, vocab, (rows,), generator=gen)
+        for b in range(3):
+            at = start[b] + torch.arange(sizes[b])
+            slots[cu[b] : cu[b + 1]] = c.tables[b, at // bs].long() * bs + at % bs
+            for i in range(1, sizes[b]):  # greedy rows take the path of first children
+                logits[cu[b] + trees[b][i], drafts[cu[b] + i]] = 40.0 - i / 4
+        new = dict(parents=torch.tensor(sum(trees, []) + [-1] * (rows - sum(sizes))), cu=torch.tensor(cu), start=torch.tensor(start),
+                   slots=slots, drafts=drafts, logits=logits, uniforms=torch.rand(rows, generator=gen), temperature=torch.tensor([0.0, 0.7, 1.0]),
+                   top_k=torch.tensor([0, 50, 0]), top_p=torch.tensor([1.0, 0.9, 0.8]), min_p=torch.tensor([0.0, 0.01, 0.0]),
+                   pool=c.pool)  # fmt: skip
+        for name in ("q", "k", "v"):
+            new[name] = torch.randn(buffers[name].shape, generator=gen)
+        for name, x in new.items():
+            buffers[name].copy_(x)
+        return sum(sizes)
+
+    refill(0)
+    step(**buffers)  # libraries and allocations are there before the capture
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(**buffers)
+    accepts = 0
+    for turn in range(4):
+        n = refill(turn)
+        pool = buffers["pool"].clone()
+        want = step(**{**buffers, "pool": pool})
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, expected in zip(captured, want):
+            assert torch.equal(got, expected)
+        assert torch.equal(buffers["pool"], pool)
+        positions, masks, out, tokens, _, _, counts = captured
+        assert not positions[n:].any() and not masks[n:].any() and not out[n:].any() and (tokens[n:] == -1).all()
+        accepts += int(counts.sum())
+    assert accepts > 12 and not error.item()
