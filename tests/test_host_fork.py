@@ -106,3 +106,45 @@ def test_compact():
     for s in seqs + [more]:
         a.free(s)
     assert a.num_free_blocks == 40 and a.compact([]) == 0
+
+
+def shared(cuts):
+    """An allocator, a sequence behind freed blocks, and forks of it at the given cuts."""
+    a = allocator(num_blocks=16)
+    first, s = sequence(a, 0, 8), sequence(a, 1, 8)
+    children = []
+    for i, n in enumerate(cuts):
+        children.append(Sequence(2 + i, [0] * 8))
+        a.fork(s, children[-1], n)
+    a.free(first)
+    return a, s, children
+
+
+@pytest.mark.parametrize("cuts", [[8], [4], [8, 8], [8, 4, 8]])
+def test_compact_refuses_owners_left_out(cuts):
+    # All blocks of a fork that was cut between two blocks belong to its parent too: without it no block is missing.
+    a, s, children = shared(cuts)
+    everyone = [s, *children]
+    before = a.pool.clone(), [list(q.block_table) for q in everyone], list(a.ref_counts), list(a._free)
+    for left_out in range(len(everyone)):
+        given = everyone[:left_out] + everyone[left_out + 1 :]
+        with pytest.raises(ValueError, match="in use"):
+            a.compact(given)
+        with pytest.raises(ValueError, match="in use"):  # one that is named twice does not stand for the other
+            a.compact(given + given[:1])
+    assert torch.equal(a.pool, before[0]) and [q.block_table for q in everyone] == before[1]
+    assert a.ref_counts == before[2] and a._free == before[3]
+    contents = [cached(a, q) for q in everyone]
+    assert a.compact(everyone + [s]) == 2
+    assert all(torch.equal(cached(a, q), x) for q, x in zip(everyone, contents))
+    for q in everyone:
+        a.free(q)
+    assert a.num_free_blocks == 16 and not any(a.ref_counts)
+
+
+def test_compact_refuses_blocks_that_are_free():
+    a, s, _ = shared([])
+    stale = Sequence(9, [0])
+    stale.block_table = [15]
+    with pytest.raises(ValueError, match="in use"):
+        a.compact([s, stale])

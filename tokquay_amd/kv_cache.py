@@ -21,6 +21,7 @@ attention straight off the pool, in place.
 from __future__ import annotations
 
 import math
+from collections import Counter
 from typing import TYPE_CHECKING
 
 import torch
@@ -138,10 +139,15 @@ class BlockAllocator:
 
     def compact(self, seqs: list[Sequence]) -> int:
         """Move the blocks in use to the lowest ids, so that the pool's end is free; returns how many moved. ``seqs`` are all
-        sequences that own blocks; those of highest id go to the lowest free ids."""
-        used = {b for s in seqs for b in s.block_table}
-        if len(used) != self.num_used_blocks:
-            raise ValueError(f"{self.num_used_blocks} blocks are in use, {len(used)} of them by these sequences")
+        sequences that own blocks, forks among them; those of highest id go to the lowest free ids."""
+        seqs = list({id(s): s for s in seqs}.values())
+        # Owner by owner: of blocks that are shared, the ids alone do not tell whether one is left out.
+        owners = Counter(b for s in seqs for b in s.block_table)
+        counts = Counter({b: count for b, count in enumerate(self.ref_counts) if count})
+        if owners != counts:
+            raise ValueError(f"{len(counts)} blocks are in use, by {counts.total()} entries of tables; these sequences have "
+                             f"{len(owners)}, by {owners.total()}")  # fmt: skip
+        used = set(owners)
         n = len(used)
         src = sorted(b for b in used if b >= n)
         dst = sorted(set(range(n)) - used)
