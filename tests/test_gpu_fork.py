@@ -101,3 +101,17 @@ def test_many_blocks_are_moved_by_several_calls(monkeypatch):
     assert alloc.compact([second]) == 11 and sorted(second.block_table) == list(range(11))
     assert torch.equal(alloc.pool[second.block_table], want)
     alloc.check_device_errors()
+
+
+def test_a_fork_that_the_copy_refuses_changes_nothing():
+    # Heads of 32: blocks of such a pool are shared, but not copied.
+    alloc = BlockAllocator(GPT2Config(n_layer=1, n_embd=32, n_head=1), 8, 4, device="cuda")
+    seq, child = Sequence(0, [0] * 10), Sequence(1, [0] * 10)
+    alloc.allocate(seq)
+    seq.num_cached_tokens = 10
+    before = list(alloc.ref_counts), list(alloc._free)
+    with pytest.raises(ValueError, match="copy_blocks"):
+        alloc.fork(seq, child)
+    assert child.block_table == [] and child.num_cached_tokens == 0 and (alloc.ref_counts, alloc._free) == before
+    alloc.fork(seq, child, 8)
+    assert child.block_table == seq.block_table[:2] and child.num_cached_tokens == 8

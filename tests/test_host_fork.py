@@ -148,3 +148,18 @@ def test_compact_refuses_blocks_that_are_free():
     stale.block_table = [15]
     with pytest.raises(ValueError, match="in use"):
         a.compact([s, stale])
+
+
+def test_a_fork_whose_copy_is_refused_changes_nothing(monkeypatch):
+    a = allocator()
+    s, child = sequence(a, 0, 10), Sequence(1, [0] * 10)
+    before = list(a.ref_counts), list(a._free), list(s.block_table)
+
+    def refuse(*args):
+        raise ValueError("copy_blocks: pool has another head size")
+
+    monkeypatch.setattr(a, "_copy", refuse)
+    with pytest.raises(ValueError, match="another head size"):
+        a.fork(s, child)
+    assert child.block_table == [] and child.num_cached_tokens == 0
+    assert (list(a.ref_counts), list(a._free), list(s.block_table)) == before

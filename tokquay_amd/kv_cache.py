@@ -130,12 +130,17 @@ class BlockAllocator:
             raise ValueError(f"sequence {seq.seq_id} has {seq.num_cached_tokens} cached tokens, not {n}")
         full, rest = divmod(n, self.block_size)
         own = self._take(1 if rest else 0)
+        if rest:
+            try:
+                self._copy([seq.block_table[full]], own, [rest])
+            except BaseException:  # a pool that the copy refuses: nothing has changed
+                self.ref_counts[own[0]] = 0
+                self._free.append(own[0])
+                raise
         for b in seq.block_table[:full]:
             self.ref_counts[b] += 1
         child.block_table = seq.block_table[:full] + own
         child.num_cached_tokens = n
-        if rest:
-            self._copy([seq.block_table[full]], own, [rest])
 
     def compact(self, seqs: list[Sequence]) -> int:
         """Move the blocks in use to the lowest ids, so that the pool's end is free; returns how many moved. ``seqs`` are all
