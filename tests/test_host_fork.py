@@ -9,6 +9,7 @@ import torch
 
 from tokquay_amd.kv_cache import BlockAllocator, OutOfBlocksError
 from tokquay_amd.model import GPT2Config
+from tokquay_amd.scheduler import RequestRejected, Scheduler, SchedulerConfig
 from tokquay_amd.sequence import Sequence
 
 TINY = GPT2Config(vocab_size=8, n_positions=64, n_embd=4, n_layer=2, n_head=1)
@@ -163,3 +164,23 @@ def test_a_fork_whose_copy_is_refused_changes_nothing(monkeypatch):
         a.fork(s, child)
     assert child.block_table == [] and child.num_cached_tokens == 0
     assert (list(a.ref_counts), list(a._free), list(s.block_table)) == before
+
+
+def test_the_scheduler_refuses_sequences_that_own_blocks():
+    # A queued sequence has none: it gets blocks for all of its tokens when it is admitted.
+    a = allocator()
+    s, child = sequence(a, 0, 9), Sequence(1, [0] * 10)
+    sched = Scheduler(a, SchedulerConfig(max_model_len=64, max_num_batched_tokens=64, watermark_blocks=0))
+    a.fork(s, child)
+    with pytest.raises(RequestRejected, match="already owns blocks"):
+        sched.add_request(child)
+    assert not sched.has_unfinished() and a.num_used_blocks == 4
+    a.free(child)
+    child.num_cached_tokens = 0
+    sched.add_request(child)
+    a.fork(s, child, 8)  # behind the queue's back: it says so, and loses nothing
+    with pytest.raises(ValueError, match="already owns blocks"):
+        sched.schedule()
+    assert len(sched.waiting) == 1 and sched.waiting[0] is child and not sched.running
+    sched.abort(child)
+    assert a.num_used_blocks == 3 and not sched.has_unfinished()

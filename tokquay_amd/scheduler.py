@@ -113,6 +113,8 @@ class Scheduler:
         reason = self.rejection_reason(seq)
         if reason is not None:
             raise RequestRejected(reason)
+        if seq.block_table:  # a fork: what is queued holds no blocks, so that a running sequence finds room
+            raise RequestRejected(f"sequence {seq.seq_id} already owns blocks")
         seq.status = SequenceStatus.WAITING
         self.waiting.append(seq)
 
@@ -171,8 +173,8 @@ class Scheduler:
             keep_free = cfg.watermark_blocks if self.running else 0
             if alloc.num_free_blocks - keep_free < alloc.blocks_needed(head.num_tokens):
                 return
-            self.waiting.popleft()
             alloc.allocate(head)
+            self.waiting.popleft()
             head.status = SequenceStatus.RUNNING
             self.running.append(head)
             on_admit(head)
