@@ -677,8 +677,8 @@ size_t tq_sample_tokens_workspace_size(int32_t num_rows, int32_t vocab);
  * [num_blocks][num_layers][2][num_kv_heads][block_size][head_dim] of dtype (tq_dtype), head_dim 64 or 128, 16-byte aligned; block_tables and
  * q_start are tq_paged_chunk's. A block that a position is moved to must be in no other sequence's table.
  *
- * A sequence past num_rows (or its block table, with a pool) sets TQ_DEVERR_LENGTH and gets no path; a bad block id sets
- * TQ_DEVERR_BLOCK_ID and that position is not moved. No counterpart in the reference.
+ * A sequence past num_rows (or its block table or 2^31 - 1 positions, with a pool) sets TQ_DEVERR_LENGTH and gets no path; a bad
+ * block id sets TQ_DEVERR_BLOCK_ID and that position is not moved. No counterpart in the reference.
  */
 tq_status tq_accept_tree(int64_t* tokens, int32_t* path, int32_t* counts, int32_t max_path, const int64_t* sampled,
                          const int64_t* draft_tokens, const int32_t* parents, const int32_t* cu_seqlens_q,

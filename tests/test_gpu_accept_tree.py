@@ -158,6 +158,29 @@ def test_errors_are_flagged():
     assert torch.equal(path, want[1]) and torch.equal(pool, c.pool)
 
 
+def test_positions_end_before_2_31():
+    # A block table of more positions than 32 bits count, all in one block: the last sequence that fits them, and those that do not.
+    bs, blocks = 1024, (1 << 21) + 1
+    c = Case([8], [0], layers=1, kv_heads=1, bs=bs, seed=14)
+    c.parents = torch.tensor([-1, 0, 0, 1, 2, 2, 3, 5], dtype=torch.int32)
+    c.drafts = torch.tensor([1, 2, 3, 4, 5, 6, 7, 8])
+    c.tokens = torch.tensor([3, 0, 6, 0, 0, 8, 0, 0])
+    c.tables = torch.zeros(1, blocks, dtype=torch.int32)
+    for start in (2**31 - 1 - 8, 2**31 - 8, 2**31 - 6, 2**31 - 1):
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        c.start[0] = start
+        tokens, path, counts, pool = c.run(err=err)
+        if start + 8 < 2**31:
+            assert path.tolist() == [[0, 2, 5, 7, -1, -1, -1, -1]] and tokens.tolist() == [[3, 6, 8, 0, -1, -1, -1, -1]]
+            want = c.pool.clone()
+            for j, node in enumerate([0, 2, 5, 7]):
+                want[0, :, :, :, (start + j) % bs] = c.pool[0, :, :, :, (start + node) % bs]
+            assert torch.equal(pool, want) and int(err) == 0
+        else:
+            assert int(err) == _lib.DEVERR_LENGTH and counts.tolist() == [0] and bool((path == -1).all())
+            assert bool((tokens == -1).all()) and torch.equal(pool, c.pool)
+
+
 def test_large_pools():
     # Blocks past 2^31 bytes and elements.
     c = Case([30, 40], [40, 3], layers=2, kv_heads=8, dim=128, seed=12, agree=1.0)

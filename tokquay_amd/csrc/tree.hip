@@ -126,11 +126,11 @@ struct AcceptArgs {
   int32_t pieces;       // of a slot, in all layers
   int32_t num_blocks;
   int32_t block_size;
-  int32_t max_blocks;
   int32_t num_rows;
   int32_t num_seqs;
   int32_t max_path;
   int32_t slices;
+  int64_t max_context;  // positions of a block table, at most 2^31 - 1: they are counted in 32 bits
 };
 
 // A workgroup takes 256 16-byte pieces of the slots of one sequence. Each of its waves walks the tree by itself; a piece's
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kMoveThreads) void accept_tree_kernel(const AcceptA
   bool fits = lo >= 0 && n > 0 && lo + n <= a.num_rows;
   if (a.pool != nullptr) {
     start = a.q_start[b];
-    fits = fits && start >= 0 && start + n <= (int64_t)a.max_blocks * a.block_size;
+    fits = fits && start >= 0 && start + n <= a.max_context;
   }
   int64_t* tokens = a.tokens + (int64_t)b * a.max_path;
   int32_t* path = a.path + (int64_t)b * a.max_path;
@@ -305,7 +305,8 @@ extern "C" tq_status tq_accept_tree(int64_t* tokens, int32_t* path, int32_t* cou
     a.slices = (a.pieces + kMoveThreads - 1) / kMoveThreads;
     a.num_blocks = (int32_t)num_blocks;
     a.block_size = block_size;
-    a.max_blocks = max_blocks_per_seq;
+    const int64_t positions = (int64_t)max_blocks_per_seq * block_size;
+    a.max_context = positions < 0x7fffffffLL ? positions : 0x7fffffffLL;
     a.block_tables = block_tables;
     a.bt_stride = block_table_stride;
     a.q_start = q_start;
