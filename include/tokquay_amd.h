@@ -62,6 +62,8 @@
  *     row is undefined but the launch is memory safe.
  *   - Only head_dim == 64 is supported (GPT-2 family), and 64 and 128 by tq_rope_cache_write,
  *     tq_paged_chunk, tq_paged_tree, tq_accept_tree and tq_copy_blocks. block_size may be any value in [1, 1024].
+ *   - A launch takes at most 2^32 - 1 threads. Calls that would need more (2^22 sampled rows, 2^24 accepted trees, 2^24 pieces of
+ *     8 KiB of copied blocks) return TQ_ERR_UNSUPPORTED and launch nothing.
  *   - Calls are not thread safe with respect to the same pool: the caller
  *     (one engine thread) orders them on one stream.
  */

@@ -8,7 +8,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from tests.test_host_chunk_ops import chunk_args, host, inner_strided, off_by_four, other_type, shorter
+from tests.test_host_chunk_ops import chunk_args, chunk_call, host, inner_strided, off_by_four, other_type, shorter, verify_call
 from tokquay_amd import _lib, ops, torch_ops
 
 BF16, F32, I32, I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
@@ -270,3 +270,41 @@ def sample_call(tokens=P, logits=P, ls=90, u=P, t=P, k=P, p=P, m=P, cu=None, seq
 ])  # fmt: skip
 def test_sample_tokens_c_refusals(status, more):
     assert sample_call(**more) == status
+
+
+# ---- more workgroups than a launch takes: 2^32 - 1 threads
+GIB = dict(nb=300, layers=16, kv=64, bs=1024, d=128, dtype=0)  # blocks of 1 GiB
+
+
+@pytest.mark.parametrize("call,more", [
+    (layout_call, dict(seqs=2**23 - 1, mq=449, words=8)), (layout_call, dict(seqs=2**26)), (accept_call, dict(seqs=2**24, pool=None)),
+    (accept_call, dict(seqs=2**18, layers=64, kv=64, d=64)), (accept_call, dict(seqs=2**30)), (copy_call, dict(GIB, pairs=128)),
+    (copy_call, dict(GIB, pairs=256)), (sample_call, dict(rows=2**22, seqs=2**22, wb=1 << 40)),
+    (sample_call, dict(rows=2**16, seqs=2**16, vocab=1 << 21, ls=1 << 21, wb=1 << 60)),
+    (sample_call, dict(rows=2**31 - 1, seqs=2**31 - 1, wb=1 << 60)), (sample_call, dict(rows=2**22, seqs=1, cu=P, wb=1 << 40)),
+    (tree_call, dict(seqs=2**26, rows=2**30)), (tree_call, dict(seqs=2**23, rows=2**30, heads=12, kv=3, qs=768, os=768)),
+    (chunk_call, dict(seqs=2**26, rows=2**30)), (verify_call, dict(rows=2**24, seqs=2**20, wb=1 << 60)),
+    (verify_call, dict(rows=2**22, seqs=2**22, wb=1 << 60)), (verify_call, dict(rows=2**24, seqs=2**24, probs=P, wb=1 << 60)),
+])  # fmt: skip
+def test_launches_that_are_too_large_are_refused(call, more):
+    assert call(**more) == UNSUPPORTED
+
+
+def test_fakes_refuse_launches_that_are_too_large():
+    with FakeTensorMode():
+        with pytest.raises(ValueError, match="tree_layout: q_start has too many sequences"):
+            ops.tree_layout(empty(5, dtype=I32), empty(2**23, dtype=I32), empty(2**23 - 1, dtype=I32), 449)
+        with pytest.raises(ValueError, match="sample_tokens: logits has too many rows"):
+            ops.sample_tokens(empty(2**22, 50), empty(2**22), empty(2**22))
+        with pytest.raises(ValueError, match="sample_tokens: logits has too many rows"):
+            ops.sample_tokens(empty(2**16, 2**21), empty(2**16), empty(2**16))
+        ids = empty(5, dtype=I64)
+        with pytest.raises(ValueError, match="accept_tree: counts has too many sequences"):
+            ops.accept_tree(ids, ids, ids.int(), empty(2**24 + 1, dtype=I32), 1)
+        with pytest.raises(ValueError, match="accept_tree: counts has too many sequences"):
+            n = 2**18
+            ops.accept_tree(ids, ids, ids.int(), empty(n + 1, dtype=I32), 1, empty(2, 64, 2, 64, 16, 64, dtype=BF16),
+                            empty(n, 4, dtype=I32), empty(n, dtype=I32))  # fmt: skip
+        pairs = empty(128, dtype=I32)
+        with pytest.raises(ValueError, match="copy_blocks: src_blocks has too many blocks of this size"):
+            ops.copy_blocks(empty(300, 16, 2, 64, 1024, 128), pairs, pairs)

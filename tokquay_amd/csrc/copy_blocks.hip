@@ -115,7 +115,7 @@ extern "C" tq_status tq_copy_blocks(void* pool, int64_t num_blocks, int32_t num_
   a.block_bytes = slabs * a.slab_bytes;
   a.turns = (num_pairs + kThreads - 1) / kThreads;
   const int64_t turn = (int64_t)kThreads * kPer * a.turns, slices = (a.block_bytes / 16 + turn - 1) / turn;
-  if (a.block_bytes / 16 > 0x7fffffffLL || slices * num_pairs > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
+  if (a.block_bytes / 16 > 0x7fffffffLL || !grid_fits(slices * num_pairs, kThreads)) return TQ_ERR_UNSUPPORTED;
   a.slot_pieces = (int32_t)(slot / 16);
   a.slabs = (int32_t)slabs;
   a.num_blocks = (int32_t)num_blocks;

@@ -1132,7 +1132,8 @@ template <int D, typename T, bool TREE>
 tq_status launch(const ChunkArgs& a, const Plan& p, hipStream_t stream) {
   const int64_t grid = (int64_t)a.num_seqs * a.kv_heads * a.row_tiles * a.parts;
   const int64_t join = (int64_t)a.num_seqs * (((int64_t)a.max_query_len * a.num_heads + kJoinPairs<D> - 1) / kJoinPairs<D>);
-  if (grid > 0x7fffffffLL || (a.parts > 1 && join > 0x7fffffffLL)) return TQ_ERR_UNSUPPORTED;
+  if (grid > 0x7fffffffLL || (!p.queue && !grid_fits(grid, kWave * kWaves)) || (a.parts > 1 && !grid_fits(join, 256)))
+    return TQ_ERR_UNSUPPORTED;
   const dim3 g((unsigned)grid), t(kWave * kWaves);
   if (p.queue) {
     hipLaunchKernelGGL(chunk_order_kernel, dim3(1), dim3(kOrderThreads), 0, stream, a, p.rows);

@@ -732,7 +732,7 @@ Plan plan_of(int32_t num_rows, int32_t vocab) {
 template <typename T>
 tq_status launch(const SampleArgs& a, const Plan& p, hipStream_t stream) {
   const int64_t stats = (int64_t)a.num_rows * a.chunks;
-  if (stats > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
+  if (!grid_fits(stats, kThreads) || !grid_fits(a.num_rows, kPick)) return TQ_ERR_UNSUPPORTED;
   if (p.per == 8)
     hipLaunchKernelGGL((sample_stats_kernel<T, 8>), dim3((unsigned)stats), dim3(kThreads), 0, stream, a);
   else

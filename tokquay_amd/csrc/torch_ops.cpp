@@ -15,6 +15,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 #include <tuple>
@@ -564,6 +565,11 @@ void exactly(const char* op, const char* name, const at::Tensor& t, at::ScalarTy
               "] tensor on ", device);
 }
 
+// One launch takes 2^32 - 1 threads.
+void launchable(const char* op, const char* what, int64_t groups, int64_t threads) {
+  TORCH_CHECK(groups <= 0xffffffffLL / threads, op, ": ", what);
+}
+
 void tree_layout(at::Tensor positions, at::Tensor masks, const at::Tensor& parents, const at::Tensor& cu_seqlens_q,
                  const at::Tensor& q_start, int64_t max_query_len, const c10::optional<at::Tensor>& d_error) {
   const char* op = "tokquay_amd::tree_layout";
@@ -575,6 +581,7 @@ void tree_layout(at::Tensor positions, at::Tensor masks, const at::Tensor& paren
   exactly(op, "cu_seqlens_q", cu_seqlens_q, at::kInt, n + 1, device);
   exactly(op, "positions", positions, at::kLong, rows, device);
   TORCH_CHECK(max_query_len >= 0 && max_query_len <= INT32_MAX, op, ": max_query_len must be a length");
+  launchable(op, "q_start has too many sequences", n + 1, 64 * std::min<int64_t>(8, std::max<int64_t>(1, (max_query_len + 63) / 64)));
   masks_of(op, masks, rows, max_query_len, device);
   if (d_error.has_value()) exactly(op, "d_error", *d_error, at::kInt, 1, device);
   check(tq_tree_layout(positions.data_ptr<int64_t>(), masks.data_ptr<int64_t>(), masks.size(1),
@@ -593,6 +600,8 @@ void sample_tokens(at::Tensor tokens, const at::Tensor& logits, const at::Tensor
   const int64_t rows = logits.size(0), vocab = logits.size(1);
   const at::Device device = logits.device();
   TORCH_CHECK(rows <= INT32_MAX && vocab >= 1 && vocab <= 1 << 21, op, ": logits must have 1 to 2097152 columns");
+  launchable(op, "logits has too many rows", rows, 1024);
+  launchable(op, "logits has too many rows", rows * ((vocab + 8191) / 8192), 256);
   const int64_t ls = vocab_rows_of(op, "logits", logits, rows, vocab);
   exactly(op, "temperature", temperature, at::kFloat, cu_seqlens_q.has_value() ? -1 : rows, device);
   const int64_t n = temperature.numel();
@@ -647,6 +656,9 @@ void accept_tree(at::Tensor tokens, at::Tensor path, at::Tensor counts, const at
     TORCH_CHECK(block_tables->size(1) <= INT32_MAX, op, ": block_tables has too many columns");
     exactly(op, "q_start", *q_start, at::kInt, n, device);
   }
+  // A workgroup takes 256 pieces of 16 bytes.
+  const int64_t pieces = pool.has_value() ? pool->numel() / (pool->size(0) * pool->size(4)) * pool->element_size() / 16 : 1;
+  launchable(op, "counts has too many sequences", n * ((pieces + 255) / 256), 256);
   check(tq_accept_tree(tokens.data_ptr<int64_t>(), path.data_ptr<int32_t>(), counts.data_ptr<int32_t>(),
                        (int32_t)tokens.size(1), sampled.data_ptr<int64_t>(), draft_tokens.data_ptr<int64_t>(),
                        parents.data_ptr<int32_t>(), cu_seqlens_q.data_ptr<int32_t>(), (int32_t)n, (int32_t)rows,
@@ -706,6 +718,9 @@ void copy_blocks(at::Tensor pool, const at::Tensor& src_blocks, const at::Tensor
   TORCH_CHECK(n <= 1 << 20, op, ": src_blocks has more than 1048576 entries");
   exactly(op, "dst_blocks", dst_blocks, at::kInt, n, p.device);
   if (num_slots.has_value()) exactly(op, "num_slots", *num_slots, at::kInt, n, p.device);
+  // A workgroup takes 8 KiB, for every 256 pairs.
+  const int64_t share = 8192 * std::max<int64_t>(1, (n + 255) / 256), block = pool.numel() / p.blocks * pool.element_size();
+  launchable(op, "src_blocks has too many blocks of this size", n * ((block + share - 1) / share), 256);
   if (d_error.has_value()) exactly(op, "d_error", *d_error, at::kInt, 1, p.device);
   check(tq_copy_blocks(pool.data_ptr(), p.blocks, p.layers, p.heads, p.block_size, p.head_dim,
                        dtype_of(pool.scalar_type()), src_blocks.data_ptr<int32_t>(), dst_blocks.data_ptr<int32_t>(),

@@ -41,6 +41,9 @@ struct TimingEvents {
 };
 TimingEvents take_timing_events();
 
+// Whether one launch takes so many workgroups: the threads of a grid's dimension are counted in 32 bits.
+inline bool grid_fits(int64_t groups, int threads) { return groups <= 0xffffffffLL / threads; }
+
 // Checks the launch that was just enqueued.
 inline tq_status check_launch() {
   hipError_t e = hipGetLastError();

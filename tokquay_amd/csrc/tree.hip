@@ -255,7 +255,8 @@ extern "C" tq_status tq_tree_layout(int64_t* positions, int64_t* masks, int64_t 
       (num_seqs > 0 && (parents == nullptr || q_start == nullptr)) || mask_words > 0x3fffffffLL ||
       mask_words * 64 < max_query_len)
     return TQ_ERR_INVALID_ARGUMENT;
-  if (num_seqs == 0x7fffffff) return TQ_ERR_UNSUPPORTED;
+  const int waves = max_query_len > kLayoutNodes - kWave ? kLayoutWaves : max_query_len > kWave ? (max_query_len + kWave - 1) / kWave : 1;
+  if (!grid_fits((int64_t)num_seqs + 1, kWave * waves)) return TQ_ERR_UNSUPPORTED;
   LayoutArgs a;
   a.positions = positions;
   a.masks = reinterpret_cast<uint64_t*>(masks);
@@ -267,7 +268,6 @@ extern "C" tq_status tq_tree_layout(int64_t* positions, int64_t* masks, int64_t 
   a.num_rows = num_rows;
   a.num_seqs = num_seqs;
   a.max_query_len = max_query_len;
-  const int waves = max_query_len > kLayoutNodes - kWave ? kLayoutWaves : max_query_len > kWave ? (max_query_len + kWave - 1) / kWave : 1;
   hipLaunchKernelGGL(tree_layout_kernel, dim3((unsigned)num_seqs + 1), dim3(kWave * waves), 0, (hipStream_t)stream, a);
   return check_launch();
 }
@@ -313,7 +313,7 @@ extern "C" tq_status tq_accept_tree(int64_t* tokens, int32_t* path, int32_t* cou
   } else {
     a.slot_pieces = 1;
   }
-  if ((int64_t)num_seqs * a.slices > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
+  if (!grid_fits((int64_t)num_seqs * a.slices, kMoveThreads)) return TQ_ERR_UNSUPPORTED;
   a.tokens = tokens;
   a.path = path;
   a.counts = counts;

@@ -458,14 +458,16 @@ template <typename T>
 tq_status launch(const VerifyArgs& a, const Plan& p, hipStream_t stream) {
   const int64_t rows = a.num_rows > a.num_seqs ? a.num_rows : a.num_seqs;
   const int64_t stats = rows * a.chunks;
-  if (stats > 0x7fffffffLL || (int64_t)a.num_seqs * a.draw_chunks > 0x7fffffffLL) return TQ_ERR_UNSUPPORTED;
+  const bool decided = p.decide || a.probs == nullptr;
+  if (!grid_fits(stats, kThreads) || (decided && !grid_fits(a.num_seqs, p.per == 8 ? kThreads : 4 * kThreads)) ||
+      (a.probs != nullptr && !grid_fits((int64_t)a.num_seqs * a.draw_chunks, kThreads)))
+    return TQ_ERR_UNSUPPORTED;
   if (p.per == 8)
     hipLaunchKernelGGL((verify_stats_kernel<T, 8>), dim3((unsigned)stats), dim3(kThreads), 0, stream, a);
   else
     hipLaunchKernelGGL((verify_stats_kernel<T, 32>), dim3((unsigned)stats), dim3(kThreads), 0, stream, a);
   tq_status st = check_launch();
   if (st != TQ_OK) return st;
-  const bool decided = p.decide || a.probs == nullptr;
   if (decided) {
     if (p.per == 8)
       hipLaunchKernelGGL((verify_decide_kernel<T, kThreads>), dim3((unsigned)a.num_seqs), dim3(kThreads), 0, stream, a);

@@ -450,6 +450,11 @@ def _slots_of(op, pool):
         _fail(op, "a slot of the pool has too many elements")
 
 
+def _launchable(op, what, groups, threads):
+    if groups > 0xFFFFFFFF // threads:
+        _fail(op, what)
+
+
 def _fake_tree_layout(positions, masks, parents, cu_seqlens_q, q_start, max_query_len, d_error):
     op, device = "tree_layout", parents.device
     if not parents.is_cuda:
@@ -461,6 +466,7 @@ def _fake_tree_layout(positions, masks, parents, cu_seqlens_q, q_start, max_quer
     _exactly(op, "positions", positions, torch.int64, rows, device)
     if not 0 <= max_query_len < 2**31:
         _fail(op, "max_query_len must be a length")
+    _launchable(op, "q_start has too many sequences", n + 1, 64 * min(8, max(1, (max_query_len + 63) // 64)))
     _masks_of(op, masks, rows, max_query_len, device)
     if d_error is not None:
         _exactly(op, "d_error", d_error, torch.int32, 1, device)
@@ -473,6 +479,8 @@ def _fake_sample_tokens(tokens, logits, uniforms, temperature, top_k, top_p, min
     rows, vocab = logits.shape
     if not (rows < 2**31 and 1 <= vocab <= 1 << 21):
         _fail(op, "logits must have 1 to 2097152 columns")
+    _launchable(op, "logits has too many rows", rows, 1024)
+    _launchable(op, "logits has too many rows", rows * ((vocab + 8191) // 8192), 256)
     if vocab > 1 and logits.stride(1) != 1:
         _fail(op, f"logits must be [{rows}, {vocab}] with contiguous rows")
     if rows > 1 and logits.stride(0) < vocab:
@@ -514,6 +522,8 @@ def _fake_accept_tree(tokens, path, counts, sampled, draft_tokens, parents, cu_s
         if block_tables.size(1) >= 2**31:
             _fail(op, "block_tables has too many columns")
         _exactly(op, "q_start", q_start, torch.int32, n, device)
+    pieces = 1 if pool is None else pool.numel() // (pool.size(0) * pool.size(4)) * pool.element_size() // 16
+    _launchable(op, "counts has too many sequences", n * ((pieces + 255) // 256), 256)
 
 
 def _fake_copy_blocks(pool, src_blocks, dst_blocks, num_slots, d_error):
@@ -527,6 +537,8 @@ def _fake_copy_blocks(pool, src_blocks, dst_blocks, num_slots, d_error):
     _exactly(op, "dst_blocks", dst_blocks, torch.int32, n, pool.device)
     if num_slots is not None:
         _exactly(op, "num_slots", num_slots, torch.int32, n, pool.device)
+    share, block = 8192 * max(1, (n + 255) // 256), pool.numel() // pool.size(0) * pool.element_size()
+    _launchable(op, "src_blocks has too many blocks of this size", n * ((block + share - 1) // share), 256)
     if d_error is not None:
         _exactly(op, "d_error", d_error, torch.int32, 1, pool.device)
 
