@@ -277,3 +277,17 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
         assert torch.equal(want.cpu(), sampled(logits.cpu(), u.cpu(), *(x.cpu() for x in s)))
+
+
+@pytest.mark.parametrize("rows", [96, 160])
+def test_draws_that_meet_the_border_of_a_chunk(rows):
+    # 16 times the same 2,048 columns, and uniform numbers of whole sixteenths: what lies before the chunk (of 2,048 columns, or of 8,192
+    # with many rows) or the round (4,096) that the token falls in is the goal itself, up to roundings to either side. The token is
+    # the first column of that sixteenth, or by those roundings the one before. Every weight is far above them.
+    g = torch.Generator().manual_seed(33)
+    logits = torch.cat([torch.rand(rows, 2048, generator=g) * -3.0] * 16, 1)
+    sixteenth = torch.arange(rows) % 16
+    for turn, t in enumerate((0.3, 0.7, 1.0, 1.3, 2.7)):
+        got, err = run(logits.roll(turn, 0), sixteenth / 16, torch.full((rows,), t))
+        off = got - 2048 * sixteenth
+        assert err == 0 and bool(((off == 0) | ((off == -1) & (sixteenth > 0))).all()), (t, off.tolist())

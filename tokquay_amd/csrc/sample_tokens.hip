@@ -349,6 +349,10 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
       for (int e = 0; e < 4; ++e) d[j][e] = x[j][e] == x[j][e] ? distance_of(x[j][e]) : kNone;
   };
 
+  // What is left of the goal behind what lies before a thread: `upto - mine` is not the sum before it bit for bit, and may be a few
+  // roundings past a goal that meets this border. Below 0 means that there is no goal yet.
+  auto behind = [](double goal, double before) { return goal < before ? 0.0 : goal - before; };
+
   // The sum of the row's weights, and for draws from all of them the chunk that the token falls in.
   double total = 0.0, rest = -1.0;
   if (s.sums()) {
@@ -361,7 +365,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
     if (s.all()) {
       const double goal = u * total;
       const int chosen = first_of(mine > 0.0 && upto > goal, mine > 0.0, part());
-      if (tid == chosen) sh.goal = goal - (upto - mine);
+      if (tid == chosen) sh.goal = behind(goal, upto - mine);
       __syncthreads();
       rest = sh.goal;
       first = chosen * a.chunk_columns;
@@ -688,7 +692,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
     upto = sums(mine, part(), all);
     const double goal = rest < 0.0 ? u * all : rest;
     r = max(first_of(mine > 0.0 && upto > goal, mine > 0.0, part()), 0);
-    if (tid == r) sh.goal = goal - (upto - mine);
+    if (tid == r) sh.goal = behind(goal, upto - mine);
     __syncthreads();
     rest = sh.goal;
     found = true;
