@@ -651,9 +651,11 @@ size_t tq_paged_tree_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t
  * entries, non-decreasing) is given, an entry a sequence, for its rows; rows of no sequence are left alone. Without cu_seqlens_q
  * num_seqs is num_rows. logits is [num_rows, vocab] of dtype (tq_dtype), vocab at most 2^21, rows logits_row_stride elements apart.
  *
- * The weights are exponentials off by at most 2.2e-12 and the draw's sums fp64. top_p's sums are whole multiples of vocab 2^-63 (of 2^-51
- * below 4,097 columns), the largest weight being 1, and so the same for every order. A token may differ from the exact rule's only where
- * a uniform number, or p times the sum, meets a border that closely.
+ * The weights are exponentials off by at most 2.2e-12. The sums of weights that are held against p times the whole are of weights in
+ * fixed point, so the same for every order of additions, and off by less than vocab 2^-51 of the whole (6e-11 at 128,000 columns). The
+ * draw's sums are fp64, and so is, without top_k, the whole that p multiplies: their order is fixed for a call, but the latter's depends on
+ * num_rows and vocab, so a row's whole may differ in its last bits between calls of other sizes. A token may differ from the exact
+ * rule's only where a uniform number, or p times the whole, meets a border as closely as all this.
  *
  * Needs tq_sample_tokens_workspace_size(...) bytes of workspace (16-byte aligned, any contents; calls that may run at the
  * same time need one each). No counterpart in the reference's kernels; it stands beside Engine._sample

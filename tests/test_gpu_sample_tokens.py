@@ -291,3 +291,25 @@ def test_draws_that_meet_the_border_of_a_chunk(rows):
         got, err = run(logits.roll(turn, 0), sixteenth / 16, torch.full((rows,), t))
         off = got - 2048 * sixteenth
         assert err == 0 and bool(((off == 0) | ((off == -1) & (sixteenth > 0))).all()), (t, off.tolist())
+
+
+@pytest.mark.parametrize("k", [0, 1_500_000])
+@pytest.mark.parametrize("octaves", [42.8, 43.2, 44.3])
+@pytest.mark.parametrize("p", [1 - 2.0**-23, 1 - 2.0**-24])
+def test_top_p_of_a_long_tail_of_tiny_weights(p, octaves, k):
+    # One likely column and 2^21 - 1 others that together weigh a few times as much as p leaves out.
+    vocab, first, u = 1 << 21, 7, 1 - 2.0**-24
+    logits = torch.full((2, vocab), -octaves * math.log(2.0))
+    logits[:, first] = 0.0
+    w = math.exp(float(logits[0, 0]))
+    total = 1 + ((k or vocab) - 1) * w
+    kept = max(0, math.ceil((p * total - 1) / w))  # of the tail: those before which less than p of the sum lies
+    goal = u * (1 + kept * w)
+    want = math.floor((goal - 1) / w)  # of the tail's columns, the one that passes it; below 0: the likely column does
+    got, err = run(logits, torch.full((2,), u), torch.ones(2), torch.full((2,), k, dtype=torch.int32), torch.full((2,), p))
+    assert err == 0
+    # Sums of 2^21 weights in fixed point are off by at most vocab 2^-52 of them; the exponentials (2.2e-12 of the tail) and fp64
+    # additions (2^-53 each, 512 rounds of them and the chunks') less than 2^-40 in all.
+    slack = (vocab * 2.0**-52 + 2.0**-40) / w + 2
+    for column in got.tolist():
+        assert abs(column - (column > first) - want) <= slack if goal > 1 else column == first, (column, want, kept, slack)

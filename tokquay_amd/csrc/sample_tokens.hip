@@ -36,6 +36,7 @@ constexpr int kListed = 8192;       // columns that are kept in LDS; rows of whi
 constexpr int kRanked = 1024;       // of them, those that are ranked by comparing each with each; at most kPick
 constexpr int kSelected = 4096;     // groups whose columns are listed; if more reach the limit, all are looked at
 constexpr int kMaxVocab = 1 << 21;
+constexpr int kFewRanks = 4096;     // of top-k: their weights' roundings in units of the vocabulary's stay below those of the row's
 constexpr int kRound = 4 * kPick;
 constexpr int kMaxRounds = kMaxVocab / kRound;
 static_assert(kMaxRounds <= kPick && kRanked <= kPick && kMaxVocab / kGroup <= 1 << 16, "an entry a thread, groups in 16 bits");
@@ -59,7 +60,7 @@ struct SampleArgs {
   int32_t chunks;
   int32_t chunk_columns;
   int32_t groups;
-  int32_t mass_bits;  // weights are counted in units of 2^-mass_bits
+  int32_t mass_bits;  // weights are counted in units of 2^-mass_bits, where the row's sum is not known
 };
 
 // A row's settings.
@@ -71,7 +72,7 @@ struct Settings {
   __device__ __forceinline__ bool nucleus() const { return p < 1.f; }
   __device__ __forceinline__ bool all() const { return k == 0 && !nucleus() && !(least > 0.f); }
   // Whether the sum of the whole row's weights is asked for.
-  __device__ __forceinline__ bool sums() const { return k == 0 && (nucleus() || !(least > 0.f)); }
+  __device__ __forceinline__ bool sums() const { return nucleus() ? k == 0 || k > kFewRanks : k == 0 && !(least > 0.f); }
 };
 
 __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int row) {
@@ -249,8 +250,9 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
     const double t = ((double)key_value((uint64_t)(key - d) << 32) - t0) * c;
     return t >= -1000.0 ? exp2_neg(t) : 0.0;
   };
-  const double unit = __builtin_ldexp(1.0, a.mass_bits);
-  auto fixed = [&](double w) {  // w below 2^(52 - mass_bits)
+  int mass_bits = a.mass_bits;
+  double unit = __builtin_ldexp(1.0, mass_bits);
+  auto fixed = [&](double w) {  // w at most 1, mass_bits at most 51
     return __builtin_bit_cast(uint64_t, __builtin_fma(w, unit, 0x1p52)) & 0xfffffffffffffull;
   };
 
@@ -259,7 +261,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
   const float cf = fminf((float)c, 1e30f);
   auto nearly = [&](uint32_t d) {
     const float w = __builtin_amdgcn_exp2f((key_value((uint64_t)(key - d) << 32) - top) * cf);
-    return (uint64_t)(uint32_t)(w * 0x1p31f) << (a.mass_bits - 31);
+    return (uint64_t)(uint32_t)(w * 0x1p31f) << (mass_bits - 31);
   };
   const double slack = 1.0 + 1e-4 + a.vocab * 0x1p-31;
 
@@ -362,6 +364,10 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
       if (t >= -1000.0) mine = st[tid].sum * exp2_neg(t);
     }
     const double upto = sums(mine, part(), total);
+    // As fine as the sum allows, that of all weights below 2^63 units: a peaked row's many tiny weights are not rounded away together.
+    // Off by half a unit each, they are off by less than vocab 2^-51 of the sum; so are up to kFewRanks in units of the vocabulary's.
+    mass_bits = min(51, 63 - __builtin_amdgcn_frexp_exp(total));
+    unit = __builtin_ldexp(1.0, mass_bits);
     if (s.all()) {
       const double goal = u * total;
       const int chosen = first_of(mine > 0.0 && upto > goal, mine > 0.0, part());
