@@ -313,3 +313,14 @@ def test_top_p_of_a_long_tail_of_tiny_weights(p, octaves, k):
     slack = (vocab * 2.0**-52 + 2.0**-40) / w + 2
     for column in got.tolist():
         assert abs(column - (column > first) - want) <= slack if goal > 1 else column == first, (column, want, kept, slack)
+
+
+def test_subnormal_temperatures_and_flat_rows():
+    # Temperatures below the normal numbers, and logits that lie as close: a distribution as flat as any other, of which top-p leaves
+    # thousands of columns.
+    g = torch.Generator().manual_seed(34)
+    for vocab in (50257, 9001):
+        logits = torch.randint(0, 8_000_000, (12, vocab), generator=g, dtype=torch.int32).view(torch.float32)
+        for bits in (30_000, 2_000_000, 6_000_000):
+            t = float(torch.tensor([bits], dtype=torch.int32).view(torch.float32))
+            check(logits, [(t, 0, 0.9, 0.0), (t, 0, 0.5, 0.0), (t, 0, 1.0, 0.0), (t, 9000, 0.7, 0.0), (t, 20000, 0.3, 0.0)], bits)

@@ -257,8 +257,9 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
   };
 
   // The same nearly, for a search that is made again with exact ones where it ends: by an exponential that is off by 2e-6 (of
-  // exponents up to 30), in units of 2^-31; `slack` is more than both.
-  const float cf = fminf((float)c, 1e30f);
+  // exponents up to 30), in units of 2^-31; `slack` is more than both. Not where T is so small that c is infinite in 32 bits: then
+  // there is no such search.
+  const float cf = (float)c;
   auto nearly = [&](uint32_t d) {
     const float w = __builtin_amdgcn_exp2f((key_value((uint64_t)(key - d) << 32) - top) * cf);
     return (uint64_t)(uint32_t)(w * 0x1p31f) << (mass_bits - 31);
@@ -401,7 +402,7 @@ __global__ __launch_bounds__(kPick) void sample_pick_kernel(const SampleArgs a) 
         make = kMaxima;
       }
     }
-    bool scouted = false;
+    bool scouted = !(cf < INFINITY);
     uint32_t lo = 0;
     uint64_t n0 = 0, m0 = 0;  // before lo
     int shift = 14;
