@@ -308,3 +308,8 @@ def test_fakes_refuse_launches_that_are_too_large():
         pairs = empty(128, dtype=I32)
         with pytest.raises(ValueError, match="copy_blocks: src_blocks has too many blocks of this size"):
             ops.copy_blocks(empty(300, 16, 2, 64, 1024, 128), pairs, pairs)
+
+
+def test_sample_tokens_without_settings_for_its_rows():
+    # Without cu_seqlens_q every row has settings of its own: none at all are too few, not a call without work.
+    assert sample_call(seqs=0) == INVALID and sample_call(seqs=0, rows=0) == OK and sample_call(seqs=0, cu=P) == OK

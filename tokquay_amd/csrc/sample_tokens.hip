@@ -771,7 +771,7 @@ extern "C" tq_status tq_sample_tokens(int64_t* tokens, const void* logits, int64
   using namespace tq;
   if (num_seqs < 0 || num_rows < 0 || vocab < 1) return TQ_ERR_INVALID_ARGUMENT;
   if ((dtype != TQ_F32 && dtype != TQ_F16 && dtype != TQ_BF16) || vocab > kMaxVocab) return TQ_ERR_UNSUPPORTED;
-  if (num_rows == 0 || num_seqs == 0) return TQ_OK;
+  if (num_rows == 0 || (num_seqs == 0 && cu_seqlens_q != nullptr)) return TQ_OK;
   if (tokens == nullptr || logits == nullptr || uniforms == nullptr || temperature == nullptr ||
       (cu_seqlens_q == nullptr && num_seqs < num_rows) || (num_rows > 1 && logits_row_stride < vocab))
     return TQ_ERR_INVALID_ARGUMENT;
