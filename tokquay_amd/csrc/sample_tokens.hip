@@ -22,6 +22,8 @@
 // make 31), 2 by its dependent steps of 1-3 us: one row of 50,257 with top-k 50 and top-p 11 us, from the temperature alone 5.6, with top-k
 // 1,000 23; 256 rows of 128,000 with settings of all kinds 24. Read and ranked by one workgroup a row in passes over all of its columns, one row
 // took 103 us and the 256 273. Top-p 0.9 of 256 x 128,000 normal logits, some 5,700 columns each, takes 96.
+#include <type_traits>
+
 #include "draw.h"
 
 namespace tq {

@@ -22,6 +22,8 @@
 //    sequence to finish finds chunk and column. A few sequences do without 2: each workgroup decides, all draw (one sequence of
 //    4 drafts: 10 us, dependent steps of 1-2 us).
 
+#include <type_traits>
+
 #include "draw.h"
 
 namespace tq {
@@ -136,6 +138,53 @@ __device__ __forceinline__ void weights(const Dist& d, const void* row, const fl
     const int at = column_of<kVec<T>, N, PER, RUNS>(i);
     put(i, at < n ? weight_of(d, x[i], (double)q[i], draft, mode, base + at) : 0.0);
   }
+}
+
+// Inclusive sums over the workgroup's N threads, in order; s_part: a word a wave.
+template <int N>
+__device__ __forceinline__ double scan(double v, double* s_part) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  auto up = [&](auto ctrl) {  // from a lane further down in the row of 16; 0 past its start
+    return __builtin_bit_cast(double, dpp_move64<decltype(ctrl)::value>(__builtin_bit_cast(uint64_t, v)));
+  };
+  v += up(std::integral_constant<int, 0x111>());  // row_shr:1, 2, 4, 8
+  v += up(std::integral_constant<int, 0x112>());
+  v += up(std::integral_constant<int, 0x114>());
+  v += up(std::integral_constant<int, 0x118>());
+  double before = 0.0;  // the rows before this one
+#pragma unroll
+  for (int r = 1; r < kWave / 16; ++r) {
+    const double row = __builtin_bit_cast(double, lane_of(__builtin_bit_cast(uint64_t, v), 16 * r - 1));
+    before += lane >= 16 * r ? row : 0.0;
+  }
+  v += before;
+  if (lane == kWave - 1) s_part[wave] = v;
+  __syncthreads();
+  before = 0.0;
+#pragma unroll
+  for (int u = 0; u < N / kWave - 1; ++u) before += u < wave ? s_part[u] : 0.0;
+  __syncthreads();
+  return before + v;
+}
+
+// The first thread with `over`, or the last with `has` where there is none; -1: none either. s_pick: two words a wave.
+template <int N>
+__device__ __forceinline__ int pick(bool over, bool has, int (*s_pick)[2]) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const uint64_t overs = __builtin_amdgcn_ballot_w64(over), those = __builtin_amdgcn_ballot_w64(has);
+  if (lane == 0) {
+    s_pick[wave][0] = overs != 0 ? wave * kWave + __builtin_ctzll(overs) : 0x7fffffff;
+    s_pick[wave][1] = those != 0 ? wave * kWave + 63 - __builtin_clzll(those) : -1;
+  }
+  __syncthreads();
+  int first = 0x7fffffff, last = -1;
+#pragma unroll
+  for (int v = 0; v < N / kWave; ++v) {
+    first = min(first, s_pick[v][0]);
+    last = max(last, s_pick[v][1]);
+  }
+  __syncthreads();
+  return first != 0x7fffffff ? first : last;
 }
 
 // What became of a sequence's drafts: how many stand, and the distribution of the row that the next token is drawn from.
