@@ -67,8 +67,6 @@ struct ChunkArgs {
   int64_t bt_stride;
   const int32_t* cu_q;
   const int32_t* q_start;
-  const uint32_t* masks;  // tq_paged_tree: row r's bits from masks + r mask_words on
-  int64_t mask_words;
   float* part_o;   // [num_q_rows][num_heads][parts][D] sums of each part, or null: one part
   float* part_ml;  // [num_q_rows][num_heads][parts][2] maximum and weight sum
   int32_t* queue;  // kQueueHead words, then (sequence, row tile) pairs: chunk_order_kernel; or null
@@ -89,6 +87,10 @@ struct ChunkArgs {
   int32_t row_tiles;    // workgroup row tiles per (sequence, K/V head)
   int32_t parts;        // key parts per row tile
   int32_t part_tokens;  // keys of a part, a multiple of kWaves * kTileKeys
+  // tq_paged_tree: row r's bits from masks + r mask_words on. Behind all others, so that those lie where they do without masks: further
+  // up, the kernels without masks fetched them otherwise (one token behind 500 12.1 -> 12.4 us, 32 x 5 drafted tokens 42.9 -> 43.5).
+  const uint32_t* masks;
+  int64_t mask_words;
 };
 
 __device__ __forceinline__ float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
