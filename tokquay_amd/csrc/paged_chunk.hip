@@ -88,7 +88,7 @@ struct ChunkArgs {
   int32_t parts;        // key parts per row tile
   int32_t part_tokens;  // keys of a part, a multiple of kWaves * kTileKeys
   // tq_paged_tree: row r's bits from masks + r mask_words on. Behind all others, so that those lie where they do without masks: further
-  // up, the kernels without masks fetched them otherwise (one token behind 500 12.1 -> 12.4 us, 32 x 5 drafted tokens 42.9 -> 43.5).
+  // up, the kernels without masks fetched them otherwise (one token behind 4,000 12.1 -> 12.4 us, 32 x 5 drafted tokens 42.9 -> 43.5).
   const uint32_t* masks;
   int64_t mask_words;
 };
