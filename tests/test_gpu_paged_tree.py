@@ -251,3 +251,19 @@ def test_offsets_past_2_to_the_31():
     want, bound = c.expected()
     c.tables += shift
     assert_within(run(c, pool=pool), want, bound)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("start,nodes", [(0, 9), (0, 90), (0, 600), (5, 9), (70, 90)])
+def test_rows_whose_scores_are_all_minus_infinity_have_no_softmax(start, nodes, dim):
+    # Not the same as a row that sees nothing: NaN, as in a line by paged_chunk.
+    c = Tree([(start, grown(nodes, 0, line=True))], 2, 1, dim, BF16, 16, seed=23)
+    c.q = c.q.abs().clamp_min(0.25)
+    c.pool[:, :, 0, :, :, 0] = -math.inf
+    out, same = run(c), torch.empty_like(c.q).cuda()
+    ops.paged_chunk(same, c.q.cuda(), c.pool.cuda(), LAYER, c.tables.cuda(), c.cu.cuda(), c.start.cuda(), c.max_new, c.max_context)
+    assert bool(same.isnan().all()) and bool(out.isnan().all())
+    c.masks[1::3] = 0
+    out = run(c)
+    blind = torch.arange(nodes) % 3 == 1 if start == 0 else torch.zeros(nodes, dtype=torch.bool)
+    assert bool((out[blind] == 0).all()) and bool(out[~blind].isnan().all())

@@ -37,7 +37,7 @@
 //
 // TREE (tq_paged_tree): the new tokens are nodes of a tree of drafts, and a row sees of them those that its mask names and that are not
 // behind itself, so a part of what it would see in a line: tiles, parts and maxima are those of a line, and tiles with new keys are
-// masked by bits. A row that sees nothing has a sum of zero, and gets zeros. 64 trees of 64 nodes behind 511-4,094 tokens, 32 / 8
+// masked by bits. A row that sees nothing has a sum of zero and gets zeros (inverse). 64 trees of 64 nodes behind 511-4,094 tokens, 32 / 8
 // heads of 128: 0.62 GB and 155 GFLOP in 202 us (as a line 196), matrix cores busy for 46 % of the time and vector units for 47.
 #include <float.h>
 
@@ -553,10 +553,20 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
-// One over a row's sum of weights; 0 for a tree's row that sees nothing, whose output is zero.
+// One over a row's sum of weights; 0 for a tree's row (token t of the sequence) that sees nothing, whose output is zero. A row that
+// sees keys, but with scores of -infinity alone, has no softmax: NaN, with or without TREE.
 template <bool TREE>
-__device__ __forceinline__ float inverse(float l) {
-  return TREE && l == 0.f ? 0.f : 1.f / l;
+__device__ __forceinline__ float inverse(const ChunkArgs& a, const Seq& s, int t, float l) {
+  if constexpr (TREE) {
+    if (l == 0.f && s.start == 0) {
+      const uint32_t* m = a.masks + (s.row0 + t) * a.mask_words;
+      uint32_t any = m[t / 32] & ((2u << t % 32) - 1u);  // none behind its own
+#pragma unroll 1
+      for (int w = 0; w < t / 32; ++w) any |= m[w];
+      if (any == 0) return 0.f;
+    }
+  }
+  return 1.f / l;
 }
 
 // Few rows: a workgroup takes 16 NT rows and one part of the keys; its waves take every fourth tile of the
@@ -693,7 +703,7 @@ __global__ __launch_bounds__(kWave* kWaves) void chunk_rows_kernel(const ChunkAr
       add_left_out<T, TREE>(a, bt, head_base + d, D, max(kbeg, (w.lo + 1) / kTileKeys * kTileKeys), min(kstop, s.start + t + 1),
                             s, t, o);
     if (a.parts == 1) {
-      const float inv = inverse<TREE>(l);
+      const float inv = inverse<TREE>(a, s, t, l);
       *reinterpret_cast<u32x2*>(a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + d) =
           u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
     } else {
@@ -822,7 +832,7 @@ __device__ __forceinline__ void row_tile(const ChunkArgs& a, const Seq& s, int b
     if (r >= total) continue;
     const int t = r / a.group, h = kvh * a.group + r - t * a.group;
     if (a.parts == 1) {
-      const float inv = inverse<TREE>(l);
+      const float inv = inverse<TREE>(a, s, t, l);
       uint16_t* op = a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + 4 * g;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d)
@@ -1062,7 +1072,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(const ChunkArgs a) {
       for (int k = 0; k < kDims; ++k) o[k] = fmaf(w, x[k], o[k]);
     }
   }
-  const float inv = inverse<TREE>(l);
+  const float inv = inverse<TREE>(a, s, t, l);
   uint16_t* to = a.out + (int64_t)(s.row0 + t) * a.out_stride + h * D + lane * kDims;
 #pragma unroll
   for (int k = 0; k < kDims; k += 2) reinterpret_cast<uint32_t*>(to)[k / 2] = pack2<T>(o[k] * inv, o[k + 1] * inv);
