@@ -695,7 +695,8 @@ tq_status tq_accept_tree(int64_t* tokens, int32_t* path, int32_t* counts, int32_
  * Copies blocks of the pool, all layers, keys and values: the first num_slots[p] slots (all block_size where num_slots is null) of block
  * src_blocks[p] to those of block dst_blocks[p], bit exact, for every pair p. A forked sequence's last block, blocks moved together.
  * Pairs with a negative id, with src_blocks[p] = dst_blocks[p], or of no slots do nothing. The copies run beside each other: a pair
- * whose destination is another such pair's source, or the destination of an earlier one, sets TQ_DEVERR_OVERLAP and is left out. An id
+ * whose destination is the source of another pair than these, or the destination of an earlier one, sets TQ_DEVERR_OVERLAP and is left
+ * out, whatever becomes of that other pair. An id
  * >= num_blocks sets TQ_DEVERR_BLOCK_ID, a count outside [0, block_size] TQ_DEVERR_LENGTH, and the pair is left out. At most 2^20 pairs,
  * since each is held against all others: more are TQ_ERR_UNSUPPORTED.
  * pool is [num_blocks][num_layers][2][num_kv_heads][block_size][head_dim] of dtype (tq_dtype), head_dim 64 or 128, 16-byte aligned.
