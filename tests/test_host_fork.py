@@ -184,3 +184,17 @@ def test_the_scheduler_refuses_sequences_that_own_blocks():
     assert len(sched.waiting) == 1 and sched.waiting[0] is child and not sched.running
     sched.abort(child)
     assert a.num_used_blocks == 3 and not sched.has_unfinished()
+
+
+def test_the_scheduler_refuses_cached_tokens_without_blocks():
+    # A fork that gave its blocks back still counts its cached tokens: admitted, it would read them from blocks that nobody has written.
+    a = allocator()
+    s, child = sequence(a, 0, 9), Sequence(1, [0] * 10)
+    sched = Scheduler(a, SchedulerConfig(max_model_len=64, max_num_batched_tokens=64, watermark_blocks=0))
+    a.fork(s, child)
+    a.free(child)
+    with pytest.raises(RequestRejected, match="cached tokens"):
+        sched.add_request(child)
+    child.reset_for_recompute()
+    sched.add_request(child)
+    assert sched.schedule().seqs == [child]

@@ -115,6 +115,8 @@ class Scheduler:
             raise RequestRejected(reason)
         if seq.block_table:  # a fork: what is queued holds no blocks, so that a running sequence finds room
             raise RequestRejected(f"sequence {seq.seq_id} already owns blocks")
+        if seq.num_cached_tokens:  # of blocks that it gave back
+            raise RequestRejected(f"sequence {seq.seq_id} counts {seq.num_cached_tokens} cached tokens, and owns no blocks")
         seq.status = SequenceStatus.WAITING
         self.waiting.append(seq)
 
